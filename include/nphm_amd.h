@@ -653,6 +653,45 @@ int nphm_dense_gpre(const float* g, const float* y, int n, int c, float beta, fl
                     void* stream);
 int nphm_dense_column_sums(const float* x, int rows, int c, float* out, void* stream);
 
+/* ---- training operators (no change of the ABI version: symbols were added, none changed) ------------------------------------
+ * Around the decoders in a training step (scripts/training/train.py: the table of latent codes, clip_grad_norm_ of decoder and
+ * codes, src/NPHM/models/training.py:111-135) and the dense layer in 16-bit storage.  dtype: 0 fp32, 1 bf16, 2 fp16.  All calls are
+ * stream-ordered, copy nothing from or to the host and can be captured; a captured call keeps using the workspace it was given.
+ *
+ *   nphm_rows_lookup : out[n] = scale * table[idx[n]]  (rows of `dim` elements; rows of the table ld elements apart; idx of idx_bits =
+ *     32 or 64 bits).  An index outside [0, rows) gives a row of NaN.  At most 2^26 - 4 rows / indices, 2^23 elements a row.
+ *   nphm_rows_grad : out [rows, dim] = scale * sum of grad[n] over the n with idx[n] = row, zeros elsewhere and in row `padding`
+ *     (-1: none); indices outside the table add nothing.  fp32 sums in the order of n: bitwise reproducible.
+ *   nphm_rows_merge : out[n] = sum of grad[m] over the m with idx[m] = idx[n] where n is the first of them, else zeros.
+ *   nphm_rows_renorm : rows named by idx whose 2-norm is above max_norm are multiplied by max_norm / (norm + 1e-7), each once;
+ *     flags: `rows` bytes of scratch. */
+int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t count,
+                     float scale, void* out, void* stream);
+size_t nphm_rows_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t count);
+int nphm_rows_grad(const void* grad, int64_t count, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t rows,
+                   int64_t padding, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+int nphm_rows_merge(const void* grad, int64_t count, int64_t dim, int dtype, const void* idx, int idx_bits, void* out, void* stream);
+int nphm_rows_renorm(void* table, int64_t rows, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t count,
+                     float max_norm, void* flags, void* stream);
+/*   nphm_clip_grads : norm (device fp32) over n tensors of counts[i] elements at in[i] (HOST arrays of device pointers; read during
+ *     the call only): kind 0 the 2-norm (squares added in fp64), 1 the largest magnitude (NaN if one is NaN).  out not NULL: out[i] =
+ *     in[i] * min(1, limit / (norm + 1e-6)), in place where out[i] = in[i]; tensors that share memory otherwise are refused.
+ *     workspace: nphm_clip_workspace_bytes(counts, n) bytes, 8-byte aligned. */
+size_t nphm_clip_workspace_bytes(const int64_t* counts, int n);
+int nphm_clip_grads(const void* const* in, void* const* out, const int64_t* counts, const int* dtypes, int n, int kind, double limit,
+                    float* norm, void* workspace, size_t workspace_bytes, void* stream);
+/*   nphm_layer16_forward : z = x W^T + bias, y = a(z) + residual; x [M, K], weight [N, K], y / z / residual [M, N], bias [N], all
+ *     contiguous bf16 or fp16; bias, residual, z (kept for the backward pass) may be NULL.  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU
+ *     (erf), 4 Softplus(beta).  M up to 2^22, N and K up to 2^20.
+ *   nphm_layer16_backward : gz = g a'(z); dx = gz W, dweight = gz^T x, dbias = column sums of gz (each may be NULL).
+ *     Workspaces: nphm_layer16_*_workspace_bytes, 256-byte aligned. */
+size_t nphm_layer16_forward_workspace_bytes(int64_t M, int64_t N, int64_t K);
+int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,
+                         int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream);
+size_t nphm_layer16_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+int nphm_layer16_backward(const void* g, const void* x, const void* weight, const void* z, void* dx, void* dweight, void* dbias, int64_t M,
+                          int64_t N, int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -14,6 +14,9 @@ CSRC = os.path.join(HERE, "csrc")
 EVAL_PARTS = [("eval_kernel.hip", ["-DNPHM_EVAL_PART=1"], "eval_kernel_api"), ("eval_kernel.hip", ["-DNPHM_EVAL_PART=10"], "eval_kernel_f32"),
               ("eval_kernel.hip", ["-DNPHM_EVAL_PART=11"], "eval_kernel_bf16"), ("eval_kernel.hip", ["-DNPHM_EVAL_PART=12"], "eval_kernel_f16")]
 SOURCES = ["prep_kernels.hip", "mlp_kernel.hip", "mlp_bwd_kernel.hip", "ident_bwd_kernel.hip", "ident_train_kernel.hip", "fit_kernels.hip", "train_loss_kernels.hip", "dense_train_kernels.hip", "mc_device.hip", "probe.hip", "marching_cubes.cpp"]
+# the training operators: NaN is a value there (a masked row, a gradient that overflowed), and no packed fp32 instructions
+TRAIN_FLAGS = ["-fhonor-nans", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
+TRAIN_PARTS = [(src, TRAIN_FLAGS, os.path.splitext(src)[0]) for src in ("layer16_kernels.hip", "rows_kernels.hip", "clip_kernels.hip")]
 OUT = os.path.join(HERE, "libnphm_amd.so")
 OBJ_CACHE = os.path.join(HERE, "..", ".build_cache")      # objects by content hash (git- and gpurun-ignored)
 
@@ -49,7 +52,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
             common.update(open(os.path.join(CSRC, f), "rb").read())
     common.update(open(os.path.join(HERE, "..", "include", "nphm_amd.h"), "rb").read())
     jobs, objs = [], []
-    units = EVAL_PARTS + [(src, [], os.path.splitext(src)[0]) for src in SOURCES]       # (the slowest first)
+    units = EVAL_PARTS + TRAIN_PARTS + [(src, [], os.path.splitext(src)[0]) for src in SOURCES]       # (the slowest first)
     for src, extra, tag in units:
         h = common.copy()
         h.update(" ".join(extra).encode())

@@ -27,6 +27,7 @@ import torch
 import torch.nn as nn
 
 from . import _lib
+from .train_ops import linear_act
 from .ensembled_deepsdf import sample_point_feature  # noqa: F401  (re-exported like the reference)
 
 _SQRT2 = float(np.sqrt(2))
@@ -258,6 +259,10 @@ class DeepSDF(nn.Module):
         self.beta = beta
         self.backend = "hip"            # "hip" | "composite"
         self.train_backend = "hip"      # with trainable parameters: "hip" = the dense training tier (evaluate_train_hip) | "composite"
+        # storage of the dense training tier's hidden layers: "fp32", or "bf16" | "fp16" (train_ops.linear_act) for the layers that
+        # read hidden values alone; the layers that read coordinates (the first, the skip layer) and the last stay in fp32 -
+        # a coordinate of 0.5 would move by up to 1e-3 in bf16
+        self.train_precision = "fp32"
         self._pack_cache = None         # (key, packed tensor)
         self._pack_bwd_cache = None     # (key, transposed pack of the backward kernel)
         # Numerics of the plain HIP evaluation (forward_hip / lattice launches; include/nphm_amd.h NPHM_MLP_*):
@@ -381,7 +386,8 @@ class DeepSDF(nn.Module):
     def evaluate_train_hip(self, pos, lat):
         """``evaluate`` with every hidden nn.Linear + activation as ONE launch of csrc/dense_train_kernels.hip and its
         backward - data, weight and bias gradients - on the same kernels (``_DenseLayerFn``): the op sequence of the reference's
-        forward (deepSDF.py:64-89: cat, skip cat / sqrt 2, Linear, Softplus), the concatenations left to torch.  The last
+        forward (deepSDF.py:64-89: cat, skip cat / sqrt 2, Linear, Softplus), the concatenations left to torch.  With ``train_precision``
+        "bf16" or "fp16" the layers between run in 16-bit storage (``linear_act``).  The last
         linear layer (out_dim <= 4 rows) stays an nn.Linear call.  pos [B,N,d_spatial]; lat [B,Lr,lat_dim], Lr in {1,N}."""
         B, N, _ = pos.shape
         lat_full = lat if lat.shape[1] == N else lat.expand(B, N, lat.shape[-1])
@@ -389,12 +395,20 @@ class DeepSDF(nn.Module):
         x = inp
         last = self.num_layers - 2
         beta = float(self.beta)
+        try:
+            half = {"fp32": None, "bf16": torch.bfloat16, "fp16": torch.float16}[self.train_precision]
+        except KeyError:
+            raise ValueError(f"train_precision is 'fp32', 'bf16' or 'fp16', not {self.train_precision!r}") from None
         for layer in range(self.num_layers - 1):
             lin = getattr(self, f"lin{layer}")
             alpha = 1.0
             if layer in self.skip_in:
-                x = torch.cat([x, inp], dim=-1)
+                x = torch.cat([x.float(), inp], dim=-1)
                 alpha = 1.0 / _SQRT2
+            if half is not None and 0 < layer < last and layer not in self.skip_in:
+                x = linear_act(x.to(half), lin.weight.to(half), lin.bias.to(half), "softplus" if beta > 0 else "relu", max(beta, 1e-6))
+                continue
+            x = x.float()
             if layer < last:
                 x = _DenseLayerFn.apply(x, lin.weight, lin.bias, alpha, beta)
             else:

@@ -1,0 +1,679 @@
+"""The training operators (nphm_amd.train_ops) against plain forms in 64 bits: rows of a table and their gradient, the 16-bit dense
+layer and its gradients, the gradient norm and clipping, and a step that uses all of them.
+
+Tolerances count roundings.  A rounding to a type moves a value by at most eps / 2 of it, ``torch.finfo(t).eps / 2``; a sum of n fp32 terms
+by at most (n - 1) 2^-24 of the sum of their magnitudes (the matrix instructions' internal adds are taken as twice that)."""
+import math
+
+import numpy as np
+import pytest
+import torch
+
+from nphm_amd import train_ops as T
+from nphm_amd._lib import NphmAmdError
+from nphm_amd.deepsdf import DeepSDF, _DenseLayerFn
+
+gpu = pytest.mark.gpu
+FLOATS = [torch.float32, torch.bfloat16, torch.float16]
+HALVES = [torch.bfloat16, torch.float16]
+F32 = 2.0 ** -24
+
+
+def half_step(t):
+    return torch.finfo(t).eps / 2
+
+
+def tiny(t):
+    return torch.finfo(t).smallest_normal * torch.finfo(t).eps       # the step below the smallest normal number
+
+
+def within(got, want, bound):
+    """|got - want| <= bound everywhere, all in fp64; says by how much the worst one misses or fits"""
+    d = (got.double() - want).abs()
+    assert bool(torch.isfinite(d).all()), "a value that is not finite"
+    worst = float((d / bound.clamp(min=1e-300)).max()) if d.numel() else 0.0
+    assert worst <= 1.0, f"{worst:.3g} of the bound"
+    return worst
+
+
+# ---- refusals (no GPU is touched) -----------------------------------------------------------------------------------------------
+
+def test_cpu_tensors_are_refused():
+    t, i = torch.zeros(4, 8), torch.zeros(3, dtype=torch.long)
+    for call in (lambda: T.lookup_rows(t, i), lambda: T.lookup_rows_grad(torch.zeros(3, 8), i, 4), lambda: T.renorm_rows_(t, i, 1.0),
+                 lambda: T.linear_act(t.bfloat16(), t.bfloat16()), lambda: T.grad_norm([t]), lambda: T.clip_grads([t], 1.0)):
+        with pytest.raises(TypeError):
+            call()
+    p = torch.nn.Parameter(torch.zeros(3))
+    p.grad = torch.ones(3)
+    with pytest.raises(TypeError):
+        T.clip_grad_norm_([p], 1.0)
+
+
+def test_module_on_cpu_needs_the_composite_backend():
+    codes = T.LatentCodes(5, 8, max_norm=1.0, scale=2.0)
+    with pytest.raises(TypeError):
+        codes(torch.tensor([1, 2]))
+    codes.backend = "composite"
+    got = codes(torch.tensor([1, 2, 1]))
+    assert torch.equal(got, 2.0 * codes.weight[torch.tensor([1, 2, 1])])
+    assert float(codes.weight[1].detach().norm()) <= 1.0 + 1e-6
+    other = torch.nn.Embedding(5, 8)
+    other.load_state_dict(codes.state_dict())
+
+
+def test_bad_arguments_are_refused():
+    for kind in (1.0, 3.0, 0.0):
+        with pytest.raises(ValueError):
+            T.grad_norm([], norm_type=kind)
+    for limit in (-1.0, math.nan):
+        with pytest.raises(ValueError):
+            T.clip_grads([], limit)
+        with pytest.raises(ValueError):
+            T.clip_grad_norm_([], limit)
+    with pytest.raises(ValueError):
+        T.clip_grads([], 1.0, out=[torch.zeros(1)])
+    assert float(T.grad_norm([])) == 0.0 and float(T.clip_grad_norm_([], 1.0)) == 0.0
+    with pytest.raises(ValueError):
+        T.LatentCodes(4, 8, scale=math.inf)
+
+
+def test_c_entries_refuse_before_any_launch():
+    """what the host can see is an error, not a launch: sizes, types, null pointers, memory that tensors share"""
+    import ctypes
+    from nphm_amd import _lib
+    lib = _lib.load()
+    assert lib.nphm_rows_lookup(None, 4, 8, 8, 0, None, 64, 1, 1.0, None, None) != 0
+    assert lib.nphm_rows_lookup(16, 4, 8, 7, 0, 16, 64, 1, 1.0, 16, None) != 0 and b"stride" in lib.nphm_last_error()
+    assert lib.nphm_rows_lookup(16, 4, 8, 8, 3, 16, 64, 1, 1.0, 16, None) != 0 and b"dtype" in lib.nphm_last_error()
+    assert lib.nphm_rows_lookup(16, 4, 8, 8, 0, 16, 16, 1, 1.0, 16, None) != 0 and b"bits" in lib.nphm_last_error()
+    assert lib.nphm_rows_grad(16, 1 << 27, 8, 8, 0, 16, 64, 4, -1, 1.0, 16, 16, 1 << 40, None) != 0 and b"sizes" in lib.nphm_last_error()
+    assert lib.nphm_rows_renorm(16, 4, 8, 8, 0, 16, 64, 1, -1.0, 16, None) != 0 and b"max_norm" in lib.nphm_last_error()
+    assert lib.nphm_layer16_forward(16, 16, None, None, 16, None, 4, 4, 4, 0, 0, 1.0, None, 0, None) != 0 and b"dtype" in lib.nphm_last_error()
+    assert lib.nphm_layer16_forward(16, 16, None, None, 16, None, 0, 4, 4, 1, 0, 1.0, None, 0, None) != 0 and b"sizes" in lib.nphm_last_error()
+    assert lib.nphm_layer16_forward(16, 16, None, None, 16, None, 4, 4, 4, 1, 9, 1.0, None, 0, None) != 0 and b"activation" in lib.nphm_last_error()
+    assert lib.nphm_layer16_backward(16, 16, 16, None, 16, 16, None, 4, 4, 4, 1, 2, 1.0, 16, 1 << 30, None) != 0 and b"null" in lib.nphm_last_error()
+    assert lib.nphm_layer16_backward(16, 16, 16, 16, 16, 16, None, 4, 4, 4, 1, 2, 1.0, 16, 0, None) != 0 and b"workspace" in lib.nphm_last_error()
+
+    def clip(ins, outs, counts, dtypes):
+        n = len(ins)
+        return lib.nphm_clip_grads((ctypes.c_void_p * n)(*ins), (ctypes.c_void_p * n)(*outs), (ctypes.c_int64 * n)(*counts),
+                                   (ctypes.c_int * n)(*dtypes), n, 0, 1.0, 16, 16, 0, None)
+    big = 1 << 20
+    assert clip([big, big + 100], [big, big + 100], [64, 64], [1, 1]) != 0 and b"share memory" in lib.nphm_last_error()
+    assert clip([big, big], [big, big], [64, 64], [1, 1]) != 0 and b"share memory" in lib.nphm_last_error()          # the same twice
+    assert clip([big], [big + 16], [64], [1]) != 0 and b"share memory" in lib.nphm_last_error()                       # shifted by a few
+    assert clip([big, 2 * big], [2 * big, 3 * big], [64, 64], [1, 1]) != 0 and b"share memory" in lib.nphm_last_error()
+    assert clip([big, big], [2 * big, 3 * big], [64, 64], [1, 1]) != 0 and b"workspace" in lib.nphm_last_error()     # read twice: fine
+    assert clip([big], [big], [-1], [1]) != 0 and b"count" in lib.nphm_last_error()
+    assert clip([big], [big], [1], [7]) != 0 and b"dtype" in lib.nphm_last_error()
+
+
+# ---- rows of a table ------------------------------------------------------------------------------------------------------------
+
+@pytest.fixture(scope="module")
+def dev():
+    assert torch.cuda.is_available(), "GPU tests need a ROCm device"
+    return torch.device("cuda:0")
+
+
+ROW_CASES = [(1, 1, 1), (7, 3, 5), (24, 1344, 16), (1000, 64, 257), (50, 200, 1), (333, 1001, 300), (4099, 40, 2500), (9, 515, 10000),
+             (70001, 24, 9001), (3, 8, 40000), (2000, 2048, 700)]
+
+
+@gpu
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("V,D,N", ROW_CASES)
+def test_lookup_and_gradient(dev, t, V, D, N):
+    gen = torch.Generator().manual_seed(V * 31 + D + N)
+    table = torch.randn(V, D, generator=gen).to(t).to(dev)
+    idx = (torch.rand(N, generator=gen) ** 3 * V).long().clamp_(0, V - 1).to(dev)
+    for kind in (torch.int64, torch.int32):
+        for s in (1.0, 0.37):
+            got = T.lookup_rows(table, idx.to(kind), scale=s)
+            want = table.double()[idx] * s
+            s32 = float(np.float32(s))
+            assert got.dtype == t and got.shape == (N, D)
+            within(got, want, want.abs() * (half_step(t) + 2 * F32 + abs(s32 - s) / s) + tiny(t))
+    if True:
+        g = torch.randn(N, D, generator=gen).to(t).to(dev)
+        pad = int(idx[0])
+        for padding in (None, pad):
+            got = T.lookup_rows_grad(g, idx, V, scale=0.37, padding_idx=padding)
+            keep = torch.ones(N, dtype=torch.bool, device=dev) if padding is None else idx != padding
+            want = torch.zeros(V, D, dtype=torch.float64, device=dev).index_put_((idx[keep],), g[keep].double(), accumulate=True) * 0.37
+            mag = torch.zeros(V, D, dtype=torch.float64, device=dev).index_put_((idx[keep],), g[keep].double().abs(), accumulate=True) * 0.37
+            many = torch.bincount(idx[keep], minlength=V)[:, None].double()
+            within(got, want, mag * (many + 2) * F32 + want.abs() * (half_step(t) + F32) + tiny(t))
+            assert torch.equal(got, T.lookup_rows_grad(g, idx.int(), V, scale=0.37, padding_idx=padding))      # bits
+
+
+@gpu
+@pytest.mark.parametrize("t", FLOATS)
+def test_rows_strides_shapes_and_alignment(dev, t):
+    gen = torch.Generator().manual_seed(5)
+    wide = torch.randn(40, 77, generator=gen).to(t).to(dev)
+    idx = torch.randint(0, 40, (3, 1, 4), generator=gen).to(dev)
+    for table in (wide[:, 3:70], wide[:, ::2], wide.t(), wide[::3], wide[:1].expand(40, 77), wide.reshape(-1)[1:1 + 40 * 70].view(40, 70)):
+        i = idx % table.shape[0]
+        got = T.lookup_rows(table, i)
+        assert torch.equal(got, table[i])
+        every_second = i.reshape(-1).repeat(2)[::2]
+        assert torch.equal(T.lookup_rows(table, every_second), table[every_second])
+    g = torch.randn(12, 77, generator=gen).to(t).to(dev)
+    for grad in (g, g[:, 1:70], g.t().contiguous().t(), g[:1].expand(12, 77)):
+        got = T.lookup_rows_grad(grad.reshape(3, 1, 4, -1), idx, 40)
+        assert torch.equal(got, T.lookup_rows_grad(grad.contiguous(), idx.reshape(-1), 40))
+    assert T.lookup_rows(wide, torch.empty(0, 2, dtype=torch.long, device=dev)).shape == (0, 2, 77)
+    assert not T.lookup_rows_grad(g[:0], torch.empty(0, dtype=torch.long, device=dev), 11).any()
+    assert torch.equal(T.lookup_rows(wide, torch.tensor(4, device=dev)), wide[4])
+
+
+@gpu
+@pytest.mark.parametrize("N", [20, 900, 20000])
+def test_indices_outside_the_table(dev, N):
+    """rows of NaN, no gradient, nothing read or written beside the table (rows around it stay)"""
+    V, D = 30, 72
+    around = torch.randn(V + 20, D, device=dev)
+    table = around[10:10 + V]
+    idx = torch.arange(N, device=dev) % V
+    idx[3], idx[7], idx[11], idx[12] = -1, V, 2 ** 40, -2 ** 62
+    bad = (idx < 0) | (idx >= V)
+    got = T.lookup_rows(table, idx)
+    assert bool(got[bad].isnan().all()) and torch.equal(got[~bad], table[idx[~bad]])
+    g = torch.randn(N, D, device=dev)
+    assert torch.equal(T.lookup_rows_grad(g, idx, V), T.lookup_rows_grad(g[~bad], idx[~bad], V))
+    assert not T.lookup_rows_grad(g, torch.full((N,), -5, device=dev), V).any()
+    before = around.clone()
+    T.renorm_rows_(table, idx, 0.5)
+    assert torch.equal(around[:10], before[:10]) and torch.equal(around[10 + V:], before[10 + V:])
+
+
+@gpu
+def test_row_gradients_do_not_overflow_in_sums(dev):
+    """fp16 rows whose partial sums leave the type's range and come back"""
+    g = torch.full((2000, 24), 60000.0, dtype=torch.float16, device=dev)
+    g[1000:] = -60000.0
+    got = T.lookup_rows_grad(g, torch.zeros(2000, dtype=torch.long, device=dev), 2)
+    assert torch.equal(got, torch.zeros_like(got))
+    g[5] = math.nan
+    assert bool(T.lookup_rows_grad(g, torch.zeros(2000, dtype=torch.long, device=dev), 2)[0].isnan().all())
+    assert not T.lookup_rows_grad(g, torch.zeros(2000, dtype=torch.long, device=dev), 2, padding_idx=0).any()      # NaN in a padded place
+
+
+@gpu
+@pytest.mark.parametrize("t", FLOATS)
+def test_renorm_scales_named_rows_once(dev, t):
+    table = (torch.randn(60, 300, generator=torch.Generator().manual_seed(2)) * torch.linspace(0.01, 0.2, 60)[:, None]).to(t).to(dev)
+    idx = torch.tensor([5, 5, 59, 40, 40, 40, 0, 30], device=dev)
+    before, version = table.clone(), table._version
+    T.renorm_rows_(table, idx, 1.0)
+    assert table._version > version
+    want = before.double()
+    for v in set(idx.tolist()):
+        n = float(want[v].norm())
+        if n > 1.0:
+            want[v] *= 1.0 / (n + 1e-7)
+    within(table, want, want.abs() * (half_step(t) + 2 * F32) + tiny(t))
+    untouched = [v for v in range(60) if v not in idx.tolist()]
+    assert torch.equal(table[untouched], before[untouched])
+    ref = torch.nn.functional.embedding(idx, before.float().clone(), max_norm=1.0)
+    assert float((T.lookup_rows(table, idx).float() - ref).abs().max()) <= float(ref.abs().max()) * (half_step(t) + 4e-7)
+
+
+@gpu
+def test_latent_codes_module_against_embedding(dev):
+    for sparse in (False, True):
+        for padding in (None, 2):
+            ours = T.LatentCodes(12, 40, padding_idx=padding, max_norm=0.9, sparse=sparse, scale=1.5, device=dev)
+            ref = torch.nn.Embedding(12, 40, padding_idx=padding, max_norm=0.9, sparse=sparse).to(dev)
+            ref.load_state_dict(ours.state_dict())
+            idx = torch.tensor([[1, 2, 1], [11, 2, 0]], device=dev)
+            a, b = ours(idx), ref(idx) * 1.5
+            go = torch.randn_like(a)
+            a.backward(go)
+            b.backward(go)
+            ga, gb = [m.weight.grad.to_dense() if sparse else m.weight.grad for m in (ours, ref)]
+            assert ours.weight.grad.is_sparse == sparse
+            assert float((a - b).detach().abs().max()) <= 1e-6 and float((ga - gb).abs().max()) <= 2e-6 * float(gb.abs().max())
+            assert float((ours.weight - ref.weight).detach().abs().max()) <= 4 * F32
+            if sparse:       # both kinds step the trainer's optimiser
+                torch.optim.SparseAdam([ours.weight], lr=1e-3).step()
+
+
+# ---- dense layer ----------------------------------------------------------------------------------------------------------------
+
+def layer_inputs(dev, t, M, N, K, bias, residual, seed=0):
+    gen = torch.Generator(device=dev).manual_seed(seed + M + 3 * N + 7 * K)
+    r = lambda *s: torch.randn(*s, device=dev, generator=gen)  # noqa: E731
+    return (r(M, K).to(t), (r(N, K) / math.sqrt(K)).to(t), (0.1 * r(N)).to(t) if bias else None, r(M, N).to(t) if residual else None,
+            r(M, N).to(t))
+
+
+def act64(z, act, beta):
+    """value and slope, from their formulas"""
+    if act == "none":
+        return z, torch.ones_like(z)
+    if act == "relu":
+        return z.clamp(min=0), (z > 0).double()
+    if act == "silu":
+        s = torch.sigmoid(z)
+        return z * s, s + z * s * (1 - s)
+    if act == "gelu":
+        c = 0.5 * torch.erfc(-z / math.sqrt(2))
+        return z * c, c + z * torch.exp(-z * z / 2) / math.sqrt(2 * math.pi)
+    return torch.logaddexp(z * beta, torch.zeros_like(z)) / beta, torch.sigmoid(z * beta)
+
+
+CURVE = {"none": 0.0, "relu": 0.0, "silu": 0.5, "gelu": 0.8}          # largest |a''|; Softplus: beta / 4
+
+
+def check_layer(dev, t, M, N, K, act, beta=1.0, bias=True, residual=False, seed=0):
+    x, w, b, r, g = layer_inputs(dev, t, M, N, K, bias, residual, seed)
+    leaves = [v.clone().requires_grad_() if v is not None else None for v in (x, w, b, r)]
+    y = T.linear_act(leaves[0], leaves[1], leaves[2], activation=act, beta=beta, residual=leaves[3])
+    y.backward(g)
+    plain = T.linear_act(x, w, b, activation=act, beta=beta, residual=r)
+    assert torch.equal(plain, y.detach()) and not plain.requires_grad
+    h = half_step(t)
+    xd, wd, gd = x.double(), w.double(), g.double()
+    z = xd @ wd.t()
+    mag = xd.abs() @ wd.abs().t()
+    if bias:
+        z, mag = z + b.double(), mag + b.double().abs()
+    ez = (K + 4) * 2 * F32 * mag
+    a, slope = act64(z, act, beta)
+    want = a + (r.double() if residual else 0)
+    # a: slope at most 1.13; exp, log and erf to 2^-20 of what enters them; Softplus above 20 / beta is z: off by exp(-20) / beta
+    ey = 1.13 * ez + 2.0 ** -20 * (a.abs() + z.abs()) + (2.1e-9 / beta if act == "softplus" else 0) + F32 * want.abs()
+    within(y.detach(), want, ey + h * (want.abs() + ey) + tiny(t))
+    # gz: z is kept with one rounding, |z a''(z)| <= 0.5 for every activation; then gz is rounded once itself
+    curve = beta / 4 if act == "softplus" else CURVE[act]
+    gz = gd * slope
+    dz = gd.abs() * ((0.55 * h if act not in ("none", "relu") else 0) + curve * ez + 2.0 ** -19)
+    if act == "relu":
+        dz = dz + gd.abs() * (z.abs() <= ez + tiny(t))
+    rounded = dz + (h * (gz.abs() + dz) + tiny(t) if act != "none" else 0)
+    wants = [(gz @ wd, rounded @ wd.abs() + (N + 4) * 2 * F32 * ((gz.abs() + rounded) @ wd.abs())),
+             (gz.t() @ xd, rounded.t() @ xd.abs() + (M + 4) * 2 * F32 * ((gz.abs() + rounded).t() @ xd.abs())),
+             (gz.sum(0), dz.sum(0) + (M + 4) * F32 * (gz.abs() + dz).sum(0))]
+    for leaf, (v, e) in zip(leaves[:3], wants):
+        if leaf is not None:
+            assert leaf.grad.dtype == t
+            within(leaf.grad, v, e + h * (v.abs() + e) + tiny(t))
+    if residual:
+        assert torch.equal(leaves[3].grad, g)
+    return leaves, y
+
+
+@gpu
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("act,beta", [("none", 1.0), ("relu", 1.0), ("silu", 1.0), ("gelu", 1.0), ("softplus", 1.0), ("softplus", 100.0)])
+@pytest.mark.parametrize("M,N,K", [(1, 1, 1), (5, 130, 515), (70, 64, 64), (300, 257, 200)])
+def test_layer_and_gradients(dev, t, act, beta, M, N, K):
+    check_layer(dev, t, M, N, K, act, beta, bias=True, residual=M != 70)
+
+
+@gpu
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("M,N,K", [(1, 1024, 512), (16, 333, 4096), (17, 40, 1000), (33, 2048, 96), (64, 3, 512), (129, 1, 8), (128, 128, 128), (256, 256, 256),
+                                   (257, 513, 129), (1000, 512, 512), (4095, 96, 515), (2, 5000, 24), (3000, 8, 1344), (515, 1030, 1032),
+                                   (20000, 64, 72)])
+@pytest.mark.parametrize("bias,residual", [(True, False), (False, True)])
+def test_layer_sizes(dev, t, M, N, K, bias, residual):
+    check_layer(dev, t, M, N, K, "softplus" if residual else "none", 20.0, bias=bias, residual=residual)
+
+
+@gpu
+def test_layer_strides_shapes_and_refusals(dev):
+    t = torch.bfloat16
+    x, w, b, r, g = layer_inputs(dev, t, 60, 48, 40, True, True)
+    want = T.linear_act(x, w, b, "gelu", residual=r)
+    wide = torch.zeros(60, 100, dtype=t, device=dev)
+    wide[:, 7:47] = x
+    spread = torch.zeros(48, 80, dtype=t, device=dev)
+    spread[:, ::2] = w
+    packed = torch.zeros(60 * 48 + 1, dtype=t, device=dev)
+    packed[1:] = r.reshape(-1)
+    for args in ((wide[:, 7:47], w, b, r), (x, w.t().contiguous().t(), b, r), (x, spread[:, ::2], b, r), (x, w, b, r.t().contiguous().t()),
+                 (x, w, b, packed[1:].view(60, 48)), (x, w, b.repeat_interleave(2)[::2], r)):
+        assert torch.equal(T.linear_act(*args[:3], "gelu", residual=args[3]), want)
+    batched = T.linear_act(x.view(3, 4, 5, 40), w, b, "gelu", residual=r.view(3, 4, 5, 48))
+    assert torch.equal(batched.view(60, 48), want)
+    assert torch.equal(T.linear_act(x[0], w, b, "gelu", residual=r[0]).view(1, 48), T.linear_act(x[:1], w, b, "gelu", residual=r[:1]))
+    empty = x[:0].clone().requires_grad_()
+    w2 = w.clone().requires_grad_()
+    T.linear_act(empty, w2, b).sum().backward()
+    assert empty.grad.shape == (0, 40) and not w2.grad.any()
+    # a gradient that is one value spread over the result
+    x2, w2 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    T.linear_act(x2, w2, b, "silu").sum().backward()
+    x3, w3 = x.clone().requires_grad_(), w.clone().requires_grad_()
+    T.linear_act(x3, w3, b, "silu").backward(torch.ones(60, 48, dtype=t, device=dev))
+    assert torch.equal(x2.grad, x3.grad) and torch.equal(w2.grad, w3.grad)
+    for bad in (dict(activation="tanh"), dict(activation="softplus", beta=0.0), dict(residual=r[0]), dict(residual=r.float()), dict(bias=b[:-1]),
+                dict(bias=b.half())):
+        with pytest.raises((ValueError, TypeError)):
+            T.linear_act(x, w, **bad)
+    for pair in ((x.float(), w.float()), (x, w[:, :-1]), (x, w.half()), (x, w.cpu())):
+        with pytest.raises((ValueError, TypeError)):
+            T.linear_act(*pair)
+    # second order is refused, not wrong
+    x4 = x.clone().requires_grad_()
+    (gx,) = torch.autograd.grad(T.linear_act(x4, w, b, "silu").sum(), x4, create_graph=True)
+    with pytest.raises(RuntimeError):
+        gx.sum().backward()
+
+
+@gpu
+@pytest.mark.parametrize("t", HALVES)
+def test_layer_gradient_against_differences(dev, t):
+    """the directional derivative of sum(y go) along d, by central differences of the 64-bit formula at the layer's own inputs; the layer's
+    dot product with its gradients is off by their bounds (checked entry by entry above): 4 roundings of t of the magnitudes"""
+    x, w, b, _, go = layer_inputs(dev, t, 40, 33, 24, True, False, seed=3)
+    leaves = [v.clone().requires_grad_() for v in (x, w, b)]
+    T.linear_act(*leaves, "gelu").backward(go)
+
+    def f(xx, ww, bb):
+        return (act64(xx @ ww.t() + bb, "gelu", 1.0)[0] * go.double()).sum()
+    gen = torch.Generator(device=dev).manual_seed(9)
+    for k in range(3):
+        d = torch.randn(leaves[k].shape, device=dev, generator=gen).double()
+        args = [v.double() for v in (x, w, b)]
+        up, down = list(args), list(args)
+        up[k], down[k] = args[k] + 1e-4 * d, args[k] - 1e-4 * d
+        numeric = float(f(*up) - f(*down)) / 2e-4
+        own = float((leaves[k].grad.double() * d).sum())
+        z = x.double() @ w.double().t() + b.double()
+        gz = (go.double() * act64(z, "gelu", 1.0)[1]).abs()
+        span = [gz @ w.double().abs(), gz.t() @ x.double().abs(), gz.sum(0)][k]
+        assert abs(own - numeric) <= 4 * half_step(t) * float((span * d.abs()).sum()) + 1e-5
+
+
+@gpu
+def test_layer_special_values(dev):
+    """NaN and infinities stay in their rows; large values do not leave a gradient that is no number"""
+    t = torch.float16
+    x, w, b, _, g = layer_inputs(dev, t, 200, 96, 64, True, False)
+    want = T.linear_act(x, w, b, "gelu")
+    x[17, 3], x[130, 5] = math.nan, math.inf
+    got = T.linear_act(x, w, b, "gelu")
+    rows = torch.ones(200, dtype=torch.bool, device=dev)
+    rows[17] = rows[130] = False
+    assert torch.equal(got[rows], want[rows]) and bool(got[17].isnan().all()) and not bool(torch.isfinite(got[130]).all())
+    big = torch.full((8, 64), 6000.0, dtype=t, device=dev, requires_grad=True)
+    one = torch.ones(16, 64, dtype=t, device=dev)
+    for act in ("silu", "gelu", "softplus", "relu"):
+        big.grad = None
+        T.linear_act(big, one, None, act).backward(torch.ones(8, 16, dtype=t, device=dev))      # z = 384 000: above the type's range
+        assert torch.equal(big.grad, torch.full_like(big, 16.0)), act
+    for act in ("silu", "gelu", "softplus", "relu"):
+        big.grad = None
+        T.linear_act(big, -one, None, act).backward(torch.ones(8, 16, dtype=t, device=dev))
+        assert not big.grad.any(), act
+
+
+@gpu
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+def test_decoder_trains_with_16_bit_hidden_layers(dev, t):
+    """DeepSDF.train_precision: the same bits as the layers called one by one, and the fp32 tier untouched by it"""
+    torch.manual_seed(0)
+    net = DeepSDF(lat_dim=32, hidden_dim=128, nlayers=6, beta=100, out_dim=1).to(dev).train()
+    xyz = torch.randn(2, 300, 3, device=dev) * 0.3
+    lat = (torch.randn(2, 1, 32, device=dev) * 0.1).requires_grad_()
+    before = net.evaluate_train_hip(xyz, lat)
+    net.train_precision = t
+    out = net.evaluate_train_hip(xyz, lat)
+    out.square().sum().backward()
+    grads = [p.grad.clone() for p in net.parameters()] + [lat.grad.clone()]
+    net.zero_grad()
+    lat.grad = None
+    h = {"bf16": torch.bfloat16, "fp16": torch.float16}[t]
+    inp = torch.cat([xyz, lat.expand(2, 300, 32)], -1).reshape(600, -1)
+    x = inp
+    for k in range(6):
+        lin = getattr(net, f"lin{k}")
+        if k == 0:
+            x = _DenseLayerFn.apply(x, lin.weight, lin.bias, 1.0, 100.0)
+        elif k == 3:
+            x = _DenseLayerFn.apply(torch.cat([x.float(), inp], -1), lin.weight, lin.bias, 1 / math.sqrt(2), 100.0)
+        else:
+            x = T.linear_act(x.to(h), lin.weight.to(h), lin.bias.to(h), "softplus", 100.0)
+    want = torch.nn.functional.linear(x.float(), net.lin6.weight, net.lin6.bias).view(2, 300, 1)
+    assert torch.equal(out, want)
+    want.square().sum().backward()
+    for a, p in zip(grads, list(net.parameters()) + [lat]):
+        assert torch.equal(a, p.grad)
+    net.train_precision = "fp32"
+    assert torch.equal(net.evaluate_train_hip(xyz, lat), before)
+    net.train_precision = "fp8"
+    with pytest.raises(ValueError):
+        net.evaluate_train_hip(xyz, lat)
+
+
+# ---- gradient norm and clipping ---------------------------------------------------------------------------------------------------
+
+def clip_bound(want, t):
+    return want.abs() * (3 * F32 + (half_step(t) if t != torch.float32 else 0)) + tiny(t)
+
+
+@gpu
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("sizes", [[1], [0, 5, 0], [3, 1, 4, 1, 5, 9, 2, 6], [8192], [16385, 1], [70000, 3, 128, 40001], [1000] * 300, [2 ** 22 + 7]])
+@pytest.mark.parametrize("limit", [0.1, 1e9])
+def test_clip(dev, t, sizes, limit):
+    gen = torch.Generator(device=dev).manual_seed(len(sizes) + sizes[0])
+    grads = [(torch.randn(n, device=dev, generator=gen) * 0.5).to(t) for n in sizes]
+    total = math.sqrt(math.fsum(float(g.double().square().sum()) for g in grads))
+    most = max([float(g.abs().max()) for g in grads if g.numel()])
+    assert abs(float(T.grad_norm(grads)) - total) <= total * 1.01 * F32
+    assert float(T.grad_norm(grads, math.inf)) == most
+    for kind, n in ((2.0, total), (math.inf, most)):
+        out = [torch.full_like(g, 7.0) for g in grads]
+        norm, got = T.clip_grads(grads, limit, norm_type=kind, out=out)
+        assert abs(float(norm) - n) <= n * 1.01 * F32 and all(a is b for a, b in zip(got, out))
+        f = min(1.0, limit / (n + 1e-6))
+        for g, o in zip(grads, out):
+            within(o, g.double() * f, clip_bound(g.double() * f, t))
+        own = [g.clone() for g in grads]
+        versions = [g._version for g in own]
+        T.clip_grads(own, limit, norm_type=kind)
+        assert all(torch.equal(a, b) for a, b in zip(own, out)) and all(g._version > v for g, v in zip(own, versions))
+
+
+@gpu
+def test_clip_mixed_types_views_and_layouts(dev):
+    gen = torch.Generator(device=dev).manual_seed(1)
+    flat = torch.randn(50000, device=dev, generator=gen)
+    halves = torch.randn(50000, device=dev, generator=gen).half()
+    base = [flat[1:4098], flat[5000:5007], halves[3:20003], torch.randn(40, 30, device=dev).bfloat16().t(), torch.randn(6, 50, device=dev)[:, ::5],
+            torch.randn(3, 4, 5, device=dev).permute(2, 0, 1), torch.randn((), device=dev), halves[20003:20004]]
+    total = math.sqrt(math.fsum(float(g.double().square().sum()) for g in base))
+    want = [g.double() * min(1.0, 0.5 / (total + 1e-6)) for g in base]
+    around = flat[4098:5000].clone(), halves[20004:].clone()
+    out = [torch.empty(g.shape, dtype=g.dtype, device=dev) for g in base]
+    T.clip_grads(base, 0.5, out=out)
+    norm, _ = T.clip_grads(base, 0.5)
+    assert abs(float(norm) - total) <= total * 1.01 * F32
+    for g, o, w in zip(base, out, want):
+        within(g, w, clip_bound(w, g.dtype))
+        assert torch.equal(g, o)
+    assert torch.equal(around[0], flat[4098:5000]) and torch.equal(around[1], halves[20004:])
+    with pytest.raises(NphmAmdError):
+        T.clip_grads([flat[:100], flat[50:150]], 1.0)
+    with pytest.raises(NphmAmdError):
+        T.clip_grads([flat[:100], flat[:100]], 1.0)
+    with pytest.raises(TypeError):
+        T.clip_grads([flat, flat.double()], 1.0)
+    with pytest.raises(TypeError):
+        T.clip_grads([flat, torch.zeros(3)], 1.0)
+    with pytest.raises(ValueError):
+        T.clip_grads([flat], 1.0, out=[flat[1:]])
+
+
+@gpu
+@pytest.mark.parametrize("value,kind", [(math.nan, 2.0), (math.nan, math.inf), (math.inf, 2.0), (-math.inf, math.inf)])
+def test_clip_values_that_are_no_numbers_as_torch(dev, value, kind):
+    def params():
+        ps = [torch.nn.Parameter(torch.zeros(5000, device=dev)) for _ in range(3)]
+        for k, p in enumerate(ps):
+            p.grad = torch.full_like(p, 0.5 + k)
+        ps[1].grad[4321] = value
+        return ps
+    a, b = params(), params()
+    na = T.clip_grad_norm_(a, 1.0, norm_type=kind)
+    nb = torch.nn.utils.clip_grad_norm_(b, 1.0, norm_type=kind)
+    assert torch.equal(na.isnan(), nb.isnan()) and (bool(na.isnan()) or float(na) == float(nb))
+    for p, q in zip(a, b):
+        assert torch.equal(p.grad.isnan(), q.grad.isnan()) and torch.equal(p.grad.nan_to_num(), q.grad.nan_to_num())
+    c = params()
+    with pytest.raises(RuntimeError):
+        T.clip_grad_norm_(c, 1.0, norm_type=kind, error_if_nonfinite=True)
+    assert float(c[0].grad[0]) == 0.5
+
+
+@gpu
+def test_norm_of_huge_and_tiny_gradients(dev):
+    """squares of these leave fp32 on both sides; the norm does not"""
+    for v in (1e30, 1e-30):
+        g = torch.full((10000,), v, device=dev)
+        assert abs(float(T.grad_norm([g])) / float(g[0].double() * 100) - 1) <= 1e-6
+        got = T.clip_grads([g.clone()], 1.0)[1][0]
+        f = min(1.0, 1.0 / (100 * float(g[0].double()) + 1e-6))
+        assert float((got.double() / (g.double() * f) - 1).abs().max()) <= 4 * F32
+    with pytest.raises(AssertionError):          # (the plain fp32 form does)
+        assert math.isfinite(float(torch.full((10000,), 1e30, device=dev).square().sum()))
+
+
+@gpu
+def test_clip_sparse_and_dense_gradients_together(dev):
+    """rows that an index names twice count as their sum, on both kinds of sparse tensors; the gradient stays the same tensor in dense form"""
+    for coalesced in (False, True):
+        gen = torch.Generator(device=dev).manual_seed(4)
+        table, w = torch.nn.Parameter(torch.zeros(50, 136, device=dev)), torch.nn.Parameter(torch.zeros(70, 30, device=dev))
+        idx = torch.tensor([[3, 49, 3, 0, 3, 7, 49]], device=dev)
+        s = torch.sparse_coo_tensor(idx, torch.randn(7, 136, device=dev, generator=gen), (50, 136))
+        table.grad = s.coalesce() if coalesced else s
+        w.grad = torch.randn(70, 30, device=dev, generator=gen)
+        unused = torch.nn.Parameter(torch.zeros(3, device=dev))
+        dense = table.grad.to_dense().double()
+        want_w = w.grad.double().clone()
+        total = math.sqrt(float(dense.square().sum()) + float(want_w.square().sum()))
+        # the magnitudes that a row's sum is made of: of the entries as they come in (the call works on them in place; read after it
+        # they are f times smaller, and the bound f^2 mag where f mag is meant)
+        mag = torch.zeros(50, 136, dtype=torch.float64, device=dev).index_add_(0, idx[0], s._values().abs().double())
+        norm = T.clip_grad_norm_(iter([table, unused, w]), 2.0)
+        assert abs(float(norm) - total) <= total * 8 * F32            # (a row's sum is rounded before its square)
+        f = 2.0 / (total + 1e-6)
+        within(table.grad.to_dense(), dense * f, mag * f * 8 * F32 + 1e-30)
+        within(w.grad, want_w * f, want_w.abs() * f * 12 * F32)
+
+
+# ---- all of them -----------------------------------------------------------------------------------------------------------------
+
+def step(dev, codes, layers, idx, pts, target):
+    """codes -> two residual layers -> loss -> gradients, clipped by one norm"""
+    x = torch.cat([codes(idx), pts], -1).to(torch.bfloat16)
+    h = T.linear_act(x, layers[0], layers[1], "softplus", 10.0)
+    h = T.linear_act(h, layers[2], layers[3], "silu", residual=h)
+    loss = (h.float() - target).square().mean()
+    for p in (codes.weight, *layers):
+        p.grad = None
+    loss.backward()
+    return loss, T.clip_grad_norm_([codes.weight, *layers], 0.05)
+
+
+def step_inputs(dev, sparse):
+    gen = torch.Generator(device=dev).manual_seed(11)
+    codes = T.LatentCodes(20, 61, max_norm=1.0, sparse=sparse, device=dev)
+    with torch.no_grad():
+        codes.weight.copy_(torch.randn(20, 61, device=dev, generator=gen) * 0.2)
+    layers = [(torch.randn(*s, device=dev, generator=gen) * 0.15).bfloat16().requires_grad_() for s in ((128, 64), (128,), (128, 128), (128,))]
+    idx = torch.randint(0, 20, (96,), device=dev, generator=gen)
+    return codes, layers, idx, torch.randn(96, 3, device=dev, generator=gen), torch.randn(96, 128, device=dev, generator=gen)
+
+
+@gpu
+@pytest.mark.parametrize("sparse", [False, True])
+def test_a_step_of_all_operators(dev, sparse):
+    """against the same step in fp64.  bf16 roundings on the way of a gradient entry: x, z, y, z, y, g, gz, dh, gz, dx - ten of 2^-8 / 2 each if
+    they all add up in one direction; as they do not, the 2-norm of each gradient is held to ten half steps of its 2-norm, and
+    clipping to the norm found"""
+    codes, layers, idx, pts, target = step_inputs(dev, sparse)
+    start = codes.weight.detach().double()
+    loss, norm = step(dev, codes, layers, idx, pts, target)
+    named = torch.unique(idx)
+    n = start[named].norm(dim=1, keepdim=True)
+    start[named] = torch.where(n > 1, start[named] / (n + 1e-7), start[named])
+    assert float((codes.weight.detach().double() - start).abs().max()) <= 4 * F32
+    t, ls = start.clone().requires_grad_(), [p.detach().double().requires_grad_() for p in layers]
+    x = torch.cat([t[idx], pts.double()], -1)
+    h = torch.nn.functional.softplus(x @ ls[0].t() + ls[1], beta=10.0)
+    h = torch.nn.functional.silu(h @ ls[2].t() + ls[3]) + h
+    ref = (h - target.double()).square().mean()
+    grads = torch.autograd.grad(ref, [t, *ls])
+    total = math.sqrt(sum(float(g.square().sum()) for g in grads))
+    room = 10 * 2.0 ** -9
+    assert abs(float(loss) - float(ref)) <= room * float(ref)
+    assert abs(float(norm) - total) <= room * total
+    for p, g in zip([codes.weight, *layers], grads):
+        own = (p.grad.to_dense() if p.grad.is_sparse else p.grad).double()
+        f = 0.05 / (total + 1e-6)
+        assert float((own - g * f).norm()) <= 2 * room * float((g * f).norm())
+    assert abs(float(T.grad_norm([p.grad.coalesce().values() if p.grad.is_sparse else p.grad for p in (codes.weight, *layers)])) - 0.05) <= 0.05 * 2.0 ** -9
+
+
+@gpu
+def test_a_captured_step_replays_as_the_eager_one(dev):
+    """graph and eager steps in turn, new inputs each time: the same bits (the graph has its own leaves: none is shared with an eager graph)"""
+    codes, layers, idx, pts, target = step_inputs(dev, False)
+    own = T.LatentCodes(20, 61, max_norm=1.0, device=dev)
+    own.load_state_dict(codes.state_dict())
+    own_layers = [p.detach().clone().requires_grad_() for p in layers]
+    s_idx, s_pts = idx.clone(), pts.clone()
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        for _ in range(2):
+            step(dev, own, own_layers, s_idx, s_pts, target)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    for p in (own.weight, *own_layers):
+        p.grad = None
+    with torch.cuda.graph(graph):
+        _, norm = step(dev, own, own_layers, s_idx, s_pts, target)
+    for k in range(4):
+        s_idx.copy_((idx + k) % 20)
+        s_pts.copy_(pts * (1 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        _, want = step(dev, codes, layers, s_idx.clone(), s_pts.clone(), target)
+        torch.cuda.synchronize()
+        assert torch.equal(norm, want)
+        for p, q in zip((own.weight, *own_layers), (codes.weight, *layers)):
+            assert torch.equal(p.grad, q.grad) and torch.equal(p, q)
+
+
+@gpu
+def test_operators_run_on_the_current_stream(dev):
+    """work queued behind a long product on another stream: the operators wait for it there, and two streams at once do not meet"""
+    x, w, b, r, g = layer_inputs(dev, torch.bfloat16, 256, 256, 256, True, True)
+    table = torch.randn(500, 256, device=dev)
+    idx = torch.randint(0, 500, (3000,), device=dev)
+    rows = torch.randn(3000, 256, device=dev)
+    want = T.linear_act(x, w, b, "silu", residual=r), T.lookup_rows_grad(rows, idx, 500), T.clip_grads([rows], 1.0, out=[torch.empty_like(rows)])[1][0]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream(), torch.cuda.Stream()]
+    got = []
+    for s in streams:
+        s.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(s):
+            big = torch.randn(4096, 4096, device=dev)
+            big = big @ big
+            late = torch.zeros_like(x).copy_(x)
+            late_rows = torch.zeros_like(rows).copy_(rows)
+            got.append((T.linear_act(late, w, b, "silu", residual=r), T.lookup_rows_grad(late_rows, idx, 500),
+                        T.clip_grads([late_rows], 1.0, out=[torch.empty_like(rows)])[1][0]))
+    torch.cuda.synchronize()
+    for trio in got:
+        assert all(torch.equal(a, b_) for a, b_ in zip(trio, want))
