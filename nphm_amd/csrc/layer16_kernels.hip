@@ -15,6 +15,7 @@
 namespace nphm {
 namespace train_ops {
 
+typedef int v4i __attribute__((ext_vector_type(4)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef fp16 fp16x8 __attribute__((ext_vector_type(8)));
@@ -51,8 +52,8 @@ __device__ __forceinline__ float act_slope(float z, int act, float beta) {
 }
 
 struct GemmArgs {
-  const void* A; int64_t a_i, a_k;       // element strides
-  const void* B; int64_t b_j, b_k;
+  const void* A; int64_t lda;            // [I, K] rows lda elements apart, or (transposed) [K, I]
+  const void* B; int64_t ldb;            // [J, K], or (transposed) [K, J]
   int I, J, K;
   int splits, k_per_split;               // > 1: partial products to `parts`
   float* parts;                          // [splits][I][J]
@@ -63,6 +64,7 @@ struct GemmArgs {
   void* z;                               // [I, J] or null: the value before the activation
   int act;
   float beta;
+  int wide;                              // J is a multiple of 8; rows of C, z and residual take 16-byte accesses
 };
 
 // z as it is kept: finite where z is (a' of an infinity is no number for some activations)
@@ -72,47 +74,256 @@ __device__ __forceinline__ T keep(float v) {
   return T(v != v ? v : fminf(fmaxf(v, -MOST), MOST));
 }
 
-constexpr int GT = 64, GK = 32, GP = GK + 8;
+constexpr int BK = 64;                   // k a step: 128 bytes of a row
 
-template <class T>
-__global__ __launch_bounds__(256) void gemm_simple_kernel(GemmArgs p) {
-  __shared__ __attribute__((aligned(16))) T sa[GT * GP], sb[GT * GP];
-  const int t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  const int i0 = blockIdx.y * GT, j0 = blockIdx.x * GT;
-  const int kb = blockIdx.z * p.k_per_split, ke = min(p.K, kb + p.k_per_split);
-  const T* A = static_cast<const T*>(p.A);
-  const T* B = static_cast<const T*>(p.B);
-  f32x16 acc = {};
-  for (int k0 = kb; k0 < ke; k0 += GK) {
-    for (int u = t; u < GT * GK; u += 256) {
-      const int r = u / GK, k = u % GK;
-      sa[r * GP + k] = (i0 + r < p.I && k0 + k < ke) ? A[int64_t(i0 + r) * p.a_i + int64_t(k0 + k) * p.a_k] : T(0.f);
-      sb[r * GP + k] = (j0 + r < p.J && k0 + k < ke) ? B[int64_t(j0 + r) * p.b_j + int64_t(k0 + k) * p.b_k] : T(0.f);
-    }
-    __syncthreads();
-    typedef typename Frag<T>::type frag;
+// One operand's tile of ROWS rows (its i or j) x 64 k, on its way from memory to LDS and from there into fragments.
+// Not transposed: memory holds k beside k.  LDS row r: 128 bytes, its eight 16-byte pieces c at place c ^ (r / 2 % 8), so that the lanes of a
+//   fragment read (32 rows, the same k) meet every bank.  A fragment's 8 k are one ds_read_b128.
+// Transposed: memory holds row beside row.  LDS row k: 2 ROWS bytes, piece c at c ^ 2 (k % 4).  A fragment's 8 k are two ds_read_b64_tr: 16 lanes
+//   read 4 k x 16 rows and get them turned round.
+// Both are written by LDS-DMA (the destination is linear in the lane: the lanes load permuted pieces instead), 1 KiB an instruction.
+// Pieces behind the operand's end have an offset behind the buffer's: they arrive as zeros.
+template <class T, int ROWS, int WAVES, bool TR>
+struct Operand {
+  static constexpr int BYTES = ROWS * BK * 2, DMA = BYTES / 1024 / WAVES, CPR = TR ? ROWS / 8 : 8;
+  static_assert(BYTES % (1024 * WAVES) == 0, "whole DMA instructions a wavefront");
+  static constexpr unsigned NOWHERE = 0x80000000u;                   // behind every buffer (each is below 2^31 bytes)
+  const char* base;
+  int64_t ld;
+  int rows, K;                                                       // valid rows from the tile's first
+  unsigned voff[DMA], lds[DMA];
+
+  __device__ __forceinline__ void init(const void* P, int64_t ld_, int r0, int I, int K_, int wave, int lane, unsigned lds0) {
+    ld = ld_;
+    K = K_;
+    rows = min(ROWS, I - r0);
+    base = static_cast<const char*>(P) + (TR ? int64_t(r0) * 2 : int64_t(r0) * ld * 2);
 #pragma unroll
-    for (int s = 0; s < GK; s += 16) {
-      const frag a = *reinterpret_cast<const frag*>(sa + ((wave >> 1) * 32 + (lane & 31)) * GP + s + 8 * (lane >> 5));
-      const frag b = *reinterpret_cast<const frag*>(sb + ((wave & 1) * 32 + (lane & 31)) * GP + s + 8 * (lane >> 5));
-      acc = mfma(a, b, acc);
+    for (int d = 0; d < DMA; ++d) {
+      const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, at = piece % CPR;
+      const int c = TR ? at ^ ((row & 3) << 1) : at ^ ((row >> 1) & 7);
+      voff[d] = unsigned(row * int(ld) * 2 + c * 16);
+      if (TR && c * 8 >= rows) voff[d] = NOWHERE;
+      lds[d] = __builtin_amdgcn_readfirstlane(lds0 + (d * WAVES + wave) * 1024);
     }
-    __syncthreads();
   }
-  const int j = j0 + (wave & 1) * 32 + (lane & 31);
-  if (j >= p.J) return;
-  const float bias = p.bias ? float(static_cast<const T*>(p.bias)[j]) : 0.f;
+  // the 64 k from k0 (below K) into the buffer `shift` bytes behind the first
+  __device__ __forceinline__ void fetch(int k0, unsigned shift, int lane, int wave) const {
+    v4i rsrc;
+    const char* p = TR ? base + int64_t(k0) * ld * 2 : base;
+    const unsigned bytes = TR ? unsigned(min(BK, K - k0)) * unsigned(ld * 2) : unsigned(rows) * unsigned(ld * 2);
+    rsrc[0] = __builtin_amdgcn_readfirstlane(int(uint32_t(uintptr_t(p))));
+    rsrc[1] = __builtin_amdgcn_readfirstlane(int(uint32_t(uintptr_t(p) >> 32) & 0xffff));
+    rsrc[2] = __builtin_amdgcn_readfirstlane(int(bytes));
+    rsrc[3] = 0x00020000;
+    const unsigned soff = __builtin_amdgcn_readfirstlane(TR ? 0 : k0 * 2);
+    const bool tail = !TR && k0 + BK > K;
 #pragma unroll
-  for (int q = 0; q < 16; ++q) {
-    const int i = i0 + (wave >> 1) * 32 + 8 * (q >> 2) + 4 * (lane >> 5) + (q & 3);
-    if (i >= p.I) continue;
-    const int64_t at = int64_t(i) * p.J + j;
-    if (p.splits > 1) { p.parts[int64_t(blockIdx.z) * p.I * p.J + at] = acc[q]; continue; }
-    float v = acc[q] + bias;
-    if (p.z) static_cast<T*>(p.z)[at] = keep<T>(v);
-    v = act_value(v, p.act, p.beta);
-    if (p.residual) v += float(static_cast<const T*>(p.residual)[at]);
-    static_cast<T*>(p.C)[at] = T(v);
+    for (int d = 0; d < DMA; ++d) {
+      unsigned v = voff[d];
+      if (tail) {
+        const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, c = (piece % CPR) ^ ((row >> 1) & 7);
+        if (k0 + c * 8 >= K) v = NOWHERE;
+      }
+      const unsigned dst = __builtin_amdgcn_readfirstlane(lds[d] + shift);
+      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(v), "s"(rsrc), "s"(dst), "s"(soff) : "memory", "m0");
+    }
+  }
+};
+
+template <bool TR, int ROWS>
+struct Reader {
+  // lane -> its place in a fragment's rows; fragment (t, ks): rows w0 + 32 t .. + 31, k 16 ks .. + 15
+  unsigned at[TR ? 2 : 4];
+  __device__ __forceinline__ void init(int w0, int lane) {
+    if constexpr (TR) {
+      const int r = (lane & 15) >> 2, q = lane & 3, kg = lane >> 5;
+#pragma unroll
+      for (int o = 0; o < 2; ++o) {
+        const int c = w0 / 8 + o * 4 + ((lane >> 4) & 1) * 2 + (q >> 1);
+        at[o] = unsigned((kg * 8 + r) * ROWS * 2 + ((c ^ (r << 1)) * 16) + (q & 1) * 8);
+      }
+    } else {
+      const int row = w0 + (lane & 31), kg = lane >> 5;
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks) at[ks] = unsigned(row * 128 + (((ks * 2 + kg) ^ ((row >> 1) & 7)) * 16));
+    }
+  }
+  template <class F>
+  __device__ __forceinline__ F read(const char* tile, int t, int ks) const {
+    if constexpr (TR) {
+      const char* p = tile + at[t & 1] + (t >> 1) * 128 + ks * (16 * ROWS * 2);
+      typedef short s4 __attribute__((ext_vector_type(4)));
+      typedef short s8 __attribute__((ext_vector_type(8)));
+      typedef __attribute__((address_space(3))) s4 lds_s4;
+      const s4 lo = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p));
+      const s4 hi = __builtin_amdgcn_ds_read_tr16_b64_v4i16((lds_s4*)(p + 4 * ROWS * 2));
+      const s8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
+      return __builtin_bit_cast(F, v);
+    } else {
+      return *reinterpret_cast<const F*>(tile + at[ks] + t * (32 * 128));
+    }
+  }
+};
+
+template <class T, class V>
+__device__ __forceinline__ void put8(T* to, const V& v, bool whole, int width) {
+  if (whole) { *reinterpret_cast<V*>(to) = v; return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < width) to[e] = v[e];
+}
+// (the choice once for eight values: it is the same for the whole launch)
+__device__ __forceinline__ void act_values(float (&v)[8], int act, float beta) {
+  if (act == ACT_NONE) return;
+#define NPHM_EACH(A) case A: _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], A, beta); break
+  switch (act) { NPHM_EACH(ACT_RELU); NPHM_EACH(ACT_SILU); NPHM_EACH(ACT_GELU); NPHM_EACH(ACT_SOFTPLUS); }
+#undef NPHM_EACH
+}
+
+enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2 };
+
+// C[i, j] = sum_k A(i, k) B(j, k): tile BM x BN, WM x WN wavefronts, two LDS buffers; one step's loads fly over the step before it.
+template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, int OUT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
+  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  typedef Operand<T, BM, WAVES, TA> OpA;
+  typedef Operand<T, BN, WAVES, TB> OpB;
+  constexpr unsigned STEP = OpA::BYTES + OpB::BYTES;
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  // Blocks go round the 8 XCDs: each XCD gets a run of consecutive tiles, 8 tiles of i to one of j, so that the 32 that it works on
+  // at a time share 8 + 4 panels in its L2.
+  const int mt = (p.I + BM - 1) / BM, nt = (p.J + BN - 1) / BN, tiles = mt * nt * p.splits, per = (tiles + 7) / 8;
+  const int tile = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
+  if (int(blockIdx.x >> 3) >= per || tile >= tiles) return;
+  const int split = tile / (mt * nt), rest = tile % (mt * nt);
+  const int group = rest / (8 * nt), m_first = group * 8, m_count = min(8, mt - m_first), in = rest - group * 8 * nt;
+  const int i0 = (m_first + in % m_count) * BM, j0 = in / m_count * BN;
+  const int kb = split * p.k_per_split, ke = min(p.K, kb + p.k_per_split);
+  const unsigned lds0 = unsigned(size_t((__attribute__((address_space(3))) char*)lds));
+
+  OpA a;
+  OpB b;
+  a.init(p.A, p.lda, i0, p.I, ke, wave, lane, lds0);
+  b.init(p.B, p.ldb, j0, p.J, ke, wave, lane, lds0 + OpA::BYTES);
+  Reader<TA, BM> ra;
+  Reader<TB, BN> rb;
+  ra.init((wave / WN) * TM * 32, lane);
+  rb.init((wave % WN) * TN * 32, lane);
+  f32x16 acc[TM][TN];
+#pragma unroll
+  for (int x = 0; x < TM; ++x)
+#pragma unroll
+    for (int y = 0; y < TN; ++y) acc[x][y] = f32x16{};
+  typedef typename Frag<T>::type frag;
+
+  a.fetch(kb, 0, lane, wave);
+  b.fetch(kb, 0, lane, wave);
+  unsigned shift = 0;
+  for (int k0 = kb; k0 < ke; k0 += BK, shift ^= STEP) {
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this step's tile has landed, the other buffer is read out
+    if (k0 + BK < ke) {
+      a.fetch(k0 + BK, shift ^ STEP, lane, wave);
+      b.fetch(k0 + BK, shift ^ STEP, lane, wave);
+    }
+    const char* ta = lds + shift;
+    const char* tb = lds + shift + OpA::BYTES;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) {
+      frag fa[TM], fb[TN];
+#pragma unroll
+      for (int x = 0; x < TM; ++x) fa[x] = ra.template read<frag>(ta, x, ks);
+#pragma unroll
+      for (int y = 0; y < TN; ++y) fb[y] = rb.template read<frag>(tb, y, ks);
+#pragma unroll
+      for (int x = 0; x < TM; ++x)
+#pragma unroll
+        for (int y = 0; y < TN; ++y) acc[x][y] = mfma(fb[y], fa[x], acc[x][y]);
+    }
+  }
+
+  // Register q of a lane: i = lane % 32, j = 8 (q / 4) + 4 (lane / 32) + q % 4 of its 32 x 32 tile.  Through LDS (every wavefront its own part
+  // of the tiles' room, 32 rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  typedef T eight __attribute__((ext_vector_type(8)));
+  constexpr int COLS = TN * 32, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
+  static_assert(WAVES * 32 * PITCH * 4 <= 2 * STEP, "the epilogue's rows fit the tiles' room");
+  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles
+  float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
+  const int j = j0 + (wave % WN) * COLS + (lane % LPR) * 8, width = min(8, p.J - j);
+  float bias[8] = {};
+  if (OUT == OUT_LAYER && p.bias) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) if (e < width) bias[e] = float(static_cast<const T*>(p.bias)[j + e]);
+  }
+#pragma unroll
+  for (int x = 0; x < TM; ++x) {
+#pragma unroll
+    for (int y = 0; y < TN; ++y)
+#pragma unroll
+      for (int q4 = 0; q4 < 4; ++q4)
+        *reinterpret_cast<f32x4*>(out + (lane & 31) * PITCH + y * 32 + 8 * q4 + 4 * (lane >> 5)) =
+            f32x4{acc[x][y][4 * q4], acc[x][y][4 * q4 + 1], acc[x][y][4 * q4 + 2], acc[x][y][4 * q4 + 3]};
+#pragma nounroll
+    for (int r = lane / LPR; r < 32; r += RPI) {
+      const int i = i0 + (wave / WN) * TM * 32 + x * 32 + r;
+      if (i >= p.I || width <= 0) continue;
+      float v[8];
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8 + 4);
+      const int64_t at = int64_t(i) * p.J + j;
+      const bool whole = p.wide;                                     // J a multiple of 8: all eight or none
+      if constexpr (OUT == OUT_PARTS) {
+        float* o = p.parts + int64_t(split) * p.I * p.J + at;
+        if (whole) {
+          *reinterpret_cast<f32x4*>(o) = *reinterpret_cast<f32x4*>(v);
+          *reinterpret_cast<f32x4*>(o + 4) = *reinterpret_cast<f32x4*>(v + 4);
+        } else {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) if (e < width) o[e] = v[e];
+        }
+      } else {
+        if constexpr (OUT == OUT_LAYER) {
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += bias[e];
+          if (p.z) {
+            eight zz;
+#pragma unroll
+            for (int e = 0; e < 8; ++e) zz[e] = keep<T>(v[e]);
+            put8(static_cast<T*>(p.z) + at, zz, whole, width);
+          }
+          eight res = {};
+          if (p.residual) {
+            const T* s = static_cast<const T*>(p.residual) + at;
+            if (whole) res = *reinterpret_cast<const eight*>(s);
+            else {
+#pragma unroll
+              for (int e = 0; e < 8; ++e) if (e < width) res[e] = s[e];
+            }
+          }
+          act_values(v, p.act, p.beta);
+          if (p.residual) {
+#pragma unroll
+            for (int e = 0; e < 8; ++e) v[e] += float(res[e]);
+          }
+        }
+        eight o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
+        put8(static_cast<T*>(p.C) + at, o, whole, width);
+      }
+    }
+  }
+}
+
+// rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(const T* src, T* dst, int64_t rows, int cols, int ld) {
+  const int64_t count = rows * ld;
+  for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < count; u += int64_t(gridDim.x) * 256) {
+    const int64_t r = u / ld;
+    const int c = int(u - r * ld);
+    dst[u] = c < cols ? src[r * cols + c] : T(0.f);
   }
 }
 
@@ -125,20 +336,24 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* parts, in
   }
 }
 
-// gz = g a'(z) and the column sums of every 64-row tile of it (before it is rounded)
+// gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every 64-row tile of it (before it is rounded)
 template <class T>
-__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, int M, int N, int act, float beta) {
+__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, int M, int N, int ld, int act, float beta) {
   const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+  if (n >= ld) return;
   const int m0 = blockIdx.y * 64, m1 = min(M, m0 + 64);
   float s = 0.f;
   for (int m = m0; m < m1; ++m) {
     const int64_t at = int64_t(m) * N + n;
-    float v = float(g[at]);
-    if (z) { v *= act_slope(float(z[at]), act, beta); gz[at] = T(v); }
-    s += v;
+    float v = 0.f;
+    if (n < N) {
+      v = float(g[at]);
+      if (z) v *= act_slope(float(z[at]), act, beta);
+      s += v;
+    }
+    if (gz) gz[int64_t(m) * ld + n] = T(v);
   }
-  if (sums) sums[int64_t(blockIdx.y) * N + n] = s;
+  if (sums && n < N) sums[int64_t(blockIdx.y) * N + n] = s;
 }
 
 template <class T>
@@ -150,34 +365,58 @@ __global__ __launch_bounds__(256) void column_sums16_kernel(const float* sums, i
   out[n] = T(s);
 }
 
-struct Plan {
-  size_t gz = 0, sums = 0, parts = 0, total = 0;    // byte offsets
-  int w_splits = 1;
-};
 inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
-inline Plan backward_plan(int64_t M, int64_t N, int64_t K, int act) {
-  Plan p;
-  const int64_t tiles = ((N + GT - 1) / GT) * ((K + GT - 1) / GT);
-  int64_t s = tiles >= 512 ? 1 : 512 / tiles;
-  if (s > (M + 255) / 256) s = (M + 255) / 256;
-  p.w_splits = int(s < 1 ? 1 : s);
-  p.gz = 0;
-  p.sums = p.gz + (act != ACT_NONE ? up(size_t(M) * N * 2) : 0);
-  p.parts = p.sums + up(size_t((M + 63) / 64) * N * 4);
-  p.total = p.parts + (p.w_splits > 1 ? up(size_t(p.w_splits) * N * K * 4) : 0);
-  return p;
+inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+
+struct Tiling { int size, splits; };               // size: 256, 128 or 64
+// Whole tiles of 256 x 256 where there are enough to fill the 256 CUs, else smaller ones, and the k range in pieces.
+inline Tiling tiling(int64_t I, int64_t J, int64_t K, bool may_split) {
+  auto tiles = [&](int64_t b) { return ((I + b - 1) / b) * ((J + b - 1) / b); };
+  if (tiles(256) >= 192) return {256, 1};
+  if (!may_split) return {tiles(128) >= 192 ? 128 : 64, 1};
+  const int size = I >= 128 && J >= 128 ? 128 : 64;
+  int64_t s = (512 + tiles(size) - 1) / tiles(size);
+  if (s > K / 512) s = K / 512;
+  if (s > 64) s = 64;
+  return {size, int(s < 1 ? 1 : s)};
 }
 
-template <class T>
-inline void gemm(hipStream_t st, GemmArgs a) {
-  a.k_per_split = ((a.K + a.splits - 1) / a.splits + GK - 1) / GK * GK;
-  hipLaunchKernelGGL((gemm_simple_kernel<T>), dim3((a.J + GT - 1) / GT, (a.I + GT - 1) / GT, a.splits), dim3(256), 0, st, a);
-  if (a.splits > 1) {
+template <class T, int B, int WM, int WN, bool TA, bool TB, int OUT>
+inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
+  constexpr unsigned LDS = 2 * 2 * B * BK * 2;
+  static_assert(LDS <= 160 * 1024, "two buffers of two tiles");
+  const int64_t tiles = ((a.I + B - 1) / B) * int64_t((a.J + B - 1) / B) * a.splits;
+  if constexpr (LDS > 65536) {
+    static hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
+                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));
+    (void)once;
+  }
+  hipLaunchKernelGGL((gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>), dim3(unsigned((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), LDS, st, a);
+}
+
+template <class T, bool TA, bool TB, int OUT>
+inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
+  a.splits = t.splits;
+  a.k_per_split = ((a.K + t.splits - 1) / t.splits + BK - 1) / BK * BK;
+  a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
+  if (t.size == 256) launch_gemm<T, 256, 2, 4, TA, TB, OUT>(st, a);
+  else if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, OUT>(st, a);
+  else launch_gemm<T, 64, 2, 2, TA, TB, OUT>(st, a);
+  if constexpr (OUT == OUT_PARTS) {
     const int64_t count = int64_t(a.I) * a.J, want = (count + 255) / 256;
     hipLaunchKernelGGL((join_splits_kernel<T>), dim3(unsigned(want < 4096 ? want : 4096)), dim3(256), 0, st, a.parts, a.splits, count,
                        static_cast<T*>(a.C));
   }
 }
+
+template <class T>
+inline void pack(hipStream_t st, const void* src, void* dst, int64_t rows, int64_t cols) {
+  const int64_t ld = round8(cols), want = (rows * ld + 255) / 256;
+  hipLaunchKernelGGL((pack_kernel<T>), dim3(unsigned(want < 8192 ? want : 8192)), dim3(256), 0, st, static_cast<const T*>(src),
+                     static_cast<T*>(dst), rows, int(cols), int(ld));
+}
+
+inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
 inline int check_layer(const char* what, int64_t M, int64_t N, int64_t K, int dtype, int act, float beta) {
   static thread_local char msg[160];
@@ -191,6 +430,23 @@ inline int check_layer(const char* what, int64_t M, int64_t N, int64_t K, int dt
   return nphm_fail_msg(msg);
 }
 
+struct Backward {
+  Tiling w;
+  size_t gz, sums, x, weight, parts, total;         // byte offsets
+};
+// (room for packed copies is there even where none is made: whether one is needed depends on addresses)
+inline Backward backward_plan(int64_t M, int64_t N, int64_t K) {
+  Backward p;
+  p.w = tiling(N, K, M, true);
+  p.gz = 0;
+  p.sums = p.gz + up(size_t(M) * round8(N) * 2);
+  p.x = p.sums + up(size_t((M + 63) / 64) * N * 4);
+  p.weight = p.x + up(size_t(M) * round8(K) * 2);
+  p.parts = p.weight + up(size_t(N) * round8(K) * 2);
+  p.total = p.parts + (p.w.splits > 1 ? up(size_t(p.w.splits) * N * K * 4) : 0);
+  return p;
+}
+
 }  // namespace train_ops
 }  // namespace nphm
 
@@ -198,63 +454,84 @@ using namespace nphm::train_ops;
 
 extern "C" {
 
-size_t nphm_layer16_forward_workspace_bytes(int64_t M, int64_t N, int64_t K) { return 0; }
+size_t nphm_layer16_forward_workspace_bytes(int64_t M, int64_t N, int64_t K) {
+  return up(size_t(M) * round8(K) * 2) + up(size_t(N) * round8(K) * 2);
+}
 
 int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,
                          int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_layer("nphm_layer16_forward", M, N, K, dtype, act, beta)) return rc;
-  if (!x || !weight || !y) return nphm_fail_msg("nphm_layer16_forward: null pointer");
-  GemmArgs a{};
-  a.A = x; a.a_i = K; a.a_k = 1;
-  a.B = weight; a.b_j = K; a.b_k = 1;
-  a.I = int(M); a.J = int(N); a.K = int(K);
-  a.splits = 1;
-  a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
+  if (!x || !weight || !y || !workspace) return nphm_fail_msg("nphm_layer16_forward: null pointer");
+  if (workspace_bytes < nphm_layer16_forward_workspace_bytes(M, N, K)) return nphm_fail_msg("nphm_layer16_forward: workspace too small");
+  hipStream_t st = static_cast<hipStream_t>(stream);
+  char* ws = static_cast<char*>(workspace);
   with_dtype(dtype, [&](auto t) {
-    if constexpr (sizeof(t) == 2) gemm<decltype(t)>(static_cast<hipStream_t>(stream), a);
+    typedef decltype(t) T;
+    if constexpr (sizeof(T) == 2) {
+      GemmArgs a{};
+      a.A = x; a.lda = K;
+      a.B = weight; a.ldb = K;
+      if (K % 8 || !aligned(x, 16)) { pack<T>(st, x, ws, M, K); a.A = ws; a.lda = round8(K); }
+      if (K % 8 || !aligned(weight, 16)) {
+        void* to = ws + up(size_t(M) * round8(K) * 2);
+        pack<T>(st, weight, to, N, K);
+        a.B = to; a.ldb = round8(K);
+      }
+      a.I = int(M); a.J = int(N); a.K = int(K);
+      a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
+      a.wide = N % 8 == 0 && aligned(y, 16) && aligned(z, 16) && aligned(residual, 16);
+      gemm<T, false, false, OUT_LAYER>(st, a, tiling(M, N, K, false));
+    }
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_layer16_forward launch", e);
   return 0;
 }
 
-size_t nphm_layer16_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) { return backward_plan(M, N, K, act).total; }
+size_t nphm_layer16_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) { return backward_plan(M, N, K).total; }
 
 int nphm_layer16_backward(const void* g, const void* x, const void* weight, const void* z, void* dx, void* dweight, void* dbias, int64_t M,
                           int64_t N, int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_layer("nphm_layer16_backward", M, N, K, dtype, act, beta)) return rc;
   if (!g || (act != ACT_NONE && !z) || (dx && !weight) || (dweight && !x) || !workspace) return nphm_fail_msg("nphm_layer16_backward: null pointer");
-  const Plan plan = backward_plan(M, N, K, act);
+  const Backward plan = backward_plan(M, N, K);
   if (workspace_bytes < plan.total) return nphm_fail_msg("nphm_layer16_backward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   with_dtype(dtype, [&](auto t) {
     typedef decltype(t) T;
     if constexpr (sizeof(T) == 2) {
-      T* gz = act == ACT_NONE ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
+      const int64_t ldn = round8(N), ldk = round8(K);
       float* sums = reinterpret_cast<float*>(ws + plan.sums);
       const unsigned tiles = unsigned((M + 63) / 64);
-      if (act != ACT_NONE || dbias)
-        hipLaunchKernelGGL((gz_kernel<T>), dim3(unsigned((N + 255) / 256), tiles), dim3(256), 0, st, static_cast<const T*>(g),
-                           act == ACT_NONE ? nullptr : static_cast<const T*>(z), gz, dbias ? sums : nullptr, int(M), int(N), act, beta);
+      const bool same = act == ACT_NONE && N % 8 == 0 && aligned(g, 16);       // g as it stands is gz
+      T* gz = same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
+      if (!same || dbias)
+        hipLaunchKernelGGL((gz_kernel<T>), dim3(unsigned((ldn + 255) / 256), tiles), dim3(256), 0, st, static_cast<const T*>(g),
+                           act == ACT_NONE ? nullptr : static_cast<const T*>(z), same ? nullptr : gz, dbias ? sums : nullptr, int(M), int(N),
+                           int(ldn), act, beta);
       if (dbias)
         hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 255) / 256)), dim3(256), 0, st, sums, int(tiles), int(N),
                            static_cast<T*>(dbias));
       if (dx) {
         GemmArgs a{};
-        a.A = gz; a.a_i = N; a.a_k = 1;
-        a.B = weight; a.b_j = 1; a.b_k = K;
+        a.A = gz; a.lda = ldn;
+        a.B = weight; a.ldb = K;
+        if (K % 8 || !aligned(weight, 16)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = ldk; }
         a.I = int(M); a.J = int(K); a.K = int(N);
-        a.splits = 1; a.C = dx;
-        gemm<T>(st, a);
+        a.C = dx; a.wide = K % 8 == 0 && aligned(dx, 16);
+        gemm<T, false, true, OUT_PLAIN>(st, a, tiling(M, K, N, false));
       }
       if (dweight) {
         GemmArgs a{};
-        a.A = gz; a.a_i = 1; a.a_k = N;
-        a.B = x; a.b_j = 1; a.b_k = K;
+        a.A = gz; a.lda = ldn;
+        a.B = x; a.ldb = K;
+        if (K % 8 || !aligned(x, 16)) { pack<T>(st, x, ws + plan.x, M, K); a.B = ws + plan.x; a.ldb = ldk; }
         a.I = int(N); a.J = int(K); a.K = int(M);
-        a.splits = plan.w_splits; a.parts = reinterpret_cast<float*>(ws + plan.parts); a.C = dweight;
-        gemm<T>(st, a);
+        a.parts = reinterpret_cast<float*>(ws + plan.parts);
+        a.C = dweight; a.wide = K % 8 == 0 && (plan.w.splits > 1 || aligned(dweight, 16));
+        if (plan.w.splits > 1) gemm<T, true, true, OUT_PARTS>(st, a, plan.w);
+        else gemm<T, true, true, OUT_PLAIN>(st, a, plan.w);
       }
     }
   });
