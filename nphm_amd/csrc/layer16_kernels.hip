@@ -107,27 +107,30 @@ struct Operand {
       lds[d] = __builtin_amdgcn_readfirstlane(lds0 + (d * WAVES + wave) * 1024);
     }
   }
-  // the 64 k from k0 (below K) into the buffer `shift` bytes behind the first
-  __device__ __forceinline__ void fetch(int k0, unsigned shift, int lane, int wave) const {
-    v4i rsrc;
+  // The 64 k from k0 (behind K: zeros, nothing is read): aim() once, then issue(d) for every instruction d, into the buffer `shift` bytes behind the first.
+  v4i rsrc;
+  unsigned soff;
+  bool tail;
+  int k_at;
+  __device__ __forceinline__ void aim(int k0) {
     const char* p = TR ? base + int64_t(k0) * ld * 2 : base;
-    const unsigned bytes = TR ? unsigned(min(BK, K - k0)) * unsigned(ld * 2) : unsigned(rows) * unsigned(ld * 2);
+    const unsigned bytes = k0 >= K ? 0u : (TR ? unsigned(min(BK, K - k0)) : unsigned(rows)) * unsigned(ld * 2);
     rsrc[0] = __builtin_amdgcn_readfirstlane(int(uint32_t(uintptr_t(p))));
     rsrc[1] = __builtin_amdgcn_readfirstlane(int(uint32_t(uintptr_t(p) >> 32) & 0xffff));
     rsrc[2] = __builtin_amdgcn_readfirstlane(int(bytes));
     rsrc[3] = 0x00020000;
-    const unsigned soff = __builtin_amdgcn_readfirstlane(TR ? 0 : k0 * 2);
-    const bool tail = !TR && k0 + BK > K;
-#pragma unroll
-    for (int d = 0; d < DMA; ++d) {
-      unsigned v = voff[d];
-      if (tail) {
-        const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, c = (piece % CPR) ^ ((row >> 1) & 7);
-        if (k0 + c * 8 >= K) v = NOWHERE;
-      }
-      const unsigned dst = __builtin_amdgcn_readfirstlane(lds[d] + shift);
-      asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(v), "s"(rsrc), "s"(dst), "s"(soff) : "memory", "m0");
+    soff = __builtin_amdgcn_readfirstlane(TR ? 0 : k0 * 2);
+    tail = !TR && k0 + BK > K;
+    k_at = k0;
+  }
+  __device__ __forceinline__ void issue(int d, unsigned shift, int lane, int wave) const {
+    unsigned v = voff[d];
+    if constexpr (!TR) {
+      const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, c = (piece % CPR) ^ ((row >> 1) & 7);
+      v = tail && k_at + c * 8 >= K ? NOWHERE : v;
     }
+    const unsigned dst = __builtin_amdgcn_readfirstlane(lds[d] + shift);
+    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(v), "s"(rsrc), "s"(dst), "s"(soff) : "memory", "m0");
   }
 };
 
@@ -217,29 +220,62 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
     for (int y = 0; y < TN; ++y) acc[x][y] = f32x16{};
   typedef typename Frag<T>::type frag;
 
-  a.fetch(kb, 0, lane, wave);
-  b.fetch(kb, 0, lane, wave);
+  // Fragments of k 16 ks .. come from LDS while the products of the 16 before them run, one read behind each product; the step's barrier
+  // stands in front of its last 16: behind it the first fragments of the next step are read and the loads of the one after it
+  // start, each behind a product too (a wavefront issues in order: a burst of either would leave the matrix pipe idle).
+  frag fa[2][TM], fb[2][TN];
+  auto read_one = [&](int set, const char* at, int ks, int n) __attribute__((always_inline)) {
+    if (n < TN) fb[set][n] = rb.template read<frag>(at + OpA::BYTES, n, ks);
+    else if (n < TN + TM) fa[set][n - TN] = ra.template read<frag>(at, n - TN, ks);
+  };
+  auto multiply = [&](int set, auto&& behind) __attribute__((always_inline)) {
+#pragma unroll
+    for (int x = 0; x < TM; ++x)
+#pragma unroll
+      for (int y = 0; y < TN; ++y) {
+        acc[x][y] = mfma(fb[set][y], fa[set][x], acc[x][y]);
+        __builtin_amdgcn_sched_barrier(0);
+        behind(x * TN + y);
+        __builtin_amdgcn_sched_barrier(0);
+      }
+  };
+  constexpr int NMUL = TM * TN, NREAD = TM + TN, NDMA = OpA::DMA + OpB::DMA;
+  constexpr int RPM = (NREAD + NMUL - 1) / NMUL, DPM = (NDMA + NMUL - 1) / NMUL;       // reads, loads behind a product
+  auto load_one = [&](int d, unsigned to) __attribute__((always_inline)) {
+    if (d < OpA::DMA) a.issue(d, to, lane, wave);
+    else if (d < NDMA) b.issue(d - OpA::DMA, to, lane, wave);
+  };
+  a.aim(kb);
+  b.aim(kb);
+#pragma unroll
+  for (int d = 0; d < NDMA; ++d) load_one(d, 0);
+  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
+  a.aim(kb + BK);
+  b.aim(kb + BK);
+#pragma unroll
+  for (int d = 0; d < NDMA; ++d) load_one(d, STEP);
   unsigned shift = 0;
+#pragma unroll
+  for (int n = 0; n < NREAD; ++n) read_one(0, lds, 0, n);
   for (int k0 = kb; k0 < ke; k0 += BK, shift ^= STEP) {
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // this step's tile has landed, the other buffer is read out
-    if (k0 + BK < ke) {
-      a.fetch(k0 + BK, shift ^ STEP, lane, wave);
-      b.fetch(k0 + BK, shift ^ STEP, lane, wave);
-    }
-    const char* ta = lds + shift;
-    const char* tb = lds + shift + OpA::BYTES;
+    const char* tile_at = lds + shift;
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks) {
-      frag fa[TM], fb[TN];
+    for (int ks = 0; ks < 3; ++ks)
+      multiply(ks & 1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-      for (int x = 0; x < TM; ++x) fa[x] = ra.template read<frag>(ta, x, ks);
+        for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one((ks + 1) & 1, tile_at, ks + 1, n);
+      });
+    // the next step's tile has landed, every wavefront has read this one out
+    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    const char* next_at = lds + (shift ^ STEP);
+    a.aim(k0 + 2 * BK);
+    b.aim(k0 + 2 * BK);
+    multiply(1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-      for (int y = 0; y < TN; ++y) fb[y] = rb.template read<frag>(tb, y, ks);
+      for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one(0, next_at, 0, n);       // (behind the last step: zeros)
 #pragma unroll
-      for (int x = 0; x < TM; ++x)
-#pragma unroll
-        for (int y = 0; y < TN; ++y) acc[x][y] = mfma(fb[y], fa[x], acc[x][y]);
-    }
+      for (int d = m * DPM; d < m * DPM + DPM; ++d) load_one(d, shift);
+    });
   }
 
   // Register q of a lane: i = lane % 32, j = 8 (q / 4) + 4 (lane / 32) + q % 4 of its 32 x 32 tile.  Through LDS (every wavefront its own part
@@ -248,7 +284,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   typedef T eight __attribute__((ext_vector_type(8)));
   constexpr int COLS = TN * 32, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
   static_assert(WAVES * 32 * PITCH * 4 <= 2 * STEP, "the epilogue's rows fit the tiles' room");
-  asm volatile("s_waitcnt lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles
+  asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles, no load is on its way
   float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   const int j = j0 + (wave % WN) * COLS + (lane % LPR) * 8, width = min(8, p.J - j);
   float bias[8] = {};
