@@ -157,10 +157,10 @@ SYMBOLS = {
     "nphm_dense_gpre": (c_int, [c_void_p, c_void_p, c_int, c_int, c_float, c_void_p, c_void_p, c_int, c_void_p, c_void_p]),
     "nphm_dense_column_sums": (c_int, [c_void_p, c_int, c_int, c_void_p, c_void_p]),
     "nphm_rows_lookup": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_float, c_void_p, c_void_p]),
-    "nphm_rows_grad_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "nphm_rows_grad_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
     "nphm_rows_grad": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float, c_void_p, c_void_p,
                                c_size_t, c_void_p]),
-    "nphm_rows_merge": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_void_p, c_void_p]),
+    "nphm_rows_merge": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "nphm_rows_renorm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_float, c_void_p, c_void_p]),
     "nphm_clip_workspace_bytes": (c_size_t, [c_void_p, c_int]),
     "nphm_clip_grads": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, ctypes.c_double, c_void_p, c_void_p, c_size_t, c_void_p]),

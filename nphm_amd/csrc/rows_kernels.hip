@@ -57,71 +57,421 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs p) {
 struct GradArgs {
   const void* grad;    // [count, dim], rows ld apart
   const void* idx;
-  void* out;           // [rows, dim]
+  void* out;           // [rows, dim]; merging: [count, dim]
   int64_t ld, count, rows;
   int dim, idx64;
   int64_t padding;     // -1: none
   float scale;
 };
 
-// One wavefront a row of the table and 64 vectors of its columns: it looks through all indices, 64 at a time, and adds the rows
-// that name its own.
 template <class T>
-__global__ __launch_bounds__(256) void grad_owner_kernel(GradArgs p) {
+__device__ __forceinline__ void load_cols(float (&v)[Vec<T>::N], const T* row, int c, int dim) {
+  constexpr int V = Vec<T>::N;
+  if (c + V <= dim) {
+    const typename Vec<T>::type x = *reinterpret_cast<const typename Vec<T>::type*>(row + c);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = float(x[k]);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = c + k < dim ? float(row[c + k]) : 0.f;
+  }
+}
+template <class T>
+__device__ __forceinline__ void store_cols(T* row, int c, int dim, const float (&v)[Vec<T>::N], float scale) {
+  constexpr int V = Vec<T>::N;
+  if (c + V <= dim) {
+    typename Vec<T>::type x;
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = T(v[k] * scale);
+    *reinterpret_cast<typename Vec<T>::type*>(row + c) = x;
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) if (c + k < dim) row[c + k] = T(v[k] * scale);
+  }
+}
+
+// ---- few indices: no sorting ----------------------------------------------------------------------------------------------------
+// One wavefront a row of the result and 64 vectors of its columns: it looks through all indices, 64 at a time, and adds the rows
+// that name its own.  One launch; MERGE: the rows of the result are those of `grad`, and all but the first of an index are zeros.
+constexpr int FEW = 256;
+
+template <class T, bool MERGE>
+__global__ __launch_bounds__(256) void grad_few_kernel(GradArgs p) {
   constexpr int V = Vec<T>::N;
   const int lane = threadIdx.x & 63;
-  const int64_t v = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (v >= p.rows) return;
+  const int64_t own = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (own >= (MERGE ? p.count : p.rows)) return;
+  const int64_t v = MERGE ? load_index(p.idx, p.idx64, own) : own;
   const int c = (blockIdx.y * 64 + lane) * V;
   float acc[V] = {};
   if (v != p.padding) {
     for (int64_t n0 = 0; n0 < p.count; n0 += 64) {
       const int64_t n = n0 + lane;
       uint64_t hit = __ballot(n < p.count && load_index(p.idx, p.idx64, n < p.count ? n : 0) == v);
+      if (MERGE && hit && n0 + __builtin_ctzll(hit) < own) break;    // an earlier row owns the sum (nothing was added yet)
       while (hit) {
         const int b = __builtin_ctzll(hit);
         hit &= hit - 1;
-        const T* g = static_cast<const T*>(p.grad) + (n0 + b) * p.ld;
+        float x[V];
+        load_cols(x, static_cast<const T*>(p.grad) + (n0 + b) * p.ld, c, p.dim);
 #pragma unroll
-        for (int k = 0; k < V; ++k)
-          if (c + k < p.dim) acc[k] += float(g[c + k]);
+        for (int k = 0; k < V; ++k) acc[k] += x[k];
       }
     }
   }
-  T* dst = static_cast<T*>(p.out) + v * p.dim;
-#pragma unroll
-  for (int k = 0; k < V; ++k)
-    if (c + k < p.dim) dst[c + k] = T(acc[k] * p.scale);
+  store_cols(static_cast<T*>(p.out) + own * p.dim, c, p.dim, acc, p.scale);
 }
 
-// out[n] = the sum of the rows that name the same index as row n, if n is the first of them, else zeros: duplicates of a row gradient
-// [count, dim] folded into one entry each, its shape unchanged
-template <class T>
-__global__ __launch_bounds__(256) void merge_kernel(GradArgs p) {
-  constexpr int V = Vec<T>::N;
-  const int lane = threadIdx.x & 63;
-  const int64_t own = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (own >= p.count) return;
-  const int c = (blockIdx.y * 64 + lane) * V;
-  const int64_t v = load_index(p.idx, p.idx64, own);
-  float acc[V] = {};
-  for (int64_t n0 = 0; n0 < p.count; n0 += 64) {
-    const int64_t n = n0 + lane;
-    uint64_t hit = __ballot(n < p.count && load_index(p.idx, p.idx64, n < p.count ? n : 0) == v);
-    if (hit && n0 + __builtin_ctzll(hit) < own) break;             // an earlier row owns the sum (nothing was added yet)
-    while (hit) {
-      const int b = __builtin_ctzll(hit);
-      hit &= hit - 1;
-      const T* g = static_cast<const T*>(p.grad) + (n0 + b) * p.ld;
+// ---- the indices, sorted ---------------------------------------------------------------------------------------------------------
+// A stable sort of the keys with their positions; keys that must not count (padding, outside the table) become `rows`, behind all others.
+__device__ __forceinline__ int key_of(const GradArgs& p, int64_t n) {
+  const int64_t i = load_index(p.idx, p.idx64, n);
+  return int(i < 0 || i >= p.rows || i == p.padding ? p.rows : i);
+}
+
+struct SortArgs {
+  int *keys, *sorted, *perm;           // [count up to a multiple of 64], [count], [count]
+  int *keys2, *perm2;                  // the other end of a radix pass
+  int* hist;                           // [blocks][1 << digit bits]
+  uint8_t* named;                      // [rows]: whether an index names the row
+  int shift, bits, per_block, blocks;
+};
+
+// keys from indices, and no row named yet
+__global__ __launch_bounds__(256) void keys_kernel(GradArgs p, SortArgs s, int key_blocks) {
+  if (int(blockIdx.x) < key_blocks) {
+    const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
+    if (n < (p.count + 63) / 64 * 64) s.keys[n] = n < p.count ? key_of(p, n) : 0x7fffffff;
+  } else {
+    const int64_t step = int64_t(gridDim.x - key_blocks) * 256;
+    for (int64_t i = int64_t(blockIdx.x - key_blocks) * 256 + threadIdx.x; i < p.rows; i += step) s.named[i] = 0;
+  }
+}
+
+// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 64 keys, its four wavefronts count over a quarter of
+// all keys each (scalar loads: the counted key is the same for all lanes): count^2 comparisons, one launch.
+constexpr int MIDDLE = 8192;
+
+__global__ __launch_bounds__(256) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
+                                                   uint8_t* __restrict__ named) {
+  __shared__ int part[4][64];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int i = blockIdx.x * 64 + lane, own = keys[i];
+  const int groups = (count + 63) / 64, quarter = (groups + 3) / 4;
+  int before = 0;
+  for (int g = wave * quarter; g < min(groups, (wave + 1) * quarter); ++g) {
+    const int* k = keys + g * 64;
+    if (g < int(blockIdx.x)) {
 #pragma unroll
-      for (int k = 0; k < V; ++k)
-        if (c + k < p.dim) acc[k] += float(g[c + k]);
+      for (int u = 0; u < 64; ++u) before += k[u] <= own;
+    } else if (g > int(blockIdx.x)) {
+#pragma unroll
+      for (int u = 0; u < 64; ++u) before += k[u] < own;
+    } else {
+#pragma unroll
+      for (int u = 0; u < 64; ++u) before += k[u] < own || (k[u] == own && u < lane);
     }
   }
-  T* dst = static_cast<T*>(p.out) + own * p.dim;
+  part[wave][lane] = before;
+  __syncthreads();
+  if (wave == 0 && i < count) {
+    const int at = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    sorted[at] = own;
+    perm[at] = i;
+    if (own < rows) named[own] = 1;
+  }
+}
+
+// More: radix passes of up to 9 bits, least first.  hist: how often each block of keys has each digit.
+constexpr int MAX_DIGIT = 9;
+
+__global__ __launch_bounds__(1024) void radix_hist_kernel(const int* __restrict__ keys, int count, SortArgs s) {
+  __shared__ int bins[1 << MAX_DIGIT];
+  const int digits = 1 << s.bits, t = threadIdx.x;
+  for (int d = t; d < digits; d += 1024) bins[d] = 0;
+  __syncthreads();
+  const int64_t first = int64_t(blockIdx.x) * s.per_block;
+  for (int u = t; u < s.per_block; u += 1024)
+    if (first + u < count) atomicAdd(&bins[(keys[first + u] >> s.shift) & (digits - 1)], 1);
+  __syncthreads();
+  for (int d = t; d < digits; d += 1024) s.hist[blockIdx.x * digits + d] = bins[d];
+}
+
+// Every block finds where its keys of each digit begin (the digits below it in all blocks, its own in the blocks before), then places its
+// keys in order, 1024 at a time: in a wavefront the lanes of one digit find each other by ballots, wavefront follows wavefront.
+template <bool FIRST, bool LAST>
+__global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict__ keys, const int* __restrict__ perm, int count, int rows, SortArgs s,
+                                                           int* __restrict__ keys_out, int* __restrict__ perm_out) {
+  __shared__ int base[1 << MAX_DIGIT], scan[1 << MAX_DIGIT], seen[16][1 << MAX_DIGIT];
+  const int digits = 1 << s.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
+  if (t < digits) {
+    int total = 0, before = 0;
+    for (int b = 0; b < s.blocks; ++b) {
+      const int h = s.hist[b * digits + t];
+      total += h;
+      before += b < int(blockIdx.x) ? h : 0;
+    }
+    base[t] = before;
+    scan[t] = total;
+  }
+  __syncthreads();
+  for (int o = 1; o < digits; o <<= 1) {
+    const int v = t < digits && t >= o ? scan[t - o] : 0;
+    __syncthreads();
+    if (t < digits) scan[t] += v;
+    __syncthreads();
+  }
+  if (t > 0 && t < digits) base[t] += scan[t - 1];
+  const int64_t first = int64_t(blockIdx.x) * s.per_block;
+  for (int u = 0; u < s.per_block; u += 1024) {
+    const int64_t n = first + u + t;
+    const bool in = n < count;
+    const int key = in ? keys[n] : 0, d = (key >> s.shift) & (digits - 1);
+    for (int q = t; q < 16 * digits; q += 1024) seen[q / digits][q % digits] = 0;
+    __syncthreads();
+    uint64_t mates = __ballot(in);
+    for (int b = 0; b < s.bits; ++b) {
+      const uint64_t ones = __ballot((d >> b) & 1);
+      mates &= (d >> b) & 1 ? ones : ~ones;
+    }
+    const int ahead = __popcll(mates & ((uint64_t(1) << lane) - 1));
+    if (in && ahead == 0) seen[wave][d] = __popcll(mates);
+    __syncthreads();
+    if (t < digits) {
+      int at = base[t];
+      for (int w = 0; w < 16; ++w) {
+        const int h = seen[w][t];
+        seen[w][t] = at;
+        at += h;
+      }
+      base[t] = at;
+    }
+    __syncthreads();
+    if (in) {
+      const int at = seen[wave][d] + ahead;
+      keys_out[at] = key;
+      perm_out[at] = FIRST ? int(n) : perm[n];
+      if (LAST && key < rows) s.named[key] = 1;
+    }
+    __syncthreads();
+  }
+}
+
+// ---- sums over runs of equal keys --------------------------------------------------------------------------------------------------
+// A wavefront adds the rows of `chunk` consecutive places (64 vectors of columns): a run that lies inside goes out, one that the
+// chunk's borders cut goes to partial[2 chunk + (begun before ? 0 : 1)] in fp32; join adds those in order, from the chunk where the run
+// begins.  So a row that takes half of all indices costs no more than any other half.
+struct SumArgs {
+  const int *sorted, *perm;
+  const uint8_t* named;
+  float* partial;
+  int chunk, chunks, tiles;
+  int64_t pitch;                       // floats a partial row
+  int sum_blocks;
+};
+
+template <class T, bool MERGE>
+__global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
+  constexpr int V = Vec<T>::N, AHEAD = 4;
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  T* out = static_cast<T*>(p.out);
+  const float nothing[V] = {};
+  if (int(blockIdx.x) >= s.sum_blocks) {                             // the rows that stay zero
+    const int64_t step = int64_t(gridDim.x - s.sum_blocks) * 4;
+    for (int64_t v = int64_t(blockIdx.x - s.sum_blocks) * 4 + wave; v < (MERGE ? p.count : p.rows); v += step) {
+      int64_t row = v;
+      if constexpr (MERGE) {
+        if (s.sorted[v] < p.rows && (v == 0 || s.sorted[v] != s.sorted[v - 1])) continue;
+        row = s.perm[v];
+      } else {
+        if (s.named[v]) continue;
+      }
+      for (int c = lane * V; c < p.dim; c += 64 * V) store_cols(out + row * p.dim, c, p.dim, nothing, 1.f);
+    }
+    return;
+  }
+  const int64_t task = int64_t(blockIdx.x) * 4 + wave;
+  if (task >= int64_t(s.chunks) * s.tiles) return;
+  const int chunk = int(task / s.tiles), c = (int(task % s.tiles) * 64 + lane) * V;
+  const int64_t p0 = int64_t(chunk) * s.chunk, p1 = min(p.count, p0 + s.chunk);
+  float acc[V] = {};
+  int key = s.sorted[p0], head = s.perm[p0];
+  bool begun = p0 > 0 && s.sorted[p0 - 1] == key;
+  auto flush = [&](bool goes_on) __attribute__((always_inline)) {
+    if (key >= p.rows) return;
+    if (!begun && !goes_on) {
+      store_cols(out + int64_t(MERGE ? head : key) * p.dim, c, p.dim, acc, p.scale);
+    } else {
+      float* to = s.partial + (2 * int64_t(chunk) + (begun ? 0 : 1)) * s.pitch + c;
+      typedef float f32x4 __attribute__((ext_vector_type(4)));
 #pragma unroll
-  for (int k = 0; k < V; ++k)
-    if (c + k < p.dim) dst[c + k] = T(acc[k]);
+      for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(to + k) = f32x4{acc[k], acc[k + 1], acc[k + 2], acc[k + 3]};
+    }
+  };
+  for (int64_t q = p0; q < p1; q += AHEAD) {
+    float x[AHEAD][V];
+    int k[AHEAD], r[AHEAD];
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      const int64_t at = min(q + a, p1 - 1);
+      k[a] = s.sorted[at];
+      r[a] = s.perm[at];
+    }
+    if (k[0] >= p.rows) break;                                       // nothing that counts from here on
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) load_cols(x[a], static_cast<const T*>(p.grad) + int64_t(r[a]) * p.ld, c, p.dim);
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) {
+      if (q + a >= p1) break;
+      if (k[a] != key) {
+        flush(false);
+        key = k[a];
+        head = r[a];
+        begun = false;
+#pragma unroll
+        for (int e = 0; e < V; ++e) acc[e] = 0.f;
+      }
+#pragma unroll
+      for (int e = 0; e < V; ++e) acc[e] += x[a][e];
+    }
+  }
+  flush(p1 < p.count && s.sorted[p1] == key);
+}
+
+template <class T, bool MERGE>
+__global__ __launch_bounds__(256) void join_kernel(GradArgs p, SumArgs s) {
+  constexpr int V = Vec<T>::N;
+  __shared__ float part[3][64][V];
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int chunk = blockIdx.x, c = (blockIdx.y * 64 + lane) * V;
+  const int64_t p0 = int64_t(chunk) * s.chunk, p1 = min(p.count, p0 + s.chunk);
+  const int key = s.sorted[p1 - 1];
+  if (p1 >= p.count || key >= p.rows || s.sorted[p1] != key) return;             // its last run does not go on
+  if (s.sorted[p0] == key && p0 > 0 && s.sorted[p0 - 1] == key) return;          // it began before this chunk
+  int last = chunk;                                                              // the chunk where it ends
+  for (;;) {
+    const int64_t at = int64_t(last + 1 + lane) * s.chunk;
+    const uint64_t on = __ballot(at < p.count && s.sorted[at < p.count ? at : 0] == key);
+    const int run = on == ~uint64_t(0) ? 64 : __builtin_ctzll(~on);
+    last += run;
+    if (run < 64) break;
+  }
+  const int n = last - chunk, each = (n + 3) / 4, from = chunk + 1 + wave * each, to = min(last + 1, from + each);
+  float acc[V] = {};
+  auto add = [&](int64_t row) __attribute__((always_inline)) {
+    const float* q = s.partial + row * s.pitch + c;
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += q[k];
+  };
+  if (wave == 0) add(2 * int64_t(chunk) + 1);
+#pragma unroll 4
+  for (int k = from; k < to; ++k) add(2 * int64_t(k));
+  if (wave) {
+#pragma unroll
+    for (int k = 0; k < V; ++k) part[wave - 1][lane][k] = acc[k];
+  }
+  __syncthreads();
+  if (wave) return;
+#pragma unroll
+  for (int w = 0; w < 3; ++w)
+#pragma unroll
+    for (int k = 0; k < V; ++k) acc[k] += part[w][lane][k];
+  int64_t row = key;
+  if constexpr (MERGE) {                                                         // the run's first place in this chunk (chunks have 64 at most)
+    const uint64_t in = __ballot(p0 + lane < p1 && s.sorted[p0 + lane < p1 ? p0 + lane : p0] == key);
+    row = s.perm[p0 + __builtin_ctzll(in)];
+  }
+  store_cols(static_cast<T*>(p.out) + row * p.dim, c, p.dim, acc, p.scale);
+}
+
+struct GradPlan {
+  int passes, bits, blocks, per_block, chunk, chunks, tiles;
+  size_t keys, sorted, perm, keys2, perm2, hist, named, partial, total;
+};
+inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element) {
+  GradPlan g{};
+  if (count <= FEW) return g;
+  auto up = [](size_t v) { return (v + 255) / 256 * 256; };
+  int bits = 1;
+  while ((int64_t(1) << bits) <= rows) ++bits;
+  g.passes = count <= MIDDLE ? 0 : (bits + MAX_DIGIT - 1) / MAX_DIGIT;
+  g.bits = g.passes ? (bits + g.passes - 1) / g.passes : 0;
+  g.per_block = int(((count + 255) / 256 + 1023) / 1024 * 1024);
+  g.blocks = int((count + g.per_block - 1) / g.per_block);
+  const int vec = 16 / element;
+  g.tiles = int((dim + 64 * vec - 1) / (64 * vec));
+  g.chunk = 8;
+  while (g.chunk < 64 && count / (2 * g.chunk) * g.tiles >= 4096) g.chunk *= 2;
+  g.chunks = int((count + g.chunk - 1) / g.chunk);
+  const size_t ints = up(size_t((count + 63) / 64 * 64) * 4);
+  g.keys = 0;
+  g.sorted = ints;
+  g.perm = 2 * ints;
+  g.keys2 = 3 * ints;
+  g.perm2 = 4 * ints;
+  g.hist = g.passes ? 5 * ints : 3 * ints;
+  g.named = g.hist + (g.passes ? up(size_t(g.blocks) * 4 << g.bits) : 0);
+  g.partial = g.named + up(size_t(rows));
+  g.total = g.partial + up(size_t(2) * g.chunks * g.tiles * 64 * vec * 4);
+  return g;
+}
+
+template <class T, bool MERGE>
+inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char* ws) {
+  const unsigned tiles = unsigned((a.dim + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N));
+  const int64_t out_rows = MERGE ? a.count : a.rows;
+  if (a.count <= FEW) {
+    hipLaunchKernelGGL((grad_few_kernel<T, MERGE>), dim3(unsigned((out_rows + 3) / 4), tiles), dim3(256), 0, st, a);
+    return;
+  }
+  const int count = int(a.count), rows = int(a.rows);
+  SortArgs s{};
+  s.keys = reinterpret_cast<int*>(ws + g.keys);
+  s.sorted = reinterpret_cast<int*>(ws + g.sorted);
+  s.perm = reinterpret_cast<int*>(ws + g.perm);
+  s.keys2 = reinterpret_cast<int*>(ws + g.keys2);
+  s.perm2 = reinterpret_cast<int*>(ws + g.perm2);
+  s.hist = reinterpret_cast<int*>(ws + g.hist);
+  s.named = reinterpret_cast<uint8_t*>(ws + g.named);
+  s.bits = g.bits;
+  s.per_block = g.per_block;
+  s.blocks = g.blocks;
+  const int key_blocks = (count + 63) / 64 * 64 / 256 + 1;
+  const int64_t clear = (a.rows + 255) / 256;
+  hipLaunchKernelGGL(keys_kernel, dim3(unsigned(key_blocks + (clear < 1024 ? clear : 1024))), dim3(256), 0, st, a, s, key_blocks);
+  if (!g.passes) {
+    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + 63) / 64)), dim3(256), 0, st, s.keys, count, rows, s.sorted, s.perm, s.named);
+  } else {
+    // the passes go keys -> other -> ... -> sorted, whatever their number
+    const int *kin = s.keys, *pin = nullptr;
+    for (int pass = 0; pass < g.passes; ++pass) {
+      const bool to_sorted = (g.passes - 1 - pass) % 2 == 0;
+      int *kout = to_sorted ? s.sorted : s.keys2, *pout = to_sorted ? s.perm : s.perm2;
+      s.shift = pass * g.bits;
+      hipLaunchKernelGGL(radix_hist_kernel, dim3(unsigned(g.blocks)), dim3(1024), 0, st, kin, count, s);
+      const dim3 grid(unsigned(g.blocks)), block(1024);
+      const bool first = pass == 0, last = pass == g.passes - 1;
+      if (first && last) hipLaunchKernelGGL((radix_place_kernel<true, true>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
+      else if (first) hipLaunchKernelGGL((radix_place_kernel<true, false>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
+      else if (last) hipLaunchKernelGGL((radix_place_kernel<false, true>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
+      else hipLaunchKernelGGL((radix_place_kernel<false, false>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
+      kin = kout;
+      pin = pout;
+    }
+  }
+  SumArgs u{};
+  u.sorted = s.sorted;
+  u.perm = s.perm;
+  u.named = s.named;
+  u.partial = reinterpret_cast<float*>(ws + g.partial);
+  u.chunk = g.chunk;
+  u.chunks = g.chunks;
+  u.tiles = g.tiles;
+  u.pitch = int64_t(g.tiles) * 64 * Vec<T>::N;
+  u.sum_blocks = int((int64_t(g.chunks) * g.tiles + 3) / 4);
+  const int64_t zero = (out_rows + 15) / 16;
+  hipLaunchKernelGGL((sum_kernel<T, MERGE>), dim3(unsigned(u.sum_blocks + (zero < 4096 ? zero : 4096))), dim3(256), 0, st, a, u);
+  hipLaunchKernelGGL((join_kernel<T, MERGE>), dim3(unsigned(g.chunks), tiles), dim3(256), 0, st, a, u);
 }
 
 // max-norm: rows that an index names are flagged, then each flagged row is rescaled ONCE however often it is named
@@ -192,34 +542,32 @@ int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, i
   return 0;
 }
 
-size_t nphm_rows_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t count) { return 0; }
+size_t nphm_rows_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t count, int dtype) {
+  return dtype_ok(dtype) ? grad_plan(rows, dim, count, dtype_size(dtype)).total : 0;
+}
 
 int nphm_rows_grad(const void* grad, int64_t count, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t rows,
                    int64_t padding, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_table("nphm_rows_grad", out, rows, dim, dim, dtype, idx, idx_bits, count)) return rc;
   if (count && (!grad || ld < dim)) return nphm_fail_msg("nphm_rows_grad: null gradient or row stride below the width");
-  if (workspace_bytes < nphm_rows_grad_workspace_bytes(rows, dim, count)) return nphm_fail_msg("nphm_rows_grad: workspace too small");
+  const GradPlan g = grad_plan(rows, dim, count, dtype_size(dtype));
+  if (workspace_bytes < g.total || (g.total && !workspace)) return nphm_fail_msg("nphm_rows_grad: workspace too small");
   GradArgs a{grad, idx, out, ld, count, rows, int(dim), idx_bits == 64, padding, scale};
-  with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    const unsigned tiles = unsigned((dim + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N));
-    hipLaunchKernelGGL((grad_owner_kernel<T>), dim3(unsigned((rows + 3) / 4), tiles), dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  });
+  with_dtype(dtype, [&](auto t) { grad_run<decltype(t), false>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_grad launch", e);
   return 0;
 }
 
-int nphm_rows_merge(const void* grad, int64_t count, int64_t dim, int dtype, const void* idx, int idx_bits, void* out, void* stream) {
-  if (int rc = check_table("nphm_rows_merge", out, 1, dim, dim, dtype, idx, idx_bits, count)) return rc;
+int nphm_rows_merge(const void* grad, int64_t count, int64_t dim, int dtype, const void* idx, int idx_bits, int64_t rows, void* out,
+                    void* workspace, size_t workspace_bytes, void* stream) {
+  if (int rc = check_table("nphm_rows_merge", out, rows, dim, dim, dtype, idx, idx_bits, count)) return rc;
   if (count == 0) return 0;
-  if (!grad) return nphm_fail_msg("nphm_rows_merge: null pointer");
-  GradArgs a{grad, idx, out, dim, count, 0, int(dim), idx_bits == 64, -1, 1.f};
-  with_dtype(dtype, [&](auto t) {
-    using T = decltype(t);
-    const unsigned tiles = unsigned((dim + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N));
-    hipLaunchKernelGGL((merge_kernel<T>), dim3(unsigned((count + 3) / 4), tiles), dim3(256), 0, static_cast<hipStream_t>(stream), a);
-  });
+  if (!grad || grad == out) return nphm_fail_msg("nphm_rows_merge: null pointer, or the result in place of the gradient");
+  const GradPlan g = grad_plan(rows, dim, count, dtype_size(dtype));
+  if (workspace_bytes < g.total || (g.total && !workspace)) return nphm_fail_msg("nphm_rows_merge: workspace too small");
+  GradArgs a{grad, idx, out, dim, count, rows, int(dim), idx_bits == 64, -1, 1.f};
+  with_dtype(dtype, [&](auto t) { grad_run<decltype(t), true>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_merge launch", e);
   return 0;

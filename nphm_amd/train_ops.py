@@ -102,7 +102,7 @@ def lookup_rows_grad(grad, idx, num_rows, scale=1.0, padding_idx=None):
     i = idx.contiguous()
     out = torch.empty(num_rows, D, dtype=grad.dtype, device=grad.device)
     lib = _lib.load()
-    need = lib.nphm_rows_grad_workspace_bytes(num_rows, D, i.numel())
+    need = lib.nphm_rows_grad_workspace_bytes(num_rows, D, i.numel(), _DTYPES[grad.dtype])
     with _on(grad.device) as stream:
         ws = torch.empty(max(need, 1), dtype=torch.uint8, device=grad.device)
         _lib.check(lib.nphm_rows_grad(g.data_ptr(), i.numel(), D, ld, _DTYPES[grad.dtype], i.data_ptr(), 8 * i.element_size(), num_rows, pad,
@@ -364,9 +364,12 @@ def _merge_rows_(g):
     if flat.numel() == 0:
         return
     out = torch.empty_like(flat)
+    lib = _lib.load()
+    need = lib.nphm_rows_grad_workspace_bytes(g.shape[0], flat.shape[1], flat.shape[0], _DTYPES[v.dtype])
     with _on(v.device) as stream:
-        _lib.check(_lib.load().nphm_rows_merge(flat.data_ptr(), flat.shape[0], flat.shape[1], _DTYPES[v.dtype], i.data_ptr(), 64,
-                                               out.data_ptr(), stream), "nphm_rows_merge")
+        ws = _workspace(need, v.device)
+        _lib.check(lib.nphm_rows_merge(flat.data_ptr(), flat.shape[0], flat.shape[1], _DTYPES[v.dtype], i.data_ptr(), 64, g.shape[0],
+                                       out.data_ptr(), ws.data_ptr(), need, stream), "nphm_rows_merge")
     v.copy_(out.view_as(v))
 
 

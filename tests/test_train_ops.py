@@ -569,6 +569,27 @@ def test_clip_sparse_and_dense_gradients_together(dev):
         within(w.grad, want_w * f, want_w.abs() * f * 12 * F32)
 
 
+@gpu
+@pytest.mark.parametrize("N,rows,D", [(200, 7, 33), (700, 50, 8), (9000, 300, 20), (30000, 3, 5), (20000, 100000, 4)])
+def test_duplicates_of_a_sparse_gradient_are_folded(dev, N, rows, D):
+    """every entry's row in order: the first entry of a row holds the sum of its entries (fp32, in their order), the others zeros"""
+    gen = torch.Generator(device=dev).manual_seed(N)
+    idx = (torch.rand(N, device=dev, generator=gen) ** 2 * rows).long().clamp_(0, rows - 1)
+    values = torch.randn(N, D, device=dev, generator=gen)
+    s = torch.sparse_coo_tensor(idx[None], values.clone(), (rows, D))
+    T._merge_rows_(s)
+    got = s._values()
+    want = torch.zeros(rows, D, dtype=torch.float64, device=dev).index_put_((idx,), values.double(), accumulate=True)
+    mag = torch.zeros(rows, D, dtype=torch.float64, device=dev).index_put_((idx,), values.double().abs(), accumulate=True)
+    many = torch.bincount(idx, minlength=rows)[:, None].double()
+    first = torch.full((rows,), N, device=dev).scatter_reduce_(0, idx, torch.arange(N, device=dev), "amin")
+    heads = first[many[:, 0] > 0]
+    within(got[heads], want[idx[heads]], (mag * (many + 1) * F32)[idx[heads]] + 1e-30)
+    rest = torch.ones(N, dtype=torch.bool, device=dev)
+    rest[heads] = False
+    assert not got[rest].any()
+
+
 # ---- all of them -----------------------------------------------------------------------------------------------------------------
 
 def step(dev, codes, layers, idx, pts, target):
