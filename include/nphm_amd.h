@@ -686,11 +686,11 @@ int nphm_clip_grads(const void* const* in, void* const* out, const int64_t* coun
  *     contiguous bf16 or fp16; bias, residual, z (kept for the backward pass) may be NULL.  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU
  *     (erf), 4 Softplus(beta).  M up to 2^22, N and K up to 2^20.
  *   nphm_layer16_backward : gz = g a'(z); dx = gz W, dweight = gz^T x, dbias = column sums of gz (each may be NULL).
- *     Workspaces: nphm_layer16_*_workspace_bytes, 256-byte aligned. */
-size_t nphm_layer16_forward_workspace_bytes(int64_t M, int64_t N, int64_t K);
+ *     Workspaces: nphm_layer16_*_workspace_bytes of the same operands (0: none is needed, NULL will do), 256-byte aligned. */
+size_t nphm_layer16_forward_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K);
 int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,
                          int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream);
-size_t nphm_layer16_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act);
+size_t nphm_layer16_backward_workspace_bytes(const void* g, const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int act);
 int nphm_layer16_backward(const void* g, const void* x, const void* weight, const void* z, void* dx, void* dweight, void* dbias, int64_t M,
                           int64_t N, int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream);
 

@@ -164,9 +164,9 @@ SYMBOLS = {
     "nphm_rows_renorm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_float, c_void_p, c_void_p]),
     "nphm_clip_workspace_bytes": (c_size_t, [c_void_p, c_int]),
     "nphm_clip_grads": (c_int, [c_void_p, c_void_p, c_void_p, c_void_p, c_int, c_int, ctypes.c_double, c_void_p, c_void_p, c_size_t, c_void_p]),
-    "nphm_layer16_forward_workspace_bytes": (c_size_t, [c_int64] * 3),
+    "nphm_layer16_forward_workspace_bytes": (c_size_t, [c_void_p] * 2 + [c_int64] * 3),
     "nphm_layer16_forward": (c_int, [c_void_p] * 6 + [c_int64] * 3 + [c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
-    "nphm_layer16_backward_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
+    "nphm_layer16_backward_workspace_bytes": (c_size_t, [c_void_p] * 3 + [c_int64] * 3 + [c_int]),
     "nphm_layer16_backward": (c_int, [c_void_p] * 7 + [c_int64] * 3 + [c_int, c_int, c_float, c_void_p, c_size_t, c_void_p]),
 }
 

@@ -16,7 +16,7 @@
 namespace nphm {
 namespace train_ops {
 
-constexpr int TABLE = 128;               // tensors a launch: 128 * 25 bytes + ... of the 4 KiB of arguments
+constexpr int TABLE = 150;               // tensors a launch: 150 x 25 bytes of the 4 KiB of arguments
 constexpr int CHUNK = 16384;             // bytes a block takes at a time
 constexpr int MAX_BLOCKS = 2048;
 
@@ -51,16 +51,18 @@ __device__ __forceinline__ double join(double a, double b, int kind) {
   return (b > a || b != b) ? b : a;
 }
 
-// the 256 threads' values -> one, in thread order
+// the block's values -> one, the same on every thread, in a fixed order
+template <int THREADS>
 __device__ __forceinline__ double block_join(double v, int kind) {
-  __shared__ double part[256];
-  part[threadIdx.x] = v;
+  __shared__ double part[THREADS / 64];
+#pragma unroll
+  for (int o = 32; o; o >>= 1) v = join(v, __shfl_xor(v, o), kind);
+  if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = v;
   __syncthreads();
-  for (int o = 128; o; o >>= 1) {
-    if (int(threadIdx.x) < o) part[threadIdx.x] = join(part[threadIdx.x], part[threadIdx.x + o], kind);
-    __syncthreads();
-  }
-  return part[0];
+  v = part[0];
+#pragma unroll
+  for (int w = 1; w < THREADS / 64; ++w) v = join(v, part[w], kind);
+  return v;
 }
 
 template <class T>
@@ -85,20 +87,28 @@ __global__ __launch_bounds__(256) void norm_kernel(ClipTable t, uint32_t chunks,
     else if (t.dtype[i] == DT_BF16) norm_chunk<bf16>(t, i, c, kind, acc);
     else norm_chunk<fp16>(t, i, c, kind, acc);
   }
-  acc = block_join(acc, kind);
+  acc = block_join<256>(acc, kind);
   if (threadIdx.x == 0) partial[blockIdx.x] = acc;
 }
 
 // partial sums -> norm (fp32) and the factor
-__global__ __launch_bounds__(256) void norm_finish_kernel(const double* partial, int n, int kind, double limit, float* norm, float* factor) {
+template <int THREADS>
+__device__ __forceinline__ void finish(const double* partial, int n, int kind, double limit, float& norm, float& factor) {
   double acc = 0;
-  for (int i = threadIdx.x; i < n; i += 256) acc = join(acc, partial[i], kind);
-  acc = block_join(acc, kind);
+  for (int i = threadIdx.x; i < n; i += THREADS) acc = join(acc, partial[i], kind);
+  acc = block_join<THREADS>(acc, kind);
+  if (kind == 0) acc = sqrt(acc);
+  const double f = limit / (acc + 1e-6);
+  norm = float(acc);
+  factor = f > 1.0 ? 1.f : float(f);
+}
+
+__global__ __launch_bounds__(1024) void finish_kernel(const double* partial, int n, int kind, double limit, float* norm, float* factor) {
+  float a, f;
+  finish<1024>(partial, n, kind, limit, a, f);
   if (threadIdx.x == 0) {
-    if (kind == 0) acc = sqrt(acc);
-    *norm = float(acc);
-    const double f = limit / (acc + 1e-6);
-    if (factor) *factor = f > 1.0 ? 1.f : float(f);
+    *norm = a;
+    if (factor) *factor = f;
   }
 }
 
@@ -118,9 +128,28 @@ __device__ __forceinline__ void scale_chunk(const ClipTable& t, int i, uint32_t 
   if (full + threadIdx.x < end) o[full + threadIdx.x] = T(float(g[full + threadIdx.x]) * f);
 }
 
-__global__ __launch_bounds__(256) void scale_kernel(ClipTable t, uint32_t chunks, const float* factor) {
-  const float f = *factor;
-  for (uint32_t c = blockIdx.x; c < chunks; c += gridDim.x) {
+// Up to FOLD partial sums every block adds up by itself (8 KiB from L2, no launch for them); more have their factor ready.
+constexpr int FOLD = 1024;
+
+struct Factor {
+  const double* partial;
+  int n, kind;
+  double limit;
+  float* norm;               // written by the first block where the partial sums are folded here
+  const float* ready;        // null: fold
+};
+
+__global__ __launch_bounds__(256) void scale_kernel(ClipTable t, uint32_t chunks, Factor s) {
+  float f;
+  if (s.ready) {
+    f = *s.ready;
+  } else {
+    float norm;
+    finish<256>(s.partial, s.n, s.kind, s.limit, norm, f);
+    if (blockIdx.x == 0 && threadIdx.x == 0 && s.norm) *s.norm = norm;
+  }
+  for (uint32_t b = blockIdx.x; b < chunks; b += gridDim.x) {
+    const uint32_t c = chunks - 1 - b;                               // the other way round: what was read last is still in the cache
     const int i = tensor_of(t, c);
     if (f == 1.f && t.in[i] == t.out[i]) continue;                 // nothing to change in place
     if (t.dtype[i] == DT_F32) scale_chunk<float>(t, i, c, f);
@@ -129,9 +158,9 @@ __global__ __launch_bounds__(256) void scale_kernel(ClipTable t, uint32_t chunks
   }
 }
 
-// cuts the list into tables: f(table, chunks)
+// cuts the list into tables, from its end where `back`: f(table, chunks)
 template <class F>
-inline void for_tables(const void* const* in, void* const* out, const int64_t* counts, const int* dtypes, int n, F&& f) {
+inline void for_tables(const void* const* in, void* const* out, const int64_t* counts, const int* dtypes, int n, bool back, F&& f) {
   ClipTable t;
   t.tensors = 0;
   uint32_t chunks = 0;
@@ -143,8 +172,8 @@ inline void for_tables(const void* const* in, void* const* out, const int64_t* c
     chunks = 0;
   };
   constexpr int64_t PIECE = int64_t(1) << 30;                      // a tensor of more elements takes several entries
-  for (int i = 0; i < n; ++i) {
-    const int e = dtype_size(dtypes[i]);
+  for (int u = 0; u < n; ++u) {
+    const int i = back ? n - 1 - u : u, e = dtype_size(dtypes[i]);
     for (int64_t at = 0; at < counts[i]; at += PIECE) {
       const int64_t m = std::min(PIECE, counts[i] - at);
       const int k = t.tensors++;
@@ -220,15 +249,18 @@ int nphm_clip_grads(const void* const* in, void* const* out, const int64_t* coun
   double* partial = static_cast<double*>(workspace);
   float* factor = reinterpret_cast<float*>(partial + size_t(table_count(counts, n)) * MAX_BLOCKS);
   int parts = 0;
-  for_tables(in, out, counts, dtypes, n, [&](const ClipTable& t, uint32_t chunks) {
+  for_tables(in, out, counts, dtypes, n, false, [&](const ClipTable& t, uint32_t chunks) {
     const uint32_t blocks = std::min<uint32_t>(chunks, MAX_BLOCKS);
     hipLaunchKernelGGL(norm_kernel, dim3(blocks), dim3(256), 0, st, t, chunks, kind, partial + parts);
     parts += int(blocks);
   });
-  hipLaunchKernelGGL(norm_finish_kernel, dim3(1), dim3(256), 0, st, partial, parts, kind, limit, norm, out ? factor : nullptr);
+  const bool fold = out && parts && parts <= FOLD;
+  if (!fold) hipLaunchKernelGGL(finish_kernel, dim3(1), dim3(1024), 0, st, partial, parts, kind, limit, norm, out ? factor : nullptr);
+  Factor s{partial, parts, kind, limit, norm, fold ? nullptr : factor};
   if (out)
-    for_tables(in, out, counts, dtypes, n, [&](const ClipTable& t, uint32_t chunks) {
-      hipLaunchKernelGGL(scale_kernel, dim3(std::min<uint32_t>(chunks, MAX_BLOCKS)), dim3(256), 0, st, t, chunks, factor);
+    for_tables(in, out, counts, dtypes, n, true, [&](const ClipTable& t, uint32_t chunks) {
+      hipLaunchKernelGGL(scale_kernel, dim3(std::min<uint32_t>(chunks, MAX_BLOCKS)), dim3(256), 0, st, t, chunks, s);
+      s.norm = nullptr;
     });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_clip_grads launch", e);

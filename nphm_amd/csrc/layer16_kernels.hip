@@ -27,16 +27,25 @@ __device__ __forceinline__ f32x16 mfma(fp16x8 a, fp16x8 b, f32x16 c) { return __
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SOFTPLUS = 4 };
 
-__device__ __forceinline__ float sigmoid(float z) { return 1.f / (1.f + __expf(-z)); }
+// exp and log in base 2 and the reciprocal are the hardware's (1 ulp): far below a 16-bit rounding
+__device__ __forceinline__ float exp_(float v) { return __builtin_amdgcn_exp2f(1.44269504f * v); }
+__device__ __forceinline__ float sigmoid(float z) { return __builtin_amdgcn_rcpf(1.f + exp_(-z)); }
+// normal distribution, P(X < z): erfc by Abramowitz & Stegun 7.1.26 (off by 1.5e-7 at most), e = exp(-z^2 / 2)
+__device__ __forceinline__ float normal_cdf(float z, float e) {
+  const float t = __builtin_amdgcn_rcpf(1.f + 0.3275911f * 0.70710678f * fabsf(z));
+  const float half = 0.5f * e * t * (0.254829592f + t * (-0.284496736f + t * (1.421413741f + t * (-1.453152027f + t * 1.061405429f))));
+  return z > 0.f ? 1.f - half : half;
+}
 
 __device__ __forceinline__ float act_value(float z, int act, float beta) {
   switch (act) {
     case ACT_RELU: return z > 0.f ? z : (z != z ? z : 0.f);
     case ACT_SILU: return z * sigmoid(z);
-    case ACT_GELU: return 0.5f * z * (1.f + erff(z * 0.70710678f));
-    case ACT_SOFTPLUS: {
-      const float t = beta * z;
-      return t > 20.f ? z : log1pf(__expf(t)) / beta;
+    case ACT_GELU: return z * normal_cdf(z, exp_(-0.5f * z * z));
+    case ACT_SOFTPLUS: {                                             // max(z, 0) + log(1 + exp(-|beta z|)) / beta
+      const float t = exp_(-fabsf(beta * z));
+      const float l = t < 1e-3f ? t - 0.5f * t * t : 0.693147181f * __builtin_amdgcn_logf(1.f + t);
+      return fmaxf(z, 0.f) + l * __builtin_amdgcn_rcpf(beta);
     }
     default: return z;
   }
@@ -45,7 +54,7 @@ __device__ __forceinline__ float act_slope(float z, int act, float beta) {
   switch (act) {
     case ACT_RELU: return z > 0.f ? 1.f : (z != z ? z : 0.f);
     case ACT_SILU: { const float s = sigmoid(z); return s + z * s * (1.f - s); }
-    case ACT_GELU: return 0.5f * (1.f + erff(z * 0.70710678f)) + z * 0.39894228f * __expf(-0.5f * z * z);
+    case ACT_GELU: { const float e = exp_(-0.5f * z * z); return normal_cdf(z, e) + z * 0.39894228f * e; }
     case ACT_SOFTPLUS: return sigmoid(beta * z);
     default: return 1.f;
   }
@@ -372,33 +381,100 @@ __global__ __launch_bounds__(256) void join_splits_kernel(const float* parts, in
   }
 }
 
-// gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every 64-row tile of it (before it is rounded)
-template <class T>
-__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, int M, int N, int ld, int act, float beta) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= ld) return;
-  const int m0 = blockIdx.y * 64, m1 = min(M, m0 + 64);
-  float s = 0.f;
-  for (int m = m0; m < m1; ++m) {
-    const int64_t at = int64_t(m) * N + n;
-    float v = 0.f;
-    if (n < N) {
-      v = float(g[at]);
-      if (z) v *= act_slope(float(z[at]), act, beta);
-      s += v;
+// gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every tile of rows of it (before it is rounded).  A
+// thread takes eight columns of eight rows; LPR threads a row, 256 / LPR rows side by side.
+constexpr int GZ_ROWS = 8;
+
+template <class T, int LPR>
+__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
+  constexpr int SIDE = 256 / LPR;
+  typedef typename Vec<T>::type vec;
+  __shared__ float part[256][9];
+  const int c = (blockIdx.x * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.y * (SIDE * GZ_ROWS) + threadIdx.x / LPR;
+  float s[8] = {};
+  if (c < ld) {
+#pragma unroll
+    for (int r = 0; r < GZ_ROWS; ++r) {
+      const int m = m0 + r * SIDE;
+      if (m >= M) continue;
+      const int64_t at = int64_t(m) * N + c;
+      float v[8] = {}, zz[8] = {};
+      if (c + 8 <= N) {
+        const vec x = *reinterpret_cast<const vec*>(g + at);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) v[e] = float(x[e]);
+        if (z) {
+          const vec y = *reinterpret_cast<const vec*>(z + at);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) zz[e] = float(y[e]);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (c + e < N) { v[e] = float(g[at + e]); if (z) zz[e] = float(z[at + e]); }
+      }
+      if (z) {
+#define NPHM_EACH(A) case A: _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] *= act_slope(zz[e], A, beta); break
+        switch (act) { NPHM_EACH(ACT_RELU); NPHM_EACH(ACT_SILU); NPHM_EACH(ACT_GELU); NPHM_EACH(ACT_SOFTPLUS); }
+#undef NPHM_EACH
+      }
+#pragma unroll
+      for (int e = 0; e < 8; ++e) s[e] += c + e < N ? v[e] : 0.f;
+      if (gz) {
+        vec o;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) o[e] = c + e < N ? T(v[e]) : T(0.f);
+        *reinterpret_cast<vec*>(gz + int64_t(m) * ld + c) = o;
+      }
     }
-    if (gz) gz[int64_t(m) * ld + n] = T(v);
   }
-  if (sums && n < N) sums[int64_t(blockIdx.y) * N + n] = s;
+  if (!sums) return;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) part[threadIdx.x][e] = s[e];
+  __syncthreads();
+  for (int u = threadIdx.x; u < LPR * 8; u += 256) {
+    const int n = blockIdx.x * LPR * 8 + u;
+    if (n >= N) continue;
+    float o = 0.f;
+#pragma unroll
+    for (int k = 0; k < SIDE; ++k) o += part[k * LPR + u / 8][u % 8];
+    if (gridDim.y == 1) dbias[n] = T(o);
+    else sums[int64_t(blockIdx.y) * N + n] = o;
+  }
 }
 
+// the tiles' sums, added up: 32 columns a block, eight threads a column
 template <class T>
 __global__ __launch_bounds__(256) void column_sums16_kernel(const float* sums, int tiles, int N, T* out) {
-  const int n = blockIdx.x * 256 + threadIdx.x;
-  if (n >= N) return;
+  __shared__ float part[8][32];
+  const int col = threadIdx.x & 31, k = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
   float s = 0.f;
-  for (int t = 0; t < tiles; ++t) s += sums[int64_t(t) * N + n];
+  if (n < N) {
+#pragma unroll 8
+    for (int t = k; t < tiles; t += 8) s += sums[int64_t(t) * N + n];
+  }
+  part[k][col] = s;
+  __syncthreads();
+  if (k || n >= N) return;
+#pragma unroll
+  for (int q = 1; q < 8; ++q) s += part[q][col];
   out[n] = T(s);
+}
+
+inline int gz_lanes(int64_t ldn) { return ldn <= 64 ? 8 : ldn <= 128 ? 16 : ldn <= 256 ? 32 : 64; }
+inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_lanes(ldn) * GZ_ROWS; return (M + rows - 1) / rows; }
+
+template <class T>
+inline void make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
+  const int lanes = gz_lanes(ld);
+  const int64_t tiles = gz_tiles(M, ld);
+  const dim3 grid(unsigned((ld + lanes * 8 - 1) / (lanes * 8)), unsigned(tiles));
+  float* s = dbias ? sums : nullptr;
+  if (lanes == 8) hipLaunchKernelGGL((gz_kernel<T, 8>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  else if (lanes == 16) hipLaunchKernelGGL((gz_kernel<T, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  else if (lanes == 32) hipLaunchKernelGGL((gz_kernel<T, 32>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  else hipLaunchKernelGGL((gz_kernel<T, 64>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  if (dbias && tiles > 1)
+    hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 31) / 32)), dim3(256), 0, st, sums, int(tiles), N, dbias);
 }
 
 inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
@@ -423,9 +499,8 @@ inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
   static_assert(LDS <= 160 * 1024, "two buffers of two tiles");
   const int64_t tiles = ((a.I + B - 1) / B) * int64_t((a.J + B - 1) / B) * a.splits;
   if constexpr (LDS > 65536) {
-    static hipError_t once = hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
-                                                 hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));
-    (void)once;
+    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
+                              hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));          // (a refusal shows at the launch)
   }
   hipLaunchKernelGGL((gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>), dim3(unsigned((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), LDS, st, a);
 }
@@ -466,19 +541,22 @@ inline int check_layer(const char* what, int64_t M, int64_t N, int64_t K, int dt
   return nphm_fail_msg(msg);
 }
 
+inline bool packed(const void* p, int64_t cols) { return cols % 8 || !aligned(p, 16); }     // rows that the tile loads do not take as they are
+
 struct Backward {
   Tiling w;
+  bool same;                                        // g as it stands is gz
   size_t gz, sums, x, weight, parts, total;         // byte offsets
 };
-// (room for packed copies is there even where none is made: whether one is needed depends on addresses)
-inline Backward backward_plan(int64_t M, int64_t N, int64_t K) {
+inline Backward backward_plan(const void* g, const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int act) {
   Backward p;
   p.w = tiling(N, K, M, true);
+  p.same = act == ACT_NONE && !packed(g, N);
   p.gz = 0;
-  p.sums = p.gz + up(size_t(M) * round8(N) * 2);
-  p.x = p.sums + up(size_t((M + 63) / 64) * N * 4);
-  p.weight = p.x + up(size_t(M) * round8(K) * 2);
-  p.parts = p.weight + up(size_t(N) * round8(K) * 2);
+  p.sums = p.gz + (p.same ? 0 : up(size_t(M) * round8(N) * 2));
+  p.x = p.sums + up(size_t(gz_tiles(M, round8(N))) * N * 4);
+  p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
+  p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
   p.total = p.parts + (p.w.splits > 1 ? up(size_t(p.w.splits) * N * K * 4) : 0);
   return p;
 }
@@ -490,15 +568,16 @@ using namespace nphm::train_ops;
 
 extern "C" {
 
-size_t nphm_layer16_forward_workspace_bytes(int64_t M, int64_t N, int64_t K) {
-  return up(size_t(M) * round8(K) * 2) + up(size_t(N) * round8(K) * 2);
+size_t nphm_layer16_forward_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K) {
+  return (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0) + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
 }
 
 int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,
                          int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_layer("nphm_layer16_forward", M, N, K, dtype, act, beta)) return rc;
-  if (!x || !weight || !y || !workspace) return nphm_fail_msg("nphm_layer16_forward: null pointer");
-  if (workspace_bytes < nphm_layer16_forward_workspace_bytes(M, N, K)) return nphm_fail_msg("nphm_layer16_forward: workspace too small");
+  if (!x || !weight || !y) return nphm_fail_msg("nphm_layer16_forward: null pointer");
+  const size_t need = nphm_layer16_forward_workspace_bytes(x, weight, M, N, K);
+  if (workspace_bytes < need || (need && !workspace)) return nphm_fail_msg("nphm_layer16_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   with_dtype(dtype, [&](auto t) {
@@ -507,12 +586,9 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       GemmArgs a{};
       a.A = x; a.lda = K;
       a.B = weight; a.ldb = K;
-      if (K % 8 || !aligned(x, 16)) { pack<T>(st, x, ws, M, K); a.A = ws; a.lda = round8(K); }
-      if (K % 8 || !aligned(weight, 16)) {
-        void* to = ws + up(size_t(M) * round8(K) * 2);
-        pack<T>(st, weight, to, N, K);
-        a.B = to; a.ldb = round8(K);
-      }
+      char* to = ws;
+      if (packed(x, K)) { pack<T>(st, x, to, M, K); a.A = to; a.lda = round8(K); to += up(size_t(M) * round8(K) * 2); }
+      if (packed(weight, K)) { pack<T>(st, weight, to, N, K); a.B = to; a.ldb = round8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
       a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
       a.wide = N % 8 == 0 && aligned(y, 16) && aligned(z, 16) && aligned(residual, 16);
@@ -524,13 +600,15 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
   return 0;
 }
 
-size_t nphm_layer16_backward_workspace_bytes(int64_t M, int64_t N, int64_t K, int act) { return backward_plan(M, N, K).total; }
+size_t nphm_layer16_backward_workspace_bytes(const void* g, const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int act) {
+  return backward_plan(g, x, weight, M, N, K, act).total;
+}
 
 int nphm_layer16_backward(const void* g, const void* x, const void* weight, const void* z, void* dx, void* dweight, void* dbias, int64_t M,
                           int64_t N, int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_layer("nphm_layer16_backward", M, N, K, dtype, act, beta)) return rc;
   if (!g || (act != ACT_NONE && !z) || (dx && !weight) || (dweight && !x) || !workspace) return nphm_fail_msg("nphm_layer16_backward: null pointer");
-  const Backward plan = backward_plan(M, N, K);
+  const Backward plan = backward_plan(g, x, weight, M, N, K, act);
   if (workspace_bytes < plan.total) return nphm_fail_msg("nphm_layer16_backward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
@@ -538,22 +616,15 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
     typedef decltype(t) T;
     if constexpr (sizeof(T) == 2) {
       const int64_t ldn = round8(N), ldk = round8(K);
-      float* sums = reinterpret_cast<float*>(ws + plan.sums);
-      const unsigned tiles = unsigned((M + 63) / 64);
-      const bool same = act == ACT_NONE && N % 8 == 0 && aligned(g, 16);       // g as it stands is gz
-      T* gz = same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
-      if (!same || dbias)
-        hipLaunchKernelGGL((gz_kernel<T>), dim3(unsigned((ldn + 255) / 256), tiles), dim3(256), 0, st, static_cast<const T*>(g),
-                           act == ACT_NONE ? nullptr : static_cast<const T*>(z), same ? nullptr : gz, dbias ? sums : nullptr, int(M), int(N),
-                           int(ldn), act, beta);
-      if (dbias)
-        hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 255) / 256)), dim3(256), 0, st, sums, int(tiles), int(N),
-                           static_cast<T*>(dbias));
+      T* gz = plan.same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
+      if (!plan.same || dbias)
+        make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
+                   reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta);
       if (dx) {
         GemmArgs a{};
         a.A = gz; a.lda = ldn;
         a.B = weight; a.ldb = K;
-        if (K % 8 || !aligned(weight, 16)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = ldk; }
+        if (packed(weight, K)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = ldk; }
         a.I = int(M); a.J = int(K); a.K = int(N);
         a.C = dx; a.wide = K % 8 == 0 && aligned(dx, 16);
         gemm<T, false, true, OUT_PLAIN>(st, a, tiling(M, K, N, false));
@@ -562,7 +633,7 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
         GemmArgs a{};
         a.A = gz; a.lda = ldn;
         a.B = x; a.ldb = K;
-        if (K % 8 || !aligned(x, 16)) { pack<T>(st, x, ws + plan.x, M, K); a.B = ws + plan.x; a.ldb = ldk; }
+        if (packed(x, K)) { pack<T>(st, x, ws + plan.x, M, K); a.B = ws + plan.x; a.ldb = ldk; }
         a.I = int(N); a.J = int(K); a.K = int(M);
         a.parts = reinterpret_cast<float*>(ws + plan.parts);
         a.C = dweight; a.wide = K % 8 == 0 && (plan.w.splits > 1 || aligned(dweight, 16));

@@ -141,41 +141,54 @@ struct SortArgs {
 __global__ __launch_bounds__(256) void keys_kernel(GradArgs p, SortArgs s, int key_blocks) {
   if (int(blockIdx.x) < key_blocks) {
     const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (n < (p.count + 63) / 64 * 64) s.keys[n] = n < p.count ? key_of(p, n) : 0x7fffffff;
+    if (n < (p.count + 63) / 64 * 64) s.keys[n] = n < p.count ? key_of(p, n) : 0x7ffffffe;
   } else {
     const int64_t step = int64_t(gridDim.x - key_blocks) * 256;
     for (int64_t i = int64_t(blockIdx.x - key_blocks) * 256 + threadIdx.x; i < p.rows; i += step) s.named[i] = 0;
   }
 }
 
-// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 64 keys, its four wavefronts count over a quarter of
-// all keys each (scalar loads: the counted key is the same for all lanes): count^2 comparisons, one launch.
-constexpr int MIDDLE = 8192;
+// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 64 keys; all keys are in LDS, and its sixteen wavefronts
+// count over a part of them each (a read of four keys is the same for all lanes): count^2 comparisons, one launch.
+constexpr int MIDDLE = 16384;
 
-__global__ __launch_bounds__(256) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
-                                                   uint8_t* __restrict__ named) {
-  __shared__ int part[4][64];
+__global__ __launch_bounds__(1024) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
+                                                    uint8_t* __restrict__ named) {
+  extern __shared__ __attribute__((aligned(16))) int all[];
+  __shared__ int part[16][64];
+  typedef int i32x4 __attribute__((ext_vector_type(4)));
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int i = blockIdx.x * 64 + lane, own = keys[i];
-  const int groups = (count + 63) / 64, quarter = (groups + 3) / 4;
+  const int groups = (count + 63) / 64;
+  for (int u = threadIdx.x; u < groups * 16; u += 1024) reinterpret_cast<i32x4*>(all)[u] = reinterpret_cast<const i32x4*>(keys)[u];
+  __syncthreads();
+  const int i = blockIdx.x * 64 + lane, own = all[i];
+  const int each = (groups + 15) / 16;
   int before = 0;
-  for (int g = wave * quarter; g < min(groups, (wave + 1) * quarter); ++g) {
-    const int* k = keys + g * 64;
-    if (g < int(blockIdx.x)) {
+  for (int g = wave * each; g < min(groups, (wave + 1) * each); ++g) {
+    const i32x4* k = reinterpret_cast<const i32x4*>(all + g * 64);
+    const int bound = g < int(blockIdx.x) ? own + 1 : own;           // an equal key in front counts
+    if (g != int(blockIdx.x)) {
 #pragma unroll
-      for (int u = 0; u < 64; ++u) before += k[u] <= own;
-    } else if (g > int(blockIdx.x)) {
+      for (int u = 0; u < 16; ++u) {
+        const i32x4 v = k[u];
 #pragma unroll
-      for (int u = 0; u < 64; ++u) before += k[u] < own;
+        for (int e = 0; e < 4; ++e) before += v[e] < bound;
+      }
     } else {
 #pragma unroll
-      for (int u = 0; u < 64; ++u) before += k[u] < own || (k[u] == own && u < lane);
+      for (int u = 0; u < 16; ++u) {
+        const i32x4 v = k[u];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) before += v[e] < own || (v[e] == own && 4 * u + e < lane);
+      }
     }
   }
   part[wave][lane] = before;
   __syncthreads();
   if (wave == 0 && i < count) {
-    const int at = part[0][lane] + part[1][lane] + part[2][lane] + part[3][lane];
+    int at = 0;
+#pragma unroll
+    for (int w = 0; w < 16; ++w) at += part[w][lane];
     sorted[at] = own;
     perm[at] = i;
     if (own < rows) named[own] = 1;
@@ -440,7 +453,10 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   const int64_t clear = (a.rows + 255) / 256;
   hipLaunchKernelGGL(keys_kernel, dim3(unsigned(key_blocks + (clear < 1024 ? clear : 1024))), dim3(256), 0, st, a, s, key_blocks);
   if (!g.passes) {
-    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + 63) / 64)), dim3(256), 0, st, s.keys, count, rows, s.sorted, s.perm, s.named);
+    const unsigned lds = unsigned((count + 63) / 64 * 64 * 4);
+    if (lds > 49152)
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&rank_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
+    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + 63) / 64)), dim3(1024), lds, st, s.keys, count, rows, s.sorted, s.perm, s.named);
   } else {
     // the passes go keys -> other -> ... -> sorted, whatever their number
     const int *kin = s.keys, *pin = nullptr;

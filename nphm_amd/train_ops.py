@@ -14,8 +14,8 @@ no PyTorch fallback, CPU tensors are refused.  Results are the same bits from ru
 graph, except where a line says that it waits for the device."""
 from __future__ import annotations
 
-import ctypes
 import math
+from array import array
 
 import torch
 import torch.nn as nn
@@ -26,87 +26,116 @@ _DTYPES = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 _ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "softplus": 4}
 
 
+_raw_stream = torch._C._cuda_getCurrentRawStream        # (torch.cuda.current_stream builds an object around it: 2 us a call)
+
+
 class _on:
-    """Launches go to the current stream of `device`, which need not be the current device."""
+    """Makes `device` the current one for the launches inside and yields the handle of its current stream (the tensors' device need not
+    be the current one)."""
 
     def __init__(self, device):
-        self.device = device
-        self.other = device.index is not None and device.index != torch.cuda.current_device()
+        self.index = device.index
 
     def __enter__(self):
-        if self.other:
-            self.before = torch.cuda.current_device()
-            torch.cuda.set_device(self.device)
-        return torch.cuda.current_stream(self.device).cuda_stream
+        self.before = torch.cuda.current_device()
+        if self.before != self.index:
+            torch.cuda.set_device(self.index)
+        return _raw_stream(self.index)
 
     def __exit__(self, *exc):
-        if self.other:
+        if self.before != self.index:
             torch.cuda.set_device(self.before)
 
 
-def _need(cond, msg, kind=ValueError):
-    if not cond:
-        raise kind(msg)
+def _workspace(nbytes, device):
+    """-> (tensor or None, its address or None)"""
+    if not nbytes:
+        return None, None
+    ws = torch.empty(nbytes, dtype=torch.uint8, device=device)
+    return ws, ws.data_ptr()
 
 
 def _on_gpu(what, t):
-    _need(isinstance(t, torch.Tensor) and t.is_cuda, f"{what}: a tensor on a ROCm device (these operators have no CPU form)", TypeError)
+    if not (isinstance(t, torch.Tensor) and t.is_cuda):
+        raise TypeError(f"{what}: a tensor on a ROCm device (these operators have no CPU form)")
 
 
 # ---- rows of a table ---------------------------------------------------------------------------------------------------------
 
-def _check_index(what, idx, device):
-    _need(isinstance(idx, torch.Tensor) and idx.dtype in (torch.int32, torch.int64), f"{what}: idx is an int32 or int64 tensor", TypeError)
-    _need(idx.device == device, f"{what}: idx is on {idx.device}, the rows on {device}")
+def _check_rows(what, rows, idx, scale):
+    """rows and indices that fit each other, on a ROCm device"""
+    _on_gpu(what, rows)
+    if rows.dtype not in _DTYPES:
+        raise TypeError(f"{what}: rows of fp32, bf16 or fp16, not {rows.dtype}")
+    if not isinstance(idx, torch.Tensor) or idx.dtype not in (torch.int64, torch.int32):
+        raise TypeError(f"{what}: idx is an int32 or int64 tensor")
+    if idx.device != rows.device:
+        raise ValueError(f"{what}: idx is on {idx.device}, the rows on {rows.device}")
+    if not math.isfinite(scale):
+        raise ValueError(f"{what}: scale {scale}")
+
+
+def _check_table(what, table):
+    if table.dim() != 2 or table.numel() == 0:
+        raise ValueError(f"{what}: a table [rows, width], not {tuple(table.shape)}")
 
 
 def _padding(what, padding_idx, rows):
     if padding_idx is None:
         return -1
-    _need(-rows <= padding_idx < rows, f"{what}: padding_idx {padding_idx} is no row of {rows}")
+    if not -rows <= padding_idx < rows:
+        raise ValueError(f"{what}: padding_idx {padding_idx} is no row of {rows}")
     return padding_idx % rows
 
 
 def _row_strided(t):
     """(t or a copy of it, elements between its rows): rows contiguous, at least a row apart"""
-    if t.shape[0] <= 1 or t.shape[1] == 0 or not (t.stride(1) == 1 or t.shape[1] == 1) or t.stride(0) < t.shape[1]:
+    if t.is_contiguous():
+        return t, t.shape[1]
+    if t.stride(1) != 1 or t.stride(0) < t.shape[1]:
         t = t.contiguous()
-        return t, max(t.shape[1], 1)
+        return t, t.shape[1]
     return t, t.stride(0)
 
 
 def _lookup(table, idx, scale):
-    rows, ld = _row_strided(table.detach())
-    i = idx.contiguous()
-    out = torch.empty(*idx.shape, table.shape[1], dtype=table.dtype, device=table.device)
+    rows, ld = _row_strided(table)
+    V, D = table.shape
+    i = idx if idx.is_contiguous() else idx.contiguous()
+    out = torch.empty((*idx.shape, D), dtype=table.dtype, device=table.device)
     with _on(table.device) as stream:
-        _lib.check(_lib.load().nphm_rows_lookup(rows.data_ptr(), rows.shape[0], rows.shape[1], ld, _DTYPES[table.dtype], i.data_ptr(),
-                                                8 * i.element_size(), i.numel(), scale, out.data_ptr(), stream), "nphm_rows_lookup")
+        rc = _lib.load().nphm_rows_lookup(rows.data_ptr(), V, D, ld, _DTYPES[table.dtype], i.data_ptr(), 64 if i.dtype == torch.int64 else 32,
+                                          i.numel(), scale, out.data_ptr(), stream)
+    if rc:
+        _lib.check(rc, "nphm_rows_lookup")
     return out
 
 
+@torch.no_grad()
 def lookup_rows_grad(grad, idx, num_rows, scale=1.0, padding_idx=None):
     """Gradient of ``lookup_rows`` w.r.t. its table of `num_rows` rows: [num_rows, D] of grad's type, ``scale`` times the sum of the rows
     of `grad` [*idx.shape, D] that name a row; zeros in rows that none names and in row `padding_idx`.  Sums are in fp32, in the
     order of the indices.  For programs that keep their own backward pass; autograd calls it by itself."""
     what = "lookup_rows_grad"
-    _on_gpu(what, grad)
-    _check_index(what, idx, grad.device)
-    _need(grad.dtype in _DTYPES, f"{what}: fp32, bf16 or fp16 rows, not {grad.dtype}", TypeError)
-    _need(grad.dim() >= 1 and grad.shape[:-1] == idx.shape, f"{what}: grad {tuple(grad.shape)} does not fit idx {tuple(idx.shape)}")
-    _need(num_rows >= 1 and grad.shape[-1] >= 1, f"{what}: an empty table")
-    _need(math.isfinite(scale), f"{what}: scale {scale}")
-    pad = _padding(what, padding_idx, num_rows)
+    _check_rows(what, grad, idx, scale)
+    if grad.dim() < 1 or grad.shape[:-1] != idx.shape:
+        raise ValueError(f"{what}: grad {tuple(grad.shape)} does not fit idx {tuple(idx.shape)}")
     D = grad.shape[-1]
-    g, ld = _row_strided(grad.detach().reshape(-1, D))
-    i = idx.contiguous()
-    out = torch.empty(num_rows, D, dtype=grad.dtype, device=grad.device)
+    if num_rows < 1 or D < 1:
+        raise ValueError(f"{what}: an empty table")
+    pad = _padding(what, padding_idx, num_rows)
+    g, ld = _row_strided(grad if grad.dim() == 2 else grad.reshape(-1, D))
+    i = idx if idx.is_contiguous() else idx.contiguous()
+    count, code = i.numel(), _DTYPES[grad.dtype]
+    out = torch.empty((num_rows, D), dtype=grad.dtype, device=grad.device)
     lib = _lib.load()
-    need = lib.nphm_rows_grad_workspace_bytes(num_rows, D, i.numel(), _DTYPES[grad.dtype])
+    need = lib.nphm_rows_grad_workspace_bytes(num_rows, D, count, code)
     with _on(grad.device) as stream:
-        ws = torch.empty(max(need, 1), dtype=torch.uint8, device=grad.device)
-        _lib.check(lib.nphm_rows_grad(g.data_ptr(), i.numel(), D, ld, _DTYPES[grad.dtype], i.data_ptr(), 8 * i.element_size(), num_rows, pad,
-                                      scale, out.data_ptr(), ws.data_ptr(), need, stream), "nphm_rows_grad")
+        ws, at = _workspace(need, grad.device)
+        rc = lib.nphm_rows_grad(g.data_ptr(), count, D, ld, code, i.data_ptr(), 64 if i.dtype == torch.int64 else 32, num_rows, pad, scale,
+                                out.data_ptr(), at, need, stream)
+    if rc:
+        _lib.check(rc, "nphm_rows_grad")
     return out
 
 
@@ -139,13 +168,11 @@ def lookup_rows(table, idx, scale=1.0, padding_idx=None, sparse=False):
     sparse one with an entry for every index.  Row `padding_idx` is read like any other and gets no gradient.  An index outside
     the table gives a row of NaN and adds nothing to the gradient (nothing on the host looks at the indices)."""
     what = "lookup_rows"
-    _on_gpu(what, table)
-    _check_index(what, idx, table.device)
-    _need(table.dtype in _DTYPES, f"{what}: a table of fp32, bf16 or fp16, not {table.dtype}", TypeError)
-    _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1, f"{what}: a table [rows, width], not {tuple(table.shape)}")
-    _need(math.isfinite(scale), f"{what}: scale {scale}")
-    _padding(what, padding_idx, table.shape[0])
-    if torch.is_grad_enabled() and table.requires_grad:
+    _check_rows(what, table, idx, scale)
+    _check_table(what, table)
+    if padding_idx is not None:
+        _padding(what, padding_idx, table.shape[0])
+    if table.requires_grad and torch.is_grad_enabled():
         return _LookupFn.apply(table, idx, float(scale), padding_idx, bool(sparse))
     return _lookup(table, idx, scale)
 
@@ -154,18 +181,20 @@ def renorm_rows_(table, idx, max_norm):
     """Rows of `table` that `idx` names and whose 2-norm is above `max_norm` are scaled down to it, in place, each once
     (nn.Embedding's max_norm, training.py:36-40)."""
     what = "renorm_rows_"
-    _on_gpu(what, table)
-    _check_index(what, idx, table.device)
-    _need(table.dtype in _DTYPES, f"{what}: a table of fp32, bf16 or fp16, not {table.dtype}", TypeError)
-    _need(table.dim() == 2 and table.shape[0] >= 1 and table.shape[1] >= 1 and (table.stride(1) == 1 or table.shape[1] == 1)
-          and (table.shape[0] == 1 or table.stride(0) >= table.shape[1]), f"{what}: a table [rows, width] with contiguous rows")
-    _need(max_norm >= 0, f"{what}: max_norm {max_norm}")
-    i = idx.contiguous()
+    _check_rows(what, table, idx, 1.0)
+    _check_table(what, table)
+    V, D = table.shape
+    if (D > 1 and table.stride(1) != 1) or (V > 1 and table.stride(0) < D):
+        raise ValueError(f"{what}: a table with contiguous rows")
+    if not max_norm >= 0:
+        raise ValueError(f"{what}: max_norm {max_norm}")
+    i = idx if idx.is_contiguous() else idx.contiguous()
     with _on(table.device) as stream:
-        flags = torch.empty(table.shape[0], dtype=torch.uint8, device=table.device)
-        _lib.check(_lib.load().nphm_rows_renorm(table.data_ptr(), table.shape[0], table.shape[1], max(table.stride(0), table.shape[1]),
-                                                _DTYPES[table.dtype], i.data_ptr(), 8 * i.element_size(), i.numel(), float(max_norm),
-                                                flags.data_ptr(), stream), "nphm_rows_renorm")
+        flags = torch.empty(V, dtype=torch.uint8, device=table.device)
+        rc = _lib.load().nphm_rows_renorm(table.data_ptr(), V, D, max(table.stride(0), D), _DTYPES[table.dtype], i.data_ptr(),
+                                          64 if i.dtype == torch.int64 else 32, i.numel(), float(max_norm), flags.data_ptr(), stream)
+    if rc:
+        _lib.check(rc, "nphm_rows_renorm")
     torch.autograd.graph.increment_version(table.detach())
     return table
 
@@ -177,7 +206,8 @@ class LatentCodes(nn.Embedding):
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, scale=1.0, sparse=False, device=None, dtype=None):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, max_norm=max_norm, sparse=sparse, device=device, dtype=dtype)
-        _need(math.isfinite(scale), f"LatentCodes: scale {scale}")
+        if not math.isfinite(scale):
+            raise ValueError(f"LatentCodes: scale {scale}")
         self.scale = float(scale)
         self.backend = "hip"            # "hip" | "composite"
 
@@ -192,56 +222,66 @@ class LatentCodes(nn.Embedding):
 
 # ---- dense layer in 16 bits --------------------------------------------------------------------------------------------------
 
-def _workspace(nbytes, device):
-    return torch.empty(max(int(nbytes), 1), dtype=torch.uint8, device=device)
+def _rows_of(t):
+    """t as contiguous rows [M, K]"""
+    t = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    return t if t.is_contiguous() else t.contiguous()
+
+
+def _layer_forward(x, weight, bias, residual, act, beta, keep):
+    """-> (y, z or None)"""
+    x2, w = _rows_of(x), weight if weight.is_contiguous() else weight.contiguous()
+    M, K = x2.shape
+    N = w.shape[0]
+    y = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
+    z = torch.empty((M, N), dtype=x.dtype, device=x.device) if keep and act else None
+    if M:
+        b = None if bias is None else bias.contiguous()
+        r = None if residual is None else residual.contiguous()
+        lib = _lib.load()
+        with _on(x.device) as stream:
+            need = lib.nphm_layer16_forward_workspace_bytes(x2.data_ptr(), w.data_ptr(), M, N, K)
+            ws, at = _workspace(need, x.device)
+            rc = lib.nphm_layer16_forward(x2.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(), None if r is None else r.data_ptr(),
+                                          y.data_ptr(), None if z is None else z.data_ptr(), M, N, K, _DTYPES[x.dtype], act, beta, at, need, stream)
+        if rc:
+            _lib.check(rc, "nphm_layer16_forward")
+    return y, z
 
 
 class _LinearActFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, x, weight, bias, residual, act, beta, keep):
-        lib = _lib.load()
-        x2, w = x.detach().reshape(-1, x.shape[-1]).contiguous(), weight.detach().contiguous()
-        M, K = x2.shape
-        N = w.shape[0]
-        y = torch.empty(*x.shape[:-1], N, dtype=x.dtype, device=x.device)
-        z = torch.empty(M, N, dtype=x.dtype, device=x.device) if keep and act else None
-        if M:
-            b = None if bias is None else bias.detach().contiguous()
-            r = None if residual is None else residual.detach().contiguous()
-            with _on(x.device) as stream:
-                need = lib.nphm_layer16_forward_workspace_bytes(M, N, K)
-                ws = _workspace(need, x.device)
-                _lib.check(lib.nphm_layer16_forward(x2.data_ptr(), w.data_ptr(), None if b is None else b.data_ptr(),
-                                                    None if r is None else r.data_ptr(), y.data_ptr(), None if z is None else z.data_ptr(),
-                                                    M, N, K, _DTYPES[x.dtype], act, beta, ws.data_ptr(), need, stream), "nphm_layer16_forward")
-        if keep:
-            ctx.save_for_backward(x, weight, z)
-            ctx.meta = (act, beta, bias is not None)
+    def forward(ctx, x, weight, bias, residual, act, beta):
+        y, z = _layer_forward(x, weight, bias, residual, act, beta, True)
+        ctx.save_for_backward(x, weight, z)
+        ctx.meta = (act, beta)
         return y
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, g):
-        lib = _lib.load()
         x, weight, z = ctx.saved_tensors
-        act, beta, _ = ctx.meta
-        x2, w = x.detach().reshape(-1, x.shape[-1]).contiguous(), weight.detach().contiguous()
+        act, beta = ctx.meta
+        x2, w = _rows_of(x), weight if weight.is_contiguous() else weight.contiguous()
         M, K = x2.shape
         N = w.shape[0]
         need_x, need_w, need_b, need_r = ctx.needs_input_grad[:4]
         new = torch.empty if M else torch.zeros
         dx = new(x.shape, dtype=x.dtype, device=x.device) if need_x else None
-        dw = new(N, K, dtype=x.dtype, device=x.device) if need_w else None
-        db = new(N, dtype=x.dtype, device=x.device) if need_b else None
+        dw = new((N, K), dtype=x.dtype, device=x.device) if need_w else None
+        db = new((N,), dtype=x.dtype, device=x.device) if need_b else None
         if M and (need_x or need_w or need_b):
-            g2 = g.reshape(M, N).contiguous()
+            g2 = _rows_of(g)
+            lib = _lib.load()
             with _on(x.device) as stream:
-                need = lib.nphm_layer16_backward_workspace_bytes(M, N, K, act)
-                ws = _workspace(need, x.device)
-                p = lambda t: None if t is None else t.data_ptr()  # noqa: E731
-                _lib.check(lib.nphm_layer16_backward(g2.data_ptr(), x2.data_ptr(), w.data_ptr(), p(z), p(dx), p(dw), p(db), M, N, K,
-                                                     _DTYPES[x.dtype], act, beta, ws.data_ptr(), need, stream), "nphm_layer16_backward")
-        return dx, dw, db, g if need_r else None, None, None, None
+                need = lib.nphm_layer16_backward_workspace_bytes(g2.data_ptr(), x2.data_ptr(), w.data_ptr(), M, N, K, act)
+                ws, at = _workspace(need, x.device)
+                rc = lib.nphm_layer16_backward(g2.data_ptr(), x2.data_ptr(), w.data_ptr(), None if z is None else z.data_ptr(),
+                                               None if dx is None else dx.data_ptr(), None if dw is None else dw.data_ptr(),
+                                               None if db is None else db.data_ptr(), M, N, K, _DTYPES[x.dtype], act, beta, at, need, stream)
+            if rc:
+                _lib.check(rc, "nphm_layer16_backward")
+        return dx, dw, db, g if need_r else None, None, None
 
 
 def linear_act(x, weight, bias=None, activation="none", beta=1.0, residual=None):
@@ -251,93 +291,123 @@ def linear_act(x, weight, bias=None, activation="none", beta=1.0, residual=None)
     kept in 16 bits for it.  No broadcasting: residual has the result's shape."""
     what = "linear_act"
     _on_gpu(what, x)
-    _need(x.dtype in (torch.bfloat16, torch.float16), f"{what}: bf16 or fp16 tensors, not {x.dtype}", TypeError)
-    _need(x.dim() >= 1 and weight.dim() == 2 and x.shape[-1] == weight.shape[1] and weight.shape[0] >= 1 and weight.shape[1] >= 1,
-          f"{what}: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
+    t, dev = x.dtype, x.device
+    if t not in (torch.bfloat16, torch.float16):
+        raise TypeError(f"{what}: bf16 or fp16 tensors, not {t}")
+    _on_gpu(what, weight)
+    if x.dim() < 1 or weight.dim() != 2 or x.shape[-1] != weight.shape[1] or weight.numel() == 0:
+        raise ValueError(f"{what}: x {tuple(x.shape)} does not fit weight {tuple(weight.shape)}")
     N = weight.shape[0]
-    _need(bias is None or tuple(bias.shape) == (N,), f"{what}: bias has the shape ({N},)")
-    _need(residual is None or tuple(residual.shape) == (*x.shape[:-1], N), f"{what}: residual has the shape of the result")
-    for t in (weight, bias, residual):
-        _need(t is None or (t.device == x.device and t.dtype == x.dtype), f"{what}: all tensors on one device, of one type", TypeError)
+    if bias is not None and bias.shape != (N,):
+        raise ValueError(f"{what}: bias has the shape ({N},)")
+    if residual is not None and residual.shape != (*x.shape[:-1], N):
+        raise ValueError(f"{what}: residual has the shape of the result")
+    grad = x.requires_grad
+    for o in (weight, bias, residual):
+        if o is not None:
+            if o.dtype != t or o.device != dev:
+                raise TypeError(f"{what}: all tensors on one device, of one type")
+            grad = grad or o.requires_grad
     act = _ACTIVATIONS.get("none" if activation is None else activation)
-    _need(act is not None, f"{what}: activation is one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
-    _need(act != 4 or (math.isfinite(beta) and beta > 0), f"{what}: Softplus takes a positive beta, not {beta}")
-    keep = torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, weight, bias, residual))
-    return _LinearActFn.apply(x, weight, bias, residual, act, float(beta), keep)
+    if act is None:
+        raise ValueError(f"{what}: activation is one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
+    if act == 4 and not (math.isfinite(beta) and beta > 0):
+        raise ValueError(f"{what}: Softplus takes a positive beta, not {beta}")
+    if grad and torch.is_grad_enabled():
+        return _LinearActFn.apply(x, weight, bias, residual, act, float(beta))
+    return _layer_forward(x, weight, bias, residual, act, float(beta), False)[0]
 
 
 # ---- global gradient norm ----------------------------------------------------------------------------------------------------
 
 def _kind(what, norm_type):
-    norm_type = float(norm_type)
-    _need(norm_type in (2.0, math.inf), f"{what}: norm_type is 2 or inf, not {norm_type}")
-    return 0 if norm_type == 2.0 else 1
+    if norm_type == 2:
+        return 0
+    if norm_type == math.inf:
+        return 1
+    raise ValueError(f"{what}: norm_type is 2 or inf, not {norm_type}")
 
 
-def _flat_order(t):
-    """the order of t's dimensions in memory if t fills its span of memory without gaps or repeats, else None"""
-    order = sorted((d for d in range(t.dim()) if t.shape[d] != 1), key=t.stride, reverse=True)
+def _limit(what, max_norm):
+    if not max_norm >= 0:
+        raise ValueError(f"{what}: max_norm {max_norm}")
+    return float(max_norm)
+
+
+def _gapless(t):
+    """whether t fills its span of memory without gaps or repeats, whatever the order of its dimensions"""
     want = 1
-    for d in reversed(order):
-        if t.stride(d) != want:
-            return None
-        want *= t.shape[d]
-    return order
+    for n, stride in sorted(((t.shape[d], t.stride(d)) for d in range(t.dim()) if t.shape[d] != 1), key=lambda v: v[1]):
+        if stride != want:
+            return False
+        want *= n
+    return True
 
 
+def _addresses(tensors):
+    return array("Q", [t.data_ptr() for t in tensors])
+
+
+@torch.no_grad()
 def _clip(what, grads, out, kind, limit):
-    """-> norm; out None: the norm alone"""
+    """-> norm; out None: the norm alone.  (A list may hold hundreds of tensors: each line here that looks at all of them costs 30 to 50 us,
+    so they are looked at by whole lists, and one by one only where something is to be said or done about one.)"""
+    for g in grads:
+        if not isinstance(g, torch.Tensor):
+            _on_gpu(what, g)
+    n = len(grads)
+    devices, types = {g.get_device() for g in grads}, [g.dtype for g in grads]
+    if len(devices) != 1 or -1 in devices:
+        for g in grads:
+            _on_gpu(what, g)
+        raise ValueError(f"{what}: gradients on {len(devices)} devices: one call takes one device's")
+    try:
+        codes = array("i", [_DTYPES[t] for t in types])
+    except KeyError as e:
+        raise TypeError(f"{what}: fp32, bf16 or fp16 gradients, not {e.args[0]}") from None
+    counts = array("q", [g.numel() for g in grads])
+    apart = out is not None and out is not grads
+    ins, outs, back = grads, out, []
+    if apart:
+        if (any(not isinstance(o, torch.Tensor) for o in out) or {o.get_device() for o in out} != devices or [o.dtype for o in out] != types
+                or [o.shape for o in out] != [g.shape for g in grads]):
+            raise ValueError(f"{what}: out has a tensor of the shape, type and device of each gradient")
+    if not all([g.is_contiguous() for g in grads]) or (apart and not all([o.is_contiguous() for o in out])):
+        ins, outs = list(grads), None if out is None else list(out)
+        for k, g in enumerate(grads):
+            o = g if out is None else out[k]
+            if (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _gapless(g)):
+                continue                                             # (any order of dimensions, the same on both sides)
+            ins[k] = g.contiguous()
+            if out is not None:
+                outs[k] = torch.empty_like(ins[k])
+                back.append((o, outs[k]))
+    p_in = _addresses(ins)
+    p_out = None if out is None else p_in if outs is ins else _addresses(outs)
     dev = grads[0].device
-    ins, outs, back = [], [], []
-    for k, g in enumerate(grads):
-        _on_gpu(what, g)
-        _need(g.dtype in _DTYPES, f"{what}: fp32, bf16 or fp16 gradients, not {g.dtype}", TypeError)
-        _need(g.device == dev, f"{what}: gradients on {dev} and {g.device}: one call takes one device's")
-        o = None if out is None else out[k]
-        if o is not None and o is not g:
-            _need(isinstance(o, torch.Tensor) and o.shape == g.shape and o.dtype == g.dtype and o.device == g.device,
-                  f"{what}: out has a tensor of the shape, type and device of each gradient")
-        if not g.is_contiguous() or (o is not None and o is not g and not o.is_contiguous()):
-            order = None if g.numel() == 0 else _flat_order(g)
-            if order is None or not (o is None or o is g or o.stride() == g.stride()):
-                g = g.contiguous()
-                if o is not None:
-                    o_flat = torch.empty_like(g)
-                    back.append((o, o_flat))
-                    o = o_flat
-        ins.append(g)
-        outs.append(o)
-    n = len(ins)
     lib = _lib.load()
-    counts = (ctypes.c_int64 * n)(*[g.numel() for g in ins])
-    dtypes = (ctypes.c_int * n)(*[_DTYPES[g.dtype] for g in ins])
-    p_in = (ctypes.c_void_p * n)(*[g.data_ptr() for g in ins])
-    p_out = None if out is None else (ctypes.c_void_p * n)(*[o.data_ptr() for o in outs])
+    at = lambda a: a.buffer_info()[0]  # noqa: E731
     with _on(dev) as stream:
-        need = lib.nphm_clip_workspace_bytes(counts, n)
-        ws = _workspace(need, dev)
+        need = lib.nphm_clip_workspace_bytes(at(counts), n)
+        ws, ws_at = _workspace(need, dev)
         norm = torch.empty((), dtype=torch.float32, device=dev)
-        _lib.check(lib.nphm_clip_grads(p_in, p_out, counts, dtypes, n, kind, limit, norm.data_ptr(), ws.data_ptr(), need, stream),
-                   "nphm_clip_grads")
-    for o, o_flat in back:
-        o.copy_(o_flat)
+        rc = lib.nphm_clip_grads(at(p_in), None if out is None else at(p_out), at(counts), at(codes), n, kind, limit, norm.data_ptr(), ws_at,
+                                 need, stream)
+    if rc:
+        _lib.check(rc, "nphm_clip_grads")
+    for o, flat in back:
+        o.copy_(flat)
     if out is not None:
-        torch.autograd.graph.increment_version([o for o in out])
+        torch.autograd.graph.increment_version(out)
     return norm
-
-
-def _detached(tensors):
-    return [t.detach() if isinstance(t, torch.Tensor) and t.requires_grad else t for t in tensors]
 
 
 def grad_norm(grads, norm_type=2.0):
     """The 2-norm (squares added in fp64) or, with norm_type = inf, the largest magnitude over all tensors of `grads` (dense; fp32, bf16,
     fp16, mixed): a 0-dim fp32 tensor on their device."""
     kind = _kind("grad_norm", norm_type)
-    grads = _detached(grads)
-    if not grads:
-        return torch.zeros(())
-    return _clip("grad_norm", grads, None, kind, 0.0)
+    grads = list(grads)
+    return _clip("grad_norm", grads, None, kind, 0.0) if grads else torch.zeros(())
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
@@ -345,16 +415,14 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     which none shares memory with another tensor of the call).  -> (norm, the scaled tensors).  As torch's clip: a norm that is
     no number makes every result NaN, an infinite one makes the finite entries 0."""
     what = "clip_grads"
-    kind = _kind(what, norm_type)
-    _need(max_norm >= 0, f"{what}: max_norm {max_norm}")
+    kind, limit = _kind(what, norm_type), _limit(what, max_norm)
     grads = list(grads)
     written = grads if out is None else list(out)
-    _need(len(written) == len(grads), f"{what}: {len(grads)} gradients, {len(written)} tensors in out")
+    if len(written) != len(grads):
+        raise ValueError(f"{what}: {len(grads)} gradients, {len(written)} tensors in out")
     if not grads:
         return torch.zeros(()), written
-    src = _detached(grads)
-    norm = _clip(what, src, src if out is None else _detached(written), kind, float(max_norm))
-    return norm, written
+    return _clip(what, grads, written, kind, limit), written
 
 
 def _merge_rows_(g):
@@ -367,36 +435,41 @@ def _merge_rows_(g):
     lib = _lib.load()
     need = lib.nphm_rows_grad_workspace_bytes(g.shape[0], flat.shape[1], flat.shape[0], _DTYPES[v.dtype])
     with _on(v.device) as stream:
-        ws = _workspace(need, v.device)
+        ws, at = _workspace(need, v.device)
         _lib.check(lib.nphm_rows_merge(flat.data_ptr(), flat.shape[0], flat.shape[1], _DTYPES[v.dtype], i.data_ptr(), 64, g.shape[0],
-                                       out.data_ptr(), ws.data_ptr(), need, stream), "nphm_rows_merge")
+                                       out.data_ptr(), at, need, stream), "nphm_rows_merge")
     v.copy_(out.view_as(v))
 
 
+@torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (training.py:128-131) with one norm over dense and row-sparse gradients: clips the ``.grad`` of `parameters`
     (a tensor or an iterable) in place and returns the norm before it (0-dim fp32).  Sparse gradients have one sparse dimension;
     entries that name the same row count as their sum.  ``error_if_nonfinite`` waits for the device and raises before
     anything is scaled."""
     what = "clip_grad_norm_"
-    kind = _kind(what, norm_type)
-    _need(max_norm >= 0, f"{what}: max_norm {max_norm}")
+    kind, limit = _kind(what, norm_type), _limit(what, max_norm)
     if isinstance(parameters, torch.Tensor):
         parameters = [parameters]
     grads = []
-    for g in [p.grad for p in parameters if p.grad is not None]:
+    for p in parameters:
+        g = p.grad
+        if g is None:
+            continue
         if g.is_sparse:
-            _need(g.sparse_dim() == 1, f"{what}: sparse gradients of whole rows (one sparse dimension)")
-            _need(g._values().is_cuda and g._values().dtype in _DTYPES, f"{what}: sparse fp32, bf16 or fp16 gradients on a ROCm device", TypeError)
+            if g.sparse_dim() != 1:
+                raise ValueError(f"{what}: sparse gradients of whole rows (one sparse dimension)")
+            v = g._values()
+            if not (v.is_cuda and v.dtype in _DTYPES):
+                raise TypeError(f"{what}: sparse fp32, bf16 or fp16 gradients on a ROCm device")
             if not g.is_coalesced():
-                _merge_rows_(g.detach())
-            g = g.detach()._values()
+                _merge_rows_(g)
+            g = v
         grads.append(g)
     if not grads:
         return torch.zeros(())
-    grads = _detached(grads)
     if error_if_nonfinite:
         norm = _clip(what, grads, None, kind, 0.0)
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"{what}: the norm of the gradients is {float(norm)}; none was scaled")
-    return _clip(what, grads, grads, kind, float(max_norm))
+    return _clip(what, grads, grads, kind, limit)
