@@ -148,47 +148,44 @@ __global__ __launch_bounds__(256) void keys_kernel(GradArgs p, SortArgs s, int k
   }
 }
 
-// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 64 keys; all keys are in LDS, and its sixteen wavefronts
-// count over a part of them each (a read of four keys is the same for all lanes): count^2 comparisons, one launch.
-constexpr int MIDDLE = 16384;
+// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 16 keys: all keys are in LDS, its four wavefronts count
+// over a quarter of them each and the four 16-lane rows of a wavefront over a quarter of that (a read of four keys is the same for 16
+// lanes).  count^2 comparisons spread over the chip, one launch: 8 us for 4097 keys against 19 for the radix passes below, which
+// are faster above 8192 (16384 keys: 57 us against 20).
+constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 16;              // keys a block places; ranges that all keys are cut into
 
-__global__ __launch_bounds__(1024) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
-                                                    uint8_t* __restrict__ named) {
+__global__ __launch_bounds__(256) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
+                                                   uint8_t* __restrict__ named) {
   extern __shared__ __attribute__((aligned(16))) int all[];
-  __shared__ int part[16][64];
+  __shared__ int part[RANGE][PLACED];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-  const int groups = (count + 63) / 64;
-  for (int u = threadIdx.x; u < groups * 16; u += 1024) reinterpret_cast<i32x4*>(all)[u] = reinterpret_cast<const i32x4*>(keys)[u];
-  __syncthreads();
-  const int i = blockIdx.x * 64 + lane, own = all[i];
-  const int each = (groups + 15) / 16;
-  int before = 0;
-  for (int g = wave * each; g < min(groups, (wave + 1) * each); ++g) {
-    const i32x4* k = reinterpret_cast<const i32x4*>(all + g * 64);
-    const int bound = g < int(blockIdx.x) ? own + 1 : own;           // an equal key in front counts
-    if (g != int(blockIdx.x)) {
-#pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const i32x4 v = k[u];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) before += v[e] < bound;
-      }
-    } else {
-#pragma unroll
-      for (int u = 0; u < 16; ++u) {
-        const i32x4 v = k[u];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) before += v[e] < own || (v[e] == own && 4 * u + e < lane);
-      }
-    }
+  const int padded = (count + 63) / 64 * 64, each = padded / RANGE, pitch = each + 4;      // (the ranges start in different banks)
+  for (int u = threadIdx.x; u < padded / 4; u += 256) {
+    const int at = u * 4;
+    *reinterpret_cast<i32x4*>(all + at / each * pitch + at % each) = reinterpret_cast<const i32x4*>(keys)[u];
   }
-  part[wave][lane] = before;
   __syncthreads();
-  if (wave == 0 && i < count) {
+  const int range = threadIdx.x / PLACED, own0 = blockIdx.x * PLACED, i = own0 + threadIdx.x % PLACED;
+  const int own = all[i / each * pitch + i % each];
+  const i32x4* k = reinterpret_cast<const i32x4*>(all + range * pitch);
+  int before = 0;
+  // an equal key in front counts: those before the block's own keys all do, those behind none, the block's own by their place
+#pragma unroll 8
+  for (int u = 0; u < each / 4; ++u) {
+    const i32x4 v = k[u];
+    const int bound = range * each + 4 * u < own0 ? own + 1 : own;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) before += v[e] < bound;
+  }
+  if (range == 0)
+#pragma unroll
+    for (int e = 0; e < PLACED; ++e) before += own0 + e < i && all[(own0 + e) / each * pitch + (own0 + e) % each] == own;
+  part[range][threadIdx.x % PLACED] = before;
+  __syncthreads();
+  if (threadIdx.x < PLACED && i < count) {
     int at = 0;
 #pragma unroll
-    for (int w = 0; w < 16; ++w) at += part[w][lane];
+    for (int w = 0; w < RANGE; ++w) at += part[w][threadIdx.x];
     sorted[at] = own;
     perm[at] = i;
     if (own < rows) named[own] = 1;
@@ -217,17 +214,28 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict
                                                            int* __restrict__ keys_out, int* __restrict__ perm_out) {
   __shared__ int base[1 << MAX_DIGIT], scan[1 << MAX_DIGIT], seen[16][1 << MAX_DIGIT];
   const int digits = 1 << s.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
-  if (t < digits) {
+  {
+    // 1024 / digits threads a digit, each over every so many blocks
+    const int d = t & (digits - 1), side = 1024 >> s.bits, k = t >> s.bits;
     int total = 0, before = 0;
-    for (int b = 0; b < s.blocks; ++b) {
-      const int h = s.hist[b * digits + t];
+#pragma unroll 8
+    for (int b = k; b < s.blocks; b += side) {
+      const int h = s.hist[b * digits + d];
       total += h;
       before += b < int(blockIdx.x) ? h : 0;
     }
-    base[t] = before;
-    scan[t] = total;
+    int* totals = &seen[0][0];                                       // [1024] and [1024] of its 8192
+    totals[t] = total;
+    totals[1024 + t] = before;
+    __syncthreads();
+    if (t < digits) {
+      total = before = 0;
+      for (int q = 0; q < side; ++q) total += totals[(q << s.bits) + t], before += totals[1024 + (q << s.bits) + t];
+      base[t] = before;
+      scan[t] = total;
+    }
+    __syncthreads();
   }
-  __syncthreads();
   for (int o = 1; o < digits; o <<= 1) {
     const int v = t < digits && t >= o ? scan[t - o] : 0;
     __syncthreads();
@@ -240,7 +248,7 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict
     const int64_t n = first + u + t;
     const bool in = n < count;
     const int key = in ? keys[n] : 0, d = (key >> s.shift) & (digits - 1);
-    for (int q = t; q < 16 * digits; q += 1024) seen[q / digits][q % digits] = 0;
+    for (int q = t; q < 16 * digits; q += 1024) seen[q >> s.bits][q & (digits - 1)] = 0;
     __syncthreads();
     uint64_t mates = __ballot(in);
     for (int b = 0; b < s.bits; ++b) {
@@ -351,10 +359,12 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   flush(p1 < p.count && s.sorted[p1] == key);
 }
 
+constexpr int JOINERS = 8;             // wavefronts that join a run
+
 template <class T, bool MERGE>
-__global__ __launch_bounds__(256) void join_kernel(GradArgs p, SumArgs s) {
+__global__ __launch_bounds__(64 * JOINERS) void join_kernel(GradArgs p, SumArgs s) {
   constexpr int V = Vec<T>::N;
-  __shared__ float part[3][64][V];
+  __shared__ float part[JOINERS - 1][64][V];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int chunk = blockIdx.x, c = (blockIdx.y * 64 + lane) * V;
   const int64_t p0 = int64_t(chunk) * s.chunk, p1 = min(p.count, p0 + s.chunk);
@@ -369,7 +379,7 @@ __global__ __launch_bounds__(256) void join_kernel(GradArgs p, SumArgs s) {
     last += run;
     if (run < 64) break;
   }
-  const int n = last - chunk, each = (n + 3) / 4, from = chunk + 1 + wave * each, to = min(last + 1, from + each);
+  const int n = last - chunk, each = (n + JOINERS - 1) / JOINERS, from = chunk + 1 + wave * each, to = min(last + 1, from + each);
   float acc[V] = {};
   auto add = [&](int64_t row) __attribute__((always_inline)) {
     const float* q = s.partial + row * s.pitch + c;
@@ -377,7 +387,7 @@ __global__ __launch_bounds__(256) void join_kernel(GradArgs p, SumArgs s) {
     for (int k = 0; k < V; ++k) acc[k] += q[k];
   };
   if (wave == 0) add(2 * int64_t(chunk) + 1);
-#pragma unroll 4
+#pragma unroll 8
   for (int k = from; k < to; ++k) add(2 * int64_t(k));
   if (wave) {
 #pragma unroll
@@ -386,7 +396,7 @@ __global__ __launch_bounds__(256) void join_kernel(GradArgs p, SumArgs s) {
   __syncthreads();
   if (wave) return;
 #pragma unroll
-  for (int w = 0; w < 3; ++w)
+  for (int w = 0; w < JOINERS - 1; ++w)
 #pragma unroll
     for (int k = 0; k < V; ++k) acc[k] += part[w][lane][k];
   int64_t row = key;
@@ -414,6 +424,8 @@ inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element)
   const int vec = 16 / element;
   g.tiles = int((dim + 64 * vec - 1) / (64 * vec));
   g.chunk = 8;
+  // the longest chunks (fewer cut runs) that still make 4096 wavefronts: 32768 rows of 2048 bf16 take 99 us in chunks of 64 (2048
+  // wavefronts), 71 in chunks of 32, 75 in chunks of 16
   while (g.chunk < 64 && count / (2 * g.chunk) * g.tiles >= 4096) g.chunk *= 2;
   g.chunks = int((count + g.chunk - 1) / g.chunk);
   const size_t ints = up(size_t((count + 63) / 64 * 64) * 4);
@@ -453,10 +465,10 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   const int64_t clear = (a.rows + 255) / 256;
   hipLaunchKernelGGL(keys_kernel, dim3(unsigned(key_blocks + (clear < 1024 ? clear : 1024))), dim3(256), 0, st, a, s, key_blocks);
   if (!g.passes) {
-    const unsigned lds = unsigned((count + 63) / 64 * 64 * 4);
+    const unsigned lds = unsigned((count + 63) / 64 * 64 * 4 + RANGE * 16);
     if (lds > 49152)
       (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&rank_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
-    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + 63) / 64)), dim3(1024), lds, st, s.keys, count, rows, s.sorted, s.perm, s.named);
+    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + PLACED - 1) / PLACED)), dim3(256), lds, st, s.keys, count, rows, s.sorted, s.perm, s.named);
   } else {
     // the passes go keys -> other -> ... -> sorted, whatever their number
     const int *kin = s.keys, *pin = nullptr;
@@ -487,7 +499,7 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   u.sum_blocks = int((int64_t(g.chunks) * g.tiles + 3) / 4);
   const int64_t zero = (out_rows + 15) / 16;
   hipLaunchKernelGGL((sum_kernel<T, MERGE>), dim3(unsigned(u.sum_blocks + (zero < 4096 ? zero : 4096))), dim3(256), 0, st, a, u);
-  hipLaunchKernelGGL((join_kernel<T, MERGE>), dim3(unsigned(g.chunks), tiles), dim3(256), 0, st, a, u);
+  hipLaunchKernelGGL((join_kernel<T, MERGE>), dim3(unsigned(g.chunks), tiles), dim3(64 * JOINERS), 0, st, a, u);
 }
 
 // max-norm: rows that an index names are flagged, then each flagged row is rescaled ONCE however often it is named
