@@ -7,7 +7,9 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
 #include <type_traits>
+#include <utility>
 
 #include "capi_common.h"
 #include "train_ops_common.h"
@@ -84,6 +86,7 @@ __device__ __forceinline__ T keep(float v) {
 }
 
 constexpr int BK = 64;                   // k a step: 128 bytes of a row
+constexpr int SLOTS = 5;                 // tiles of one operand in LDS or on their way: two steps and a half
 
 // One operand's tile of ROWS rows (its i or j) x 64 k, on its way from memory to LDS and from there into fragments.
 // Not transposed: memory holds k beside k.  LDS row r: 128 bytes, its eight 16-byte pieces c at place c ^ (r / 2 % 8), so that the lanes of a
@@ -116,7 +119,7 @@ struct Operand {
       lds[d] = __builtin_amdgcn_readfirstlane(lds0 + (d * WAVES + wave) * 1024);
     }
   }
-  // The 64 k from k0 (behind K: zeros, nothing is read): aim() once, then issue(d) for every instruction d, into the buffer `shift` bytes behind the first.
+  // The 64 k from k0 (behind K: zeros, nothing is read): aim() once, then issue(d) for every instruction d, into the slot `shift` bytes behind the first.
   v4i rsrc;
   unsigned soff;
   bool tail;
@@ -200,7 +203,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   typedef Operand<T, BM, WAVES, TA> OpA;
   typedef Operand<T, BN, WAVES, TB> OpB;
-  constexpr unsigned STEP = OpA::BYTES + OpB::BYTES;
+  constexpr unsigned SLOT = OpA::BYTES;
+  static_assert(OpA::BYTES == OpB::BYTES, "slots take tiles of either operand");
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   // Blocks go round the 8 XCDs: each XCD gets a run of consecutive tiles, 8 tiles of i to one of j, so that the 32 that it works on
@@ -217,7 +221,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   OpA a;
   OpB b;
   a.init(p.A, p.lda, i0, p.I, ke, wave, lane, lds0);
-  b.init(p.B, p.ldb, j0, p.J, ke, wave, lane, lds0 + OpA::BYTES);
+  b.init(p.B, p.ldb, j0, p.J, ke, wave, lane, lds0);
   Reader<TA, BM> ra;
   Reader<TB, BN> rb;
   ra.init((wave / WN) * TM * 32, lane);
@@ -233,8 +237,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   // stands in front of its last 16: behind it the first fragments of the next step are read and the loads of the one after it
   // start, each behind a product too (a wavefront issues in order: a burst of either would leave the matrix pipe idle).
   frag fa[2][TM], fb[2][TN];
-  auto read_one = [&](int set, const char* at, int ks, int n) __attribute__((always_inline)) {
-    if (n < TN) fb[set][n] = rb.template read<frag>(at + OpA::BYTES, n, ks);
+  auto read_one = [&](int set, const char* at, const char* bt, int ks, int n) __attribute__((always_inline)) {
+    if (n < TN) fb[set][n] = rb.template read<frag>(bt, n, ks);
     else if (n < TN + TM) fa[set][n - TN] = ra.template read<frag>(at, n - TN, ks);
   };
   auto multiply = [&](int set, auto&& behind) __attribute__((always_inline)) {
@@ -248,43 +252,53 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
         __builtin_amdgcn_sched_barrier(0);
       }
   };
-  constexpr int NMUL = TM * TN, NREAD = TM + TN, NDMA = OpA::DMA + OpB::DMA;
-  constexpr int RPM = (NREAD + NMUL - 1) / NMUL, DPM = (NDMA + NMUL - 1) / NMUL;       // reads, loads behind a product
-  auto load_one = [&](int d, unsigned to) __attribute__((always_inline)) {
-    if (d < OpA::DMA) a.issue(d, to, lane, wave);
-    else if (d < NDMA) b.issue(d - OpA::DMA, to, lane, wave);
-  };
-  a.aim(kb);
-  b.aim(kb);
+  constexpr int NMUL = TM * TN, NREAD = TM + TN;
+  constexpr int RPM = (NREAD + NMUL - 1) / NMUL;                      // reads behind a product
+  // LDS holds five tiles, A and B in turn: A of step t in slot 2 t, B in slot 2 t + 1 (modulo 5).  Step t loads A of step t + 2 into the slot
+  // that B of step t - 1 has left, spread over its first three quarters, and behind the barrier B of step t + 2 into A's own slot:
+  // the loads' rate is two thirds of what the path takes, in bursts it would hold up the products.
+  auto load_a = [&](int d, unsigned to) __attribute__((always_inline)) { a.issue(d, to, lane, wave); };
+  auto load_b = [&](int d, unsigned to) __attribute__((always_inline)) { b.issue(d, to, lane, wave); };
 #pragma unroll
-  for (int d = 0; d < NDMA; ++d) load_one(d, 0);
-  asm volatile("s_waitcnt vmcnt(0)\n\ts_barrier" ::: "memory");
-  a.aim(kb + BK);
-  b.aim(kb + BK);
+  for (int u = 0; u < 4; ++u) {
+    if (u & 1) {
+      b.aim(kb + u / 2 * BK);
 #pragma unroll
-  for (int d = 0; d < NDMA; ++d) load_one(d, STEP);
-  unsigned shift = 0;
+      for (int d = 0; d < OpB::DMA; ++d) load_b(d, u * SLOT);
+    } else {
+      a.aim(kb + u / 2 * BK);
 #pragma unroll
-  for (int n = 0; n < NREAD; ++n) read_one(0, lds, 0, n);
-  for (int k0 = kb; k0 < ke; k0 += BK, shift ^= STEP) {
-    const char* tile_at = lds + shift;
+      for (int d = 0; d < OpA::DMA; ++d) load_a(d, u * SLOT);
+    }
+  }
+  asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(OpA::DMA + OpB::DMA) : "memory");
+  unsigned sa = 0, sb = SLOT, sfree = 4 * SLOT;
+  auto two_on = [](unsigned slot) { const unsigned v = slot + 2 * SLOT; return v >= SLOTS * SLOT ? v - SLOTS * SLOT : v; };
+#pragma unroll
+  for (int n = 0; n < NREAD; ++n) read_one(0, lds + sa, lds + sb, 0, n);
+  for (int k0 = kb; k0 < ke; k0 += BK) {
+    a.aim(k0 + 2 * BK);
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks)
       multiply(ks & 1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-        for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one((ks + 1) & 1, tile_at, ks + 1, n);
+        for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one((ks + 1) & 1, lds + sa, lds + sb, ks + 1, n);
+#pragma unroll
+        for (int d = 0; d < OpA::DMA; ++d) if (d * 3 * NMUL / OpA::DMA == ks * NMUL + m) load_a(d, sfree);
       });
-    // the next step's tile has landed, every wavefront has read this one out
-    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-    const char* next_at = lds + (shift ^ STEP);
-    a.aim(k0 + 2 * BK);
+    // the next step's tiles have landed (the A behind them may still be on its way), every wavefront has read this step's out
+    asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(OpA::DMA) : "memory");
+    const unsigned na = two_on(sa), nb = two_on(sb);
     b.aim(k0 + 2 * BK);
     multiply(1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
-      for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one(0, next_at, 0, n);       // (behind the last step: zeros)
+      for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one(0, lds + na, lds + nb, 0, n);       // (behind the last step: zeros)
 #pragma unroll
-      for (int d = m * DPM; d < m * DPM + DPM; ++d) load_one(d, shift);
+      for (int d = 0; d < OpB::DMA; ++d) if (d * NMUL / OpB::DMA == m) load_b(d, sa);
     });
+    sfree = sb;
+    sa = na;
+    sb = nb;
   }
 
   // Register q of a lane: i = lane % 32, j = 8 (q / 4) + 4 (lane / 32) + q % 4 of its 32 x 32 tile.  Through LDS (every wavefront its own part
@@ -292,7 +306,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
   typedef T eight __attribute__((ext_vector_type(8)));
   constexpr int COLS = TN * 32, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
-  static_assert(WAVES * 32 * PITCH * 4 <= 2 * STEP, "the epilogue's rows fit the tiles' room");
+  static_assert(WAVES * 32 * PITCH * 4 <= SLOTS * SLOT, "the epilogue's rows fit the tiles' room");
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles, no load is on its way
   float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   const int j = j0 + (wave % WN) * COLS + (lane % LPR) * 8, width = min(8, p.J - j);
@@ -361,23 +375,70 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   }
 }
 
-// rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them
+// rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them; 16 lanes a row
 template <class T>
 __global__ __launch_bounds__(256) void pack_kernel(const T* src, T* dst, int64_t rows, int cols, int ld) {
-  const int64_t count = rows * ld;
-  for (int64_t u = int64_t(blockIdx.x) * 256 + threadIdx.x; u < count; u += int64_t(gridDim.x) * 256) {
-    const int64_t r = u / ld;
-    const int c = int(u - r * ld);
-    dst[u] = c < cols ? src[r * cols + c] : T(0.f);
+  typedef typename Vec<T>::type vec;
+  const int64_t r = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
+  if (r >= rows) return;
+  const T* s = src + r * cols;
+  T* d = dst + r * ld;
+  for (int c = (threadIdx.x % 16) * 8; c < ld; c += 128) {
+    vec v;
+    if (c + 8 <= cols) {
+      v = *reinterpret_cast<const vec*>(s + c);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? s[c + e] : T(0.f);
+    }
+    *reinterpret_cast<vec*>(d + c) = v;
   }
 }
 
-template <class T>
-__global__ __launch_bounds__(256) void join_splits_kernel(const float* parts, int splits, int64_t count, T* out) {
-  for (int64_t i = int64_t(blockIdx.x) * 256 + threadIdx.x; i < count; i += int64_t(gridDim.x) * 256) {
-    float s = 0.f;
-    for (int z = 0; z < splits; ++z) s += parts[int64_t(z) * count + i];
-    out[i] = T(s);
+// the partial products of all k ranges, added in order, and what the tiles' epilogue does otherwise; a thread takes eight elements beside
+// each other (J a multiple of 8) or one
+template <class T, int OUT, int W>
+__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) {
+  typedef float f32x4 __attribute__((ext_vector_type(4)));
+  typedef T eight __attribute__((ext_vector_type(W)));
+  const int64_t count = int64_t(p.I) * p.J;
+  for (int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W; at < count; at += int64_t(gridDim.x) * 256 * W) {
+    float v[W] = {};
+#pragma unroll 4
+    for (int s = 0; s < p.splits; ++s) {
+      const float* q = p.parts + int64_t(s) * count + at;
+      if constexpr (W == 8) {
+        const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
+      } else {
+        v[0] += *q;
+      }
+    }
+    if constexpr (OUT == OUT_LAYER) {
+      const int j = int(at % p.J);
+      if (p.bias) {
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += float(static_cast<const T*>(p.bias)[j + e]);
+      }
+      if (p.z) {
+        eight zz;
+#pragma unroll
+        for (int e = 0; e < W; ++e) zz[e] = keep<T>(v[e]);
+        *reinterpret_cast<eight*>(static_cast<T*>(p.z) + at) = zz;
+      }
+      if constexpr (W == 8) act_values(v, p.act, p.beta);
+      else v[0] = act_value(v[0], p.act, p.beta);
+      if (p.residual) {
+        const eight r = *reinterpret_cast<const eight*>(static_cast<const T*>(p.residual) + at);
+#pragma unroll
+        for (int e = 0; e < W; ++e) v[e] += float(r[e]);
+      }
+    }
+    eight o;
+#pragma unroll
+    for (int e = 0; e < W; ++e) o[e] = T(v[e]);
+    *reinterpret_cast<eight*>(static_cast<T*>(p.C) + at) = o;
   }
 }
 
@@ -460,6 +521,7 @@ __global__ __launch_bounds__(256) void column_sums16_kernel(const float* sums, i
   out[n] = T(s);
 }
 
+inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
 inline int gz_lanes(int64_t ldn) { return ldn <= 64 ? 8 : ldn <= 128 ? 16 : ldn <= 256 ? 32 : 64; }
 inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_lanes(ldn) * GZ_ROWS; return (M + rows - 1) / rows; }
 
@@ -477,26 +539,32 @@ inline void make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, 
     hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 31) / 32)), dim3(256), 0, st, sums, int(tiles), N, dbias);
 }
 
-inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
 inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 
 struct Tiling { int size, splits; };               // size: 256, 128 or 64
-// Whole tiles of 256 x 256 where there are enough to fill the 256 CUs, else smaller ones, and the k range in pieces.
-inline Tiling tiling(int64_t I, int64_t J, int64_t K, bool may_split) {
+// The largest tiles that still fill the 256 CUs: the larger, the less a product reads (16384 x 1024 x 1024: 36 us in tiles of 256, 43 of 128,
+// 67 of 64; 2048 x 2048 x 2048: 39 split in two, 24, 30).  Where none does, the k range in pieces, added by a second launch, if
+// there is enough of it: pieces of 1024 with tiles of 128 (1024 x 1024 x 16384: 46 us in four, 56 in tiles of 64), of 512 with tiles of 64
+// (1 x 4096 x 4096: 9.6 us in eight, 32 whole; 1024 x 1024 x 1024: 8.5 us whole, 14 in two).
+inline Tiling tiling(int64_t I, int64_t J, int64_t K) {
   auto tiles = [&](int64_t b) { return ((I + b - 1) / b) * ((J + b - 1) / b); };
   if (tiles(256) >= 192) return {256, 1};
-  if (!may_split) return {tiles(128) >= 192 ? 128 : 64, 1};
-  const int size = I >= 128 && J >= 128 ? 128 : 64;
-  int64_t s = (512 + tiles(size) - 1) / tiles(size);
-  if (s > K / 512) s = K / 512;
-  if (s > 64) s = 64;
-  return {size, int(s < 1 ? 1 : s)};
+  const int64_t t128 = tiles(128), t64 = tiles(64);
+  if (t128 >= 192) return {128, 1};
+  if (t64 >= 192) {
+    const int64_t s = (256 + t128 - 1) / t128;
+    return K >= 4096 && s * 1024 <= K ? Tiling{128, int(s)} : Tiling{64, 1};
+  }
+  if (K <= 1024) return {64, 1};
+  const int64_t fill = I <= 64 ? 512 : 256, s = std::min<int64_t>({(fill + t64 - 1) / t64, K / 512, 16});
+  return {64, int(std::max<int64_t>(s, 1))};
 }
+inline size_t parts_bytes(const Tiling& t, int64_t I, int64_t J) { return t.splits > 1 ? up(size_t(t.splits) * I * J * 4) : 0; }
 
 template <class T, int B, int WM, int WN, bool TA, bool TB, int OUT>
 inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
-  constexpr unsigned LDS = 2 * 2 * B * BK * 2;
-  static_assert(LDS <= 160 * 1024, "two buffers of two tiles");
+  constexpr unsigned LDS = SLOTS * B * BK * 2;
+  static_assert(LDS <= 160 * 1024, "the slots fit");
   const int64_t tiles = ((a.I + B - 1) / B) * int64_t((a.J + B - 1) / B) * a.splits;
   if constexpr (LDS > 65536) {
     (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
@@ -505,26 +573,33 @@ inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
   hipLaunchKernelGGL((gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>), dim3(unsigned((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), LDS, st, a);
 }
 
+// the product, with its k range in t.splits pieces where that is more than one: `a.parts` has room for parts_bytes
 template <class T, bool TA, bool TB, int OUT>
 inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
-  a.splits = t.splits;
   a.k_per_split = ((a.K + t.splits - 1) / t.splits + BK - 1) / BK * BK;
   a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
-  if (t.size == 256) launch_gemm<T, 256, 2, 4, TA, TB, OUT>(st, a);
-  else if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, OUT>(st, a);
-  else launch_gemm<T, 64, 2, 2, TA, TB, OUT>(st, a);
-  if constexpr (OUT == OUT_PARTS) {
-    const int64_t count = int64_t(a.I) * a.J, want = (count + 255) / 256;
-    hipLaunchKernelGGL((join_splits_kernel<T>), dim3(unsigned(want < 4096 ? want : 4096)), dim3(256), 0, st, a.parts, a.splits, count,
-                       static_cast<T*>(a.C));
-  }
+  auto launch = [&](auto out) {
+    constexpr int O = decltype(out)::value;
+    if (t.size == 256) launch_gemm<T, 256, 2, 4, TA, TB, O>(st, a);
+    else if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, O>(st, a);
+    else launch_gemm<T, 64, 2, 2, TA, TB, O>(st, a);
+  };
+  if (a.splits == 1) return launch(std::integral_constant<int, OUT>{});
+  GemmArgs part = a;
+  part.wide = a.J % 8 == 0;
+  std::swap(a, part);
+  launch(std::integral_constant<int, OUT_PARTS>{});
+  std::swap(a, part);
+  const int64_t count = int64_t(a.I) * a.J / (a.wide ? 8 : 1), want = (count + 255) / 256;
+  const dim3 grid(unsigned(want < 8192 ? want : 8192));
+  if (a.wide) hipLaunchKernelGGL((join_splits_kernel<T, OUT, 8>), grid, dim3(256), 0, st, a);
+  else hipLaunchKernelGGL((join_splits_kernel<T, OUT, 1>), grid, dim3(256), 0, st, a);
 }
 
 template <class T>
 inline void pack(hipStream_t st, const void* src, void* dst, int64_t rows, int64_t cols) {
-  const int64_t ld = round8(cols), want = (rows * ld + 255) / 256;
-  hipLaunchKernelGGL((pack_kernel<T>), dim3(unsigned(want < 8192 ? want : 8192)), dim3(256), 0, st, static_cast<const T*>(src),
-                     static_cast<T*>(dst), rows, int(cols), int(ld));
+  hipLaunchKernelGGL((pack_kernel<T>), dim3(unsigned((rows + 15) / 16)), dim3(256), 0, st, static_cast<const T*>(src), static_cast<T*>(dst),
+                     rows, int(cols), int(round8(cols)));
 }
 
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -543,21 +618,36 @@ inline int check_layer(const char* what, int64_t M, int64_t N, int64_t K, int dt
 
 inline bool packed(const void* p, int64_t cols) { return cols % 8 || !aligned(p, 16); }     // rows that the tile loads do not take as they are
 
+struct Forward {
+  Tiling t;
+  size_t x, weight, parts, total;
+};
+inline Forward forward_plan(const void* x, const void* weight, int64_t M, int64_t N, int64_t K) {
+  Forward p;
+  p.t = tiling(M, N, K);
+  p.x = 0;
+  p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
+  p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
+  p.total = p.parts + parts_bytes(p.t, M, N);
+  return p;
+}
+
 struct Backward {
-  Tiling w;
+  Tiling x_t, w_t;
   bool same;                                        // g as it stands is gz
   size_t gz, sums, x, weight, parts, total;         // byte offsets
 };
 inline Backward backward_plan(const void* g, const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int act) {
   Backward p;
-  p.w = tiling(N, K, M, true);
+  p.x_t = tiling(M, K, N);
+  p.w_t = tiling(N, K, M);
   p.same = act == ACT_NONE && !packed(g, N);
   p.gz = 0;
   p.sums = p.gz + (p.same ? 0 : up(size_t(M) * round8(N) * 2));
   p.x = p.sums + up(size_t(gz_tiles(M, round8(N))) * N * 4);
   p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
   p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
-  p.total = p.parts + (p.w.splits > 1 ? up(size_t(p.w.splits) * N * K * 4) : 0);
+  p.total = p.parts + std::max(parts_bytes(p.x_t, M, K), parts_bytes(p.w_t, N, K));     // (one product after the other)
   return p;
 }
 
@@ -569,15 +659,15 @@ using namespace nphm::train_ops;
 extern "C" {
 
 size_t nphm_layer16_forward_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K) {
-  return (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0) + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
+  return forward_plan(x, weight, M, N, K).total;
 }
 
 int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,
                          int64_t K, int dtype, int act, float beta, void* workspace, size_t workspace_bytes, void* stream) {
   if (int rc = check_layer("nphm_layer16_forward", M, N, K, dtype, act, beta)) return rc;
   if (!x || !weight || !y) return nphm_fail_msg("nphm_layer16_forward: null pointer");
-  const size_t need = nphm_layer16_forward_workspace_bytes(x, weight, M, N, K);
-  if (workspace_bytes < need || (need && !workspace)) return nphm_fail_msg("nphm_layer16_forward: workspace too small");
+  const Forward plan = forward_plan(x, weight, M, N, K);
+  if (workspace_bytes < plan.total || (plan.total && !workspace)) return nphm_fail_msg("nphm_layer16_forward: workspace too small");
   hipStream_t st = static_cast<hipStream_t>(stream);
   char* ws = static_cast<char*>(workspace);
   with_dtype(dtype, [&](auto t) {
@@ -586,13 +676,13 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       GemmArgs a{};
       a.A = x; a.lda = K;
       a.B = weight; a.ldb = K;
-      char* to = ws;
-      if (packed(x, K)) { pack<T>(st, x, to, M, K); a.A = to; a.lda = round8(K); to += up(size_t(M) * round8(K) * 2); }
-      if (packed(weight, K)) { pack<T>(st, weight, to, N, K); a.B = to; a.ldb = round8(K); }
+      if (packed(x, K)) { pack<T>(st, x, ws + plan.x, M, K); a.A = ws + plan.x; a.lda = round8(K); }
+      if (packed(weight, K)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = round8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
       a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
       a.wide = N % 8 == 0 && aligned(y, 16) && aligned(z, 16) && aligned(residual, 16);
-      gemm<T, false, false, OUT_LAYER>(st, a, tiling(M, N, K, false));
+      a.parts = reinterpret_cast<float*>(ws + plan.parts);
+      gemm<T, false, false, OUT_LAYER>(st, a, plan.t);
     }
   });
   hipError_t e = hipGetLastError();
@@ -627,7 +717,8 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
         if (packed(weight, K)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = ldk; }
         a.I = int(M); a.J = int(K); a.K = int(N);
         a.C = dx; a.wide = K % 8 == 0 && aligned(dx, 16);
-        gemm<T, false, true, OUT_PLAIN>(st, a, tiling(M, K, N, false));
+        a.parts = reinterpret_cast<float*>(ws + plan.parts);
+        gemm<T, false, true, OUT_PLAIN>(st, a, plan.x_t);
       }
       if (dweight) {
         GemmArgs a{};
@@ -636,9 +727,8 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
         if (packed(x, K)) { pack<T>(st, x, ws + plan.x, M, K); a.B = ws + plan.x; a.ldb = ldk; }
         a.I = int(N); a.J = int(K); a.K = int(M);
         a.parts = reinterpret_cast<float*>(ws + plan.parts);
-        a.C = dweight; a.wide = K % 8 == 0 && (plan.w.splits > 1 || aligned(dweight, 16));
-        if (plan.w.splits > 1) gemm<T, true, true, OUT_PARTS>(st, a, plan.w);
-        else gemm<T, true, true, OUT_PLAIN>(st, a, plan.w);
+        a.C = dweight; a.wide = K % 8 == 0 && aligned(dweight, 16);
+        gemm<T, true, true, OUT_PLAIN>(st, a, plan.w_t);
       }
     }
   });
