@@ -199,7 +199,7 @@ struct Range { uintptr_t begin, end; };
 inline bool before(const Range& x, const Range& y) { return x.begin < y.begin; }
 // whether two written ranges meet, or a read one meets a written one (a tensor clipped in place is among the written ones only)
 inline bool meet(std::vector<Range>& written, std::vector<Range>& read) {
-  std::sort(written.begin(), written.end(), before);
+  if (!std::is_sorted(written.begin(), written.end(), before)) std::sort(written.begin(), written.end(), before);
   for (size_t i = 1; i < written.size(); ++i)
     if (written[i].begin < written[i - 1].end) return true;
   for (const Range& r : read) {

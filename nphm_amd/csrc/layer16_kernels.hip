@@ -8,6 +8,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <atomic>
 #include <type_traits>
 #include <utility>
 
@@ -375,14 +376,21 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   }
 }
 
-// rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them; 16 lanes a row
+// rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them; 16 lanes a row; one or two operands
+struct Pack {
+  const void* src;
+  void* dst;
+  int64_t rows;
+};
+
 template <class T>
-__global__ __launch_bounds__(256) void pack_kernel(const T* src, T* dst, int64_t rows, int cols, int ld) {
+__global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned blocks, int cols, int ld) {
   typedef typename Vec<T>::type vec;
-  const int64_t r = int64_t(blockIdx.x) * 16 + threadIdx.x / 16;
-  if (r >= rows) return;
-  const T* s = src + r * cols;
-  T* d = dst + r * ld;
+  if (blockIdx.x >= blocks) p = q;
+  const int64_t r = int64_t(blockIdx.x >= blocks ? blockIdx.x - blocks : blockIdx.x) * 16 + threadIdx.x / 16;
+  if (r >= p.rows) return;
+  const T* s = static_cast<const T*>(p.src) + r * cols;
+  T* d = static_cast<T*>(p.dst) + r * ld;
   for (int c = (threadIdx.x % 16) * 8; c < ld; c += 128) {
     vec v;
     if (c + 8 <= cols) {
@@ -567,8 +575,15 @@ inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
   static_assert(LDS <= 160 * 1024, "the slots fit");
   const int64_t tiles = ((a.I + B - 1) / B) * int64_t((a.J + B - 1) / B) * a.splits;
   if constexpr (LDS > 65536) {
-    (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
-                              hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));          // (a refusal shows at the launch)
+    static std::atomic<uint64_t> told{0};                            // devices that know of it, by their numbers (a refusal shows at the launch)
+    int dev = 0;
+    (void)hipGetDevice(&dev);
+    const uint64_t bit = uint64_t(1) << (dev & 63);
+    if (!(told.load(std::memory_order_relaxed) & bit)) {
+      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
+                                hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));
+      told.fetch_or(bit, std::memory_order_relaxed);
+    }
   }
   hipLaunchKernelGGL((gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>), dim3(unsigned((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), LDS, st, a);
 }
@@ -596,10 +611,13 @@ inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
   else hipLaunchKernelGGL((join_splits_kernel<T, OUT, 1>), grid, dim3(256), 0, st, a);
 }
 
+// packs p, q or both (rows 0: not)
 template <class T>
-inline void pack(hipStream_t st, const void* src, void* dst, int64_t rows, int64_t cols) {
-  hipLaunchKernelGGL((pack_kernel<T>), dim3(unsigned((rows + 15) / 16)), dim3(256), 0, st, static_cast<const T*>(src), static_cast<T*>(dst),
-                     rows, int(cols), int(round8(cols)));
+inline void pack(hipStream_t st, Pack p, Pack q, int64_t cols) {
+  if (!p.rows) std::swap(p, q);
+  if (!p.rows) return;
+  const unsigned a = unsigned((p.rows + 15) / 16), b = unsigned((q.rows + 15) / 16);
+  hipLaunchKernelGGL((pack_kernel<T>), dim3(a + b), dim3(256), 0, st, p, q, a, int(cols), int(round8(cols)));
 }
 
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
@@ -676,8 +694,10 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       GemmArgs a{};
       a.A = x; a.lda = K;
       a.B = weight; a.ldb = K;
-      if (packed(x, K)) { pack<T>(st, x, ws + plan.x, M, K); a.A = ws + plan.x; a.lda = round8(K); }
-      if (packed(weight, K)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = round8(K); }
+      const bool px = packed(x, K), pw = packed(weight, K);
+      pack<T>(st, Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
+      if (px) { a.A = ws + plan.x; a.lda = round8(K); }
+      if (pw) { a.B = ws + plan.weight; a.ldb = round8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
       a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
       a.wide = N % 8 == 0 && aligned(y, 16) && aligned(z, 16) && aligned(residual, 16);
@@ -710,11 +730,13 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
       if (!plan.same || dbias)
         make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
                    reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta);
+      const bool px = dweight && packed(x, K), pw = dx && packed(weight, K);
+      pack<T>(st, Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
       if (dx) {
         GemmArgs a{};
         a.A = gz; a.lda = ldn;
         a.B = weight; a.ldb = K;
-        if (packed(weight, K)) { pack<T>(st, weight, ws + plan.weight, N, K); a.B = ws + plan.weight; a.ldb = ldk; }
+        if (pw) { a.B = ws + plan.weight; a.ldb = ldk; }
         a.I = int(M); a.J = int(K); a.K = int(N);
         a.C = dx; a.wide = K % 8 == 0 && aligned(dx, 16);
         a.parts = reinterpret_cast<float*>(ws + plan.parts);
@@ -724,7 +746,7 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
         GemmArgs a{};
         a.A = gz; a.lda = ldn;
         a.B = x; a.ldb = K;
-        if (packed(x, K)) { pack<T>(st, x, ws + plan.x, M, K); a.B = ws + plan.x; a.ldb = ldk; }
+        if (px) { a.B = ws + plan.x; a.ldb = ldk; }
         a.I = int(N); a.J = int(K); a.K = int(M);
         a.parts = reinterpret_cast<float*>(ws + plan.parts);
         a.C = dweight; a.wide = K % 8 == 0 && aligned(dweight, 16);

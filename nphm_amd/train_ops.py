@@ -16,6 +16,7 @@ from __future__ import annotations
 
 import math
 from array import array
+from operator import attrgetter
 
 import torch
 import torch.nn as nn
@@ -344,46 +345,49 @@ def _gapless(t):
     return True
 
 
-def _addresses(tensors):
-    return array("Q", [t.data_ptr() for t in tensors])
+_Tensor = torch.Tensor
+_dtype_of = attrgetter("dtype")
 
 
 @torch.no_grad()
 def _clip(what, grads, out, kind, limit):
-    """-> norm; out None: the norm alone.  (A list may hold hundreds of tensors: each line here that looks at all of them costs 30 to 50 us,
-    so they are looked at by whole lists, and one by one only where something is to be said or done about one.)"""
-    for g in grads:
-        if not isinstance(g, torch.Tensor):
-            _on_gpu(what, g)
+    """-> norm; out None: the norm alone.  (A list may hold hundreds of tensors, and a look at each of them costs 0.1 us a question: they are
+    asked as few as will do, by maps, and one by one only where something is to be said or done about one.)"""
+    apart = out is not None and out is not grads
+    for tensors in (grads, out) if apart else (grads,):
+        if not set(map(type, tensors)) <= {_Tensor, nn.Parameter}:
+            for t in tensors:
+                _on_gpu(what, t)
     n = len(grads)
-    devices, types = {g.get_device() for g in grads}, [g.dtype for g in grads]
+    devices, types = set(map(_Tensor.get_device, grads)), set(map(_dtype_of, grads))
     if len(devices) != 1 or -1 in devices:
         for g in grads:
             _on_gpu(what, g)
         raise ValueError(f"{what}: gradients on {len(devices)} devices: one call takes one device's")
-    try:
-        codes = array("i", [_DTYPES[t] for t in types])
-    except KeyError as e:
-        raise TypeError(f"{what}: fp32, bf16 or fp16 gradients, not {e.args[0]}") from None
-    counts = array("q", [g.numel() for g in grads])
-    apart = out is not None and out is not grads
-    ins, outs, back = grads, out, []
+    if not types <= _DTYPES.keys():
+        raise TypeError(f"{what}: fp32, bf16 or fp16 gradients, not {', '.join(map(str, types - _DTYPES.keys()))}")
+    one = len(types) == 1
+    codes = array("i", [_DTYPES[types.pop()]]) * n if one else array("i", [_DTYPES[t] for t in map(_dtype_of, grads)])
+    counts = array("q", map(_Tensor.numel, grads))
+    plain = all(map(_Tensor.is_contiguous, grads))
     if apart:
-        if (any(not isinstance(o, torch.Tensor) for o in out) or {o.get_device() for o in out} != devices or [o.dtype for o in out] != types
-                or [o.shape for o in out] != [g.shape for g in grads]):
-            raise ValueError(f"{what}: out has a tensor of the shape, type and device of each gradient")
-    if not all([g.is_contiguous() for g in grads]) or (apart and not all([o.is_contiguous() for o in out])):
+        if (array("q", map(_Tensor.numel, out)) != counts or set(map(_Tensor.get_device, out)) != devices
+                or (set(map(_dtype_of, out)) != {grads[0].dtype} if one else list(map(_dtype_of, out)) != list(map(_dtype_of, grads)))):
+            raise ValueError(f"{what}: out has a tensor of the size, type and device of each gradient")
+        plain = plain and all(map(_Tensor.is_contiguous, out))
+    ins, outs, back = grads, out, []
+    if not plain:
         ins, outs = list(grads), None if out is None else list(out)
         for k, g in enumerate(grads):
             o = g if out is None else out[k]
-            if (g.is_contiguous() and o.is_contiguous()) or (g.stride() == o.stride() and _gapless(g)):
+            if (g.is_contiguous() and o.is_contiguous()) or (g.shape == o.shape and g.stride() == o.stride() and _gapless(g)):
                 continue                                             # (any order of dimensions, the same on both sides)
             ins[k] = g.contiguous()
             if out is not None:
                 outs[k] = torch.empty_like(ins[k])
                 back.append((o, outs[k]))
-    p_in = _addresses(ins)
-    p_out = None if out is None else p_in if outs is ins else _addresses(outs)
+    p_in = array("Q", map(_Tensor.data_ptr, ins))
+    p_out = None if out is None else p_in if outs is ins else array("Q", map(_Tensor.data_ptr, outs))
     dev = grads[0].device
     lib = _lib.load()
     at = lambda a: a.buffer_info()[0]  # noqa: E731
@@ -396,7 +400,7 @@ def _clip(what, grads, out, kind, limit):
     if rc:
         _lib.check(rc, "nphm_clip_grads")
     for o, flat in back:
-        o.copy_(flat)
+        o.copy_(flat.view(o.shape))
     if out is not None:
         torch.autograd.graph.increment_version(out)
     return norm
@@ -411,8 +415,8 @@ def grad_norm(grads, norm_type=2.0):
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
-    """Scales the dense tensors of `grads` by min(1, max_norm / (norm + 1e-6)), in place, or into the tensors `out` (same shapes and types, of
-    which none shares memory with another tensor of the call).  -> (norm, the scaled tensors).  As torch's clip: a norm that is
+    """Scales the dense tensors of `grads` by min(1, max_norm / (norm + 1e-6)), in place, or into the tensors `out` (of the same sizes and types,
+    in row-major order: pieces of a flat buffer will do; none shares memory with another tensor of the call).  -> (norm, the scaled tensors).  As torch's clip: a norm that is
     no number makes every result NaN, an infinite one makes the finite entries 0."""
     what = "clip_grads"
     kind, limit = _kind(what, norm_type), _limit(what, max_norm)
