@@ -466,8 +466,6 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   hipLaunchKernelGGL(keys_kernel, dim3(unsigned(key_blocks + (clear < 1024 ? clear : 1024))), dim3(256), 0, st, a, s, key_blocks);
   if (!g.passes) {
     const unsigned lds = unsigned((count + 63) / 64 * 64 * 4 + RANGE * 16);
-    if (lds > 49152)
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&rank_kernel), hipFuncAttributeMaxDynamicSharedMemorySize, int(lds));
     hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + PLACED - 1) / PLACED)), dim3(256), lds, st, s.keys, count, rows, s.sorted, s.perm, s.named);
   } else {
     // the passes go keys -> other -> ... -> sorted, whatever their number

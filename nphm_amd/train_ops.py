@@ -121,7 +121,7 @@ def lookup_rows_grad(grad, idx, num_rows, scale=1.0, padding_idx=None):
     _check_rows(what, grad, idx, scale)
     if grad.dim() < 1 or grad.shape[:-1] != idx.shape:
         raise ValueError(f"{what}: grad {tuple(grad.shape)} does not fit idx {tuple(idx.shape)}")
-    D = grad.shape[-1]
+    D, scale = grad.shape[-1], float(scale)
     if num_rows < 1 or D < 1:
         raise ValueError(f"{what}: an empty table")
     pad = _padding(what, padding_idx, num_rows)
@@ -175,7 +175,7 @@ def lookup_rows(table, idx, scale=1.0, padding_idx=None, sparse=False):
         _padding(what, padding_idx, table.shape[0])
     if table.requires_grad and torch.is_grad_enabled():
         return _LookupFn.apply(table, idx, float(scale), padding_idx, bool(sparse))
-    return _lookup(table, idx, scale)
+    return _lookup(table, idx, float(scale))
 
 
 def renorm_rows_(table, idx, max_norm):
