@@ -98,34 +98,38 @@ constexpr int SLOTS = 5;                 // tiles of one operand in LDS or on th
 // Pieces behind the operand's end have an offset behind the buffer's: they arrive as zeros.
 template <class T, int ROWS, int WAVES, bool TR>
 struct Operand {
-  static constexpr int BYTES = ROWS * BK * 2, DMA = BYTES / 1024 / WAVES, CPR = TR ? ROWS / 8 : 8;
+  static constexpr int BYTES = ROWS * BK * 2, DMA = BYTES / 1024 / WAVES, CPR = TR ? ROWS / 8 : BK / 8;
   static_assert(BYTES % (1024 * WAVES) == 0, "whole DMA instructions a wavefront");
   static constexpr unsigned NOWHERE = 0x80000000u;                   // behind every buffer (each is below 2^31 bytes)
   const char* base;
   int64_t ld;
   int rows, K;                                                       // valid rows from the tile's first
-  unsigned voff[DMA], lds[DMA];
+  unsigned voff[DMA];
+  unsigned lds0;                                                     // this wavefront's first KiB of a slot
+  v4i rsrc;
+  unsigned soff;
 
-  __device__ __forceinline__ void init(const void* P, int64_t ld_, int r0, int I, int K_, int wave, int lane, unsigned lds0) {
+  // the piece of a row (not transposed) or the piece and row (transposed) that lane `lane` takes in instruction d
+  __device__ __forceinline__ static int row_of(int d, int wave, int lane) { return ((d * WAVES + wave) * 64 + lane) / CPR; }
+  __device__ __forceinline__ static int piece_of(int d, int wave, int lane) {
+    const int row = row_of(d, wave, lane), at = lane % CPR;
+    return TR ? at ^ ((row & 3) << 1) : at ^ ((row >> 1) & 7);
+  }
+  __device__ __forceinline__ void init(const void* P, int64_t ld_, int r0, int I, int K_, int wave, int lane, unsigned lds_first) {
     ld = ld_;
     K = K_;
     rows = min(ROWS, I - r0);
     base = static_cast<const char*>(P) + (TR ? int64_t(r0) * 2 : int64_t(r0) * ld * 2);
+    lds0 = __builtin_amdgcn_readfirstlane(lds_first + wave * 1024);
 #pragma unroll
     for (int d = 0; d < DMA; ++d) {
-      const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, at = piece % CPR;
-      const int c = TR ? at ^ ((row & 3) << 1) : at ^ ((row >> 1) & 7);
-      voff[d] = unsigned(row * int(ld) * 2 + c * 16);
-      if (TR && c * 8 >= rows) voff[d] = NOWHERE;
-      lds[d] = __builtin_amdgcn_readfirstlane(lds0 + (d * WAVES + wave) * 1024);
+      const int c = piece_of(d, wave, lane);
+      voff[d] = TR && c * 8 >= rows ? NOWHERE : unsigned(row_of(d, wave, lane) * int(ld) * 2 + c * 16);
     }
   }
-  // The 64 k from k0 (behind K: zeros, nothing is read): aim() once, then issue(d) for every instruction d, into the slot `shift` bytes behind the first.
-  v4i rsrc;
-  unsigned soff;
-  bool tail;
-  int k_at;
-  __device__ __forceinline__ void aim(int k0) {
+  // The 64 k from k0 (behind K: zeros, nothing is read), in ascending order of k0: aim() once, then issue(d) for every instruction d, into the
+  // slot `shift` bytes behind the first.
+  __device__ __forceinline__ void aim(int k0, int lane, int wave) {
     const char* p = TR ? base + int64_t(k0) * ld * 2 : base;
     const unsigned bytes = k0 >= K ? 0u : (TR ? unsigned(min(BK, K - k0)) : unsigned(rows)) * unsigned(ld * 2);
     rsrc[0] = __builtin_amdgcn_readfirstlane(int(uint32_t(uintptr_t(p))));
@@ -133,19 +137,27 @@ struct Operand {
     rsrc[2] = __builtin_amdgcn_readfirstlane(int(bytes));
     rsrc[3] = 0x00020000;
     soff = __builtin_amdgcn_readfirstlane(TR ? 0 : k0 * 2);
-    tail = !TR && k0 + BK > K;
-    k_at = k0;
-  }
-  __device__ __forceinline__ void issue(int d, unsigned shift, int lane, int wave) const {
-    unsigned v = voff[d];
-    if constexpr (!TR) {
-      const int piece = (d * WAVES + wave) * 64 + lane, row = piece / CPR, c = (piece % CPR) ^ ((row >> 1) & 7);
-      v = tail && k_at + c * 8 >= K ? NOWHERE : v;
+    if (!TR && k0 < K && k0 + BK > K) {                              // the last, cut step: pieces behind K are nowhere from here on
+#pragma unroll
+      for (int d = 0; d < DMA; ++d) if (k0 + piece_of(d, wave, lane) * 8 >= K) voff[d] = NOWHERE;
     }
-    const unsigned dst = __builtin_amdgcn_readfirstlane(lds[d] + shift);
-    asm volatile("s_mov_b32 m0, %2\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(v), "s"(rsrc), "s"(dst), "s"(soff) : "memory", "m0");
+  }
+  template <int D>
+  __device__ __forceinline__ void issue(unsigned shift) const {
+    const unsigned to = __builtin_amdgcn_readfirstlane(lds0 + shift);
+    asm volatile("s_add_u32 m0, %2, %4\n\ts_nop 0\n\tbuffer_load_dwordx4 %0, %1, %3 offen lds" ::"v"(voff[D]), "s"(rsrc), "s"(to), "s"(soff),
+                 "n"(D * WAVES * 1024)
+                 : "memory", "m0", "scc");
   }
 };
+
+template <int N, class F>
+__device__ __forceinline__ void each(F&& f) {
+  if constexpr (N > 0) {
+    each<N - 1>(f);
+    f(std::integral_constant<int, N - 1>{});
+  }
+}
 
 template <bool TR, int ROWS>
 struct Reader {
@@ -258,18 +270,14 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   // LDS holds five tiles, A and B in turn: A of step t in slot 2 t, B in slot 2 t + 1 (modulo 5).  Step t loads A of step t + 2 into the slot
   // that B of step t - 1 has left, spread over its first three quarters, and behind the barrier B of step t + 2 into A's own slot:
   // the loads' rate is two thirds of what the path takes, in bursts it would hold up the products.
-  auto load_a = [&](int d, unsigned to) __attribute__((always_inline)) { a.issue(d, to, lane, wave); };
-  auto load_b = [&](int d, unsigned to) __attribute__((always_inline)) { b.issue(d, to, lane, wave); };
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
     if (u & 1) {
-      b.aim(kb + u / 2 * BK);
-#pragma unroll
-      for (int d = 0; d < OpB::DMA; ++d) load_b(d, u * SLOT);
+      b.aim(kb + u / 2 * BK, lane, wave);
+      each<OpB::DMA>([&](auto d) __attribute__((always_inline)) { b.template issue<decltype(d)::value>(u * SLOT); });
     } else {
-      a.aim(kb + u / 2 * BK);
-#pragma unroll
-      for (int d = 0; d < OpA::DMA; ++d) load_a(d, u * SLOT);
+      a.aim(kb + u / 2 * BK, lane, wave);
+      each<OpA::DMA>([&](auto d) __attribute__((always_inline)) { a.template issue<decltype(d)::value>(u * SLOT); });
     }
   }
   asm volatile("s_waitcnt vmcnt(%0)\n\ts_barrier" ::"i"(OpA::DMA + OpB::DMA) : "memory");
@@ -278,24 +286,26 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
 #pragma unroll
   for (int n = 0; n < NREAD; ++n) read_one(0, lds + sa, lds + sb, 0, n);
   for (int k0 = kb; k0 < ke; k0 += BK) {
-    a.aim(k0 + 2 * BK);
+    a.aim(k0 + 2 * BK, lane, wave);
 #pragma unroll
     for (int ks = 0; ks < 3; ++ks)
       multiply(ks & 1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
         for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one((ks + 1) & 1, lds + sa, lds + sb, ks + 1, n);
-#pragma unroll
-        for (int d = 0; d < OpA::DMA; ++d) if (d * 3 * NMUL / OpA::DMA == ks * NMUL + m) load_a(d, sfree);
+        each<OpA::DMA>([&](auto d) __attribute__((always_inline)) {
+          if (decltype(d)::value * 3 * NMUL / OpA::DMA == ks * NMUL + m) a.template issue<decltype(d)::value>(sfree);
+        });
       });
     // the next step's tiles have landed (the A behind them may still be on its way), every wavefront has read this step's out
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(OpA::DMA) : "memory");
     const unsigned na = two_on(sa), nb = two_on(sb);
-    b.aim(k0 + 2 * BK);
+    b.aim(k0 + 2 * BK, lane, wave);
     multiply(1, [&](int m) __attribute__((always_inline)) {
 #pragma unroll
       for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one(0, lds + na, lds + nb, 0, n);       // (behind the last step: zeros)
-#pragma unroll
-      for (int d = 0; d < OpB::DMA; ++d) if (d * NMUL / OpB::DMA == m) load_b(d, sa);
+      each<OpB::DMA>([&](auto d) __attribute__((always_inline)) {
+        if (decltype(d)::value * NMUL / OpB::DMA == m) b.template issue<decltype(d)::value>(sa);
+      });
     });
     sfree = sb;
     sa = na;
