@@ -469,7 +469,7 @@ __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, 
   constexpr int SIDE = 256 / LPR;
   typedef typename Vec<T>::type vec;
   __shared__ float part[256][9];
-  const int c = (blockIdx.x * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.y * (SIDE * GZ_ROWS) + threadIdx.x / LPR;
+  const int c = (blockIdx.y * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.x * (SIDE * GZ_ROWS) + threadIdx.x / LPR;
   float s[8] = {};
   if (c < ld) {
 #pragma unroll
@@ -511,13 +511,13 @@ __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, 
   for (int e = 0; e < 8; ++e) part[threadIdx.x][e] = s[e];
   __syncthreads();
   for (int u = threadIdx.x; u < LPR * 8; u += 256) {
-    const int n = blockIdx.x * LPR * 8 + u;
+    const int n = blockIdx.y * LPR * 8 + u;
     if (n >= N) continue;
     float o = 0.f;
 #pragma unroll
     for (int k = 0; k < SIDE; ++k) o += part[k * LPR + u / 8][u % 8];
-    if (gridDim.y == 1) dbias[n] = T(o);
-    else sums[int64_t(blockIdx.y) * N + n] = o;
+    if (gridDim.x == 1) dbias[n] = T(o);
+    else sums[int64_t(blockIdx.x) * N + n] = o;
   }
 }
 
@@ -547,7 +547,7 @@ template <class T>
 inline void make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
   const int lanes = gz_lanes(ld);
   const int64_t tiles = gz_tiles(M, ld);
-  const dim3 grid(unsigned((ld + lanes * 8 - 1) / (lanes * 8)), unsigned(tiles));
+  const dim3 grid(unsigned(tiles), unsigned((ld + lanes * 8 - 1) / (lanes * 8)));
   float* s = dbias ? sums : nullptr;
   if (lanes == 8) hipLaunchKernelGGL((gz_kernel<T, 8>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
   else if (lanes == 16) hipLaunchKernelGGL((gz_kernel<T, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);

@@ -56,6 +56,14 @@ def _workspace(nbytes, device):
     return ws, ws.data_ptr()
 
 
+def _written(tensors):
+    """tells autograd that the tensors were written (inference tensors keep no version)"""
+    try:
+        torch.autograd.graph.increment_version(tensors)
+    except RuntimeError:
+        torch.autograd.graph.increment_version([t for t in tensors if not t.is_inference()])
+
+
 def _on_gpu(what, t):
     if not (isinstance(t, torch.Tensor) and t.is_cuda):
         raise TypeError(f"{what}: a tensor on a ROCm device (these operators have no CPU form)")
@@ -196,7 +204,7 @@ def renorm_rows_(table, idx, max_norm):
                                           64 if i.dtype == torch.int64 else 32, i.numel(), float(max_norm), flags.data_ptr(), stream)
     if rc:
         _lib.check(rc, "nphm_rows_renorm")
-    torch.autograd.graph.increment_version(table.detach())
+    _written([table.detach()])
     return table
 
 
@@ -402,7 +410,7 @@ def _clip(what, grads, out, kind, limit):
     for o, flat in back:
         o.copy_(flat.view(o.shape))
     if out is not None:
-        torch.autograd.graph.increment_version(out)
+        _written(out)
     return norm
 
 

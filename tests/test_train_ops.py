@@ -9,6 +9,7 @@ import numpy as np
 import pytest
 import torch
 
+import _util as U
 from nphm_amd import train_ops as T
 from nphm_amd._lib import NphmAmdError
 from nphm_amd.deepsdf import DeepSDF, _DenseLayerFn
@@ -199,6 +200,26 @@ def test_row_gradients_do_not_overflow_in_sums(dev):
     g[5] = math.nan
     assert bool(T.lookup_rows_grad(g, torch.zeros(2000, dtype=torch.long, device=dev), 2)[0].isnan().all())
     assert not T.lookup_rows_grad(g, torch.zeros(2000, dtype=torch.long, device=dev), 2, padding_idx=0).any()      # NaN in a padded place
+
+
+@gpu
+def test_row_offsets_behind_32_bits(dev):
+    """a table of 1.2e9 values (4.9 GB): rows at its end, and a gradient of its size"""
+    V, D = 1200001, 1024
+    table = torch.empty(V, D, device=dev)
+    idx = torch.tensor([V - 1, 0, V - 1, 1048576, V - 2, 524288, 2097151 % V], device=dev).repeat(60)
+    table[idx] = torch.randn(len(idx), D, device=dev)
+    assert torch.equal(T.lookup_rows(table, idx), table[idx])
+    g = torch.randn(len(idx), D, device=dev)
+    for n in (7, len(idx)):
+        got = T.lookup_rows_grad(g[:n], idx[:n], V)
+        want = torch.zeros(V, D, device=dev, dtype=torch.float64).index_put_((idx[:n],), g[:n].double(), accumulate=True)
+        named = torch.unique(idx[:n])
+        within(got[named], want[named], want[named].abs() * F32 + n * F32 * g[:n].abs().max().double() * n / 3)
+        assert int((got != 0).any(1).sum()) == len(named)
+        del got, want
+    T.renorm_rows_(table, idx, 1.0)
+    assert float(table[idx].norm(dim=1).max()) <= 1 + 1e-6
 
 
 @gpu
@@ -414,6 +435,102 @@ def test_layer_special_values(dev):
 
 
 @gpu
+def test_layer_gradients_asked_one_by_one(dev):
+    """whatever subset of the four gradients is asked for, each has the same bits"""
+    x, w, b, r, g = layer_inputs(dev, torch.bfloat16, 200, 72, 130, True, True)
+    full = [v.clone().requires_grad_() for v in (x, w, b, r)]
+    T.linear_act(*full[:3], "silu", residual=full[3]).backward(g)
+    for mask in range(1, 16):
+        leaves = [v.clone().requires_grad_(bool(mask >> k & 1)) for k, v in enumerate((x, w, b, r))]
+        T.linear_act(*leaves[:3], "silu", residual=leaves[3]).backward(g)
+        for k, (leaf, ref) in enumerate(zip(leaves, full)):
+            assert (leaf.grad is None) == (not mask >> k & 1)
+            assert leaf.grad is None or torch.equal(leaf.grad, ref.grad)
+
+
+@gpu
+def test_saved_tensors_that_change_are_noticed(dev):
+    x, w, b, _, g = layer_inputs(dev, torch.bfloat16, 20, 16, 24, True, False)
+    w.requires_grad_()
+    y = T.linear_act(x, w, b, "gelu")
+    x.zero_()
+    with pytest.raises(RuntimeError):
+        y.backward(g)
+    table, idx = torch.randn(5, 8, device=dev, requires_grad=True), torch.tensor([1, 2], device=dev)
+    rows = T.lookup_rows(table, idx)
+    idx.add_(1)
+    with pytest.raises(RuntimeError):
+        rows.sum().backward()
+
+
+@gpu
+def test_inference_mode(dev):
+    with torch.inference_mode():
+        x, w, b, r, _ = layer_inputs(dev, torch.bfloat16, 20, 16, 24, True, True)
+        g = [torch.randn(100, device=dev), torch.randn(7, device=dev)]
+        table, idx = torch.randn(5, 8, device=dev), torch.tensor([1, 2], device=dev)
+        assert T.linear_act(x, w, b, "gelu", residual=r).shape == (20, 16)
+        T.clip_grads(g, 0.1)
+        assert abs(float(T.grad_norm(g)) - 0.1) <= 1e-6
+        T.renorm_rows_(table, idx, 0.5)
+        assert float(T.lookup_rows(table, idx).norm(dim=1).max()) <= 0.5 * (1 + 4 * F32)
+
+
+@gpu
+def test_layer_offsets_behind_32_bits(dev):
+    """a result of 2.3e9 values (4.6 GB) and its gradients: spot checks in the last rows against 64 bits, and the whole-sum gradients"""
+    t, M, N, K = torch.bfloat16, 70000, 32768, 64
+    x, w, b, _, _ = layer_inputs(dev, t, M, N, K, True, False)
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    y = T.linear_act(*leaves, "relu")
+    at = torch.tensor([0, 1, 40000, 65536, M - 2, M - 1], device=dev)
+    xd, wd, bd = x.detach().double(), w.detach().double(), b.detach().double()
+    z = xd[at] @ wd.t() + bd
+    ez = (K + 4) * 2 * F32 * (xd[at].abs() @ wd.abs().t() + bd.abs())
+    within(y.detach()[at], z.clamp(min=0), ez + half_step(t) * (z.abs() + ez) + tiny(t))
+    go = torch.zeros(M, N, dtype=t, device=dev)
+    go[at] = torch.randn(len(at), N, device=dev).to(t)
+    y.backward(go)
+    live = (z > 0) & (z.abs() > ez)
+    edge = (z.abs() <= ez).double() * go[at].double().abs()
+    gz = go[at].double() * live
+    # e: what a gradient is off before it is rounded (an entry whose z lies within its own error of 0 counts on one side and not on the other);
+    # the rounding is then one of |gradient| + e, not of |gradient|: 1.002 of the bound was seen without it, at an entry with |ref| 0.05, e 2.09
+    h = half_step(t)
+
+    def bound(ref, e):
+        return e + h * (ref.abs() + e) + tiny(t)
+    ref = gz @ wd
+    within(x.grad[at], ref, bound(ref, edge @ wd.abs() + (N + 4) * 2 * F32 * (gz.abs() @ wd.abs())))
+    rest = torch.ones(M, dtype=torch.bool, device=dev)
+    rest[at] = False
+    assert not x.grad[rest].any()
+    ref = gz.t() @ xd[at]
+    within(w.grad, ref, bound(ref, edge.t() @ xd[at].abs() + 16 * F32 * (gz.abs().t() @ xd[at].abs())))
+    within(b.grad, gz.sum(0), bound(gz.sum(0), edge.sum(0) + 16 * F32 * gz.abs().sum(0)))
+
+
+@gpu
+def test_layer_with_more_rows_than_a_grid_axis(dev):
+    """2^21 + 3 rows: more tiles of rows than one axis of a launch may have blocks"""
+    t, M, N, K = torch.float16, (1 << 21) + 3, 8, 8
+    x, w, b, _, g = layer_inputs(dev, t, M, N, K, True, False)
+    leaves = [v.requires_grad_() for v in (x, w, b)]
+    y = T.linear_act(*leaves, "silu")
+    y.backward(g)
+    z = x.detach().double() @ w.detach().double().t() + b.detach().double()
+    a, slope = act64(z, "silu", 1.0)
+    gz = g.double() * slope
+    want = gz.sum(0)
+    # fp32 sums over M entries in tiles: at most tile height + tiles adds follow one another, 2^14 here
+    dz = g.double().abs() * (0.55 * half_step(t) + 2.0 ** -19 + 0.5 * 24 * F32 * (1 + z.abs()))
+    within(b.grad, want, dz.sum(0) + 2 ** 14 * F32 * gz.abs().sum(0) + half_step(t) * want.abs())
+    within(y.detach()[-5:], a[-5:], half_step(t) * a[-5:].abs() + 1e-5)
+    within(x.grad[-5:], gz[-5:] @ w.detach().double(), (dz[-5:] + half_step(t) * gz[-5:].abs()) @ w.detach().double().abs() * 1.01
+           + half_step(t) * (gz[-5:] @ w.detach().double()).abs() + tiny(t))
+
+
+@gpu
 @pytest.mark.parametrize("t", ["bf16", "fp16"])
 def test_decoder_trains_with_16_bit_hidden_layers(dev, t):
     """DeepSDF.train_precision: the same bits as the layers called one by one, and the fp32 tier untouched by it"""
@@ -546,6 +663,20 @@ def test_norm_of_huge_and_tiny_gradients(dev):
 
 
 @gpu
+def test_clip_of_a_tensor_behind_32_bits(dev):
+    """2^31 + 13 bf16 values: more than one piece of the launch's table"""
+    n = (1 << 31) + 13
+    g = torch.empty(n, dtype=torch.bfloat16, device=dev).normal_()
+    total = math.sqrt(math.fsum(float(c.double().square().sum()) for c in g.split(1 << 27)))
+    out = torch.zeros_like(g)
+    norm, _ = T.clip_grads([g[:5], g[5:]], 3.0, out=[out[:5], out[5:]])
+    assert abs(float(norm) - total) <= total * 1.01 * F32
+    f = 3.0 / (total + 1e-6)
+    for a, b in zip(g.split(1 << 27), out.split(1 << 27)):
+        within(b, a.double() * f, clip_bound(a.double() * f, torch.bfloat16))
+
+
+@gpu
 def test_clip_sparse_and_dense_gradients_together(dev):
     """rows that an index names twice count as their sum, on both kinds of sparse tensors; the gradient stays the same tensor in dense form"""
     for coalesced in (False, True):
@@ -642,6 +773,45 @@ def test_a_step_of_all_operators(dev, sparse):
         f = 0.05 / (total + 1e-6)
         assert float((own - g * f).norm()) <= 2 * room * float((g * f).norm())
     assert abs(float(T.grad_norm([p.grad.coalesce().values() if p.grad.is_sparse else p.grad for p in (codes.weight, *layers)])) - 0.05) <= 0.05 * 2.0 ** -9
+
+
+@gpu
+def test_training_script_with_the_operators(dev):
+    """training.py's step (compute_loss, backward, two clips, AdamW + SparseAdam) with LatentCodes and clip_grad_norm_ in place of nn.Embedding and
+    torch's clip, which takes no sparse gradient: losses of the same first step, and a code gradient of the same norm"""
+    from nphm_amd.loss_functions import compute_loss
+    decoder = U.build_identity(device=dev).train()
+    gen = torch.Generator().manual_seed(11)
+    B, box = 4, torch.tensor([0.5, 0.6, 0.5])
+    pts = lambda n: (torch.rand(B, n, 3, generator=gen) - 0.5) * box + torch.tensor([0.0, 0.05, 0.05])  # noqa: E731
+    nrm = lambda n: torch.nn.functional.normalize(torch.randn(B, n, 3, generator=gen), dim=-1)  # noqa: E731
+    face, non = pts(96), pts(8)
+    batch = {"points_face": face, "normals_face": nrm(96), "points_non_face": non, "normals_non_face": nrm(8), "sup_grad_far": nrm(12) * 0.4,
+             "sup_grad_near": torch.cat([face, non], 1) + 0.01 * torch.randn(B, 104, 3, generator=gen),
+             "gt_anchors": torch.from_numpy(U.anchors_mean()).float().reshape(1, 39, 3).repeat(B, 1, 1),
+             "idx": torch.tensor([[3], [1], [3], [0]]), "path": ["x"] * B}
+    lambdas = {"surf_sdf": 2.0, "normals": 0.3, "space_sdf": 0.01, "grad": 0.1, "lat_reg": 0.005, "anchors": 7.5, "symm_dist": 0.005, "middle_dist": 0.001}
+    start = torch.randn(6, decoder.lat_dim, generator=gen).to(dev) * 0.1
+    seen = []
+    for kind in (T.LatentCodes, torch.nn.Embedding):
+        codes = kind(6, decoder.lat_dim, max_norm=1.0, sparse=True).to(dev)
+        with torch.no_grad():
+            codes.weight.copy_(start)
+        decoder.zero_grad()
+        losses = compute_loss(dict(batch), decoder, codes, dev)
+        sum(lambdas[k] * losses[k] for k in losses).backward()
+        norm = T.clip_grad_norm_(codes.parameters(), 1e-4)
+        dense = codes.weight.grad.to_dense()
+        assert abs(float(dense.double().norm()) - 1e-4) <= 1e-4 * 0.02           # (1e-6 beside a norm of 1e-4 in the factor's formula)
+        seen.append(({k: float(v.detach()) for k, v in losses.items()}, float(norm), codes))
+    for k, v in seen[1][0].items():
+        assert abs(seen[0][0][k] - v) <= 2e-5 * max(1.0, abs(v)), k
+    assert abs(seen[0][1] - seen[1][1]) <= 1e-3 * seen[1][1]
+    norm = T.clip_grad_norm_(decoder.parameters(), 0.1)
+    assert math.isfinite(float(norm))
+    torch.optim.AdamW(decoder.parameters(), lr=1e-4).step()
+    torch.optim.SparseAdam(list(seen[0][2].parameters()), lr=1e-3).step()
+    assert bool(torch.isfinite(seen[0][2].weight).all())
 
 
 @gpu
