@@ -6,6 +6,8 @@
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include <algorithm>
+
 #include "capi_common.h"
 #include "train_ops_common.h"
 
@@ -90,36 +92,99 @@ __device__ __forceinline__ void store_cols(T* row, int c, int dim, const float (
   }
 }
 
-// ---- few indices: no sorting ----------------------------------------------------------------------------------------------------
-// One wavefront a row of the result and 64 vectors of its columns: it looks through all indices, 64 at a time, and adds the rows
-// that name its own.  One launch; MERGE: the rows of the result are those of `grad`, and all but the first of an index are zeros.
-constexpr int FEW = 256;
-
-template <class T, bool MERGE>
-__global__ __launch_bounds__(256) void grad_few_kernel(GradArgs p) {
+// `count` elements from `to` on become zeros, by `threads` threads of which this is number `t`: whole 16-byte places but for the ends
+template <class T>
+__device__ __forceinline__ void zero_run(T* to, int64_t count, int t, int threads) {
   constexpr int V = Vec<T>::N;
-  const int lane = threadIdx.x & 63;
-  const int64_t own = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
-  if (own >= (MERGE ? p.count : p.rows)) return;
-  const int64_t v = MERGE ? load_index(p.idx, p.idx64, own) : own;
-  const int c = (blockIdx.y * 64 + lane) * V;
-  float acc[V] = {};
-  if (v != p.padding) {
-    for (int64_t n0 = 0; n0 < p.count; n0 += 64) {
-      const int64_t n = n0 + lane;
-      uint64_t hit = __ballot(n < p.count && load_index(p.idx, p.idx64, n < p.count ? n : 0) == v);
-      if (MERGE && hit && n0 + __builtin_ctzll(hit) < own) break;    // an earlier row owns the sum (nothing was added yet)
-      while (hit) {
-        const int b = __builtin_ctzll(hit);
-        hit &= hit - 1;
-        float x[V];
-        load_cols(x, static_cast<const T*>(p.grad) + (n0 + b) * p.ld, c, p.dim);
+  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
+  const int head = int(min(count, int64_t((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / int64_t(sizeof(T))));
+  const int64_t whole = (count - head) / V;
+  u32x4* p = reinterpret_cast<u32x4*>(to + head);
+  for (int64_t i = t; i < whole; i += threads) p[i] = u32x4{};
+  if (t < head) to[t] = T(0.f);
+  const int64_t last = head + whole * V + t;
+  if (last < count) to[last] = T(0.f);                               // (V - 1 elements at most on either end, at least 64 threads)
+}
+
+// ---- few indices: no sorting ----------------------------------------------------------------------------------------------------
+// One launch.  A block owns `rows_each` rows of the table (one, if a row is longer than SPAN vectors: then blockIdx.y cuts it into pieces of
+// them) and makes one run of zeros of them; one thread an index finds out which indices fall into them, and then each row that is named
+// becomes the sum of its own, in the order of the indices.
+constexpr int FEW = 256, SPAN = 1024;
+
+template <class T>
+__global__ __launch_bounds__(256) void grad_few_kernel(GradArgs p, int rows_each) {
+  constexpr int V = Vec<T>::N;
+  __shared__ uint64_t found[4], lead[4];
+  __shared__ int64_t index[FEW];
+  const int t = threadIdx.x;
+  const int64_t v0 = int64_t(blockIdx.x) * rows_each, v1 = min(p.rows, v0 + rows_each);
+  const int c0 = blockIdx.y * (SPAN * V), c1 = min(p.dim, c0 + SPAN * V);
+  const int64_t i = t < p.count ? load_index(p.idx, p.idx64, t) : -1;
+  index[t] = i;
+  const bool in = i >= v0 && i < v1 && i != p.padding;
+  const uint64_t hit = __ballot(in);
+  if ((t & 63) == 0) found[t >> 6] = hit;
+  T* out = static_cast<T*>(p.out);
+  if (c0 == 0 && c1 == p.dim) zero_run(out + v0 * p.dim, (v1 - v0) * p.dim, t, 256);
+  else zero_run(out + v0 * p.dim + c0, c1 - c0, t, 256);             // (one row)
+  __syncthreads();
+  if (!(found[0] | found[1] | found[2] | found[3])) return;
+  bool leads = in;                                                   // the first index of its row
+  for (int n = 0; leads && n < t; ++n) leads = index[n] != i;
+  const uint64_t leader = __ballot(leads);
+  if ((t & 63) == 0) lead[t >> 6] = leader;
+  __syncthreads();                                                   // (orders the sums below behind the zeros, too)
+  for (int u = 0; u < 4; ++u) {
+    uint64_t rows = lead[u];
+    while (rows) {
+      const int first = u * 64 + __builtin_ctzll(rows);
+      rows &= rows - 1;
+      const int64_t v = index[first];
+      for (int c = c0 + t * V; c < c1; c += 256 * V) {
+        float acc[V] = {};
+        for (int w = u; w < 4; ++w) {
+          uint64_t mask = found[w];
+          while (mask) {
+            const int n = w * 64 + __builtin_ctzll(mask);
+            mask &= mask - 1;
+            if (index[n] != v) continue;
+            float x[V];
+            load_cols(x, static_cast<const T*>(p.grad) + n * p.ld, c, p.dim);
 #pragma unroll
-        for (int k = 0; k < V; ++k) acc[k] += x[k];
+            for (int k = 0; k < V; ++k) acc[k] += x[k];
+          }
+        }
+        store_cols(out + v * p.dim, c, p.dim, acc, p.scale);
       }
     }
   }
-  store_cols(static_cast<T*>(p.out) + own * p.dim, c, p.dim, acc, p.scale);
+}
+
+// merging few: one wavefront a row and 64 vectors of its columns; all but the first row of an index become zeros
+template <class T>
+__global__ __launch_bounds__(256) void merge_few_kernel(GradArgs p) {
+  constexpr int V = Vec<T>::N;
+  const int lane = threadIdx.x & 63;
+  const int64_t own = int64_t(blockIdx.x) * 4 + (threadIdx.x >> 6);
+  if (own >= p.count) return;
+  const int64_t v = load_index(p.idx, p.idx64, own);
+  const int c = (blockIdx.y * 64 + lane) * V;
+  float acc[V] = {};
+  for (int64_t n0 = 0; n0 < p.count; n0 += 64) {
+    const int64_t n = n0 + lane;
+    uint64_t hit = __ballot(n < p.count && load_index(p.idx, p.idx64, n < p.count ? n : 0) == v);
+    if (hit && n0 + __builtin_ctzll(hit) < own) break;               // an earlier row owns the sum (nothing was added yet)
+    while (hit) {
+      const int b = __builtin_ctzll(hit);
+      hit &= hit - 1;
+      float x[V];
+      load_cols(x, static_cast<const T*>(p.grad) + (n0 + b) * p.ld, c, p.dim);
+#pragma unroll
+      for (int k = 0; k < V; ++k) acc[k] += x[k];
+    }
+  }
+  store_cols(static_cast<T*>(p.out) + own * p.dim, c, p.dim, acc, 1.f);
 }
 
 // ---- the indices, sorted ---------------------------------------------------------------------------------------------------------
@@ -296,7 +361,6 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   constexpr int V = Vec<T>::N, AHEAD = 4;
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* out = static_cast<T*>(p.out);
-  const float nothing[V] = {};
   if (int(blockIdx.x) >= s.sum_blocks) {                             // the rows that stay zero
     const int64_t step = int64_t(gridDim.x - s.sum_blocks) * 4;
     for (int64_t v = int64_t(blockIdx.x - s.sum_blocks) * 4 + wave; v < (MERGE ? p.count : p.rows); v += step) {
@@ -307,7 +371,7 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
       } else {
         if (s.named[v]) continue;
       }
-      for (int c = lane * V; c < p.dim; c += 64 * V) store_cols(out + row * p.dim, c, p.dim, nothing, 1.f);
+      zero_run(out + row * p.dim, p.dim, lane, 64);
     }
     return;
   }
@@ -446,7 +510,15 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   const unsigned tiles = unsigned((a.dim + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N));
   const int64_t out_rows = MERGE ? a.count : a.rows;
   if (a.count <= FEW) {
-    hipLaunchKernelGGL((grad_few_kernel<T, MERGE>), dim3(unsigned((out_rows + 3) / 4), tiles), dim3(256), 0, st, a);
+    if constexpr (MERGE) {
+      hipLaunchKernelGGL((merge_few_kernel<T>), dim3(unsigned((out_rows + 3) / 4), tiles), dim3(256), 0, st, a);
+    } else {
+      // up to 64 KiB of rows a block, as long as there are 1024 blocks
+      const int span = SPAN * Vec<T>::N;
+      const int64_t fit = a.dim <= span ? 65536 / (int64_t(a.dim) * int64_t(sizeof(T))) : 1, each = std::max<int64_t>(1, std::min(a.rows / 1024, fit));
+      hipLaunchKernelGGL((grad_few_kernel<T>), dim3(unsigned((a.rows + each - 1) / each), unsigned((a.dim + span - 1) / span)), dim3(256), 0, st, a,
+                         int(each));
+    }
     return;
   }
   const int count = int(a.count), rows = int(a.rows);

@@ -119,7 +119,8 @@ def dev():
 
 
 ROW_CASES = [(1, 1, 1), (7, 3, 5), (24, 1344, 16), (1000, 64, 257), (50, 200, 1), (333, 1001, 300), (4099, 40, 2500), (9, 515, 10000),
-             (70001, 24, 9001), (3, 8, 40000), (2000, 2048, 700)]
+             (70001, 24, 9001), (3, 8, 40000), (2000, 2048, 700),
+             (3000, 5000, 10), (3000, 20000, 7), (300000, 8, 256), (5000, 100, 200), (2, 9000, 256)]
 
 
 @gpu
