@@ -30,7 +30,8 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int idx64, int64_
   return idx64 ? static_cast<const int64_t*>(idx)[n] : int64_t(static_cast<const int*>(idx)[n]);
 }
 
-// A group of LPR lanes takes one row (LPR * 16 bytes of it at a time); a wavefront 64 / LPR rows, so that narrow rows fill it too.
+// A group of LPR lanes takes one row (LPR * 16 bytes of it at a time); a wavefront 64 / LPR rows, so that narrow rows fill it too.  Few rows
+// are cut along blockIdx.y.  Bound by memory: 16384 rows of 4096 bf16 out of 50000 take 54.6 us, 248 MB at 4.5 TB/s (a copy: 5.1).
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs p) {
   constexpr int V = Vec<T>::N, ROWS = 256 / LPR;
@@ -195,89 +196,98 @@ __device__ __forceinline__ int key_of(const GradArgs& p, int64_t n) {
 }
 
 struct SortArgs {
-  int *keys, *sorted, *perm;           // [count up to a multiple of 64], [count], [count]
-  int *keys2, *perm2;                  // the other end of a radix pass
+  int *sorted, *perm;                  // [count]
+  int *sorted2, *perm2;                // the other end of a radix pass
   int* hist;                           // [blocks][1 << digit bits]
-  uint8_t* named;                      // [rows]: whether an index names the row
   int shift, bits, per_block, blocks;
 };
 
-// keys from indices, and no row named yet
-__global__ __launch_bounds__(256) void keys_kernel(GradArgs p, SortArgs s, int key_blocks) {
-  if (int(blockIdx.x) < key_blocks) {
-    const int64_t n = int64_t(blockIdx.x) * 256 + threadIdx.x;
-    if (n < (p.count + 63) / 64 * 64) s.keys[n] = n < p.count ? key_of(p, n) : 0x7ffffffe;
-  } else {
-    const int64_t step = int64_t(gridDim.x - key_blocks) * 256;
-    for (int64_t i = int64_t(blockIdx.x - key_blocks) * 256 + threadIdx.x; i < p.rows; i += step) s.named[i] = 0;
-  }
+// The rows that no index names are zeros: the launches that sort, which leave most of the chip idle, clear the whole result with the
+// blocks behind their own, a share each, and the sums are written over it (50000 x 2048 bf16, 32768 indices: 102 us with the
+// rows told apart by a flag and cleared beside the sums, 94 so).  In units of 16 bits.
+struct Zero {
+  void* out;
+  int64_t first, last;
+  int blocks;                          // the launch's own, in front
+};
+constexpr int64_t ZERO_UNITS = 32768;                                // 64 KiB a block
+__device__ __forceinline__ bool cleared(const Zero& z) {             // whether this was one of the blocks that clear
+  if (int(blockIdx.x) < z.blocks) return false;
+  const int64_t at = z.first + int64_t(blockIdx.x - z.blocks) * ZERO_UNITS;
+  zero_run(static_cast<bf16*>(z.out) + at, min(ZERO_UNITS, z.last - at), threadIdx.x, blockDim.x);
+  return true;
 }
 
 // Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 16 keys: all keys are in LDS, its four wavefronts count
 // over a quarter of them each and the four 16-lane rows of a wavefront over a quarter of that (a read of four keys is the same for 16
-// lanes).  count^2 comparisons spread over the chip, one launch: 8 us for 4097 keys against 19 for the radix passes below, which
+// lanes).  count^2 comparisons spread over the chip, one launch: 10 us for 4097 keys against 19 for the radix passes below, which
 // are faster above 8192 (16384 keys: 57 us against 20).
-constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 16;              // keys a block places; ranges that all keys are cut into
+constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 16;               // keys a block places; ranges that all keys are cut into
 
-__global__ __launch_bounds__(256) void rank_kernel(const int* __restrict__ keys, int count, int rows, int* __restrict__ sorted, int* __restrict__ perm,
-                                                   uint8_t* __restrict__ named) {
+__global__ __launch_bounds__(256) void rank_kernel(GradArgs p, SortArgs s, Zero z) {
   extern __shared__ __attribute__((aligned(16))) int all[];
   __shared__ int part[RANGE][PLACED];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
-  const int padded = (count + 63) / 64 * 64, each = padded / RANGE, pitch = each + 4;      // (the ranges start in different banks)
-  for (int u = threadIdx.x; u < padded / 4; u += 256) {
-    const int at = u * 4;
-    *reinterpret_cast<i32x4*>(all + at / each * pitch + at % each) = reinterpret_cast<const i32x4*>(keys)[u];
-  }
+  if (cleared(z)) return;
+  const int count = int(p.count), padded = (count + 63) / 64 * 64, each = padded / RANGE;
+#pragma unroll 8
+  for (int n = threadIdx.x; n < padded; n += 256) all[n] = n < count ? key_of(p, n) : 0x7ffffffe;
   __syncthreads();
   const int range = threadIdx.x / PLACED, own0 = blockIdx.x * PLACED, i = own0 + threadIdx.x % PLACED;
-  const int own = all[i / each * pitch + i % each];
-  const i32x4* k = reinterpret_cast<const i32x4*>(all + range * pitch);
+  const int own = all[i];
+  const i32x4* k = reinterpret_cast<const i32x4*>(all + range * each);
   int before = 0;
-  // an equal key in front counts: those before the block's own keys all do, those behind none, the block's own by their place
+  // an equal key in front counts: those before the block's own keys all do, those behind none, the block's own by their place.  Each range
+  // starts one read further on than the one before it: the ranges of a wavefront then meet different banks.
+  const int reads = each / 4;
+  int u = range % reads;
 #pragma unroll 8
-  for (int u = 0; u < each / 4; ++u) {
+  for (int step = 0; step < reads; ++step) {
     const i32x4 v = k[u];
     const int bound = range * each + 4 * u < own0 ? own + 1 : own;
 #pragma unroll
     for (int e = 0; e < 4; ++e) before += v[e] < bound;
+    u = u + 1 == reads ? 0 : u + 1;
   }
   if (range == 0)
 #pragma unroll
-    for (int e = 0; e < PLACED; ++e) before += own0 + e < i && all[(own0 + e) / each * pitch + (own0 + e) % each] == own;
+    for (int e = 0; e < PLACED; ++e) before += own0 + e < i && all[own0 + e] == own;
   part[range][threadIdx.x % PLACED] = before;
   __syncthreads();
   if (threadIdx.x < PLACED && i < count) {
     int at = 0;
 #pragma unroll
     for (int w = 0; w < RANGE; ++w) at += part[w][threadIdx.x];
-    sorted[at] = own;
-    perm[at] = i;
-    if (own < rows) named[own] = 1;
+    s.sorted[at] = own;
+    s.perm[at] = i;
   }
 }
 
-// More: radix passes of up to 9 bits, least first.  hist: how often each block of keys has each digit.
+// More: radix passes of up to 9 bits, least first.  hist: how often each block of keys has each digit.  The first pass takes its keys from
+// the indices.
 constexpr int MAX_DIGIT = 9;
 
-__global__ __launch_bounds__(1024) void radix_hist_kernel(const int* __restrict__ keys, int count, SortArgs s) {
+template <bool FIRST>
+__global__ __launch_bounds__(1024) void radix_hist_kernel(GradArgs p, const int* __restrict__ keys, SortArgs s, Zero z) {
   __shared__ int bins[1 << MAX_DIGIT];
+  if (cleared(z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x;
   for (int d = t; d < digits; d += 1024) bins[d] = 0;
   __syncthreads();
   const int64_t first = int64_t(blockIdx.x) * s.per_block;
   for (int u = t; u < s.per_block; u += 1024)
-    if (first + u < count) atomicAdd(&bins[(keys[first + u] >> s.shift) & (digits - 1)], 1);
+    if (first + u < p.count) atomicAdd(&bins[((FIRST ? key_of(p, first + u) : keys[first + u]) >> s.shift) & (digits - 1)], 1);
   __syncthreads();
   for (int d = t; d < digits; d += 1024) s.hist[blockIdx.x * digits + d] = bins[d];
 }
 
 // Every block finds where its keys of each digit begin (the digits below it in all blocks, its own in the blocks before), then places its
 // keys in order, 1024 at a time: in a wavefront the lanes of one digit find each other by ballots, wavefront follows wavefront.
-template <bool FIRST, bool LAST>
-__global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict__ keys, const int* __restrict__ perm, int count, int rows, SortArgs s,
-                                                           int* __restrict__ keys_out, int* __restrict__ perm_out) {
+template <bool FIRST>
+__global__ __launch_bounds__(1024) void radix_place_kernel(GradArgs p, const int* __restrict__ keys, const int* __restrict__ perm, SortArgs s,
+                                                           int* __restrict__ keys_out, int* __restrict__ perm_out, Zero z) {
   __shared__ int base[1 << MAX_DIGIT], scan[1 << MAX_DIGIT], seen[16][1 << MAX_DIGIT];
+  if (cleared(z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   {
     // 1024 / digits threads a digit, each over every so many blocks
@@ -311,8 +321,8 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict
   const int64_t first = int64_t(blockIdx.x) * s.per_block;
   for (int u = 0; u < s.per_block; u += 1024) {
     const int64_t n = first + u + t;
-    const bool in = n < count;
-    const int key = in ? keys[n] : 0, d = (key >> s.shift) & (digits - 1);
+    const bool in = n < p.count;
+    const int key = !in ? 0 : FIRST ? key_of(p, n) : keys[n], d = (key >> s.shift) & (digits - 1);
     for (int q = t; q < 16 * digits; q += 1024) seen[q >> s.bits][q & (digits - 1)] = 0;
     __syncthreads();
     uint64_t mates = __ballot(in);
@@ -337,7 +347,6 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict
       const int at = seen[wave][d] + ahead;
       keys_out[at] = key;
       perm_out[at] = FIRST ? int(n) : perm[n];
-      if (LAST && key < rows) s.named[key] = 1;
     }
     __syncthreads();
   }
@@ -349,41 +358,43 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(const int* __restrict
 // begins.  So a row that takes half of all indices costs no more than any other half.
 struct SumArgs {
   const int *sorted, *perm;
-  const uint8_t* named;
   float* partial;
   int chunk, chunks, tiles;
   int64_t pitch;                       // floats a partial row
-  int sum_blocks;
 };
+
+template <class T>
+__device__ __forceinline__ typename Vec<T>::type load_raw(const T* row, int c, int dim) {
+  constexpr int V = Vec<T>::N;
+  typename Vec<T>::type x;
+  if (c + V <= dim) {
+    x = *reinterpret_cast<const typename Vec<T>::type*>(row + c);
+  } else {
+#pragma unroll
+    for (int k = 0; k < V; ++k) x[k] = c + k < dim ? row[c + k] : T(0.f);
+  }
+  return x;
+}
 
 template <class T, bool MERGE>
 __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
-  constexpr int V = Vec<T>::N, AHEAD = 4;
+  constexpr int V = Vec<T>::N, AHEAD = 8;                            // rows on their way
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   T* out = static_cast<T*>(p.out);
-  if (int(blockIdx.x) >= s.sum_blocks) {                             // the rows that stay zero
-    const int64_t step = int64_t(gridDim.x - s.sum_blocks) * 4;
-    for (int64_t v = int64_t(blockIdx.x - s.sum_blocks) * 4 + wave; v < (MERGE ? p.count : p.rows); v += step) {
-      int64_t row = v;
-      if constexpr (MERGE) {
-        if (s.sorted[v] < p.rows && (v == 0 || s.sorted[v] != s.sorted[v - 1])) continue;
-        row = s.perm[v];
-      } else {
-        if (s.named[v]) continue;
-      }
-      zero_run(out + row * p.dim, p.dim, lane, 64);
-    }
-    return;
-  }
+  const T* grad = static_cast<const T*>(p.grad);
   const int64_t task = int64_t(blockIdx.x) * 4 + wave;
   if (task >= int64_t(s.chunks) * s.tiles) return;
   const int chunk = int(task / s.tiles), c = (int(task % s.tiles) * 64 + lane) * V;
-  const int64_t p0 = int64_t(chunk) * s.chunk, p1 = min(p.count, p0 + s.chunk);
+  const int64_t p0 = int64_t(chunk) * s.chunk;
+  const int n = int(min(p.count - p0, int64_t(s.chunk)));            // 64 at most: a lane holds a place's key and row
+  const int keys = s.sorted[p0 + min(lane, n - 1)], rows = s.perm[p0 + min(lane, n - 1)];
+  const int before = p0 > 0 ? s.sorted[p0 - 1] : -1, after = p0 + n < p.count ? s.sorted[p0 + n] : -1;
+  const int live = __popcll(__ballot(lane < n && keys < p.rows));    // the places that count are in front
+  if (!live) return;
   float acc[V] = {};
-  int key = s.sorted[p0], head = s.perm[p0];
-  bool begun = p0 > 0 && s.sorted[p0 - 1] == key;
+  int key = __builtin_amdgcn_readlane(keys, 0), head = __builtin_amdgcn_readlane(rows, 0);
+  bool begun = before == key;
   auto flush = [&](bool goes_on) __attribute__((always_inline)) {
-    if (key >= p.rows) return;
     if (!begun && !goes_on) {
       store_cols(out + int64_t(MERGE ? head : key) * p.dim, c, p.dim, acc, p.scale);
     } else {
@@ -393,34 +404,27 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
       for (int k = 0; k < V; k += 4) *reinterpret_cast<f32x4*>(to + k) = f32x4{acc[k], acc[k + 1], acc[k + 2], acc[k + 3]};
     }
   };
-  for (int64_t q = p0; q < p1; q += AHEAD) {
-    float x[AHEAD][V];
-    int k[AHEAD], r[AHEAD];
+  typename Vec<T>::type x[AHEAD];
+  for (int q = 0; q < live; q += AHEAD) {
+#pragma unroll
+    for (int a = 0; a < AHEAD; ++a) x[a] = load_raw(grad + int64_t(__builtin_amdgcn_readlane(rows, min(q + a, live - 1))) * p.ld, c, p.dim);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
-      const int64_t at = min(q + a, p1 - 1);
-      k[a] = s.sorted[at];
-      r[a] = s.perm[at];
-    }
-    if (k[0] >= p.rows) break;                                       // nothing that counts from here on
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) load_cols(x[a], static_cast<const T*>(p.grad) + int64_t(r[a]) * p.ld, c, p.dim);
-#pragma unroll
-    for (int a = 0; a < AHEAD; ++a) {
-      if (q + a >= p1) break;
-      if (k[a] != key) {
+      if (q + a >= live) break;
+      const int k = __builtin_amdgcn_readlane(keys, q + a);
+      if (k != key) {
         flush(false);
-        key = k[a];
-        head = r[a];
+        key = k;
+        head = __builtin_amdgcn_readlane(rows, q + a);
         begun = false;
 #pragma unroll
         for (int e = 0; e < V; ++e) acc[e] = 0.f;
       }
 #pragma unroll
-      for (int e = 0; e < V; ++e) acc[e] += x[a][e];
+      for (int e = 0; e < V; ++e) acc[e] += float(x[a][e]);
     }
   }
-  flush(p1 < p.count && s.sorted[p1] == key);
+  flush(live == n && after == key);
 }
 
 constexpr int JOINERS = 8;             // wavefronts that join a run
@@ -473,7 +477,7 @@ __global__ __launch_bounds__(64 * JOINERS) void join_kernel(GradArgs p, SumArgs 
 
 struct GradPlan {
   int passes, bits, blocks, per_block, chunk, chunks, tiles;
-  size_t keys, sorted, perm, keys2, perm2, hist, named, partial, total;
+  size_t sorted, perm, sorted2, perm2, hist, partial, total;
 };
 inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element) {
   GradPlan g{};
@@ -492,15 +496,13 @@ inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element)
   // wavefronts), 71 in chunks of 32, 75 in chunks of 16
   while (g.chunk < 64 && count / (2 * g.chunk) * g.tiles >= 4096) g.chunk *= 2;
   g.chunks = int((count + g.chunk - 1) / g.chunk);
-  const size_t ints = up(size_t((count + 63) / 64 * 64) * 4);
-  g.keys = 0;
-  g.sorted = ints;
-  g.perm = 2 * ints;
-  g.keys2 = 3 * ints;
-  g.perm2 = 4 * ints;
-  g.hist = g.passes ? 5 * ints : 3 * ints;
-  g.named = g.hist + (g.passes ? up(size_t(g.blocks) * 4 << g.bits) : 0);
-  g.partial = g.named + up(size_t(rows));
+  const size_t ints = up(size_t(count) * 4), other = g.passes > 1 ? ints : 0;
+  g.sorted = 0;
+  g.perm = ints;
+  g.sorted2 = 2 * ints;
+  g.perm2 = g.sorted2 + other;
+  g.hist = g.perm2 + other;
+  g.partial = g.hist + (g.passes ? up(size_t(g.blocks) * 4 << g.bits) : 0);
   g.total = g.partial + up(size_t(2) * g.chunks * g.tiles * 64 * vec * 4);
   return g;
 }
@@ -521,54 +523,51 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
     }
     return;
   }
-  const int count = int(a.count), rows = int(a.rows);
   SortArgs s{};
-  s.keys = reinterpret_cast<int*>(ws + g.keys);
   s.sorted = reinterpret_cast<int*>(ws + g.sorted);
   s.perm = reinterpret_cast<int*>(ws + g.perm);
-  s.keys2 = reinterpret_cast<int*>(ws + g.keys2);
+  s.sorted2 = reinterpret_cast<int*>(ws + g.sorted2);
   s.perm2 = reinterpret_cast<int*>(ws + g.perm2);
   s.hist = reinterpret_cast<int*>(ws + g.hist);
-  s.named = reinterpret_cast<uint8_t*>(ws + g.named);
   s.bits = g.bits;
   s.per_block = g.per_block;
   s.blocks = g.blocks;
-  const int key_blocks = (count + 63) / 64 * 64 / 256 + 1;
-  const int64_t clear = (a.rows + 255) / 256;
-  hipLaunchKernelGGL(keys_kernel, dim3(unsigned(key_blocks + (clear < 1024 ? clear : 1024))), dim3(256), 0, st, a, s, key_blocks);
+  // launch k of `launches` clears its share with the blocks behind its own
+  const int launches = g.passes ? 2 * g.passes : 1;
+  const int64_t units = out_rows * a.dim * int64_t(sizeof(T) / 2), share = (units / launches + ZERO_UNITS) / ZERO_UNITS * ZERO_UNITS;
+  auto zero = [&](int k, int blocks, unsigned& grid) {
+    Zero z{a.out, std::min(units, k * share), std::min(units, (k + 1) * share), blocks};
+    grid = unsigned(blocks + (z.last - z.first + ZERO_UNITS - 1) / ZERO_UNITS);
+    return z;
+  };
+  unsigned grid = 0;
   if (!g.passes) {
-    const unsigned lds = unsigned((count + 63) / 64 * 64 * 4 + RANGE * 16);
-    hipLaunchKernelGGL(rank_kernel, dim3(unsigned((count + PLACED - 1) / PLACED)), dim3(256), lds, st, s.keys, count, rows, s.sorted, s.perm, s.named);
-  } else {
-    // the passes go keys -> other -> ... -> sorted, whatever their number
-    const int *kin = s.keys, *pin = nullptr;
-    for (int pass = 0; pass < g.passes; ++pass) {
-      const bool to_sorted = (g.passes - 1 - pass) % 2 == 0;
-      int *kout = to_sorted ? s.sorted : s.keys2, *pout = to_sorted ? s.perm : s.perm2;
-      s.shift = pass * g.bits;
-      hipLaunchKernelGGL(radix_hist_kernel, dim3(unsigned(g.blocks)), dim3(1024), 0, st, kin, count, s);
-      const dim3 grid(unsigned(g.blocks)), block(1024);
-      const bool first = pass == 0, last = pass == g.passes - 1;
-      if (first && last) hipLaunchKernelGGL((radix_place_kernel<true, true>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
-      else if (first) hipLaunchKernelGGL((radix_place_kernel<true, false>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
-      else if (last) hipLaunchKernelGGL((radix_place_kernel<false, true>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
-      else hipLaunchKernelGGL((radix_place_kernel<false, false>), grid, block, 0, st, kin, pin, count, rows, s, kout, pout);
-      kin = kout;
-      pin = pout;
-    }
+    const Zero z = zero(0, int((a.count + PLACED - 1) / PLACED), grid);
+    hipLaunchKernelGGL(rank_kernel, dim3(grid), dim3(256), unsigned((a.count + 63) / 64 * 64 * 4), st, a, s, z);
+  }
+  const int *kin = nullptr, *pin = nullptr;
+  for (int pass = 0; pass < g.passes; ++pass) {                      // indices -> other -> ... -> sorted, whatever the number of passes
+    const bool to_sorted = (g.passes - 1 - pass) % 2 == 0;
+    int *kout = to_sorted ? s.sorted : s.sorted2, *pout = to_sorted ? s.perm : s.perm2;
+    s.shift = pass * g.bits;
+    Zero z = zero(2 * pass, g.blocks, grid);
+    if (pass == 0) hipLaunchKernelGGL((radix_hist_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, s, z);
+    else hipLaunchKernelGGL((radix_hist_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, s, z);
+    z = zero(2 * pass + 1, g.blocks, grid);
+    if (pass == 0) hipLaunchKernelGGL((radix_place_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
+    else hipLaunchKernelGGL((radix_place_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
+    kin = kout;
+    pin = pout;
   }
   SumArgs u{};
   u.sorted = s.sorted;
   u.perm = s.perm;
-  u.named = s.named;
   u.partial = reinterpret_cast<float*>(ws + g.partial);
   u.chunk = g.chunk;
   u.chunks = g.chunks;
   u.tiles = g.tiles;
   u.pitch = int64_t(g.tiles) * 64 * Vec<T>::N;
-  u.sum_blocks = int((int64_t(g.chunks) * g.tiles + 3) / 4);
-  const int64_t zero = (out_rows + 15) / 16;
-  hipLaunchKernelGGL((sum_kernel<T, MERGE>), dim3(unsigned(u.sum_blocks + (zero < 4096 ? zero : 4096))), dim3(256), 0, st, a, u);
+  hipLaunchKernelGGL((sum_kernel<T, MERGE>), dim3(unsigned((int64_t(g.chunks) * g.tiles + 3) / 4)), dim3(256), 0, st, a, u);
   hipLaunchKernelGGL((join_kernel<T, MERGE>), dim3(unsigned(g.chunks), tiles), dim3(64 * JOINERS), 0, st, a, u);
 }
 
@@ -631,9 +630,10 @@ int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, i
     using T = decltype(t);
     const int64_t vecs = (dim + Vec<T>::N - 1) / Vec<T>::N;
     hipStream_t st = static_cast<hipStream_t>(stream);
-    if (vecs <= 8) hipLaunchKernelGGL((lookup_kernel<T, 8>), dim3((count + 31) / 32), dim3(256), 0, st, a);
-    else if (vecs <= 16) hipLaunchKernelGGL((lookup_kernel<T, 16>), dim3((count + 15) / 16), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((lookup_kernel<T, 64>), dim3((count + 3) / 4), dim3(256), 0, st, a);
+    const int64_t blocks = (count + 3) / 4, cuts = std::max<int64_t>(1, std::min<int64_t>((vecs + 63) / 64, 1024 / blocks));
+    if (vecs <= 8) hipLaunchKernelGGL((lookup_kernel<T, 8>), dim3(unsigned((count + 31) / 32)), dim3(256), 0, st, a);
+    else if (vecs <= 16) hipLaunchKernelGGL((lookup_kernel<T, 16>), dim3(unsigned((count + 15) / 16)), dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((lookup_kernel<T, 64>), dim3(unsigned(blocks), unsigned(cuts)), dim3(256), 0, st, a);
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_lookup launch", e);
