@@ -12,6 +12,8 @@ from ctypes import c_char_p, c_float, c_int, c_int64, c_size_t, c_void_p
 _HERE = os.path.dirname(os.path.abspath(__file__))
 LIB_PATH = os.environ.get("NPHM_AMD_LIB") or os.path.join(_HERE, "libnphm_amd.so")   # override: dev builds
 
+TORCH_LIB_PATH = os.path.join(_HERE, "libnphm_torch.so")
+
 NPHM_PREC_F32 = 0
 NPHM_PREC_BF16X3 = 1
 NPHM_PREC_BF16X3_ADAPTIVE = 2
@@ -195,6 +197,31 @@ def load():
         raise NphmAmdError("libnphm_amd.so ABI version mismatch")
     _lib = lib
     return lib
+
+
+# C entries that libnphm_torch.so reaches the kernels by, in the order of its table
+_TORCH_ENTRIES = ("nphm_last_error", "nphm_rows_lookup", "nphm_rows_grad_workspace_bytes", "nphm_rows_grad", "nphm_rows_merge",
+                  "nphm_rows_renorm", "nphm_clip_workspace_bytes", "nphm_clip_grads", "nphm_layer16_forward_workspace_bytes",
+                  "nphm_layer16_forward", "nphm_layer16_backward_workspace_bytes", "nphm_layer16_backward")
+_torch_ops = None
+
+
+def load_torch():
+    """torch.ops.nphm_amd: the training operators of libnphm_torch.so on the kernels of the library that ``load`` has loaded (once).  Raises
+    NphmAmdError if either is not built."""
+    global _torch_ops
+    if _torch_ops is not None:
+        return _torch_ops
+    lib = load()
+    if not os.path.exists(TORCH_LIB_PATH):
+        raise NphmAmdError(f"{TORCH_LIB_PATH} not found: build it with `python -c 'import __graft_entry__ as g; g.build()'`")
+    import torch
+    torch.ops.load_library(TORCH_LIB_PATH)
+    table = (c_void_p * len(_TORCH_ENTRIES))(*[ctypes.cast(getattr(lib, name), c_void_p).value for name in _TORCH_ENTRIES])
+    if ctypes.CDLL(TORCH_LIB_PATH).nphm_torch_bind(table, len(table)) != 0:
+        raise NphmAmdError("libnphm_torch.so and nphm_amd are of different versions: build them again")
+    _torch_ops = torch.ops.nphm_amd
+    return _torch_ops
 
 
 def check(rc: int, what: str):

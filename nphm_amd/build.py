@@ -18,13 +18,14 @@ SOURCES = ["prep_kernels.hip", "mlp_kernel.hip", "mlp_bwd_kernel.hip", "ident_bw
 TRAIN_FLAGS = ["-fhonor-nans", "-Xclang", "-target-feature", "-Xclang", "-packed-fp32-ops"]
 TRAIN_PARTS = [(src, TRAIN_FLAGS, os.path.splitext(src)[0]) for src in ("layer16_kernels.hip", "rows_kernels.hip", "clip_kernels.hip")]
 OUT = os.path.join(HERE, "libnphm_amd.so")
+TORCH_OUT = os.path.join(HERE, "libnphm_torch.so")       # the training operators' side towards PyTorch (host code only)
 OBJ_CACHE = os.path.join(HERE, "..", ".build_cache")      # objects by content hash (git- and gpurun-ignored)
 
 
 def _stale() -> bool:
-    if not os.path.exists(OUT):
+    if not os.path.exists(OUT) or not os.path.exists(TORCH_OUT):
         return True
-    t = os.path.getmtime(OUT)
+    t = min(os.path.getmtime(OUT), os.path.getmtime(TORCH_OUT))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "nphm_amd.h")]
     return any(os.path.getmtime(d) > t for d in deps)
 
@@ -70,6 +71,7 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if proc.wait() != 0:
             raise subprocess.CalledProcessError(proc.returncode, cmd)
         os.replace(tmp, obj)
+    _build_torch(force, verbose)
     out_tmp = f"{OUT}.{os.getpid()}.tmp"
     link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-pthread"] + objs + ["-o", out_tmp]
     if verbose:
@@ -83,6 +85,34 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if f.endswith(".o") and f not in keep and f.rsplit("-", 1)[0] in stems:
             os.remove(os.path.join(OBJ_CACHE, f))
     return OUT
+
+
+def _build_torch(force: bool, verbose: bool):
+    """csrc/torch_ops.cpp -> libnphm_torch.so: host code against the headers and libraries of the installed PyTorch.  It reaches the
+    kernels through addresses handed over at load time and links against neither library's other half."""
+    import torch
+    from torch.utils import cpp_extension
+    src = os.path.join(CSRC, "torch_ops.cpp")
+    h = hashlib.sha256(torch.__version__.encode())
+    for f in (src, os.path.join(HERE, "..", "include", "nphm_amd.h")):
+        h.update(open(f, "rb").read())
+    obj = os.path.join(OBJ_CACHE, f"torch_ops-{h.hexdigest()[:20]}.o")
+    if force or not os.path.exists(obj):
+        inc = [f for p in cpp_extension.include_paths("cuda") for f in ("-isystem", p)]
+        cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+               f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc + ["-c", src, "-o", f"{obj}.{os.getpid()}.tmp"]
+        if verbose:
+            print(" ".join(cmd))
+        subprocess.run(cmd, check=True)
+        os.replace(f"{obj}.{os.getpid()}.tmp", obj)
+    tmp = f"{TORCH_OUT}.{os.getpid()}.tmp"
+    libs = [f for p in cpp_extension.library_paths("cuda") for f in ("-L", p)]
+    subprocess.run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", obj] + libs + ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-o", tmp],
+                   check=True)
+    os.replace(tmp, TORCH_OUT)
+    for f in os.listdir(OBJ_CACHE):
+        if f.startswith("torch_ops-") and f.endswith(".o") and f != os.path.basename(obj):
+            os.remove(os.path.join(OBJ_CACHE, f))
 
 
 if __name__ == "__main__":

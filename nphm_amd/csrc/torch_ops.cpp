@@ -1,0 +1,348 @@
+// torch_ops.cpp — the training operators (nphm_amd/train_ops.py) as seen from PyTorch: checks of arguments, outputs and workspaces, the
+// autograd nodes.  The kernels are those of libnphm_amd.so, reached through the C entries that nphm_torch_bind hands over (whichever
+// build of that library the process has loaded).  In C++ because a layer of a few hundred rows takes 20 us on the card, and
+// the same node written in Python took 130 on the host (its backward pass runs in a thread of autograd's own and waits for the
+// interpreter there); a list of 500 gradients took 280 to look through.
+#include <ATen/ATen.h>
+#include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPStream.h>
+#include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/library.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstring>
+#include <optional>
+#include <string>
+#include <tuple>
+#include <vector>
+
+#include "../../include/nphm_amd.h"
+
+namespace {
+
+using at::Tensor;
+using torch::autograd::AutogradContext;
+using torch::autograd::variable_list;
+
+struct Entries {
+  decltype(&nphm_last_error) last_error;
+  decltype(&nphm_rows_lookup) rows_lookup;
+  decltype(&nphm_rows_grad_workspace_bytes) rows_grad_ws;
+  decltype(&nphm_rows_grad) rows_grad;
+  decltype(&nphm_rows_merge) rows_merge;
+  decltype(&nphm_rows_renorm) rows_renorm;
+  decltype(&nphm_clip_workspace_bytes) clip_ws;
+  decltype(&nphm_clip_grads) clip;
+  decltype(&nphm_layer16_forward_workspace_bytes) forward_ws;
+  decltype(&nphm_layer16_forward) forward;
+  decltype(&nphm_layer16_backward_workspace_bytes) backward_ws;
+  decltype(&nphm_layer16_backward) backward;
+};
+Entries lib{};
+
+void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "nphm: ", what, " failed (", rc, "): ", lib.last_error()); }
+
+int code_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
+void on_gpu(const char* what, const Tensor& t) {
+  TORCH_CHECK_TYPE(t.is_cuda(), what, ": a tensor on a ROCm device (these operators have no CPU form)");
+}
+void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// (address 0 and no tensor where nothing is needed)
+Tensor workspace(size_t bytes, const Tensor& like) { return bytes ? at::empty({int64_t(bytes)}, like.options().dtype(at::kByte)) : Tensor(); }
+void* at_of(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
+const void* const_of(const Tensor& t) { return t.defined() ? t.const_data_ptr() : nullptr; }
+void written(const Tensor& t) {
+  if (!t.is_inference()) t.unsafeGetTensorImpl()->bump_version();
+}
+// a gradient that is not differentiable itself: asked for with create_graph it carries a node that says so
+variable_list once(variable_list grads, const char* what) {
+  if (!at::GradMode::is_enabled()) return grads;
+  for (Tensor& g : grads)
+    if (g.defined()) g = g.detach().set_requires_grad(true);
+  auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": its gradients are not differentiable", int64_t(grads.size()));
+  return (*node)(std::move(grads));
+}
+
+// ---- rows of a table -----------------------------------------------------------------------------------------------------------
+
+void check_rows(const char* what, const Tensor& rows, const Tensor& idx, double scale) {
+  on_gpu(what, rows);
+  TORCH_CHECK_TYPE(code_of(rows.scalar_type()) >= 0, what, ": rows of fp32, bf16 or fp16, not ", rows.scalar_type());
+  TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, what, ": idx is an int32 or int64 tensor");
+  TORCH_CHECK_VALUE(idx.device() == rows.device(), what, ": idx is on ", idx.device(), ", the rows on ", rows.device());
+  TORCH_CHECK_VALUE(std::isfinite(scale), what, ": scale ", scale);
+}
+void check_table(const char* what, const Tensor& table) {
+  TORCH_CHECK_VALUE(table.dim() == 2 && table.numel() > 0, what, ": a table [rows, width], not ", table.sizes());
+}
+int64_t padding_of(const char* what, std::optional<int64_t> padding, int64_t rows) {
+  if (!padding) return -1;
+  TORCH_CHECK_VALUE(-rows <= *padding && *padding < rows, what, ": padding_idx ", *padding, " is no row of ", rows);
+  return *padding < 0 ? *padding + rows : *padding;
+}
+// rows contiguous, at least a row apart (a copy where they are not) -> elements between them
+int64_t row_strided(Tensor& t) {
+  if (!t.is_contiguous() && (t.stride(1) != 1 || t.stride(0) < t.size(1))) t = t.contiguous();
+  return t.is_contiguous() ? t.size(1) : t.stride(0);
+}
+int bits_of(const Tensor& idx) { return idx.scalar_type() == at::kLong ? 64 : 32; }
+
+Tensor lookup(Tensor table, const Tensor& idx, double scale) {
+  const c10::DeviceGuard guard(table.device());
+  const int64_t ld = row_strided(table);
+  const Tensor i = idx.contiguous();
+  auto sizes = idx.sizes().vec();
+  sizes.push_back(table.size(1));
+  Tensor out = at::empty(sizes, table.options());
+  check(lib.rows_lookup(const_of(table), table.size(0), table.size(1), ld, code_of(table.scalar_type()), const_of(i), bits_of(i), i.numel(),
+                        float(scale), at_of(out), stream_of(table)), "nphm_rows_lookup");
+  return out;
+}
+
+Tensor rows_grad(const Tensor& grad, const Tensor& idx, int64_t rows, double scale, std::optional<int64_t> padding) {
+  const char* what = "lookup_rows_grad";
+  check_rows(what, grad, idx, scale);
+  TORCH_CHECK_VALUE(grad.dim() >= 1 && grad.sizes().slice(0, grad.dim() - 1) == idx.sizes(), what, ": grad ", grad.sizes(), " does not fit idx ",
+                    idx.sizes());
+  const int64_t D = grad.size(-1), count = idx.numel();
+  TORCH_CHECK_VALUE(rows >= 1 && D >= 1, what, ": an empty table");
+  const int64_t pad = padding_of(what, padding, rows);
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(grad.device());
+  Tensor g = grad.dim() == 2 ? grad : grad.reshape({-1, D});
+  const int64_t ld = row_strided(g);
+  const Tensor i = idx.contiguous();
+  const int code = code_of(grad.scalar_type());
+  const size_t need = lib.rows_grad_ws(rows, D, count, code);
+  Tensor out = at::empty({rows, D}, grad.options()), ws = workspace(need, grad);
+  check(lib.rows_grad(const_of(g), count, D, ld, code, const_of(i), bits_of(i), rows, pad, float(scale), at_of(out), at_of(ws), need,
+                      stream_of(grad)), "nphm_rows_grad");
+  return out;
+}
+
+struct LookupNode : torch::autograd::Function<LookupNode> {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& idx, double scale, int64_t padding, bool sparse) {
+    ctx->save_for_backward({idx});
+    ctx->saved_data["meta"] = std::vector<int64_t>{table.size(0), padding, sparse};
+    ctx->saved_data["scale"] = scale;
+    return lookup(table, idx, scale);
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const Tensor idx = ctx->get_saved_variables()[0], &g = grads[0];
+    const auto meta = ctx->saved_data["meta"].toIntVector();
+    const int64_t rows = meta[0], padding = meta[1];
+    const double scale = ctx->saved_data["scale"].toDouble();
+    Tensor out;
+    if (!meta[2]) {
+      out = rows_grad(g, idx, rows, scale, padding < 0 ? std::nullopt : std::optional<int64_t>(padding));
+    } else {
+      // an entry an index, as nn.Embedding(sparse=True) leaves it; an entry that must not count names a row that exists and adds zeros
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(g.device());
+      const Tensor i = idx.reshape({-1}).to(at::kLong);
+      Tensor keep = at::logical_and(i >= 0, i < rows);
+      if (padding >= 0) keep = at::logical_and(keep, i != padding);
+      Tensor values = at::where(keep.unsqueeze(1), g.reshape({i.numel(), g.size(-1)}) * scale, at::zeros({}, g.options()));
+      out = at::_sparse_coo_tensor_unsafe(at::where(keep, i, at::zeros_like(i)).unsqueeze(0), values, {rows, g.size(-1)}, values.options().layout(at::kSparse));
+    }
+    return once({out, Tensor(), Tensor(), Tensor(), Tensor()}, "lookup_rows");
+  }
+};
+
+Tensor lookup_rows(const Tensor& table, const Tensor& idx, double scale, std::optional<int64_t> padding_idx, bool sparse) {
+  const char* what = "lookup_rows";
+  check_rows(what, table, idx, scale);
+  check_table(what, table);
+  const int64_t padding = padding_of(what, padding_idx, table.size(0));
+  if (table.requires_grad() && at::GradMode::is_enabled()) return LookupNode::apply(table, idx, scale, padding, sparse);
+  return lookup(table, idx, scale);
+}
+
+void renorm_rows(const Tensor& table, const Tensor& idx, double max_norm) {
+  const char* what = "renorm_rows_";
+  check_rows(what, table, idx, 1.0);
+  check_table(what, table);
+  const int64_t V = table.size(0), D = table.size(1);
+  TORCH_CHECK_VALUE((D == 1 || table.stride(1) == 1) && (V == 1 || table.stride(0) >= D), what, ": a table with contiguous rows");
+  TORCH_CHECK_VALUE(max_norm >= 0, what, ": max_norm ", max_norm);
+  const c10::DeviceGuard guard(table.device());
+  const Tensor i = idx.contiguous();
+  Tensor flags = at::empty({V}, table.options().dtype(at::kByte).requires_grad(false));
+  check(lib.rows_renorm(at_of(table), V, D, std::max(table.stride(0), D), code_of(table.scalar_type()), const_of(i), bits_of(i), i.numel(),
+                        float(max_norm), at_of(flags), stream_of(table)), "nphm_rows_renorm");
+  written(table);
+}
+
+// ---- dense layer in 16 bits ------------------------------------------------------------------------------------------------------
+
+Tensor rows_of(const Tensor& t) { return (t.dim() == 2 ? t : t.reshape({-1, t.size(-1)})).contiguous(); }
+
+std::tuple<Tensor, Tensor> layer_forward(const Tensor& x, const Tensor& weight, const Tensor& bias, const Tensor& residual, int64_t act, double beta,
+                                         bool keep) {
+  const c10::DeviceGuard guard(x.device());
+  const Tensor w = weight.contiguous();
+  const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
+  auto sizes = x.sizes().vec();
+  sizes.back() = N;
+  Tensor y = at::empty(sizes, x.options()), z;
+  if (keep && act) z = at::empty({M, N}, x.options());
+  if (M) {
+    const Tensor x2 = rows_of(x), b = bias.defined() ? bias.contiguous() : bias, r = residual.defined() ? residual.contiguous() : residual;
+    const size_t need = lib.forward_ws(const_of(x2), const_of(w), M, N, K);
+    Tensor ws = workspace(need, x);
+    check(lib.forward(const_of(x2), const_of(w), const_of(b), const_of(r), at_of(y), at_of(z), M, N, K, code_of(x.scalar_type()), int(act), float(beta),
+                      at_of(ws), need, stream_of(x)), "nphm_layer16_forward");
+  }
+  return {y, z};
+}
+
+struct LayerNode : torch::autograd::Function<LayerNode> {
+  // the inputs that ask for a gradient: one bit each (x, weight, bias, residual)
+  static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
+                        const std::optional<Tensor>& residual, int64_t act, double beta, int64_t asked) {
+    auto [y, z] = layer_forward(x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), act, beta, true);
+    ctx->save_for_backward({x, weight, z});
+    ctx->saved_data["meta"] = act << 4 | asked;
+    ctx->saved_data["beta"] = beta;
+    return y;
+  }
+  static variable_list backward(AutogradContext* ctx, variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const Tensor &x = saved[0], &weight = saved[1], &z = saved[2], &g = grads[0];
+    const int64_t meta = ctx->saved_data["meta"].toInt(), act = meta >> 4, asked = meta & 15;
+    const double beta = ctx->saved_data["beta"].toDouble();
+    variable_list out(7);                                            // (one for each argument of forward)
+    {
+      const at::NoGradGuard no_grad;
+      const c10::DeviceGuard guard(x.device());
+      const Tensor w = weight.contiguous();
+      const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
+      auto made = [&](int64_t bit, at::IntArrayRef sizes) {
+        if (!(asked & bit)) return Tensor();
+        return M ? at::empty(sizes, x.options()) : at::zeros(sizes, x.options());
+      };
+      const Tensor dx = made(1, x.sizes()), dw = made(2, {N, K}), db = made(4, {N});
+      if (M && (asked & 7)) {
+        const Tensor g2 = rows_of(g), x2 = rows_of(x);
+        const size_t need = lib.backward_ws(const_of(g2), const_of(x2), const_of(w), M, N, K, int(act));
+        const Tensor ws = workspace(need, x);
+        check(lib.backward(const_of(g2), const_of(x2), const_of(w), const_of(z), at_of(dx), at_of(dw), at_of(db), M, N, K, code_of(x.scalar_type()),
+                           int(act), float(beta), at_of(ws), need, stream_of(x)), "nphm_layer16_backward");
+      }
+      out[0] = dx;
+      out[1] = dw;
+      out[2] = db;
+      if (asked & 8) out[3] = g;
+    }
+    return once(std::move(out), "linear_act");
+  }
+};
+
+Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_, const std::optional<Tensor>& residual_, int64_t act,
+                  double beta) {
+  const char* what = "linear_act";
+  const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
+  on_gpu(what, x);
+  on_gpu(what, weight);
+  TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what, ": bf16 or fp16 tensors, not ", x.scalar_type());
+  TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.numel() > 0, what, ": x ", x.sizes(),
+                    " does not fit weight ", weight.sizes());
+  const int64_t N = weight.size(0);
+  TORCH_CHECK_VALUE(!bias.defined() || (bias.dim() == 1 && bias.size(0) == N), what, ": bias has the shape (", N, ",)");
+  if (residual.defined())
+    TORCH_CHECK_VALUE(residual.dim() == x.dim() && residual.size(-1) == N
+                          && residual.sizes().slice(0, x.dim() - 1) == x.sizes().slice(0, x.dim() - 1), what, ": residual has the shape of the result");
+  int64_t asked = x.requires_grad() ? 1 : 0;
+  int bit = 2;
+  for (const Tensor* t : {&weight, &bias, &residual}) {
+    if (t->defined()) {
+      TORCH_CHECK_TYPE(t->scalar_type() == x.scalar_type() && t->device() == x.device(), what, ": all tensors on one device, of one type");
+      if (t->requires_grad()) asked |= bit;
+    }
+    bit *= 2;
+  }
+  TORCH_CHECK_VALUE(act != 4 || (std::isfinite(beta) && beta > 0), what, ": Softplus takes a positive beta, not ", beta);
+  if (asked && at::GradMode::is_enabled()) return LayerNode::apply(x, weight, bias_, residual_, act, beta, asked);
+  return std::get<0>(layer_forward(x, weight, bias, residual, act, beta, false));
+}
+
+// ---- global gradient norm ----------------------------------------------------------------------------------------------------------
+
+// -> norm; `out` empty: the norm alone.  out[i] may be grads[i] itself.
+Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, int64_t kind, double limit, const std::string& what) {
+  const size_t n = grads.size();
+  const bool writes = !out.empty();
+  const at::NoGradGuard no_grad;
+  for (const Tensor& g : grads) {
+    TORCH_CHECK_TYPE(g.is_cuda() && g.layout() == at::kStrided, what, ": dense tensors on a ROCm device (these operators have no CPU form)");
+    TORCH_CHECK_TYPE(code_of(g.scalar_type()) >= 0, what, ": fp32, bf16 or fp16 gradients, not ", g.scalar_type());
+    TORCH_CHECK_VALUE(g.device() == grads[0].device(), what, ": gradients on ", grads[0].device(), " and ", g.device(), ": one call takes one device's");
+  }
+  const c10::DeviceGuard guard(grads[0].device());
+  std::vector<const void*> from(n);
+  std::vector<void*> to(writes ? n : 0);
+  std::vector<int64_t> counts(n);
+  std::vector<int> codes(n);
+  std::vector<Tensor> held;                                          // copies that the launches read or write
+  std::vector<std::pair<Tensor, Tensor>> back;
+  for (size_t i = 0; i < n; ++i) {
+    Tensor g = grads[i], o = writes ? out[i] : g;
+    TORCH_CHECK_VALUE(o.numel() == g.numel() && o.scalar_type() == g.scalar_type() && o.device() == g.device() && o.layout() == at::kStrided, what,
+                      ": out has a tensor of the size, type and device of each gradient");
+    // any order of dimensions will do, if it is the same on both sides and leaves no gap
+    if (!(g.is_contiguous() && o.is_contiguous()) && !(g.is_non_overlapping_and_dense() && g.sizes() == o.sizes() && g.strides() == o.strides())) {
+      g = g.contiguous();
+      if (writes) {
+        Tensor flat = at::empty_like(g);
+        back.emplace_back(o, flat);
+        o = flat;
+      }
+      held.push_back(g);
+    }
+    from[i] = const_of(g);
+    if (writes) to[i] = at_of(o);
+    counts[i] = g.numel();
+    codes[i] = code_of(g.scalar_type());
+  }
+  const size_t need = lib.clip_ws(counts.data(), int(n));
+  Tensor ws = workspace(need, grads[0]), norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
+  check(lib.clip(from.data(), writes ? to.data() : nullptr, counts.data(), codes.data(), int(n), int(kind), limit,
+                 static_cast<float*>(norm.mutable_data_ptr()), at_of(ws), need, stream_of(grads[0])), "nphm_clip_grads");
+  for (auto& [o, flat] : back) o.copy_(flat.view(o.sizes()));
+  for (const Tensor& o : out) written(o);
+  return norm;
+}
+
+// the duplicates of an uncoalesced row gradient folded, in place: the sum at a row's first entry, zeros at the others
+void merge_rows(const Tensor& index, const Tensor& values, int64_t rows) {
+  const at::NoGradGuard no_grad;
+  const c10::DeviceGuard guard(values.device());
+  if (values.numel() == 0) return;
+  const Tensor i = index.contiguous(), flat = values.reshape({values.size(0), -1}).contiguous();
+  const int code = code_of(values.scalar_type());
+  const size_t need = lib.rows_grad_ws(rows, flat.size(1), flat.size(0), code);
+  Tensor out = at::empty_like(flat), ws = workspace(need, flat);
+  check(lib.rows_merge(const_of(flat), flat.size(0), flat.size(1), code, const_of(i), bits_of(i), rows, at_of(out), at_of(ws), need, stream_of(values)),
+        "nphm_rows_merge");
+  values.copy_(out.view(values.sizes()));
+}
+
+}  // namespace
+
+// the C entries, in the order of `Entries`
+extern "C" __attribute__((visibility("default"))) int nphm_torch_bind(void* const* entries, int n) {
+  if (n != int(sizeof(Entries) / sizeof(void*))) return -1;
+  memcpy(&lib, entries, sizeof(Entries));
+  return 0;
+}
+
+TORCH_LIBRARY(nphm_amd, m) {
+  m.def("lookup_rows(Tensor table, Tensor idx, float scale, int? padding_idx, bool sparse) -> Tensor", &lookup_rows);
+  m.def("lookup_rows_grad(Tensor grad, Tensor idx, int num_rows, float scale, int? padding_idx) -> Tensor", &rows_grad);
+  m.def("renorm_rows_(Tensor(a!) table, Tensor idx, float max_norm) -> ()", &renorm_rows);
+  m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float beta) -> Tensor", &linear_act);
+  m.def("clip(Tensor[] grads, Tensor[] out, int kind, float limit, str what) -> Tensor", &clip);
+  m.def("merge_rows_(Tensor index, Tensor(a!) values, int rows) -> ()", &merge_rows);
+}
