@@ -208,11 +208,11 @@ __device__ __forceinline__ void act_values(float (&v)[8], int act, float beta) {
 #undef NPHM_EACH
 }
 
-enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2 };
+enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
 
-// C[i, j] = sum_k A(i, k) B(j, k): tile BM x BN, WM x WN wavefronts, two LDS buffers; one step's loads fly over the step before it.
+// One tile BM x BN of C[i, j] = sum_k A(i, k) B(j, k), by WM x WN wavefronts.
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, int OUT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
+__device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
   typedef Operand<T, BM, WAVES, TA> OpA;
   typedef Operand<T, BN, WAVES, TB> OpB;
@@ -223,8 +223,8 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   // Blocks go round the 8 XCDs: each XCD gets a run of consecutive tiles, 8 tiles of i to one of j, so that the 32 that it works on
   // at a time share 8 + 4 panels in its L2.
   const int mt = (p.I + BM - 1) / BM, nt = (p.J + BN - 1) / BN, tiles = mt * nt * p.splits, per = (tiles + 7) / 8;
-  const int tile = int(blockIdx.x & 7) * per + int(blockIdx.x >> 3);
-  if (int(blockIdx.x >> 3) >= per || tile >= tiles) return;
+  const int tile = (block & 7) * per + (block >> 3);
+  if ((block >> 3) >= per || tile >= tiles) return;
   const int split = tile / (mt * nt), rest = tile % (mt * nt);
   const int group = rest / (8 * nt), m_first = group * 8, m_count = min(8, mt - m_first), in = rest - group * 8 * nt;
   const int i0 = (m_first + in % m_count) * BM, j0 = in / m_count * BN;
@@ -343,7 +343,7 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
       *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8 + 4);
       const int64_t at = int64_t(i) * p.J + j;
       const bool whole = p.wide;                                     // J a multiple of 8: all eight or none
-      if constexpr (OUT == OUT_PARTS) {
+      if (OUT == OUT_PARTS || (OUT == OUT_EITHER && p.splits > 1)) {
         float* o = p.parts + int64_t(split) * p.I * p.J + at;
         if (whole) {
           *reinterpret_cast<f32x4*>(o) = *reinterpret_cast<f32x4*>(v);
@@ -386,6 +386,11 @@ __global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
   }
 }
 
+template <class T, int B, int WM, int WN, bool TA, bool TB, int OUT>
+__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
+  gemm_tile<T, B, B, WM, WN, TA, TB, OUT>(p, blockIdx.x);
+}
+
 // rows of `cols` elements -> rows of `ld` elements (whole 16-byte pieces), zeros behind them; 16 lanes a row; one or two operands
 struct Pack {
   const void* src;
@@ -416,11 +421,11 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned bloc
 // the partial products of all k ranges, added in order, and what the tiles' epilogue does otherwise; a thread takes eight elements beside
 // each other (J a multiple of 8) or one
 template <class T, int OUT, int W>
-__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) {
+__device__ __forceinline__ void join_splits(const GemmArgs& p, int block, int blocks) {
   typedef float f32x4 __attribute__((ext_vector_type(4)));
   typedef T eight __attribute__((ext_vector_type(W)));
   const int64_t count = int64_t(p.I) * p.J;
-  for (int64_t at = (int64_t(blockIdx.x) * 256 + threadIdx.x) * W; at < count; at += int64_t(gridDim.x) * 256 * W) {
+  for (int64_t at = (int64_t(block) * 256 + threadIdx.x) * W; at < count; at += int64_t(blocks) * 256 * W) {
     float v[W] = {};
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
@@ -460,9 +465,20 @@ __global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) {
   }
 }
 
+template <class T, int OUT, int W>
+__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) { join_splits<T, OUT, W>(p, blockIdx.x, gridDim.x); }
+
+// both products' partial products: blocks below `first` take p, the others q
+template <class T, int W>
+__global__ __launch_bounds__(256) void join_pair_kernel(GemmArgs p, GemmArgs q, int first) {
+  const int b = blockIdx.x;
+  if (b < first) join_splits<T, OUT_PLAIN, W>(p, b, first);
+  else join_splits<T, OUT_PLAIN, W>(q, b - first, int(gridDim.x) - first);
+}
+
 // gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every tile of rows of it (before it is rounded).  A
-// thread takes eight columns of eight rows; LPR threads a row, 256 / LPR rows side by side.
-constexpr int GZ_ROWS = 8;
+// thread takes eight columns of four rows; LPR threads a row, 256 / LPR rows side by side.
+constexpr int GZ_ROWS = 4;
 
 template <class T, int LPR>
 __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
@@ -521,11 +537,18 @@ __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, 
   }
 }
 
-// the tiles' sums, added up: 32 columns a block, eight threads a column
+// the tiles' sums, added up: 32 columns a block, eight threads a column (part: [8][32])
+struct Columns {
+  const float* sums;
+  void* out;
+  int tiles, N;
+};
 template <class T>
-__global__ __launch_bounds__(256) void column_sums16_kernel(const float* sums, int tiles, int N, T* out) {
-  __shared__ float part[8][32];
-  const int col = threadIdx.x & 31, k = threadIdx.x >> 5, n = blockIdx.x * 32 + col;
+__device__ __forceinline__ void column_sums(const Columns& c, int block, float (*part)[32]) {
+  const float* sums = c.sums;
+  T* out = static_cast<T*>(c.out);
+  const int tiles = c.tiles, N = c.N;
+  const int col = threadIdx.x & 31, k = threadIdx.x >> 5, n = block * 32 + col;
   float s = 0.f;
   if (n < N) {
 #pragma unroll 8
@@ -538,13 +561,30 @@ __global__ __launch_bounds__(256) void column_sums16_kernel(const float* sums, i
   for (int q = 1; q < 8; ++q) s += part[q][col];
   out[n] = T(s);
 }
+template <class T>
+__global__ __launch_bounds__(256) void column_sums16_kernel(Columns c) {
+  __shared__ float part[8][32];
+  column_sums<T>(c, blockIdx.x, part);
+}
+
+// dx, dW and the last sums of db side by side in one launch, where none of them fills the chip: blocks [0, bx) make dx in tiles of BX,
+// [bx, bw) dW in tiles of BW, the others db (4095 x 515 -> 1024: 30 us, 37 + 4 one after the other).
+template <class T, int BX, int BW>
+__global__ __launch_bounds__(256) void gradients_kernel(GemmArgs x, GemmArgs w, Columns c, int bx, int bw) {
+  extern __shared__ __attribute__((aligned(1024))) char lds[];
+  const int b = blockIdx.x;
+  if (b < bx) gemm_tile<T, BX, BX, 2, 2, false, true, OUT_EITHER>(x, b);
+  else if (b < bw) gemm_tile<T, BW, BW, 2, 2, true, true, OUT_EITHER>(w, b - bx);
+  else column_sums<T>(c, b - bw, reinterpret_cast<float(*)[32]>(lds));
+}
 
 inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
 inline int gz_lanes(int64_t ldn) { return ldn <= 64 ? 8 : ldn <= 128 ? 16 : ldn <= 256 ? 32 : 64; }
 inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_lanes(ldn) * GZ_ROWS; return (M + rows - 1) / rows; }
 
+// -> what is left to add up for dbias (tiles 0: nothing)
 template <class T>
-inline void make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
+inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
   const int lanes = gz_lanes(ld);
   const int64_t tiles = gz_tiles(M, ld);
   const dim3 grid(unsigned(tiles), unsigned((ld + lanes * 8 - 1) / (lanes * 8)));
@@ -553,8 +593,7 @@ inline void make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, 
   else if (lanes == 16) hipLaunchKernelGGL((gz_kernel<T, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
   else if (lanes == 32) hipLaunchKernelGGL((gz_kernel<T, 32>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
   else hipLaunchKernelGGL((gz_kernel<T, 64>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
-  if (dbias && tiles > 1)
-    hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 31) / 32)), dim3(256), 0, st, sums, int(tiles), N, dbias);
+  return Columns{sums, dbias, dbias && tiles > 1 ? int(tiles) : 0, N};
 }
 
 inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
@@ -579,30 +618,44 @@ inline Tiling tiling(int64_t I, int64_t J, int64_t K) {
 }
 inline size_t parts_bytes(const Tiling& t, int64_t I, int64_t J) { return t.splits > 1 ? up(size_t(t.splits) * I * J * 4) : 0; }
 
+// tells the device once of a kernel that takes more LDS than it would give unasked (a refusal shows at the launch)
+template <auto KERNEL>
+inline void allow_lds(unsigned bytes) {
+  if (bytes <= 65536) return;
+  static std::atomic<uint64_t> told{0};                              // devices that know, by their numbers
+  int dev = 0;
+  (void)hipGetDevice(&dev);
+  const uint64_t bit = uint64_t(1) << (dev & 63);
+  if (told.load(std::memory_order_relaxed) & bit) return;
+  (void)hipFuncSetAttribute(reinterpret_cast<const void*>(KERNEL), hipFuncAttributeMaxDynamicSharedMemorySize, int(bytes));
+  told.fetch_or(bit, std::memory_order_relaxed);
+}
+constexpr unsigned lds_of(int size) { return SLOTS * size * BK * 2; }
+static_assert(lds_of(256) <= 160 * 1024, "the slots fit");
+// blocks of a product in tiles of `size`, whole rounds of the XCDs
+inline int64_t blocks_of(const GemmArgs& a, int size) {
+  return (((a.I + size - 1) / size) * int64_t((a.J + size - 1) / size) * a.splits + 7) / 8 * 8;
+}
+
 template <class T, int B, int WM, int WN, bool TA, bool TB, int OUT>
 inline void launch_gemm(hipStream_t st, const GemmArgs& a) {
-  constexpr unsigned LDS = SLOTS * B * BK * 2;
-  static_assert(LDS <= 160 * 1024, "the slots fit");
-  const int64_t tiles = ((a.I + B - 1) / B) * int64_t((a.J + B - 1) / B) * a.splits;
-  if constexpr (LDS > 65536) {
-    static std::atomic<uint64_t> told{0};                            // devices that know of it, by their numbers (a refusal shows at the launch)
-    int dev = 0;
-    (void)hipGetDevice(&dev);
-    const uint64_t bit = uint64_t(1) << (dev & 63);
-    if (!(told.load(std::memory_order_relaxed) & bit)) {
-      (void)hipFuncSetAttribute(reinterpret_cast<const void*>(&gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>),
-                                hipFuncAttributeMaxDynamicSharedMemorySize, int(LDS));
-      told.fetch_or(bit, std::memory_order_relaxed);
-    }
-  }
-  hipLaunchKernelGGL((gemm_kernel<T, B, B, WM, WN, TA, TB, OUT>), dim3(unsigned((tiles + 7) / 8 * 8)), dim3(64 * WM * WN), LDS, st, a);
+  allow_lds<&gemm_kernel<T, B, WM, WN, TA, TB, OUT>>(lds_of(B));
+  hipLaunchKernelGGL((gemm_kernel<T, B, WM, WN, TA, TB, OUT>), dim3(unsigned(blocks_of(a, B))), dim3(64 * WM * WN), lds_of(B), st, a);
+}
+
+inline void split(GemmArgs& a, int splits) {
+  a.k_per_split = ((a.K + splits - 1) / splits + BK - 1) / BK * BK;
+  a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
+}
+inline int64_t join_blocks(const GemmArgs& a) {
+  const int64_t want = (int64_t(a.I) * a.J / (a.wide ? 8 : 1) + 255) / 256;
+  return want < 8192 ? want : 8192;
 }
 
 // the product, with its k range in t.splits pieces where that is more than one: `a.parts` has room for parts_bytes
 template <class T, bool TA, bool TB, int OUT>
 inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
-  a.k_per_split = ((a.K + t.splits - 1) / t.splits + BK - 1) / BK * BK;
-  a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
+  split(a, t.splits);
   auto launch = [&](auto out) {
     constexpr int O = decltype(out)::value;
     if (t.size == 256) launch_gemm<T, 256, 2, 4, TA, TB, O>(st, a);
@@ -615,10 +668,26 @@ inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
   std::swap(a, part);
   launch(std::integral_constant<int, OUT_PARTS>{});
   std::swap(a, part);
-  const int64_t count = int64_t(a.I) * a.J / (a.wide ? 8 : 1), want = (count + 255) / 256;
-  const dim3 grid(unsigned(want < 8192 ? want : 8192));
+  const dim3 grid{unsigned(join_blocks(a))};
   if (a.wide) hipLaunchKernelGGL((join_splits_kernel<T, OUT, 8>), grid, dim3(256), 0, st, a);
   else hipLaunchKernelGGL((join_splits_kernel<T, OUT, 1>), grid, dim3(256), 0, st, a);
+}
+
+// dx, dW and db together (x, w: their own tilings of 64 or 128, rooms of their own for partial products)
+template <class T, int BX, int BW>
+inline void launch_gradients(hipStream_t st, GemmArgs x, GemmArgs w, const Columns& c) {
+  constexpr unsigned LDS = lds_of(BX > BW ? BX : BW);
+  allow_lds<&gradients_kernel<T, BX, BW>>(LDS);
+  const bool wide = x.wide && w.wide, even = x.J % 8 == 0;
+  if (x.splits > 1) x.wide = even;
+  if (w.splits > 1) w.wide = even;
+  const int64_t bx = blocks_of(x, BX), bw = bx + blocks_of(w, BW), all = bw + (c.tiles ? (c.N + 31) / 32 : 0);
+  hipLaunchKernelGGL((gradients_kernel<T, BX, BW>), dim3(unsigned(all)), dim3(256), LDS, st, x, w, c, int(bx), int(bw));
+  x.wide = w.wide = wide;
+  const int64_t jx = x.splits > 1 ? join_blocks(x) : 0, jw = w.splits > 1 ? join_blocks(w) : 0;
+  if (jx + jw == 0) return;
+  if (wide) hipLaunchKernelGGL((join_pair_kernel<T, 8>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
+  else hipLaunchKernelGGL((join_pair_kernel<T, 1>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
 }
 
 // packs p, q or both (rows 0: not)
@@ -663,7 +732,7 @@ inline Forward forward_plan(const void* x, const void* weight, int64_t M, int64_
 struct Backward {
   Tiling x_t, w_t;
   bool same;                                        // g as it stands is gz
-  size_t gz, sums, x, weight, parts, total;         // byte offsets
+  size_t gz, sums, x, weight, parts_x, parts_w, total;      // byte offsets
 };
 inline Backward backward_plan(const void* g, const void* x, const void* weight, int64_t M, int64_t N, int64_t K, int act) {
   Backward p;
@@ -674,8 +743,9 @@ inline Backward backward_plan(const void* g, const void* x, const void* weight, 
   p.sums = p.gz + (p.same ? 0 : up(size_t(M) * round8(N) * 2));
   p.x = p.sums + up(size_t(gz_tiles(M, round8(N))) * N * 4);
   p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
-  p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
-  p.total = p.parts + std::max(parts_bytes(p.x_t, M, K), parts_bytes(p.w_t, N, K));     // (one product after the other)
+  p.parts_x = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
+  p.parts_w = p.parts_x + parts_bytes(p.x_t, M, K);
+  p.total = p.parts_w + parts_bytes(p.w_t, N, K);
   return p;
 }
 
@@ -737,30 +807,37 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
     if constexpr (sizeof(T) == 2) {
       const int64_t ldn = round8(N), ldk = round8(K);
       T* gz = plan.same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
+      Columns columns{};
       if (!plan.same || dbias)
-        make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
-                   reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta);
+        columns = make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
+                             reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta);
       const bool px = dweight && packed(x, K), pw = dx && packed(weight, K);
       pack<T>(st, Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
-      if (dx) {
-        GemmArgs a{};
-        a.A = gz; a.lda = ldn;
-        a.B = weight; a.ldb = K;
-        if (pw) { a.B = ws + plan.weight; a.ldb = ldk; }
-        a.I = int(M); a.J = int(K); a.K = int(N);
-        a.C = dx; a.wide = K % 8 == 0 && aligned(dx, 16);
-        a.parts = reinterpret_cast<float*>(ws + plan.parts);
-        gemm<T, false, true, OUT_PLAIN>(st, a, plan.x_t);
-      }
-      if (dweight) {
-        GemmArgs a{};
-        a.A = gz; a.lda = ldn;
-        a.B = x; a.ldb = K;
-        if (px) { a.B = ws + plan.x; a.ldb = ldk; }
-        a.I = int(N); a.J = int(K); a.K = int(M);
-        a.parts = reinterpret_cast<float*>(ws + plan.parts);
-        a.C = dweight; a.wide = K % 8 == 0 && aligned(dweight, 16);
-        gemm<T, true, true, OUT_PLAIN>(st, a, plan.w_t);
+      GemmArgs ax{}, aw{};
+      ax.A = aw.A = gz;
+      ax.lda = aw.lda = ldn;
+      ax.B = pw ? ws + plan.weight : weight;
+      ax.ldb = pw ? ldk : K;
+      aw.B = px ? ws + plan.x : x;
+      aw.ldb = px ? ldk : K;
+      ax.I = int(M); ax.J = int(K); ax.K = int(N);
+      aw.I = int(N); aw.J = int(K); aw.K = int(M);
+      ax.C = dx; ax.wide = K % 8 == 0 && aligned(dx, 16);
+      aw.C = dweight; aw.wide = K % 8 == 0 && aligned(dweight, 16);
+      ax.parts = reinterpret_cast<float*>(ws + plan.parts_x);
+      aw.parts = reinterpret_cast<float*>(ws + plan.parts_w);
+      if (dx && dweight && plan.x_t.size <= 128 && plan.w_t.size <= 128) {
+        split(ax, plan.x_t.splits);
+        split(aw, plan.w_t.splits);
+        if (plan.x_t.size == 128 && plan.w_t.size == 128) launch_gradients<T, 128, 128>(st, ax, aw, columns);
+        else if (plan.x_t.size == 128) launch_gradients<T, 128, 64>(st, ax, aw, columns);
+        else if (plan.w_t.size == 128) launch_gradients<T, 64, 128>(st, ax, aw, columns);
+        else launch_gradients<T, 64, 64>(st, ax, aw, columns);
+      } else {
+        if (columns.tiles)
+          hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 31) / 32)), dim3(256), 0, st, columns);
+        if (dx) gemm<T, false, true, OUT_PLAIN>(st, ax, plan.x_t);
+        if (dweight) gemm<T, true, true, OUT_PLAIN>(st, aw, plan.w_t);
       }
     }
   });
