@@ -76,7 +76,6 @@ struct GemmArgs {
   void* z;                               // [I, J] or null: the value before the activation
   int act;
   float beta;
-  int wide;                              // J is a multiple of 8; rows of C, z and residual take 16-byte accesses
 };
 
 // z as it is kept: finite where z is (a' of an infinity is no number for some activations)
@@ -194,11 +193,35 @@ struct Reader {
   }
 };
 
-template <class T, class V>
-__device__ __forceinline__ void put8(T* to, const V& v, bool whole, int width) {
-  if (whole) { *reinterpret_cast<V*>(to) = v; return; }
+// eight values beside each other, `width` of them there (more than eight: all); a row may start anywhere
+template <class T>
+__device__ __forceinline__ void put8(T* to, const float (&v)[8], int width) {
+  typename Vec<T>::type o;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
+  if (width >= 8) { *reinterpret_cast<typename Vec<T>::type*>(to) = o; return; }
+#pragma unroll
+  for (int e = 0; e < 8; ++e) if (e < width) to[e] = o[e];
+}
+__device__ __forceinline__ void put8(float* to, const float (&v)[8], int width) {
+  if (width >= 8) {
+    *reinterpret_cast<f32x4_u*>(to) = f32x4_u{v[0], v[1], v[2], v[3]};
+    *reinterpret_cast<f32x4_u*>(to + 4) = f32x4_u{v[4], v[5], v[6], v[7]};
+    return;
+  }
 #pragma unroll
   for (int e = 0; e < 8; ++e) if (e < width) to[e] = v[e];
+}
+template <class T>
+__device__ __forceinline__ void get8(float (&v)[8], const T* from, int width) {
+  if (width >= 8) {
+    const typename Vec<T>::type x = *reinterpret_cast<const typename Vec<T>::type*>(from);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = float(x[e]);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] = e < width ? float(from[e]) : 0.f;
+  }
 }
 // (the choice once for eight values: it is the same for the whole launch)
 __device__ __forceinline__ void act_values(float (&v)[8], int act, float beta) {
@@ -206,6 +229,25 @@ __device__ __forceinline__ void act_values(float (&v)[8], int act, float beta) {
 #define NPHM_EACH(A) case A: _Pragma("unroll") for (int e = 0; e < 8; ++e) v[e] = act_value(v[e], A, beta); break
   switch (act) { NPHM_EACH(ACT_RELU); NPHM_EACH(ACT_SILU); NPHM_EACH(ACT_GELU); NPHM_EACH(ACT_SOFTPLUS); }
 #undef NPHM_EACH
+}
+
+// what follows a product of the forward pass, for eight values with their bias: z as it is kept, then y
+template <class T>
+__device__ __forceinline__ void layer_out(float (&v)[8], const GemmArgs& p, int64_t at, int width) {
+  if (p.z) {
+    float k[8];
+#pragma unroll
+    for (int e = 0; e < 8; ++e) k[e] = float(keep<T>(v[e]));
+    put8(static_cast<T*>(p.z) + at, k, width);
+  }
+  float r[8] = {};
+  if (p.residual) get8(r, static_cast<const T*>(p.residual) + at, width);
+  act_values(v, p.act, p.beta);
+  if (p.residual) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[e] += r[e];
+  }
+  put8(static_cast<T*>(p.C) + at, v, width);
 }
 
 enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
@@ -315,17 +357,13 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   // Register q of a lane: i = lane % 32, j = 8 (q / 4) + 4 (lane / 32) + q % 4 of its 32 x 32 tile.  Through LDS (every wavefront its own part
   // of the tiles' room, 32 rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
   typedef float f32x4 __attribute__((ext_vector_type(4)));
-  typedef T eight __attribute__((ext_vector_type(8)));
   constexpr int COLS = TN * 32, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
   static_assert(WAVES * 32 * PITCH * 4 <= SLOTS * SLOT, "the epilogue's rows fit the tiles' room");
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles, no load is on its way
   float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
   const int j = j0 + (wave % WN) * COLS + (lane % LPR) * 8, width = min(8, p.J - j);
   float bias[8] = {};
-  if (OUT == OUT_LAYER && p.bias) {
-#pragma unroll
-    for (int e = 0; e < 8; ++e) if (e < width) bias[e] = float(static_cast<const T*>(p.bias)[j + e]);
-  }
+  if (OUT == OUT_LAYER && p.bias && width > 0) get8(bias, static_cast<const T*>(p.bias) + j, width);
 #pragma unroll
   for (int x = 0; x < TM; ++x) {
 #pragma unroll
@@ -342,45 +380,14 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
       *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8);
       *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8 + 4);
       const int64_t at = int64_t(i) * p.J + j;
-      const bool whole = p.wide;                                     // J a multiple of 8: all eight or none
       if (OUT == OUT_PARTS || (OUT == OUT_EITHER && p.splits > 1)) {
-        float* o = p.parts + int64_t(split) * p.I * p.J + at;
-        if (whole) {
-          *reinterpret_cast<f32x4*>(o) = *reinterpret_cast<f32x4*>(v);
-          *reinterpret_cast<f32x4*>(o + 4) = *reinterpret_cast<f32x4*>(v + 4);
-        } else {
+        put8(p.parts + int64_t(split) * p.I * p.J + at, v, width);
+      } else if constexpr (OUT == OUT_LAYER) {
 #pragma unroll
-          for (int e = 0; e < 8; ++e) if (e < width) o[e] = v[e];
-        }
+        for (int e = 0; e < 8; ++e) v[e] += bias[e];
+        layer_out<T>(v, p, at, width);
       } else {
-        if constexpr (OUT == OUT_LAYER) {
-#pragma unroll
-          for (int e = 0; e < 8; ++e) v[e] += bias[e];
-          if (p.z) {
-            eight zz;
-#pragma unroll
-            for (int e = 0; e < 8; ++e) zz[e] = keep<T>(v[e]);
-            put8(static_cast<T*>(p.z) + at, zz, whole, width);
-          }
-          eight res = {};
-          if (p.residual) {
-            const T* s = static_cast<const T*>(p.residual) + at;
-            if (whole) res = *reinterpret_cast<const eight*>(s);
-            else {
-#pragma unroll
-              for (int e = 0; e < 8; ++e) if (e < width) res[e] = s[e];
-            }
-          }
-          act_values(v, p.act, p.beta);
-          if (p.residual) {
-#pragma unroll
-            for (int e = 0; e < 8; ++e) v[e] += float(res[e]);
-          }
-        }
-        eight o;
-#pragma unroll
-        for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
-        put8(static_cast<T*>(p.C) + at, o, whole, width);
+        put8(static_cast<T*>(p.C) + at, v, width);
       }
     }
   }
@@ -419,77 +426,64 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned bloc
 }
 
 // the partial products of all k ranges, added in order, and what the tiles' epilogue does otherwise; a thread takes eight elements beside
-// each other (J a multiple of 8) or one
-template <class T, int OUT, int W>
+// each other, across the ends of rows
+template <class T, int OUT>
 __device__ __forceinline__ void join_splits(const GemmArgs& p, int block, int blocks) {
-  typedef float f32x4 __attribute__((ext_vector_type(4)));
-  typedef T eight __attribute__((ext_vector_type(W)));
   const int64_t count = int64_t(p.I) * p.J;
-  for (int64_t at = (int64_t(block) * 256 + threadIdx.x) * W; at < count; at += int64_t(blocks) * 256 * W) {
-    float v[W] = {};
+  for (int64_t at = (int64_t(block) * 256 + threadIdx.x) * 8; at < count; at += int64_t(blocks) * 2048) {
+    const int width = int(min(count - at, int64_t(8)));
+    float v[8] = {};
 #pragma unroll 4
     for (int s = 0; s < p.splits; ++s) {
       const float* q = p.parts + int64_t(s) * count + at;
-      if constexpr (W == 8) {
-        const f32x4 lo = *reinterpret_cast<const f32x4*>(q), hi = *reinterpret_cast<const f32x4*>(q + 4);
+      if (width == 8) {
+        const f32x4_u lo = *reinterpret_cast<const f32x4_u*>(q), hi = *reinterpret_cast<const f32x4_u*>(q + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
       } else {
-        v[0] += *q;
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (e < width) v[e] += q[e];
       }
     }
     if constexpr (OUT == OUT_LAYER) {
-      const int j = int(at % p.J);
       if (p.bias) {
+        int j = int(at % p.J);
 #pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += float(static_cast<const T*>(p.bias)[j + e]);
+        for (int e = 0; e < 8; ++e) {
+          v[e] += float(static_cast<const T*>(p.bias)[j]);
+          j = j + 1 == p.J ? 0 : j + 1;
+        }
       }
-      if (p.z) {
-        eight zz;
-#pragma unroll
-        for (int e = 0; e < W; ++e) zz[e] = keep<T>(v[e]);
-        *reinterpret_cast<eight*>(static_cast<T*>(p.z) + at) = zz;
-      }
-      if constexpr (W == 8) act_values(v, p.act, p.beta);
-      else v[0] = act_value(v[0], p.act, p.beta);
-      if (p.residual) {
-        const eight r = *reinterpret_cast<const eight*>(static_cast<const T*>(p.residual) + at);
-#pragma unroll
-        for (int e = 0; e < W; ++e) v[e] += float(r[e]);
-      }
+      layer_out<T>(v, p, at, width);
+    } else {
+      put8(static_cast<T*>(p.C) + at, v, width);
     }
-    eight o;
-#pragma unroll
-    for (int e = 0; e < W; ++e) o[e] = T(v[e]);
-    *reinterpret_cast<eight*>(static_cast<T*>(p.C) + at) = o;
   }
 }
 
-template <class T, int OUT, int W>
-__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) { join_splits<T, OUT, W>(p, blockIdx.x, gridDim.x); }
+template <class T, int OUT>
+__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) { join_splits<T, OUT>(p, blockIdx.x, gridDim.x); }
 
 // both products' partial products: blocks below `first` take p, the others q
-template <class T, int W>
+template <class T>
 __global__ __launch_bounds__(256) void join_pair_kernel(GemmArgs p, GemmArgs q, int first) {
   const int b = blockIdx.x;
-  if (b < first) join_splits<T, OUT_PLAIN, W>(p, b, first);
-  else join_splits<T, OUT_PLAIN, W>(q, b - first, int(gridDim.x) - first);
+  if (b < first) join_splits<T, OUT_PLAIN>(p, b, first);
+  else join_splits<T, OUT_PLAIN>(q, b - first, int(gridDim.x) - first);
 }
 
 // gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every tile of rows of it (before it is rounded).  A
-// thread takes eight columns of four rows; LPR threads a row, 256 / LPR rows side by side.
-constexpr int GZ_ROWS = 4;
-
-template <class T, int LPR>
+// thread takes eight columns of ROWS rows; LPR threads a row, 256 / LPR rows side by side.
+template <class T, int LPR, int ROWS>
 __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
   constexpr int SIDE = 256 / LPR;
   typedef typename Vec<T>::type vec;
   __shared__ float part[256][9];
-  const int c = (blockIdx.y * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.x * (SIDE * GZ_ROWS) + threadIdx.x / LPR;
+  const int c = (blockIdx.y * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.x * (SIDE * ROWS) + threadIdx.x / LPR;
   float s[8] = {};
   if (c < ld) {
-#pragma unroll
-    for (int r = 0; r < GZ_ROWS; ++r) {
+#pragma unroll 4
+    for (int r = 0; r < ROWS; ++r) {
       const int m = m0 + r * SIDE;
       if (m >= M) continue;
       const int64_t at = int64_t(m) * N + c;
@@ -580,7 +574,12 @@ __global__ __launch_bounds__(256) void gradients_kernel(GemmArgs x, GemmArgs w, 
 
 inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
 inline int gz_lanes(int64_t ldn) { return ldn <= 64 ? 8 : ldn <= 128 ? 16 : ldn <= 256 ? 32 : 64; }
-inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_lanes(ldn) * GZ_ROWS; return (M + rows - 1) / rows; }
+// rows a thread: 16 where that leaves 512 blocks, for fewer sums to add up (16384 x 1024: 30 us, 32 with 4), else 4 (4095 x 1024: 11 us, 13 with 8)
+inline int gz_rows(int64_t M, int64_t ldn) {
+  const int64_t lanes = gz_lanes(ldn), rows = 256 / lanes * 16;
+  return (M + rows - 1) / rows * ((ldn + lanes * 8 - 1) / (lanes * 8)) >= 512 ? 16 : 4;
+}
+inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_lanes(ldn) * gz_rows(M, ldn); return (M + rows - 1) / rows; }
 
 // -> what is left to add up for dbias (tiles 0: nothing)
 template <class T>
@@ -589,28 +588,42 @@ inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sum
   const int64_t tiles = gz_tiles(M, ld);
   const dim3 grid(unsigned(tiles), unsigned((ld + lanes * 8 - 1) / (lanes * 8)));
   float* s = dbias ? sums : nullptr;
-  if (lanes == 8) hipLaunchKernelGGL((gz_kernel<T, 8>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
-  else if (lanes == 16) hipLaunchKernelGGL((gz_kernel<T, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
-  else if (lanes == 32) hipLaunchKernelGGL((gz_kernel<T, 32>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
-  else hipLaunchKernelGGL((gz_kernel<T, 64>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  const bool many = gz_rows(M, ld) == 16;
+  auto go = [&](auto lanes_c) {
+    constexpr int L = decltype(lanes_c)::value;
+    if (many) hipLaunchKernelGGL((gz_kernel<T, L, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+    else hipLaunchKernelGGL((gz_kernel<T, L, 4>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+  };
+  if (lanes == 8) go(std::integral_constant<int, 8>{});
+  else if (lanes == 16) go(std::integral_constant<int, 16>{});
+  else if (lanes == 32) go(std::integral_constant<int, 32>{});
+  else go(std::integral_constant<int, 64>{});
   return Columns{sums, dbias, dbias && tiles > 1 ? int(tiles) : 0, N};
 }
 
 inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 
 struct Tiling { int size, splits; };               // size: 256, 128 or 64
-// The largest tiles that still fill the 256 CUs: the larger, the less a product reads (16384 x 1024 x 1024: 36 us in tiles of 256, 43 of 128,
-// 67 of 64; 2048 x 2048 x 2048: 39 split in two, 24, 30).  Where none does, the k range in pieces, added by a second launch, if
-// there is enough of it: pieces of 1024 with tiles of 128 (1024 x 1024 x 16384: 46 us in four, 56 in tiles of 64), of 512 with tiles of 64
-// (1 x 4096 x 4096: 9.6 us in eight, 32 whole; 1024 x 1024 x 1024: 8.5 us whole, 14 in two).
+// Among the tiles that fill the 256 CUs the one with the least work, counting what it reaches over the ends: an element of a 128-tile costs 1.2
+// of one of a 256-tile, of a 64-tile 1.5 (16384 x 1024 x 1024: 36, 43, 67 us; 200000 x 64 x 64: 83, 42, 26); with one step of k all
+// cost about the same (5000 x 5000 x 64: 46, 42, 38).  Where none fills them, 64-tiles, or the k range in pieces, added by a second launch,
+// if there is enough of it: pieces of 1024 with tiles of 128 (1024 x 1024 x 16384: 46 us in four, 56 in tiles of 64), of 512 with tiles
+// of 64 (1 x 4096 x 4096: 9.6 us in eight, 32 whole; 1024 x 1024 x 1024: 8.5 us whole, 14 in two).
 inline Tiling tiling(int64_t I, int64_t J, int64_t K) {
   auto tiles = [&](int64_t b) { return ((I + b - 1) / b) * ((J + b - 1) / b); };
-  if (tiles(256) >= 192) return {256, 1};
   const int64_t t128 = tiles(128), t64 = tiles(64);
-  if (t128 >= 192) return {128, 1};
-  if (t64 >= 192) {
+  const bool one = K <= BK;
+  int best = 0;
+  double least = 0;
+  for (int size : {64, 128, 256}) {
+    if (tiles(size) < 192) continue;
+    const double cost = double(tiles(size)) * size * size * (size == 256 ? one ? 1.1 : 1.0 : size == 128 ? one ? 1.05 : 1.2 : one ? 1.0 : 1.5);
+    if (!best || cost < least) best = size, least = cost;
+  }
+  if (best > 64) return {best, 1};
+  if (best == 64) {
     const int64_t s = (256 + t128 - 1) / t128;
-    return K >= 4096 && s * 1024 <= K ? Tiling{128, int(s)} : Tiling{64, 1};
+    return t128 < 192 && K >= 4096 && s * 1024 <= K ? Tiling{128, int(s)} : Tiling{64, 1};
   }
   if (K <= 1024) return {64, 1};
   const int64_t fill = I <= 64 ? 512 : 256, s = std::min<int64_t>({(fill + t64 - 1) / t64, K / 512, 16});
@@ -648,7 +661,7 @@ inline void split(GemmArgs& a, int splits) {
   a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
 }
 inline int64_t join_blocks(const GemmArgs& a) {
-  const int64_t want = (int64_t(a.I) * a.J / (a.wide ? 8 : 1) + 255) / 256;
+  const int64_t want = (int64_t(a.I) * a.J + 2047) / 2048;
   return want < 8192 ? want : 8192;
 }
 
@@ -663,14 +676,8 @@ inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
     else launch_gemm<T, 64, 2, 2, TA, TB, O>(st, a);
   };
   if (a.splits == 1) return launch(std::integral_constant<int, OUT>{});
-  GemmArgs part = a;
-  part.wide = a.J % 8 == 0;
-  std::swap(a, part);
   launch(std::integral_constant<int, OUT_PARTS>{});
-  std::swap(a, part);
-  const dim3 grid{unsigned(join_blocks(a))};
-  if (a.wide) hipLaunchKernelGGL((join_splits_kernel<T, OUT, 8>), grid, dim3(256), 0, st, a);
-  else hipLaunchKernelGGL((join_splits_kernel<T, OUT, 1>), grid, dim3(256), 0, st, a);
+  hipLaunchKernelGGL((join_splits_kernel<T, OUT>), dim3(unsigned(join_blocks(a))), dim3(256), 0, st, a);
 }
 
 // dx, dW and db together (x, w: their own tilings of 64 or 128, rooms of their own for partial products)
@@ -678,16 +685,11 @@ template <class T, int BX, int BW>
 inline void launch_gradients(hipStream_t st, GemmArgs x, GemmArgs w, const Columns& c) {
   constexpr unsigned LDS = lds_of(BX > BW ? BX : BW);
   allow_lds<&gradients_kernel<T, BX, BW>>(LDS);
-  const bool wide = x.wide && w.wide, even = x.J % 8 == 0;
-  if (x.splits > 1) x.wide = even;
-  if (w.splits > 1) w.wide = even;
   const int64_t bx = blocks_of(x, BX), bw = bx + blocks_of(w, BW), all = bw + (c.tiles ? (c.N + 31) / 32 : 0);
   hipLaunchKernelGGL((gradients_kernel<T, BX, BW>), dim3(unsigned(all)), dim3(256), LDS, st, x, w, c, int(bx), int(bw));
-  x.wide = w.wide = wide;
   const int64_t jx = x.splits > 1 ? join_blocks(x) : 0, jw = w.splits > 1 ? join_blocks(w) : 0;
   if (jx + jw == 0) return;
-  if (wide) hipLaunchKernelGGL((join_pair_kernel<T, 8>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
-  else hipLaunchKernelGGL((join_pair_kernel<T, 1>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
+  hipLaunchKernelGGL((join_pair_kernel<T>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
 }
 
 // packs p, q or both (rows 0: not)
@@ -780,7 +782,6 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       if (pw) { a.B = ws + plan.weight; a.ldb = round8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
       a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
-      a.wide = N % 8 == 0 && aligned(y, 16) && aligned(z, 16) && aligned(residual, 16);
       a.parts = reinterpret_cast<float*>(ws + plan.parts);
       gemm<T, false, false, OUT_LAYER>(st, a, plan.t);
     }
@@ -822,8 +823,8 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
       aw.ldb = px ? ldk : K;
       ax.I = int(M); ax.J = int(K); ax.K = int(N);
       aw.I = int(N); aw.J = int(K); aw.K = int(M);
-      ax.C = dx; ax.wide = K % 8 == 0 && aligned(dx, 16);
-      aw.C = dweight; aw.wide = K % 8 == 0 && aligned(dweight, 16);
+      ax.C = dx;
+      aw.C = dweight;
       ax.parts = reinterpret_cast<float*>(ws + plan.parts_x);
       aw.parts = reinterpret_cast<float*>(ws + plan.parts_w);
       if (dx && dweight && plan.x_t.size <= 128 && plan.w_t.size <= 128) {

@@ -42,6 +42,7 @@ struct Entries {
 };
 Entries lib{};
 
+void bound() { TORCH_CHECK(lib.last_error, "nphm: the kernels' library is not bound (nphm_amd._lib.load_torch does it)"); }
 void check(int rc, const char* what) { TORCH_CHECK(rc == 0, "nphm: ", what, " failed (", rc, "): ", lib.last_error()); }
 
 int code_of(at::ScalarType t) { return t == at::kFloat ? 0 : t == at::kBFloat16 ? 1 : t == at::kHalf ? 2 : -1; }
@@ -68,6 +69,7 @@ variable_list once(variable_list grads, const char* what) {
 // ---- rows of a table -----------------------------------------------------------------------------------------------------------
 
 void check_rows(const char* what, const Tensor& rows, const Tensor& idx, double scale) {
+  bound();
   on_gpu(what, rows);
   TORCH_CHECK_TYPE(code_of(rows.scalar_type()) >= 0, what, ": rows of fp32, bf16 or fp16, not ", rows.scalar_type());
   TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, what, ": idx is an int32 or int64 tensor");
@@ -243,6 +245,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
 Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias_, const std::optional<Tensor>& residual_, int64_t act,
                   double beta) {
   const char* what = "linear_act";
+  bound();
   const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
   on_gpu(what, x);
   on_gpu(what, weight);
@@ -272,8 +275,10 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
 
 // -> norm; `out` empty: the norm alone.  out[i] may be grads[i] itself.
 Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, int64_t kind, double limit, const std::string& what) {
+  bound();
   const size_t n = grads.size();
   const bool writes = !out.empty();
+  TORCH_CHECK_VALUE(n && (!writes || out.size() == n), what, ": ", n, " gradients, ", out.size(), " tensors in out");
   const at::NoGradGuard no_grad;
   for (const Tensor& g : grads) {
     TORCH_CHECK_TYPE(g.is_cuda() && g.layout() == at::kStrided, what, ": dense tensors on a ROCm device (these operators have no CPU form)");
@@ -317,6 +322,7 @@ Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, in
 
 // the duplicates of an uncoalesced row gradient folded, in place: the sum at a row's first entry, zeros at the others
 void merge_rows(const Tensor& index, const Tensor& values, int64_t rows) {
+  bound();
   const at::NoGradGuard no_grad;
   const c10::DeviceGuard guard(values.device());
   if (values.numel() == 0) return;
