@@ -662,6 +662,8 @@ int nphm_dense_column_sums(const float* x, int rows, int c, float* out, void* st
  *     32 or 64 bits).  An index outside [0, rows) gives a row of NaN.  At most 2^26 - 4 rows / indices, 2^23 elements a row.
  *   nphm_rows_grad : out [rows, dim] = scale * sum of grad[n] over the n with idx[n] = row, zeros elsewhere and in row `padding`
  *     (-1: none); indices outside the table add nothing.  fp32 sums in the order of n: bitwise reproducible.
+ *   nphm_rows_entries : the same gradient with an entry for every index: index[n] = idx[n], values[n] = scale * grad[n]; where idx[n] is
+ *     `padding` or outside the table, row 0 and zeros.
  *   nphm_rows_merge : out[n] = sum of grad[m] over the m with idx[m] = idx[n] where n is the first of them, else zeros (indices in
  *     [0, rows)).  Workspaces of both: nphm_rows_grad_workspace_bytes, 256-byte aligned.
  *   nphm_rows_renorm : rows named by idx whose 2-norm is above max_norm are multiplied by max_norm / (norm + 1e-7), each once;
@@ -671,6 +673,8 @@ int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, i
 size_t nphm_rows_grad_workspace_bytes(int64_t rows, int64_t dim, int64_t count, int dtype);
 int nphm_rows_grad(const void* grad, int64_t count, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t rows,
                    int64_t padding, float scale, void* out, void* workspace, size_t workspace_bytes, void* stream);
+int nphm_rows_entries(const void* grad, int64_t count, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t rows,
+                      int64_t padding, float scale, int64_t* index, void* values, void* stream);
 int nphm_rows_merge(const void* grad, int64_t count, int64_t dim, int dtype, const void* idx, int idx_bits, int64_t rows, void* out,
                     void* workspace, size_t workspace_bytes, void* stream);
 int nphm_rows_renorm(void* table, int64_t rows, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t count,

@@ -162,6 +162,7 @@ SYMBOLS = {
     "nphm_rows_grad_workspace_bytes": (c_size_t, [c_int64] * 3 + [c_int]),
     "nphm_rows_grad": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float, c_void_p, c_void_p,
                                c_size_t, c_void_p]),
+    "nphm_rows_entries": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_int64, c_float, c_void_p, c_void_p, c_void_p]),
     "nphm_rows_merge": (c_int, [c_void_p, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_void_p, c_void_p, c_size_t, c_void_p]),
     "nphm_rows_renorm": (c_int, [c_void_p, c_int64, c_int64, c_int64, c_int, c_void_p, c_int, c_int64, c_float, c_void_p, c_void_p]),
     "nphm_clip_workspace_bytes": (c_size_t, [c_void_p, c_int]),
@@ -200,7 +201,7 @@ def load():
 
 
 # C entries that libnphm_torch.so reaches the kernels by, in the order of its table
-_TORCH_ENTRIES = ("nphm_last_error", "nphm_rows_lookup", "nphm_rows_grad_workspace_bytes", "nphm_rows_grad", "nphm_rows_merge",
+_TORCH_ENTRIES = ("nphm_last_error", "nphm_rows_lookup", "nphm_rows_grad_workspace_bytes", "nphm_rows_grad", "nphm_rows_entries", "nphm_rows_merge",
                   "nphm_rows_renorm", "nphm_clip_workspace_bytes", "nphm_clip_grads", "nphm_layer16_forward_workspace_bytes",
                   "nphm_layer16_forward", "nphm_layer16_backward_workspace_bytes", "nphm_layer16_backward")
 _torch_ops = None

@@ -7,6 +7,7 @@
 #include <stdint.h>
 
 #include <algorithm>
+#include <type_traits>
 
 #include "capi_common.h"
 #include "train_ops_common.h"
@@ -54,6 +55,43 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs p) {
   if (blockIdx.y == 0) {
     const int c = full + sub;                       // V - 1 elements at most, LPR >= 8 lanes
     if (c < p.dim) dst[c] = ok ? T(float(src[c]) * p.scale) : T(__builtin_nanf(""));
+  }
+}
+
+struct EntryArgs {
+  const void* grad;    // [count, dim], rows ld apart
+  const void* idx;
+  int64_t* index;      // [count]
+  void* values;        // [count, dim]
+  int64_t ld, count, rows, padding;
+  int dim, idx64;
+  float scale;
+};
+
+// The gradient of the table with an entry for every index: the lookup's copy the other way round.  What must not count (padding, outside
+// the table) becomes an entry of zeros for row 0, so that nobody has to know on the host how many there are.
+template <class T, int LPR>
+__global__ __launch_bounds__(256) void entries_kernel(EntryArgs p) {
+  constexpr int V = Vec<T>::N, ROWS = 256 / LPR;
+  typedef typename Vec<T>::type vec;
+  const int sub = threadIdx.x % LPR;
+  const int64_t n = int64_t(blockIdx.x) * ROWS + threadIdx.x / LPR;
+  if (n >= p.count) return;
+  const int64_t i = load_index(p.idx, p.idx64, n);
+  const bool ok = i >= 0 && i < p.rows && i != p.padding;
+  const T* src = static_cast<const T*>(p.grad) + n * p.ld;
+  T* dst = static_cast<T*>(p.values) + n * p.dim;
+  const int full = p.dim / V * V;
+  for (int c = (blockIdx.y * LPR + sub) * V; c < full; c += gridDim.y * LPR * V) {
+    vec v = *reinterpret_cast<const vec*>(src + c);
+#pragma unroll
+    for (int k = 0; k < V; ++k) v[k] = ok ? T(float(v[k]) * p.scale) : T(0.f);
+    *reinterpret_cast<vec*>(dst + c) = v;
+  }
+  if (blockIdx.y == 0) {
+    const int c = full + sub;                       // V - 1 elements at most, LPR >= 8 lanes
+    if (c < p.dim) dst[c] = ok ? T(float(src[c]) * p.scale) : T(0.f);
+    if (sub == 0) p.index[n] = ok ? i : 0;
   }
 }
 
@@ -599,6 +637,15 @@ __global__ __launch_bounds__(256) void renorm_kernel(T* table, int64_t ld, int64
 
 constexpr int64_t MAX_ROWS = (int64_t(1) << 26) - 4;      // a wavefront a row: fewer than 2^32 threads in a launch
 
+// f(lanes a row, grid) for `count` rows of `vecs` vectors
+template <class F>
+inline void for_rows(int64_t count, int64_t vecs, F&& f) {
+  const int64_t blocks = (count + 3) / 4, cuts = std::max<int64_t>(1, std::min<int64_t>((vecs + 63) / 64, 1024 / blocks));
+  if (vecs <= 8) f(std::integral_constant<int, 8>{}, dim3(unsigned((count + 31) / 32)));
+  else if (vecs <= 16) f(std::integral_constant<int, 16>{}, dim3(unsigned((count + 15) / 16)));
+  else f(std::integral_constant<int, 64>{}, dim3(unsigned(blocks), unsigned(cuts)));
+}
+
 inline int check_table(const char* what, const void* table, int64_t rows, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits,
                        int64_t count) {
   static thread_local char msg[160];
@@ -628,12 +675,9 @@ int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, i
   LookupArgs a{table, idx, out, ld, count, rows, int(dim), idx_bits == 64, scale};
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
-    const int64_t vecs = (dim + Vec<T>::N - 1) / Vec<T>::N;
-    hipStream_t st = static_cast<hipStream_t>(stream);
-    const int64_t blocks = (count + 3) / 4, cuts = std::max<int64_t>(1, std::min<int64_t>((vecs + 63) / 64, 1024 / blocks));
-    if (vecs <= 8) hipLaunchKernelGGL((lookup_kernel<T, 8>), dim3(unsigned((count + 31) / 32)), dim3(256), 0, st, a);
-    else if (vecs <= 16) hipLaunchKernelGGL((lookup_kernel<T, 16>), dim3(unsigned((count + 15) / 16)), dim3(256), 0, st, a);
-    else hipLaunchKernelGGL((lookup_kernel<T, 64>), dim3(unsigned(blocks), unsigned(cuts)), dim3(256), 0, st, a);
+    for_rows(count, (dim + Vec<T>::N - 1) / Vec<T>::N, [&](auto lanes, dim3 grid) {
+      hipLaunchKernelGGL((lookup_kernel<T, decltype(lanes)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    });
   });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_lookup launch", e);
@@ -654,6 +698,23 @@ int nphm_rows_grad(const void* grad, int64_t count, int64_t dim, int64_t ld, int
   with_dtype(dtype, [&](auto t) { grad_run<decltype(t), false>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_grad launch", e);
+  return 0;
+}
+
+int nphm_rows_entries(const void* grad, int64_t count, int64_t dim, int64_t ld, int dtype, const void* idx, int idx_bits, int64_t rows,
+                      int64_t padding, float scale, int64_t* index, void* values, void* stream) {
+  if (count == 0) return 0;
+  if (int rc = check_table("nphm_rows_entries", grad, rows, dim, ld, dtype, idx, idx_bits, count)) return rc;
+  if (!index || !values) return nphm_fail_msg("nphm_rows_entries: null pointer");
+  const EntryArgs a{grad, idx, index, values, ld, count, rows, padding, int(dim), idx_bits == 64, scale};
+  with_dtype(dtype, [&](auto t) {
+    using T = decltype(t);
+    for_rows(count, (dim + Vec<T>::N - 1) / Vec<T>::N, [&](auto lanes, dim3 grid) {
+      hipLaunchKernelGGL((entries_kernel<T, decltype(lanes)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+    });
+  });
+  hipError_t e = hipGetLastError();
+  if (e != hipSuccess) return nphm_fail("nphm_rows_entries launch", e);
   return 0;
 }
 

@@ -31,6 +31,7 @@ struct Entries {
   decltype(&nphm_rows_lookup) rows_lookup;
   decltype(&nphm_rows_grad_workspace_bytes) rows_grad_ws;
   decltype(&nphm_rows_grad) rows_grad;
+  decltype(&nphm_rows_entries) rows_entries;
   decltype(&nphm_rows_merge) rows_merge;
   decltype(&nphm_rows_renorm) rows_renorm;
   decltype(&nphm_clip_workspace_bytes) clip_ws;
@@ -143,11 +144,14 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
       // an entry an index, as nn.Embedding(sparse=True) leaves it; an entry that must not count names a row that exists and adds zeros
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(g.device());
-      const Tensor i = idx.reshape({-1}).to(at::kLong);
-      Tensor keep = at::logical_and(i >= 0, i < rows);
-      if (padding >= 0) keep = at::logical_and(keep, i != padding);
-      Tensor values = at::where(keep.unsqueeze(1), g.reshape({i.numel(), g.size(-1)}) * scale, at::zeros({}, g.options()));
-      out = at::_sparse_coo_tensor_unsafe(at::where(keep, i, at::zeros_like(i)).unsqueeze(0), values, {rows, g.size(-1)}, values.options().layout(at::kSparse));
+      const Tensor i = idx.contiguous();
+      const int64_t count = i.numel(), D = g.size(-1);
+      Tensor g2 = g.dim() == 2 ? g : g.reshape({count, D});
+      const int64_t ld = row_strided(g2);
+      Tensor index = at::empty({1, count}, i.options().dtype(at::kLong)), values = at::empty({count, D}, g.options());
+      check(lib.rows_entries(const_of(g2), count, D, ld, code_of(g.scalar_type()), const_of(i), bits_of(i), rows, padding, float(scale),
+                             static_cast<int64_t*>(at_of(index)), at_of(values), stream_of(g)), "nphm_rows_entries");
+      out = at::_sparse_coo_tensor_unsafe(index, values, {rows, D}, values.options().layout(at::kSparse));
     }
     return once({out, Tensor(), Tensor(), Tensor(), Tensor()}, "lookup_rows");
   }

@@ -245,6 +245,11 @@ class DeepSDF(nn.Module):
     the input is re-injected (concatenated, divided by sqrt 2) before layer ``nlayers//2``;
     Softplus(beta) activations (ReLU if beta <= 0); optional geometric init of the last layer."""
 
+    # storage of the dense training tier's hidden layers: "fp32", or "bf16" | "fp16" (train_ops.linear_act) for the layers that
+    # read hidden values alone; the layers that read coordinates (the first, the skip layer) and the last stay in fp32 -
+    # a coordinate of 0.5 would move by up to 1e-3 in bf16.  (On the class: modules pickled whole without it still train.)
+    train_precision = "fp32"
+
     def __init__(self, lat_dim, hidden_dim, nlayers=8, geometric_init=True, radius_init=1, beta=100,
                  out_dim=1, num_freq_bands=None, input_dim=3):
         super().__init__()
@@ -259,10 +264,6 @@ class DeepSDF(nn.Module):
         self.beta = beta
         self.backend = "hip"            # "hip" | "composite"
         self.train_backend = "hip"      # with trainable parameters: "hip" = the dense training tier (evaluate_train_hip) | "composite"
-        # storage of the dense training tier's hidden layers: "fp32", or "bf16" | "fp16" (train_ops.linear_act) for the layers that
-        # read hidden values alone; the layers that read coordinates (the first, the skip layer) and the last stay in fp32 -
-        # a coordinate of 0.5 would move by up to 1e-3 in bf16
-        self.train_precision = "fp32"
         self._pack_cache = None         # (key, packed tensor)
         self._pack_bwd_cache = None     # (key, transposed pack of the backward kernel)
         # Numerics of the plain HIP evaluation (forward_hip / lattice launches; include/nphm_amd.h NPHM_MLP_*):
@@ -403,12 +404,13 @@ class DeepSDF(nn.Module):
             lin = getattr(self, f"lin{layer}")
             alpha = 1.0
             if layer in self.skip_in:
-                x = torch.cat([x.float(), inp], dim=-1)
+                x = torch.cat([x if half is None else x.float(), inp], dim=-1)
                 alpha = 1.0 / _SQRT2
             if half is not None and 0 < layer < last and layer not in self.skip_in:
                 x = linear_act(x.to(half), lin.weight.to(half), lin.bias.to(half), "softplus" if beta > 0 else "relu", max(beta, 1e-6))
                 continue
-            x = x.float()
+            if half is not None:
+                x = x.float()
             if layer < last:
                 x = _DenseLayerFn.apply(x, lin.weight, lin.bias, alpha, beta)
             else:

@@ -192,6 +192,29 @@ def test_indices_outside_the_table(dev, N):
 
 
 @gpu
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("V,D,N", [(1, 1, 1), (7, 3, 5), (24, 1344, 16), (50, 61, 300), (4099, 130, 9001), (6, 20000, 3)])
+def test_sparse_gradient_has_an_entry_for_every_index(dev, t, V, D, N):
+    """in the order of the indices, one rounding of scale * g each; padding and indices outside the table: row 0 and zeros, NaN or not"""
+    gen = torch.Generator().manual_seed(V + D + N)
+    table = torch.randn(V, D, generator=gen).to(t).to(dev).requires_grad_()
+    wide = torch.randn(N, D + 3, generator=gen).to(t).to(dev)
+    idx = torch.randint(-1, V + 1, (N,), generator=gen).to(dev)
+    padding = V // 2
+    kept = (idx >= 0) & (idx < V) & (idx != padding)
+    for kind in (torch.int64, torch.int32):
+        for g in (wide[:, :D].contiguous(), wide[:, 2:D + 2], wide[:1, :D].expand(N, D), wide[:, :D].index_fill(0, (~kept).nonzero()[:, 0], math.nan)):
+            grad, = torch.autograd.grad(T.lookup_rows(table, idx.to(kind), 0.37, padding_idx=padding, sparse=True), table, g)
+            assert grad.is_sparse and grad.dtype == t and grad.shape == (V, D) and grad._indices().dtype == torch.int64
+            assert torch.equal(grad._indices()[0], torch.where(kept, idx, 0))
+            assert not grad._values()[~kept].any()
+            want = g[kept].double() * 0.37
+            within(grad._values()[kept], want, want.abs() * (half_step(t) + 3 * F32) + tiny(t))
+    grad, = torch.autograd.grad(T.lookup_rows(table, idx[:0].reshape(0, 2), sparse=True), table, wide[:0, :D].reshape(0, 2, D))
+    assert grad.is_sparse and grad._nnz() == 0 and not grad.to_dense().any()
+
+
+@gpu
 def test_row_gradients_do_not_overflow_in_sums(dev):
     """fp16 rows whose partial sums leave the type's range and come back"""
     g = torch.full((2000, 24), 60000.0, dtype=torch.float16, device=dev)
