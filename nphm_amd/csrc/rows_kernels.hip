@@ -394,6 +394,8 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(GradArgs p, const int
 // A wavefront adds the rows of `chunk` consecutive places (64 vectors of columns): a run that lies inside goes out, one that the
 // chunk's borders cut goes to partial[2 chunk + (begun before ? 0 : 1)] in fp32; join adds those in order, from the chunk where the run
 // begins.  So a row that takes half of all indices costs no more than any other half.
+// Bound by memory: 32768 rows of 2048 bf16 for 50000, 46 us at 5 TB/s (read once, named rows written once); sorting takes 36 beside
+// the clearing and joining 8, most of it the way through seven launches.
 struct SumArgs {
   const int *sorted, *perm;
   float* partial;

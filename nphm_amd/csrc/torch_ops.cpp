@@ -315,6 +315,12 @@ Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, in
     counts[i] = g.numel();
     codes[i] = code_of(g.scalar_type());
   }
+  if (back.size() > 1) {                                             // (the others' memory is compared behind the C entry)
+    std::vector<const void*> starts;
+    for (const auto& pair : back) starts.push_back(pair.first.const_data_ptr());
+    std::sort(starts.begin(), starts.end());
+    TORCH_CHECK(std::adjacent_find(starts.begin(), starts.end()) == starts.end(), "nphm: ", what, ": two of the tensors share memory");
+  }
   const size_t need = lib.clip_ws(counts.data(), int(n));
   Tensor ws = workspace(need, grads[0]), norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
   check(lib.clip(from.data(), writes ? to.data() : nullptr, counts.data(), codes.data(), int(n), int(kind), limit,

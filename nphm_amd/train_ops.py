@@ -8,10 +8,12 @@ clip_grad_norm_ between ``compute_loss`` and the optimisers, src/NPHM/models/tra
     clip_grad_norm_(decoder.parameters(), 0.1)
     clip_grad_norm_(codes.parameters(), 0.1)                                            # row gradients too
 
-Every function runs on libnphm_amd.so (csrc/rows_kernels.hip, clip_kernels.hip, layer16_kernels.hip; csrc/torch_ops.cpp checks its arguments,
-allocates and holds its autograd node), on the current stream of its tensors' device, raises ``ValueError`` / ``TypeError`` for what it does not take and ``NphmAmdError`` if the library is missing; there is
-no PyTorch fallback, CPU tensors are refused.  Results are the same bits from run to run.  All of it can be captured into a
-graph, except where a line says that it waits for the device."""
+Every function runs on libnphm_amd.so (csrc/rows_kernels.hip, clip_kernels.hip, layer16_kernels.hip; csrc/torch_ops.cpp checks its
+arguments, allocates and holds its autograd node), on the current stream of its tensors' device.  It raises ``ValueError`` /
+``TypeError`` for what it does not take and ``NphmAmdError`` if the library is missing or a call fails; there is no PyTorch fallback,
+CPU tensors are refused.  Results are the same bits from run to run.  All of it can be captured into a graph, except where a
+line says that it waits for the device.  (A backward pass is captured on leaves of which no graph of eager calls is alive: autograd would
+make the capturing stream wait for work outside the capture.)"""
 from __future__ import annotations
 
 import math
@@ -132,8 +134,9 @@ def grad_norm(grads, norm_type=2.0):
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """Scales the dense tensors of `grads` by min(1, max_norm / (norm + 1e-6)), in place, or into the tensors `out` (of the same sizes and types,
-    in row-major order: pieces of a flat buffer will do; none shares memory with another tensor of the call).  -> (norm, the scaled tensors).  As torch's clip: a norm that is
-    no number makes every result NaN, an infinite one makes the finite entries 0."""
+    in row-major order: pieces of a flat buffer will do).  A tensor that shares memory with another of the call, or is named twice, is
+    refused.  -> (norm, the scaled tensors).  As torch's clip: a norm that is no number makes every result NaN, an infinite one makes the
+    finite entries 0."""
     what = "clip_grads"
     kind, limit = _kind(what, norm_type), _limit(what, max_norm)
     grads = list(grads)

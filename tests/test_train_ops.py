@@ -674,6 +674,24 @@ def test_clip_values_that_are_no_numbers_as_torch(dev, value, kind):
 
 
 @gpu
+def test_clip_refuses_a_tensor_named_twice(dev):
+    """in place and into `out`, with and without gaps between its elements; what is only read may be named as often as one likes"""
+    buf = torch.randn(64, 8, device=dev)
+    for t in (buf, buf[:, ::2], buf.t()):
+        before = buf.clone()
+        with pytest.raises(NphmAmdError, match="share memory"):
+            T.clip_grads([t, t], 0.1)
+        with pytest.raises(NphmAmdError, match="share memory"):
+            T.clip_grads([buf + 1, buf + 2] if t is buf else [t + 1, t + 2], 0.1, out=[t, t])
+        assert torch.equal(buf, before)
+        norm, (a, b) = T.clip_grads([t, t], 0.1, out=[torch.empty_like(t, memory_format=torch.contiguous_format) for _ in range(2)])
+        assert abs(float(norm) - float(t.double().norm()) * 2 ** 0.5) <= float(norm) * 2.0 ** -22 and torch.equal(a, b)
+    halves = buf.clone()
+    T.clip_grads([halves[:, ::2], halves[:, 1::2]], 0.1)              # interleaved, but no element twice
+    within(halves, buf.double() * (0.1 / (buf.double().norm() + 1e-6)), buf.double().abs() * 4 * F32)
+
+
+@gpu
 def test_norm_of_huge_and_tiny_gradients(dev):
     """squares of these leave fp32 on both sides; the norm does not"""
     for v in (1e30, 1e-30):
