@@ -258,8 +258,9 @@ __device__ __forceinline__ void layer_out(float (&v)[8], const GemmArgs& p, int6
 enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
 
 // One tile BM x BN of C[i, j] = sum_k A(i, k) B(j, k), by WM x WN wavefronts.  256 x 256 by eight: a wavefront's 128 x 64 is 128 accumulators a
-// lane, and its fragments take 6 LDS reads for 8 matrix instructions.  Four wavefronts of 128 x 128 spill, slots of 32 k have a
-// barrier twice as often; both were slower.
+// lane, and its fragments take 6 LDS reads for 8 matrix instructions.  Four wavefronts of 128 x 128 read less, but
+// nothing stands in for one that waits (8192 x 4096 x 4096: 218 us, 206 with eight); slots of 32 k have a barrier twice as often.  Blocks that
+// stay and fetch the next tile's first steps while the last one's results leave: 209 us, for loads wait behind a wavefront's stores.
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, int OUT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
@@ -413,23 +414,26 @@ struct Pack {
 };
 
 template <class T>
-__global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned blocks, int cols, int ld) {
+__device__ __forceinline__ void pack_rows(Pack p, const Pack& q, unsigned blocks, unsigned block, int cols, int ld) {
   typedef typename Vec<T>::type vec;
-  if (blockIdx.x >= blocks) p = q;
-  const int64_t r = int64_t(blockIdx.x >= blocks ? blockIdx.x - blocks : blockIdx.x) * 16 + threadIdx.x / 16;
+  if (block >= blocks) p = q, block -= blocks;
+  const int64_t r = int64_t(block) * 16 + threadIdx.x / 16;
   if (r >= p.rows) return;
   const T* s = static_cast<const T*>(p.src) + r * cols;
   T* d = static_cast<T*>(p.dst) + r * ld;
-  for (int c = (threadIdx.x % 16) * 8; c < ld; c += 128) {
+  const int whole = cols / 8 * 8, c0 = (threadIdx.x % 16) * 8;
+#pragma unroll 4
+  for (int c = c0; c < whole; c += 128) *reinterpret_cast<vec*>(d + c) = *reinterpret_cast<const vec*>(s + c);
+  if (whole < ld && c0 == whole % 128) {
     vec v;
-    if (c + 8 <= cols) {
-      v = *reinterpret_cast<const vec*>(s + c);
-    } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = c + e < cols ? s[c + e] : T(0.f);
-    }
-    *reinterpret_cast<vec*>(d + c) = v;
+    for (int e = 0; e < 8; ++e) v[e] = whole + e < cols ? s[whole + e] : T(0.f);
+    *reinterpret_cast<vec*>(d + whole) = v;
   }
+}
+template <class T>
+__global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned blocks, int cols, int ld) {
+  pack_rows<T>(p, q, blocks, blockIdx.x, cols, ld);
 }
 
 // the partial products of all k ranges, added in order, and what the tiles' epilogue does otherwise; a thread takes eight elements beside
@@ -482,12 +486,22 @@ __global__ __launch_bounds__(256) void join_pair_kernel(GemmArgs p, GemmArgs q, 
 // gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every tile of rows of it (before it is rounded).  A
 // thread takes eight columns of ROWS rows; LPR threads a row, 256 / LPR rows side by side.  Bound by memory: 16384 x 1024 with Softplus,
 // 101 MB in 18 us (5.5 TB/s, some of it still in the last cache).
+// The blocks behind its own pack the operands of the products that follow (a launch less: 4095 x 515 -> 1024, 4 us).
+struct Packs {
+  Pack p, q;
+  unsigned blocks;                       // of p
+  int cols, ld;
+};
+
 template <class T, int LPR, int ROWS>
-__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
+__global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta,
+                                                 int tiles, unsigned own, Packs packs) {
   constexpr int SIDE = 256 / LPR;
   typedef typename Vec<T>::type vec;
   __shared__ float part[256][9];
-  const int c = (blockIdx.y * LPR + threadIdx.x % LPR) * 8, m0 = blockIdx.x * (SIDE * ROWS) + threadIdx.x / LPR;
+  if (blockIdx.x >= own) return pack_rows<T>(packs.p, packs.q, packs.blocks, blockIdx.x - own, packs.cols, packs.ld);
+  const int tile = int(blockIdx.x % unsigned(tiles)), side = int(blockIdx.x / unsigned(tiles));
+  const int c = (side * LPR + threadIdx.x % LPR) * 8, m0 = tile * (SIDE * ROWS) + threadIdx.x / LPR;
   float s[8] = {};
   if (c < ld) {
 #pragma unroll 4
@@ -529,13 +543,13 @@ __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, 
   for (int e = 0; e < 8; ++e) part[threadIdx.x][e] = s[e];
   __syncthreads();
   for (int u = threadIdx.x; u < LPR * 8; u += 256) {
-    const int n = blockIdx.y * LPR * 8 + u;
+    const int n = side * LPR * 8 + u;
     if (n >= N) continue;
     float o = 0.f;
 #pragma unroll
     for (int k = 0; k < SIDE; ++k) o += part[k * LPR + u / 8][u % 8];
-    if (gridDim.x == 1) dbias[n] = T(o);
-    else sums[int64_t(blockIdx.x) * N + n] = o;
+    if (tiles == 1) dbias[n] = T(o);
+    else sums[int64_t(tile) * N + n] = o;
   }
 }
 
@@ -580,6 +594,7 @@ __global__ __launch_bounds__(256) void gradients_kernel(GemmArgs x, GemmArgs w, 
   else column_sums<T>(c, b - bw, reinterpret_cast<float(*)[32]>(lds));
 }
 
+inline unsigned pack_blocks(const Pack& p) { return unsigned((p.rows + 15) / 16); }
 inline size_t up(size_t v) { return (v + 255) / 256 * 256; }
 inline int gz_lanes(int64_t ldn) { return ldn <= 64 ? 8 : ldn <= 128 ? 16 : ldn <= 256 ? 32 : 64; }
 // rows a thread: 16 where that leaves 512 blocks, for fewer sums to add up (16384 x 1024: 30 us, 32 with 4), else 4 (4095 x 1024: 11 us, 13 with 8)
@@ -591,22 +606,21 @@ inline int64_t gz_tiles(int64_t M, int64_t ldn) { const int64_t rows = 256 / gz_
 
 // -> what is left to add up for dbias (tiles 0: nothing)
 template <class T>
-inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta) {
-  const int lanes = gz_lanes(ld);
-  const int64_t tiles = gz_tiles(M, ld);
-  const dim3 grid(unsigned(tiles), unsigned((ld + lanes * 8 - 1) / (lanes * 8)));
+inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta, const Packs& packs) {
+  const int lanes = gz_lanes(ld), tiles = int(gz_tiles(M, ld));
+  const unsigned own = unsigned(tiles) * unsigned((ld + lanes * 8 - 1) / (lanes * 8)), grid = own + packs.blocks + pack_blocks(packs.q);
   float* s = dbias ? sums : nullptr;
   const bool many = gz_rows(M, ld) == 16;
   auto go = [&](auto lanes_c) {
     constexpr int L = decltype(lanes_c)::value;
-    if (many) hipLaunchKernelGGL((gz_kernel<T, L, 16>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
-    else hipLaunchKernelGGL((gz_kernel<T, L, 4>), grid, dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta);
+    if (many) hipLaunchKernelGGL((gz_kernel<T, L, 16>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
+    else hipLaunchKernelGGL((gz_kernel<T, L, 4>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
   };
   if (lanes == 8) go(std::integral_constant<int, 8>{});
   else if (lanes == 16) go(std::integral_constant<int, 16>{});
   else if (lanes == 32) go(std::integral_constant<int, 32>{});
   else go(std::integral_constant<int, 64>{});
-  return Columns{sums, dbias, dbias && tiles > 1 ? int(tiles) : 0, N};
+  return Columns{sums, dbias, dbias && tiles > 1 ? tiles : 0, N};
 }
 
 inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
@@ -700,14 +714,13 @@ inline void launch_gradients(hipStream_t st, GemmArgs x, GemmArgs w, const Colum
   hipLaunchKernelGGL((join_pair_kernel<T>), dim3(unsigned(jx + jw)), dim3(256), 0, st, x, w, int(jx));
 }
 
-// packs p, q or both (rows 0: not)
+// p, q or both (rows 0: not) in a launch of their own
 template <class T>
-inline void pack(hipStream_t st, Pack p, Pack q, int64_t cols) {
-  if (!p.rows) std::swap(p, q);
-  if (!p.rows) return;
-  const unsigned a = unsigned((p.rows + 15) / 16), b = unsigned((q.rows + 15) / 16);
-  hipLaunchKernelGGL((pack_kernel<T>), dim3(a + b), dim3(256), 0, st, p, q, a, int(cols), int(round8(cols)));
+inline void pack(hipStream_t st, const Packs& k) {
+  const unsigned blocks = k.blocks + pack_blocks(k.q);
+  if (blocks) hipLaunchKernelGGL((pack_kernel<T>), dim3(blocks), dim3(256), 0, st, k.p, k.q, k.blocks, k.cols, k.ld);
 }
+inline Packs packs_of(const Pack& p, const Pack& q, int64_t cols) { return Packs{p, q, pack_blocks(p), int(cols), int(round8(cols))}; }
 
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -785,7 +798,7 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       a.A = x; a.lda = K;
       a.B = weight; a.ldb = K;
       const bool px = packed(x, K), pw = packed(weight, K);
-      pack<T>(st, Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
+      pack<T>(st, packs_of(Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K));
       if (px) { a.A = ws + plan.x; a.lda = round8(K); }
       if (pw) { a.B = ws + plan.weight; a.ldb = round8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
@@ -816,12 +829,14 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
     if constexpr (sizeof(T) == 2) {
       const int64_t ldn = round8(N), ldk = round8(K);
       T* gz = plan.same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
+      const bool px = dweight && packed(x, K), pw = dx && packed(weight, K);
+      const Packs packs = packs_of(Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
       Columns columns{};
       if (!plan.same || dbias)
         columns = make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
-                             reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta);
-      const bool px = dweight && packed(x, K), pw = dx && packed(weight, K);
-      pack<T>(st, Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
+                             reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta, packs);
+      else
+        pack<T>(st, packs);
       GemmArgs ax{}, aw{};
       ax.A = aw.A = gz;
       ax.lda = aw.lda = ldn;
