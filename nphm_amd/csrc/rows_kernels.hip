@@ -240,17 +240,33 @@ struct SortArgs {
   int shift, bits, per_block, blocks;
 };
 
-// The rows that no index names are zeros: the launches that sort, which leave most of the chip idle, clear the whole result with the
-// blocks behind their own, a share each, and the sums are written over it (50000 x 2048 bf16, 32768 indices: 102 us with the
-// rows told apart by a flag and cleared beside the sums, 94 so).  In units of 16 bits.
+// The rows that no index names are zeros: the launches that sort, which leave most of the chip idle, clear the result with the blocks
+// behind their own, a share each.  Either all of it, and the sums are written over it, or, where rows are long and enough of them are
+// named, only the others: the first launch writes a place where it met a row to mark[row], and a row is named if the place that its
+// mark holds names it (so marks are never cleared: whatever an untouched one holds, its place is looked up).  In units of 16 bits.
 struct Zero {
   void* out;
-  int64_t first, last;
+  int64_t first, last;                 // with marks: rows
   int blocks;                          // the launch's own, in front
+  const int* mark;                     // null: all is cleared
+  int each;                            // rows a wavefront
+  int64_t row;                         // units of one
 };
 constexpr int64_t ZERO_UNITS = 32768;                                // 64 KiB a block
-__device__ __forceinline__ bool cleared(const Zero& z) {             // whether this was one of the blocks that clear
+__device__ __forceinline__ bool cleared(const GradArgs& p, const Zero& z) {      // whether this was one of the blocks that clear
   if (int(blockIdx.x) < z.blocks) return false;
+  if (z.mark) {
+    const int lane = threadIdx.x & 63;
+    const int64_t v0 = z.first + (int64_t(blockIdx.x - z.blocks) * (blockDim.x >> 6) + (threadIdx.x >> 6)) * z.each, v = v0 + lane;
+    bool open = lane < z.each && v < z.last;
+    if (open) {
+      const int m = z.mark[v];
+      open = m < 0 || m >= p.count || key_of(p, m) != v;
+    }
+    for (uint64_t rows = __ballot(open); rows; rows &= rows - 1)
+      zero_run(static_cast<bf16*>(z.out) + (v0 + __builtin_ctzll(rows)) * z.row, z.row, lane, 64);
+    return true;
+  }
   const int64_t at = z.first + int64_t(blockIdx.x - z.blocks) * ZERO_UNITS;
   zero_run(static_cast<bf16*>(z.out) + at, min(ZERO_UNITS, z.last - at), threadIdx.x, blockDim.x);
   return true;
@@ -266,7 +282,7 @@ __global__ __launch_bounds__(256) void rank_kernel(GradArgs p, SortArgs s, Zero 
   extern __shared__ __attribute__((aligned(16))) int all[];
   __shared__ int part[RANGE][PLACED];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
-  if (cleared(z)) return;
+  if (cleared(p, z)) return;
   const int count = int(p.count), padded = (count + 63) / 64 * 64, each = padded / RANGE;
 #pragma unroll 8
   for (int n = threadIdx.x; n < padded; n += 256) all[n] = n < count ? key_of(p, n) : 0x7ffffffe;
@@ -306,15 +322,19 @@ __global__ __launch_bounds__(256) void rank_kernel(GradArgs p, SortArgs s, Zero 
 constexpr int MAX_DIGIT = 9;
 
 template <bool FIRST>
-__global__ __launch_bounds__(1024) void radix_hist_kernel(GradArgs p, const int* __restrict__ keys, SortArgs s, Zero z) {
+__global__ __launch_bounds__(1024) void radix_hist_kernel(GradArgs p, const int* __restrict__ keys, SortArgs s, int* mark, Zero z) {
   __shared__ int bins[1 << MAX_DIGIT];
-  if (cleared(z)) return;
+  if (cleared(p, z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x;
   for (int d = t; d < digits; d += 1024) bins[d] = 0;
   __syncthreads();
   const int64_t first = int64_t(blockIdx.x) * s.per_block;
-  for (int u = t; u < s.per_block; u += 1024)
-    if (first + u < p.count) atomicAdd(&bins[((FIRST ? key_of(p, first + u) : keys[first + u]) >> s.shift) & (digits - 1)], 1);
+  for (int u = t; u < s.per_block; u += 1024) {
+    if (first + u >= p.count) break;
+    const int key = FIRST ? key_of(p, first + u) : keys[first + u];
+    atomicAdd(&bins[(key >> s.shift) & (digits - 1)], 1);
+    if (FIRST && mark && key < p.rows) mark[key] = int(first + u);   // (any of them)
+  }
   __syncthreads();
   for (int d = t; d < digits; d += 1024) s.hist[blockIdx.x * digits + d] = bins[d];
 }
@@ -325,7 +345,7 @@ template <bool FIRST>
 __global__ __launch_bounds__(1024) void radix_place_kernel(GradArgs p, const int* __restrict__ keys, const int* __restrict__ perm, SortArgs s,
                                                            int* __restrict__ keys_out, int* __restrict__ perm_out, Zero z) {
   __shared__ int base[1 << MAX_DIGIT], scan[1 << MAX_DIGIT], seen[16][1 << MAX_DIGIT];
-  if (cleared(z)) return;
+  if (cleared(p, z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   {
     // 1024 / digits threads a digit, each over every so many blocks
@@ -517,7 +537,8 @@ __global__ __launch_bounds__(64 * JOINERS) void join_kernel(GradArgs p, SumArgs 
 
 struct GradPlan {
   int passes, bits, blocks, per_block, chunk, chunks, tiles;
-  size_t sorted, perm, sorted2, perm2, hist, partial, total;
+  bool marks;
+  size_t sorted, perm, sorted2, perm2, hist, mark, partial, total;
 };
 inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element) {
   GradPlan g{};
@@ -542,7 +563,10 @@ inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element)
   g.sorted2 = 2 * ints;
   g.perm2 = g.sorted2 + other;
   g.hist = g.perm2 + other;
-  g.partial = g.hist + (g.passes ? up(size_t(g.blocks) * 4 << g.bits) : 0);
+  // marks (a look at each row for those that need not be cleared): 50000 x 2048 bf16 with 24 000 rows named
+  g.marks = g.passes && dim * element >= 1024 && count >= rows / 8;
+  g.mark = g.hist + (g.passes ? up(size_t(g.blocks) * 4 << g.bits) : 0);
+  g.partial = g.mark + (g.marks ? up(size_t(rows) * 4) : 0);
   g.total = g.partial + up(size_t(2) * g.chunks * g.tiles * 64 * vec * 4);
   return g;
 }
@@ -575,8 +599,16 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   // launch k of `launches` clears its share with the blocks behind its own
   const int launches = g.passes ? 2 * g.passes : 1;
   const int64_t units = out_rows * a.dim * int64_t(sizeof(T) / 2), share = (units / launches + ZERO_UNITS) / ZERO_UNITS * ZERO_UNITS;
+  int* const marks = !MERGE && g.marks ? reinterpret_cast<int*>(ws + g.mark) : nullptr;
   auto zero = [&](int k, int blocks, unsigned& grid) {
-    Zero z{a.out, std::min(units, k * share), std::min(units, (k + 1) * share), blocks};
+    if (marks) {                                                     // (not in the first launch: it makes the marks)
+      const int64_t each = std::max<int64_t>(1, std::min<int64_t>(64, 8192 / (a.dim * int64_t(sizeof(T))))), block = 16 * each;
+      const int64_t part = (a.rows / (launches - 1) + block) / block * block;
+      Zero z{a.out, k ? std::min(a.rows, (k - 1) * part) : 0, std::min(a.rows, k * part), blocks, marks, int(each), a.dim * int64_t(sizeof(T) / 2)};
+      grid = unsigned(blocks + (z.last - z.first + block - 1) / block);
+      return z;
+    }
+    Zero z{a.out, std::min(units, k * share), std::min(units, (k + 1) * share), blocks, nullptr, 0, 0};
     grid = unsigned(blocks + (z.last - z.first + ZERO_UNITS - 1) / ZERO_UNITS);
     return z;
   };
@@ -591,8 +623,8 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
     int *kout = to_sorted ? s.sorted : s.sorted2, *pout = to_sorted ? s.perm : s.perm2;
     s.shift = pass * g.bits;
     Zero z = zero(2 * pass, g.blocks, grid);
-    if (pass == 0) hipLaunchKernelGGL((radix_hist_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, s, z);
-    else hipLaunchKernelGGL((radix_hist_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, s, z);
+    if (pass == 0) hipLaunchKernelGGL((radix_hist_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
+    else hipLaunchKernelGGL((radix_hist_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
     z = zero(2 * pass + 1, g.blocks, grid);
     if (pass == 0) hipLaunchKernelGGL((radix_place_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
     else hipLaunchKernelGGL((radix_place_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);

@@ -215,6 +215,27 @@ def test_sparse_gradient_has_an_entry_for_every_index(dev, t, V, D, N):
 
 
 @gpu
+@pytest.mark.parametrize("t", FLOATS)
+@pytest.mark.parametrize("V,D,N", [(9, 600, 9000), (700, 515, 9001), (20011, 640, 9000), (60000, 512, 8193), (5000, 5001, 10000)])
+def test_long_rows_named_by_many_indices(dev, t, V, D, N):
+    """one call after another on the memory that the call before left: rows that nobody names are zeros, padding and foreign indices too"""
+    gen = torch.Generator().manual_seed(V + D + N)
+    g = torch.randn(N, D, generator=gen).to(t).to(dev)
+    for turn in range(3):
+        idx = torch.randint(-2, V + 2, (N,), generator=gen)
+        idx[: N // 3] = (idx[: N // 3] % max(1, V // 50)) * min(V, 49)        # some rows over and over, and rows that nobody names
+        idx = idx.clamp(max=V + 1).to(dev)
+        padding = None if turn == 0 else V // 2
+        keep = (idx >= 0) & (idx < V) & (idx != (-7 if padding is None else padding))
+        got = T.lookup_rows_grad(g, idx.int() if turn == 2 else idx, V, padding_idx=padding)
+        want = torch.zeros(V, D, dtype=torch.float64, device=dev).index_put_((idx[keep],), g[keep].double(), accumulate=True)
+        mag = torch.zeros(V, D, dtype=torch.float64, device=dev).index_put_((idx[keep],), g[keep].double().abs(), accumulate=True)
+        many = torch.bincount(idx[keep], minlength=V)[:, None].double()
+        within(got, want, mag * (many + 2) * F32 + want.abs() * (half_step(t) + F32) + tiny(t))
+        assert not got[many[:, 0] == 0].any()
+
+
+@gpu
 def test_row_gradients_do_not_overflow_in_sums(dev):
     """fp16 rows whose partial sums leave the type's range and come back"""
     g = torch.full((2000, 24), 60000.0, dtype=torch.float16, device=dev)
