@@ -272,20 +272,22 @@ __device__ __forceinline__ bool cleared(const GradArgs& p, const Zero& z) {     
   return true;
 }
 
-// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 16 keys: all keys are in LDS, its four wavefronts count
-// over a quarter of them each and the four 16-lane rows of a wavefront over a quarter of that (a read of four keys is the same for 16
-// lanes).  count^2 comparisons spread over the chip, one launch: 10 us for 4097 keys against 19 for the radix passes below, which
-// are faster above 8192 (16384 keys: 57 us against 20).
-constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 16;               // keys a block places; ranges that all keys are cut into
+// Up to MIDDLE keys: a key's place is the number of keys before it.  A block places 16 keys: all keys are in LDS, its 64 rows of 16 lanes
+// count over a 64th of them each (a read of four keys is the same for 16 lanes).  count^2 comparisons spread over the chip, one
+// launch: 8.6 us for 4097 keys (14 with four wavefronts a block: one a SIMD waits for every read); a whole gradient of 8192 rows of
+// 64 takes 21 us against 27 with the radix passes below, of 15000 rows 45 against 31.
+constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 64;               // keys a block places; ranges that all keys are cut into
 
-__global__ __launch_bounds__(256) void rank_kernel(GradArgs p, SortArgs s, Zero z) {
+__host__ __device__ inline int rank_room(int count) { return (count + 4 * RANGE - 1) / (4 * RANGE) * (4 * RANGE); }     // (whole reads a range)
+
+__global__ __launch_bounds__(PLACED * RANGE) void rank_kernel(GradArgs p, SortArgs s, Zero z) {
   extern __shared__ __attribute__((aligned(16))) int all[];
   __shared__ int part[RANGE][PLACED];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
   if (cleared(p, z)) return;
-  const int count = int(p.count), padded = (count + 63) / 64 * 64, each = padded / RANGE;
+  const int count = int(p.count), padded = rank_room(count), each = padded / RANGE;
 #pragma unroll 8
-  for (int n = threadIdx.x; n < padded; n += 256) all[n] = n < count ? key_of(p, n) : 0x7ffffffe;
+  for (int n = threadIdx.x; n < padded; n += PLACED * RANGE) all[n] = n < count ? key_of(p, n) : 0x7ffffffe;
   __syncthreads();
   const int range = threadIdx.x / PLACED, own0 = blockIdx.x * PLACED, i = own0 + threadIdx.x % PLACED;
   const int own = all[i];
@@ -615,7 +617,7 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   unsigned grid = 0;
   if (!g.passes) {
     const Zero z = zero(0, int((a.count + PLACED - 1) / PLACED), grid);
-    hipLaunchKernelGGL(rank_kernel, dim3(grid), dim3(256), unsigned((a.count + 63) / 64 * 64 * 4), st, a, s, z);
+    hipLaunchKernelGGL(rank_kernel, dim3(grid), dim3(PLACED * RANGE), unsigned(rank_room(int(a.count)) * 4), st, a, s, z);
   }
   const int *kin = nullptr, *pin = nullptr;
   for (int pass = 0; pass < g.passes; ++pass) {                      // indices -> other -> ... -> sorted, whatever the number of passes
