@@ -205,12 +205,13 @@ _TORCH_ENTRIES = ("nphm_last_error", "nphm_rows_lookup", "nphm_rows_grad_workspa
                   "nphm_rows_renorm", "nphm_clip_workspace_bytes", "nphm_clip_grads", "nphm_layer16_forward_workspace_bytes",
                   "nphm_layer16_forward", "nphm_layer16_backward_workspace_bytes", "nphm_layer16_backward")
 _torch_ops = None
+torch_clip = None                        # (grads, out, kind, limit, what) -> norm, once load_torch has run
 
 
 def load_torch():
     """torch.ops.nphm_amd: the training operators of libnphm_torch.so on the kernels of the library that ``load`` has loaded (once).  Raises
     NphmAmdError if either is not built."""
-    global _torch_ops
+    global _torch_ops, torch_clip
     if _torch_ops is not None:
         return _torch_ops
     lib = load()
@@ -221,6 +222,8 @@ def load_torch():
     table = (c_void_p * len(_TORCH_ENTRIES))(*[ctypes.cast(getattr(lib, name), c_void_p).value for name in _TORCH_ENTRIES])
     if ctypes.CDLL(TORCH_LIB_PATH).nphm_torch_bind(table, len(table)) != 0:
         raise NphmAmdError("libnphm_torch.so and nphm_amd are of different versions: build them again")
+    torch_clip = ctypes.PyDLL(TORCH_LIB_PATH).nphm_torch_clip
+    torch_clip.restype, torch_clip.argtypes = ctypes.py_object, [ctypes.py_object, ctypes.py_object, c_int, ctypes.c_double, c_char_p]
     _torch_ops = torch.ops.nphm_amd
     return _torch_ops
 

@@ -6,6 +6,7 @@ import hashlib
 import os
 import shutil
 import subprocess
+import sysconfig
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -98,7 +99,7 @@ def _build_torch(force: bool, verbose: bool):
         h.update(open(f, "rb").read())
     obj = os.path.join(OBJ_CACHE, f"torch_ops-{h.hexdigest()[:20]}.o")
     if force or not os.path.exists(obj):
-        inc = [f for p in cpp_extension.include_paths("cuda") for f in ("-isystem", p)]
+        inc = [f for p in cpp_extension.include_paths("cuda") + [sysconfig.get_paths()["include"]] for f in ("-isystem", p)]
         cmd = [os.environ.get("CXX", "g++"), "-O2", "-std=c++17", "-fPIC", "-fvisibility=hidden", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
                f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"] + inc + ["-c", src, "-o", f"{obj}.{os.getpid()}.tmp"]
         if verbose:
@@ -107,7 +108,7 @@ def _build_torch(force: bool, verbose: bool):
         os.replace(f"{obj}.{os.getpid()}.tmp", obj)
     tmp = f"{TORCH_OUT}.{os.getpid()}.tmp"
     libs = [f for p in cpp_extension.library_paths("cuda") for f in ("-L", p)]
-    subprocess.run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", obj] + libs + ["-ltorch", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-o", tmp],
+    subprocess.run([os.environ.get("CXX", "g++"), "-shared", "-fPIC", obj] + libs + ["-ltorch", "-ltorch_python", "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip", "-o", tmp],
                    check=True)
     os.replace(tmp, TORCH_OUT)
     for f in os.listdir(OBJ_CACHE):

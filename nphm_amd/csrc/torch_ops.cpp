@@ -3,11 +3,15 @@
 // build of that library the process has loaded).  In C++ because a layer of a few hundred rows takes 20 us on the card, and
 // the same node written in Python took 130 on the host (its backward pass runs in a thread of autograd's own and waits for the
 // interpreter there); a list of 500 gradients took 280 to look through.
+#include <Python.h>
+
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
+#include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
 
 #include <algorithm>
@@ -277,19 +281,34 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
 
 // ---- global gradient norm ----------------------------------------------------------------------------------------------------------
 
-// -> norm; `out` empty: the norm alone.  out[i] may be grads[i] itself.
-Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, int64_t kind, double limit, const std::string& what) {
+// the tensors of a Python list (of the caller's own: it keeps them alive)
+std::vector<const Tensor*> tensors_of(const std::string& what, PyObject* list) {
+  TORCH_CHECK_TYPE(PyList_Check(list), what, ": a list of tensors");
+  std::vector<const Tensor*> all(size_t(PyList_GET_SIZE(list)));
+  for (size_t i = 0; i < all.size(); ++i) {
+    PyObject* item = PyList_GET_ITEM(list, Py_ssize_t(i));
+    TORCH_CHECK_TYPE(THPVariable_Check(item), what, ": tensors, not ", Py_TYPE(item)->tp_name);
+    all[i] = &THPVariable_Unpack(item);
+  }
+  return all;
+}
+
+// -> norm; `out` None: the norm alone, the list itself: in place.  out[i] may be grads[i].
+Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, int kind, double limit) {
   bound();
+  const std::vector<const Tensor*> grads = tensors_of(what, grad_list),
+                                   out = out_list == Py_None ? std::vector<const Tensor*>{} : out_list == grad_list ? grads : tensors_of(what, out_list);
   const size_t n = grads.size();
-  const bool writes = !out.empty();
+  const bool writes = !out.empty(), in_place = out_list == grad_list;
   TORCH_CHECK_VALUE(n && (!writes || out.size() == n), what, ": ", n, " gradients, ", out.size(), " tensors in out");
   const at::NoGradGuard no_grad;
-  for (const Tensor& g : grads) {
-    TORCH_CHECK_TYPE(g.is_cuda() && g.layout() == at::kStrided, what, ": dense tensors on a ROCm device (these operators have no CPU form)");
-    TORCH_CHECK_TYPE(code_of(g.scalar_type()) >= 0, what, ": fp32, bf16 or fp16 gradients, not ", g.scalar_type());
-    TORCH_CHECK_VALUE(g.device() == grads[0].device(), what, ": gradients on ", grads[0].device(), " and ", g.device(), ": one call takes one device's");
+  const at::Device device = grads[0]->device();
+  for (const Tensor* g : grads) {
+    TORCH_CHECK_TYPE(g->is_cuda() && g->layout() == at::kStrided, what, ": dense tensors on a ROCm device (these operators have no CPU form)");
+    TORCH_CHECK_TYPE(code_of(g->scalar_type()) >= 0, what, ": fp32, bf16 or fp16 gradients, not ", g->scalar_type());
+    TORCH_CHECK_VALUE(g->device() == device, what, ": gradients on ", device, " and ", g->device(), ": one call takes one device's");
   }
-  const c10::DeviceGuard guard(grads[0].device());
+  const c10::DeviceGuard guard(device);
   std::vector<const void*> from(n);
   std::vector<void*> to(writes ? n : 0);
   std::vector<int64_t> counts(n);
@@ -297,23 +316,23 @@ Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, in
   std::vector<Tensor> held;                                          // copies that the launches read or write
   std::vector<std::pair<Tensor, Tensor>> back;
   for (size_t i = 0; i < n; ++i) {
-    Tensor g = grads[i], o = writes ? out[i] : g;
-    TORCH_CHECK_VALUE(o.numel() == g.numel() && o.scalar_type() == g.scalar_type() && o.device() == g.device() && o.layout() == at::kStrided, what,
-                      ": out has a tensor of the size, type and device of each gradient");
+    const Tensor *g = grads[i], *o = writes ? out[i] : g;
+    TORCH_CHECK_VALUE(in_place || (o->numel() == g->numel() && o->scalar_type() == g->scalar_type() && o->device() == device && o->layout() == at::kStrided),
+                      what, ": out has a tensor of the size, type and device of each gradient");
+    counts[i] = g->numel();
+    codes[i] = code_of(g->scalar_type());
     // any order of dimensions will do, if it is the same on both sides and leaves no gap
-    if (!(g.is_contiguous() && o.is_contiguous()) && !(g.is_non_overlapping_and_dense() && g.sizes() == o.sizes() && g.strides() == o.strides())) {
-      g = g.contiguous();
-      if (writes) {
-        Tensor flat = at::empty_like(g);
-        back.emplace_back(o, flat);
-        o = flat;
-      }
-      held.push_back(g);
+    if (!(g->is_contiguous() && (in_place || o->is_contiguous()))
+        && !(g->is_non_overlapping_and_dense() && g->sizes() == o->sizes() && g->strides() == o->strides())) {
+      held.push_back(g->contiguous());
+      from[i] = held.back().const_data_ptr();
+      if (!writes) continue;
+      back.emplace_back(*o, at::empty_like(held.back()));
+      to[i] = back.back().second.mutable_data_ptr();
+      continue;
     }
-    from[i] = const_of(g);
-    if (writes) to[i] = at_of(o);
-    counts[i] = g.numel();
-    codes[i] = code_of(g.scalar_type());
+    from[i] = g->const_data_ptr();
+    if (writes) to[i] = o->mutable_data_ptr();
   }
   if (back.size() > 1) {                                             // (the others' memory is compared behind the C entry)
     std::vector<const void*> starts;
@@ -322,11 +341,15 @@ Tensor clip(const std::vector<Tensor>& grads, const std::vector<Tensor>& out, in
     TORCH_CHECK(std::adjacent_find(starts.begin(), starts.end()) == starts.end(), "nphm: ", what, ": two of the tensors share memory");
   }
   const size_t need = lib.clip_ws(counts.data(), int(n));
-  Tensor ws = workspace(need, grads[0]), norm = at::empty({}, grads[0].options().dtype(at::kFloat).requires_grad(false));
-  check(lib.clip(from.data(), writes ? to.data() : nullptr, counts.data(), codes.data(), int(n), int(kind), limit,
-                 static_cast<float*>(norm.mutable_data_ptr()), at_of(ws), need, stream_of(grads[0])), "nphm_clip_grads");
+  const Tensor ws = workspace(need, *grads[0]), norm = at::empty({}, grads[0]->options().dtype(at::kFloat).requires_grad(false));
+  void* const stream = stream_of(*grads[0]);
+  PyThreadState* const python = PyEval_SaveThread();                 // (no exception leaves a C entry)
+  const int rc = lib.clip(from.data(), writes ? to.data() : nullptr, counts.data(), codes.data(), int(n), kind, limit,
+                          static_cast<float*>(norm.mutable_data_ptr()), at_of(ws), need, stream);
+  PyEval_RestoreThread(python);
+  check(rc, "nphm_clip_grads");
   for (auto& [o, flat] : back) o.copy_(flat.view(o.sizes()));
-  for (const Tensor& o : out) written(o);
+  for (const Tensor* o : out) written(*o);
   return norm;
 }
 
@@ -354,11 +377,18 @@ extern "C" __attribute__((visibility("default"))) int nphm_torch_bind(void* cons
   return 0;
 }
 
+// clip for Python: through the dispatcher 500 tensors in two lists took 60 us to hand over, 10 so.  A new reference to the norm, or null with the
+// exception set.
+extern "C" __attribute__((visibility("default"))) PyObject* nphm_torch_clip(PyObject* grads, PyObject* out, int kind, double limit, const char* what) {
+  HANDLE_TH_ERRORS
+  return THPVariable_Wrap(clip(what, grads, out, kind, limit));
+  END_HANDLE_TH_ERRORS
+}
+
 TORCH_LIBRARY(nphm_amd, m) {
   m.def("lookup_rows(Tensor table, Tensor idx, float scale, int? padding_idx, bool sparse) -> Tensor", &lookup_rows);
   m.def("lookup_rows_grad(Tensor grad, Tensor idx, int num_rows, float scale, int? padding_idx) -> Tensor", &rows_grad);
   m.def("renorm_rows_(Tensor(a!) table, Tensor idx, float max_norm) -> ()", &renorm_rows);
   m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float beta) -> Tensor", &linear_act);
-  m.def("clip(Tensor[] grads, Tensor[] out, int kind, float limit, str what) -> Tensor", &clip);
   m.def("merge_rows_(Tensor index, Tensor(a!) values, int rows) -> ()", &merge_rows);
 }

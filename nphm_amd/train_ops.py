@@ -31,7 +31,8 @@ class _Ops:
     """The operators of libnphm_torch.so; the library is loaded at the first use of one."""
 
     def __getattr__(self, name):
-        op = getattr(_lib.load_torch(), name).default
+        ops = _lib.load_torch()
+        op = _lib.torch_clip if name == "clip" else getattr(ops, name).default
 
         def call(*args):
             try:
@@ -129,7 +130,7 @@ def grad_norm(grads, norm_type=2.0):
     fp16, mixed): a 0-dim fp32 tensor on their device."""
     kind = _kind("grad_norm", norm_type)
     grads = list(grads)
-    return _ops.clip(grads, [], kind, 0.0, "grad_norm") if grads else torch.zeros(())
+    return _ops.clip(grads, None, kind, 0.0, b"grad_norm") if grads else torch.zeros(())
 
 
 def clip_grads(grads, max_norm, norm_type=2.0, out=None):
@@ -145,7 +146,7 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
         raise ValueError(f"{what}: {len(grads)} gradients, {len(written)} tensors in out")
     if not grads:
         return torch.zeros(()), written
-    return _ops.clip(grads, written, kind, limit, what), written
+    return _ops.clip(grads, written, kind, limit, what.encode()), written
 
 
 def _merge_rows_(g):
@@ -181,7 +182,7 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
     if not grads:
         return torch.zeros(())
     if error_if_nonfinite:
-        norm = _ops.clip(grads, [], kind, 0.0, what)
+        norm = _ops.clip(grads, None, kind, 0.0, what.encode())
         if not bool(torch.isfinite(norm)):
             raise RuntimeError(f"{what}: the norm of the gradients is {float(norm)}; none was scaled")
-    return _ops.clip(grads, grads, kind, limit, what)
+    return _ops.clip(grads, grads, kind, limit, what.encode())
