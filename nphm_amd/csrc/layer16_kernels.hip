@@ -437,25 +437,45 @@ __global__ __launch_bounds__(256) void pack_kernel(Pack p, Pack q, unsigned bloc
 }
 
 // the partial products of all k ranges, added in order, and what the tiles' epilogue does otherwise; a thread takes eight elements beside
-// each other, across the ends of rows
+// each other, across the ends of rows.  From SLICED ranges on (small results, then) eight threads share them, every eighth range each.
+constexpr int SLICED = 16, SLICES = 8;
+
 template <class T, int OUT>
 __device__ __forceinline__ void join_splits(const GemmArgs& p, int block, int blocks) {
+  __shared__ float part[SLICES - 1][256 / SLICES][9];
   const int64_t count = int64_t(p.I) * p.J;
-  for (int64_t at = (int64_t(block) * 256 + threadIdx.x) * 8; at < count; at += int64_t(blocks) * 2048) {
+  const bool sliced = p.splits >= SLICED;
+  const int step = sliced ? SLICES : 1, per = 256 / step, slice = sliced ? threadIdx.x / per : 0, piece = threadIdx.x % per;
+  for (int64_t base = int64_t(block) * per * 8; base < count; base += int64_t(blocks) * per * 8) {
+    const int64_t at = base + piece * 8;
     const int width = int(min(count - at, int64_t(8)));
     float v[8] = {};
+    if (width == 8) {
 #pragma unroll 4
-    for (int s = 0; s < p.splits; ++s) {
-      const float* q = p.parts + int64_t(s) * count + at;
-      if (width == 8) {
+      for (int s = slice; s < p.splits; s += step) {
+        const float* q = p.parts + int64_t(s) * count + at;
         const f32x4_u lo = *reinterpret_cast<const f32x4_u*>(q), hi = *reinterpret_cast<const f32x4_u*>(q + 4);
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] += lo[e], v[4 + e] += hi[e];
-      } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) if (e < width) v[e] += q[e];
       }
+    } else {
+      for (int s = slice; s < p.splits; s += step)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) if (e < width) v[e] += p.parts[int64_t(s) * count + at + e];
     }
+    if (sliced) {
+      if (slice)
+#pragma unroll
+        for (int e = 0; e < 8; ++e) part[slice - 1][piece][e] = v[e];
+      __syncthreads();
+      if (!slice)
+#pragma unroll
+        for (int w = 0; w < SLICES - 1; ++w)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) v[e] += part[w][piece][e];
+      __syncthreads();
+    }
+    if (slice || width <= 0) continue;
     if constexpr (OUT == OUT_LAYER) {
       if (p.bias) {
         int j = int(at % p.J);
@@ -626,29 +646,32 @@ inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sum
 inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
 
 struct Tiling { int size, splits; };               // size: 256, 128 or 64
-// Among the tiles that fill the 256 CUs the one with the least work, counting what it reaches over the ends: an element of a 128-tile costs 1.2
-// of one of a 256-tile, of a 64-tile 1.5 (16384 x 1024 x 1024: 36, 43, 67 us; 200000 x 64 x 64: 83, 42, 26); with one step of k all
-// cost about the same (5000 x 5000 x 64: 46, 42, 38).  Where none fills them, 64-tiles, or the k range in pieces, added by a second launch,
-// if there is enough of it: pieces of 1024 with tiles of 128 (1024 x 1024 x 16384: 46 us in four, 56 in tiles of 64), of 512 with tiles
-// of 64 (1 x 4096 x 4096: 9.6 us in eight, 32 whole; 1024 x 1024 x 1024: 8.5 us whole, 14 in two).
+// Among the tiles that fill the 256 CUs the size whose fullest CU is done first: a tile takes its steps of 64 k, times what an element of it
+// costs against one of a 256-tile (LDS is read more often for a smaller one), and as many steps again for its first loads and its
+// epilogue, of which small tiles hide more behind each other.  Fitted to 16384 x 1024 x 1024 (36, 43, 67 us in tiles of 256, 128, 64),
+// 5000 x 1000 x 5000 (-, 86, 120), 200000 x 64 x 64 (83, 42, 26), 5000 x 5000 x 64 (46, 42, 38); 35200 x 512 x 512: 33 us, 39 in tiles of 256,
+// of which the second round has 20.  Where none fills them, or 128-tiles do with the k range in pieces of 1024 and more, pieces, added by a
+// second launch: with tiles of 128 (1024 x 1024 x 16384: 46 us in four, 56 whole in tiles of 64; 1024 x 512 x 32768: 48 in eight, 104 in
+// two with tiles of 64), else of 64 (1 x 4096 x 4096: 9.6 us in eight, 32 whole; 128 x 128 x 100000: 18 us in 64, 46 in 16; 1024 x 1024 x
+// 1024: 8.5 us whole, 14 in two).
 inline Tiling tiling(int64_t I, int64_t J, int64_t K) {
   auto tiles = [&](int64_t b) { return ((I + b - 1) / b) * ((J + b - 1) / b); };
   const int64_t t128 = tiles(128), t64 = tiles(64);
-  const bool one = K <= BK;
-  int best = 0;
+  const double steps = double((K + BK - 1) / BK);
+  Tiling best{64, 1};
   double least = 0;
-  for (int size : {64, 128, 256}) {
-    if (tiles(size) < 192) continue;
-    const double cost = double(tiles(size)) * size * size * (size == 256 ? one ? 1.1 : 1.0 : size == 128 ? one ? 1.05 : 1.2 : one ? 1.0 : 1.5);
-    if (!best || cost < least) best = size, least = cost;
-  }
-  if (best > 64) return {best, 1};
-  if (best == 64) {
-    const int64_t s = (256 + t128 - 1) / t128;
-    return t128 < 192 && K >= 4096 && s * 1024 <= K ? Tiling{128, int(s)} : Tiling{64, 1};
-  }
-  if (K <= 1024) return {64, 1};
-  const int64_t fill = I <= 64 ? 512 : 256, s = std::min<int64_t>({(fill + t64 - 1) / t64, K / 512, 16});
+  auto offer = [&](int size, double element, double ends) {
+    if (tiles(size) < 192) return;
+    const double cost = double((tiles(size) + 255) / 256) * size * size * (element * steps + ends);
+    if (least == 0 || cost < least) best.size = size, least = cost;
+  };
+  offer(256, 1.0, 8.0);
+  offer(128, 1.4, 7.0);
+  offer(64, 2.8, 4.7);
+  const int64_t s128 = (256 + t128 - 1) / t128;
+  if (t128 < 192 && I > 64 && J > 64 && K >= 4096 && s128 * 1024 <= K) return {128, int(s128)};
+  if (least > 0 || K <= 1024) return best;
+  const int64_t fill = I <= 64 ? 512 : 256, s = std::min<int64_t>((fill + t64 - 1) / t64, K / 512);
   return {64, int(std::max<int64_t>(s, 1))};
 }
 inline size_t parts_bytes(const Tiling& t, int64_t I, int64_t J) { return t.splits > 1 ? up(size_t(t.splits) * I * J * 4) : 0; }
@@ -683,7 +706,7 @@ inline void split(GemmArgs& a, int splits) {
   a.splits = (a.K + a.k_per_split - 1) / a.k_per_split;
 }
 inline int64_t join_blocks(const GemmArgs& a) {
-  const int64_t want = (int64_t(a.I) * a.J + 2047) / 2048;
+  const int64_t each = a.splits >= SLICED ? 2048 / SLICES : 2048, want = (int64_t(a.I) * a.J + each - 1) / each;
   return want < 8192 ? want : 8192;
 }
 

@@ -384,7 +384,7 @@ def test_layer_and_gradients(dev, t, act, beta, M, N, K):
 @pytest.mark.parametrize("t", HALVES)
 @pytest.mark.parametrize("M,N,K", [(1, 1024, 512), (16, 333, 4096), (17, 40, 1000), (33, 2048, 96), (64, 3, 512), (129, 1, 8), (128, 128, 128), (256, 256, 256),
                                    (257, 513, 129), (1000, 512, 512), (4095, 96, 515), (2, 5000, 24), (3000, 8, 1344), (515, 1030, 1032),
-                                   (20000, 64, 72)])
+                                   (20000, 64, 72), (9, 70, 30000), (70000, 40, 72), (40000, 200, 130), (17000, 513, 300)])
 @pytest.mark.parametrize("bias,residual", [(True, False), (False, True)])
 def test_layer_sizes(dev, t, M, N, K, bias, residual):
     check_layer(dev, t, M, N, K, "softplus" if residual else "none", 20.0, bias=bias, residual=residual)
