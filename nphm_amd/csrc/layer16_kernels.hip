@@ -24,14 +24,16 @@ namespace nphm {
 namespace train_ops {
 
 typedef int v4i __attribute__((ext_vector_type(4)));
-typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef fp16 fp16x8 __attribute__((ext_vector_type(8)));
 template <class T> struct Frag;
 template <> struct Frag<bf16> { typedef bf16x8 type; };
 template <> struct Frag<fp16> { typedef fp16x8 type; };
-__device__ __forceinline__ f32x16 mfma(bf16x8 a, bf16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
-__device__ __forceinline__ f32x16 mfma(fp16x8 a, fp16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+// 16 x 16 x 32: on random numbers the chip's power lets it sustain 1990 TFLOP/s of these from registers, 1780 of the 32 x 32 x 16 ones, whose
+// accumulators move twice as often
+__device__ __forceinline__ f32x4 mfma(bf16x8 a, bf16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+__device__ __forceinline__ f32x4 mfma(fp16x8 a, fp16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
 enum { ACT_NONE = 0, ACT_RELU = 1, ACT_SILU = 2, ACT_GELU = 3, ACT_SOFTPLUS = 4 };
 
@@ -95,11 +97,14 @@ constexpr int SLOTS = 5;                 // tiles of one operand in LDS or on th
 
 // One operand's tile of ROWS rows (its i or j) x 64 k, on its way from memory to LDS and from there into fragments.
 // Not transposed: memory holds k beside k.  LDS row r: 128 bytes, its eight 16-byte pieces c at place c ^ (r / 2 % 8), so that the lanes of a
-//   fragment read (32 rows, the same k) meet every bank.  A fragment's 8 k are one ds_read_b128.
-// Transposed: memory holds row beside row.  LDS row k: 2 ROWS bytes, piece c at c ^ 2 (k % 4).  A fragment's 8 k are two ds_read_b64_tr: 16 lanes
-//   read 4 k x 16 rows and get them turned round.
+//   fragment read (16 rows, the same k) meet every bank.  A fragment's 8 k are one ds_read_b128.
+// Transposed: memory holds row beside row.  LDS row k: 2 ROWS bytes, piece c at c ^ 2 turn(k).  A fragment's 8 k are two ds_read_b64_tr: 16 lanes
+//   read 4 k x 16 rows and get them turned round; 32 lanes read k, k + 1, k + 2, k + 3 and the four 8 on, in different banks by turn.
 // Both are written by LDS-DMA (the destination is linear in the lane: the lanes load permuted pieces instead), 1 KiB an instruction.
 // Pieces behind the operand's end have an offset behind the buffer's: they arrive as zeros.
+template <int ROWS>
+__device__ __forceinline__ int turn(int k) { return ROWS >= 128 ? (k & 3) | ((k >> 3) & 1) << 2 : ((k >> 1) & 1) | ((k >> 3) & 1) << 1; }
+
 template <class T, int ROWS, int WAVES, bool TR>
 struct Operand {
   static constexpr int BYTES = ROWS * BK * 2, DMA = BYTES / 1024 / WAVES, CPR = TR ? ROWS / 8 : BK / 8;
@@ -117,7 +122,7 @@ struct Operand {
   __device__ __forceinline__ static int row_of(int d, int wave, int lane) { return ((d * WAVES + wave) * 64 + lane) / CPR; }
   __device__ __forceinline__ static int piece_of(int d, int wave, int lane) {
     const int row = row_of(d, wave, lane), at = lane % CPR;
-    return TR ? at ^ ((row & 3) << 1) : at ^ ((row >> 1) & 7);
+    return TR ? at ^ (turn<ROWS>(row) << 1) : at ^ ((row >> 1) & 7);
   }
   __device__ __forceinline__ void init(const void* P, int64_t ld_, int r0, int I, int K_, int wave, int lane, unsigned lds_first) {
     ld = ld_;
@@ -165,26 +170,22 @@ __device__ __forceinline__ void each(F&& f) {
 
 template <bool TR, int ROWS>
 struct Reader {
-  // lane -> its place in a fragment's rows; fragment (t, ks): rows w0 + 32 t .. + 31, k 16 ks .. + 15
-  unsigned at[TR ? 2 : 4];
+  // lane -> its place in a fragment's rows; fragment (t, ks): rows w0 + 16 t .. + 15, k 32 ks .. + 31
+  unsigned at;
   __device__ __forceinline__ void init(int w0, int lane) {
+    const int kg = lane >> 4;
     if constexpr (TR) {
-      const int r = (lane & 15) >> 2, q = lane & 3, kg = lane >> 5;
-#pragma unroll
-      for (int o = 0; o < 2; ++o) {
-        const int c = w0 / 8 + o * 4 + ((lane >> 4) & 1) * 2 + (q >> 1);
-        at[o] = unsigned((kg * 8 + r) * ROWS * 2 + ((c ^ (r << 1)) * 16) + (q & 1) * 8);
-      }
+      const int k = kg * 8 + ((lane & 15) >> 2), q = lane & 3, c = w0 / 8 + (q >> 1);
+      at = unsigned(k * ROWS * 2 + ((c ^ (turn<ROWS>(k) << 1)) * 16) + (q & 1) * 8);
     } else {
-      const int row = w0 + (lane & 31), kg = lane >> 5;
-#pragma unroll
-      for (int ks = 0; ks < 4; ++ks) at[ks] = unsigned(row * 128 + (((ks * 2 + kg) ^ ((row >> 1) & 7)) * 16));
+      const int row = w0 + (lane & 15);
+      at = unsigned(row * 128 + ((kg ^ ((row >> 1) & 7)) * 16));
     }
   }
   template <class F>
   __device__ __forceinline__ F read(const char* tile, int t, int ks) const {
     if constexpr (TR) {
-      const char* p = tile + at[t & 1] + (t >> 1) * 128 + ks * (16 * ROWS * 2);
+      const char* p = tile + (at ^ (t << 5)) + ks * (32 * ROWS * 2);
       typedef short s4 __attribute__((ext_vector_type(4)));
       typedef short s8 __attribute__((ext_vector_type(8)));
       typedef __attribute__((address_space(3))) s4 lds_s4;
@@ -193,7 +194,7 @@ struct Reader {
       const s8 v = {lo[0], lo[1], lo[2], lo[3], hi[0], hi[1], hi[2], hi[3]};
       return __builtin_bit_cast(F, v);
     } else {
-      return *reinterpret_cast<const F*>(tile + at[ks] + t * (32 * 128));
+      return *reinterpret_cast<const F*>(tile + (at ^ (ks << 6)) + t * (16 * 128));
     }
   }
 };
@@ -263,7 +264,7 @@ enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // E
 // stay and fetch the next tile's first steps while the last one's results leave: 209 us, for loads wait behind a wavefront's stores.
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, int OUT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
-  constexpr int WAVES = WM * WN, TM = BM / WM / 32, TN = BN / WN / 32;
+  constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
   typedef Operand<T, BM, WAVES, TA> OpA;
   typedef Operand<T, BN, WAVES, TB> OpB;
   constexpr unsigned SLOT = OpA::BYTES;
@@ -287,38 +288,48 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   b.init(p.B, p.ldb, j0, p.J, ke, wave, lane, lds0);
   Reader<TA, BM> ra;
   Reader<TB, BN> rb;
-  ra.init((wave / WN) * TM * 32, lane);
-  rb.init((wave % WN) * TN * 32, lane);
-  f32x16 acc[TM][TN];
+  ra.init((wave / WN) * TM * 16, lane);
+  rb.init((wave % WN) * TN * 16, lane);
+  f32x4 acc[TM][TN];
 #pragma unroll
   for (int x = 0; x < TM; ++x)
 #pragma unroll
-    for (int y = 0; y < TN; ++y) acc[x][y] = f32x16{};
+    for (int y = 0; y < TN; ++y) acc[x][y] = f32x4{};
   typedef typename Frag<T>::type frag;
 
-  // Fragments of k 16 ks .. come from LDS while the products of the 16 before them run, one read behind each product; the step's barrier
-  // stands in front of its last 16: behind it the first fragments of the next step are read and the loads of the one after it
-  // start, each behind a product too (a wavefront issues in order: a burst of either would leave the matrix pipe idle).
-  frag fa[2][TM], fb[2][TN];
+  // Fragments come from LDS while products run that do not need them, one or two reads behind a product: B's for the next 32 k beside those
+  // in use, an A fragment's successor into its own registers as soon as its last product is issued.  The step's barrier stands LEAD
+  // fragments of A into its last 32 k: the last read of this step is then old enough not to be waited for, and behind it the first
+  // fragments of the next step are read and the loads of the one after it start, each behind a product too (a wavefront issues in
+  // order: a burst of either would leave the matrix pipe idle).
+  constexpr int NMUL = TM * TN, NREAD = TM + TN, LEAD = TM >= 8 ? 2 : 1, EARLY = NMUL + LEAD * TN, LATE = NMUL - LEAD * TN;
+  frag fa[TM], fb[2][TN];
   auto read_one = [&](int set, const char* at, const char* bt, int ks, int n) __attribute__((always_inline)) {
     if (n < TN) fb[set][n] = rb.template read<frag>(bt, n, ks);
-    else if (n < TN + TM) fa[set][n - TN] = ra.template read<frag>(at, n - TN, ks);
+    else fa[n - TN] = ra.template read<frag>(at, n - TN, ks);
   };
-  auto multiply = [&](int set, auto&& behind) __attribute__((always_inline)) {
+  // behind product `m` of 32 k: those of the NREAD reads whose turn it is, spread over the products from `from` on; an A fragment's not before
+  // its last product
+  auto reads = [&](int set, const char* at, const char* bt, int ks, int m, int from) __attribute__((always_inline)) {
 #pragma unroll
-    for (int x = 0; x < TM; ++x)
-#pragma unroll
-      for (int y = 0; y < TN; ++y) {
-        acc[x][y] = mfma(fb[set][y], fa[set][x], acc[x][y]);
-        __builtin_amdgcn_sched_barrier(0);
-        behind(x * TN + y);
-        __builtin_amdgcn_sched_barrier(0);
-      }
+    for (int n = 0; n < NREAD; ++n) {
+      const int even = from + n * (NMUL - from) / NREAD, last = n < TN ? 0 : (n - TN + 1) * TN - 1;
+      if (m == (even > last ? even : last)) read_one(set, at, bt, ks, n);
+    }
   };
-  constexpr int NMUL = TM * TN, NREAD = TM + TN;
-  constexpr int RPM = (NREAD + NMUL - 1) / NMUL;                      // reads behind a product
+  // products [from, to) of 32 k
+  auto multiply = [&](int set, int from, int to, auto&& behind) __attribute__((always_inline)) {
+#pragma unroll
+    for (int m = 0; m < NMUL; ++m) {
+      if (m < from || m >= to) continue;
+      acc[m / TN][m % TN] = mfma(fb[set][m % TN], fa[m / TN], acc[m / TN][m % TN]);
+      __builtin_amdgcn_sched_barrier(0);
+      behind(m);
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
   // LDS holds five tiles, A and B in turn: A of step t in slot 2 t, B in slot 2 t + 1 (modulo 5).  Step t loads A of step t + 2 into the slot
-  // that B of step t - 1 has left, spread over its first three quarters, and behind the barrier B of step t + 2 into A's own slot:
+  // that B of step t - 1 has left, spread over what is in front of its barrier, and behind it B of step t + 2 into A's own slot:
   // the loads' rate is two thirds of what the path takes, in bursts it would hold up the products.
 #pragma unroll
   for (int u = 0; u < 4; ++u) {
@@ -337,24 +348,24 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   for (int n = 0; n < NREAD; ++n) read_one(0, lds + sa, lds + sb, 0, n);
   for (int k0 = kb; k0 < ke; k0 += BK) {
     a.aim(k0 + 2 * BK, lane, wave);
-#pragma unroll
-    for (int ks = 0; ks < 3; ++ks)
-      multiply(ks & 1, [&](int m) __attribute__((always_inline)) {
-#pragma unroll
-        for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one((ks + 1) & 1, lds + sa, lds + sb, ks + 1, n);
-        each<OpA::DMA>([&](auto d) __attribute__((always_inline)) {
-          if (decltype(d)::value * 3 * NMUL / OpA::DMA == ks * NMUL + m) a.template issue<decltype(d)::value>(sfree);
-        });
+    auto load_a = [&](int m) __attribute__((always_inline)) {
+      each<OpA::DMA>([&](auto d) __attribute__((always_inline)) {
+        if (decltype(d)::value * EARLY / OpA::DMA == m) a.template issue<decltype(d)::value>(sfree);
       });
+    };
+    multiply(0, 0, NMUL, [&](int m) __attribute__((always_inline)) {
+      reads(1, lds + sa, lds + sb, 1, m, 0);
+      load_a(m);
+    });
+    multiply(1, 0, LEAD * TN, [&](int m) __attribute__((always_inline)) { load_a(NMUL + m); });
     // the next step's tiles have landed (the A behind them may still be on its way), every wavefront has read this step's out
     asm volatile("s_waitcnt vmcnt(%0) lgkmcnt(0)\n\ts_barrier" ::"i"(OpA::DMA) : "memory");
     const unsigned na = two_on(sa), nb = two_on(sb);
     b.aim(k0 + 2 * BK, lane, wave);
-    multiply(1, [&](int m) __attribute__((always_inline)) {
-#pragma unroll
-      for (int n = m * RPM; n < m * RPM + RPM; ++n) read_one(0, lds + na, lds + nb, 0, n);       // (behind the last step: zeros)
+    multiply(1, LEAD * TN, NMUL, [&](int m) __attribute__((always_inline)) {
+      reads(0, lds + na, lds + nb, 0, m, LEAD * TN);                    // (behind the last step: nothing that is used)
       each<OpB::DMA>([&](auto d) __attribute__((always_inline)) {
-        if (decltype(d)::value * NMUL / OpB::DMA == m) b.template issue<decltype(d)::value>(sa);
+        if (LEAD * TN + decltype(d)::value * LATE / OpB::DMA == m) b.template issue<decltype(d)::value>(sa);
       });
     });
     sfree = sb;
@@ -362,10 +373,9 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
     sb = nb;
   }
 
-  // Register q of a lane: i = lane % 32, j = 8 (q / 4) + 4 (lane / 32) + q % 4 of its 32 x 32 tile.  Through LDS (every wavefront its own part
-  // of the tiles' room, 32 rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
-  typedef float f32x4 __attribute__((ext_vector_type(4)));
-  constexpr int COLS = TN * 32, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
+  // Register q of a lane: i = lane % 16, j = 4 (lane / 16) + q of its 16 x 16 tile.  Through LDS (every wavefront its own part of the tiles'
+  // room, 32 rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
+  constexpr int COLS = TN * 16, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
   static_assert(WAVES * 32 * PITCH * 4 <= SLOTS * SLOT, "the epilogue's rows fit the tiles' room");
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles, no load is on its way
   float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
@@ -373,16 +383,14 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   float bias[8] = {};
   if (OUT == OUT_LAYER && p.bias && width > 0) get8(bias, static_cast<const T*>(p.bias) + j, width);
 #pragma unroll
-  for (int x = 0; x < TM; ++x) {
+  for (int x = 0; x < TM / 2; ++x) {
 #pragma unroll
-    for (int y = 0; y < TN; ++y)
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-      for (int q4 = 0; q4 < 4; ++q4)
-        *reinterpret_cast<f32x4*>(out + (lane & 31) * PITCH + y * 32 + 8 * q4 + 4 * (lane >> 5)) =
-            f32x4{acc[x][y][4 * q4], acc[x][y][4 * q4 + 1], acc[x][y][4 * q4 + 2], acc[x][y][4 * q4 + 3]};
+      for (int y = 0; y < TN; ++y) *reinterpret_cast<f32x4*>(out + (h * 16 + (lane & 15)) * PITCH + y * 16 + 4 * (lane >> 4)) = acc[2 * x + h][y];
 #pragma nounroll
     for (int r = lane / LPR; r < 32; r += RPI) {
-      const int i = i0 + (wave / WN) * TM * 32 + x * 32 + r;
+      const int i = i0 + (wave / WN) * TM * 16 + x * 32 + r;
       if (i >= p.I || width <= 0) continue;
       float v[8];
       *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8);
@@ -401,8 +409,12 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   }
 }
 
+// wavefronts a SIMD that LDS has room for: told to the compiler, which would put fragments into accumulator registers and back for more
+// (1024 x 1024 x 16384 in tiles of 128: 62 us so, 44 told)
+constexpr int waves_of(int size) { return size == 64 ? 4 : 2; }
+
 template <class T, int B, int WM, int WN, bool TA, bool TB, int OUT>
-__global__ __launch_bounds__(64 * WM * WN) void gemm_kernel(GemmArgs p) {
+__global__ __launch_bounds__(64 * WM * WN) __attribute__((amdgpu_waves_per_eu(waves_of(B), waves_of(B)))) void gemm_kernel(GemmArgs p) {
   gemm_tile<T, B, B, WM, WN, TA, TB, OUT>(p, blockIdx.x);
 }
 
@@ -606,7 +618,7 @@ __global__ __launch_bounds__(256) void column_sums16_kernel(Columns c) {
 // dx, dW and the last sums of db side by side in one launch, where none of them fills the chip: blocks [0, bx) make dx in tiles of BX,
 // [bx, bw) dW in tiles of BW, the others db (4095 x 515 -> 1024: 25 us, 33 + 4 one after the other).
 template <class T, int BX, int BW>
-__global__ __launch_bounds__(256) void gradients_kernel(GemmArgs x, GemmArgs w, Columns c, int bx, int bw) {
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(waves_of(BX > BW ? BX : BW), waves_of(BX > BW ? BX : BW)))) void gradients_kernel(GemmArgs x, GemmArgs w, Columns c, int bx, int bw) {
   extern __shared__ __attribute__((aligned(1024))) char lds[];
   const int b = blockIdx.x;
   if (b < bx) gemm_tile<T, BX, BX, 2, 2, false, true, OUT_EITHER>(x, b);
