@@ -256,6 +256,37 @@ __device__ __forceinline__ void layer_out(float (&v)[8], const GemmArgs& p, int6
   put8(static_cast<T*>(p.C) + at, v, width);
 }
 
+// the same for U rows `row` elements apart, all there: what is asked once for them stands between them, not in front of each
+template <class T, int ACT, int U>
+__device__ __forceinline__ void layer_rows(float (&v)[U][8], const GemmArgs& p, int64_t at, int64_t row) {
+  if (p.z) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      float k[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) k[e] = float(keep<T>(v[u][e]));
+      put8(static_cast<T*>(p.z) + at + u * row, k, 8);
+    }
+  }
+  typename Vec<T>::type r[U];
+  if (p.residual) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) r[u] = *reinterpret_cast<const typename Vec<T>::type*>(static_cast<const T*>(p.residual) + at + u * row);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v[u][e] = act_value(v[u][e], ACT, p.beta);
+  if (p.residual) {
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+#pragma unroll
+      for (int e = 0; e < 8; ++e) v[u][e] += float(r[u][e]);
+  }
+#pragma unroll
+  for (int u = 0; u < U; ++u) put8(static_cast<T*>(p.C) + at + u * row, v[u], 8);
+}
+
 enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
 
 // One tile BM x BN of C[i, j] = sum_k A(i, k) B(j, k), by WM x WN wavefronts.  256 x 256 by eight: a wavefront's 128 x 64 is 128 accumulators a
@@ -374,36 +405,73 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   }
 
   // Register q of a lane: i = lane % 16, j = 4 (lane / 16) + q of its 16 x 16 tile.  Through LDS (every wavefront its own part of the tiles'
-  // room, 32 rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
-  constexpr int COLS = TN * 16, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR;
-  static_assert(WAVES * 32 * PITCH * 4 <= SLOTS * SLOT, "the epilogue's rows fit the tiles' room");
+  // room, AT rows at a time) to eight j beside each other a lane: whole 128-byte pieces of C, z and the residual.
+  constexpr int COLS = TN * 16, PITCH = COLS + 4, LPR = COLS / 8, RPI = 64 / LPR, AT = TM * 16 < 64 ? TM * 16 : 64, U = AT / RPI < 4 ? AT / RPI : 4;
+  static_assert(WAVES * AT * PITCH * 4 <= SLOTS * SLOT, "the epilogue's rows fit the tiles' room");
   asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");      // every wavefront has left the tiles, no load is on its way
-  float* out = reinterpret_cast<float*>(lds) + wave * 32 * PITCH;
+  float* out = reinterpret_cast<float*>(lds) + wave * AT * PITCH;
   const int j = j0 + (wave % WN) * COLS + (lane % LPR) * 8, width = min(8, p.J - j);
+  const bool inside = i0 + BM <= p.I && j0 + BN <= p.J;
+  const bool parts = OUT == OUT_PARTS || (OUT == OUT_EITHER && p.splits > 1);
+  float* const to_parts = p.parts + int64_t(split) * p.I * p.J;
   float bias[8] = {};
   if (OUT == OUT_LAYER && p.bias && width > 0) get8(bias, static_cast<const T*>(p.bias) + j, width);
-#pragma unroll
-  for (int x = 0; x < TM / 2; ++x) {
-#pragma unroll
-    for (int h = 0; h < 2; ++h)
-#pragma unroll
-      for (int y = 0; y < TN; ++y) *reinterpret_cast<f32x4*>(out + (h * 16 + (lane & 15)) * PITCH + y * 16 + 4 * (lane >> 4)) = acc[2 * x + h][y];
 #pragma nounroll
-    for (int r = lane / LPR; r < 32; r += RPI) {
-      const int i = i0 + (wave / WN) * TM * 16 + x * 32 + r;
-      if (i >= p.I || width <= 0) continue;
-      float v[8];
-      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8);
-      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(out + r * PITCH + (lane % LPR) * 8 + 4);
-      const int64_t at = int64_t(i) * p.J + j;
-      if (OUT == OUT_PARTS || (OUT == OUT_EITHER && p.splits > 1)) {
-        put8(p.parts + int64_t(split) * p.I * p.J + at, v, width);
-      } else if constexpr (OUT == OUT_LAYER) {
+  for (int x0 = 0; x0 < TM; x0 += AT / 16) {
+    each<TM * 16 / AT>([&](auto part) __attribute__((always_inline)) {
+      if (decltype(part)::value * (AT / 16) != x0) return;
+#pragma unroll
+      for (int x = 0; x < AT / 16; ++x)
+#pragma unroll
+        for (int y = 0; y < TN; ++y)
+          *reinterpret_cast<f32x4*>(out + (x * 16 + (lane & 15)) * PITCH + y * 16 + 4 * (lane >> 4)) = acc[decltype(part)::value * (AT / 16) + x][y];
+    });
+    const int i = i0 + (wave / WN) * TM * 16 + x0 * 16 + lane / LPR;
+    const float* from = out + lane / LPR * PITCH + (lane % LPR) * 8;
+    auto take = [&](float (&v)[8], int r) __attribute__((always_inline)) {
+      *reinterpret_cast<f32x4*>(v) = *reinterpret_cast<const f32x4*>(from + r * PITCH);
+      *reinterpret_cast<f32x4*>(v + 4) = *reinterpret_cast<const f32x4*>(from + r * PITCH + 4);
+      if constexpr (OUT == OUT_LAYER) {
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] += bias[e];
-        layer_out<T>(v, p, at, width);
+      }
+    };
+    if (inside) {                                                      // U rows at a time, without a look at the ends
+      auto rows = [&](auto act) __attribute__((always_inline)) {
+#pragma nounroll
+        for (int r = 0; r < AT; r += U * RPI) {
+          float v[U][8];
+          const int64_t at = int64_t(i + r) * p.J + j, row = int64_t(RPI) * p.J;
+#pragma unroll
+          for (int u = 0; u < U; ++u) take(v[u], r + u * RPI);
+          if constexpr (OUT == OUT_LAYER) {
+            layer_rows<T, decltype(act)::value, U>(v, p, at, row);
+          } else {
+#pragma unroll
+            for (int u = 0; u < U; ++u) {
+              if (parts) put8(to_parts + at + u * row, v[u], 8);
+              else put8(static_cast<T*>(p.C) + at + u * row, v[u], 8);
+            }
+          }
+        }
+      };
+      if constexpr (OUT == OUT_LAYER) {
+#define NPHM_EACH(A) case A: rows(std::integral_constant<int, A>{}); break
+        switch (p.act) { NPHM_EACH(ACT_NONE); NPHM_EACH(ACT_RELU); NPHM_EACH(ACT_SILU); NPHM_EACH(ACT_GELU); NPHM_EACH(ACT_SOFTPLUS); }
+#undef NPHM_EACH
       } else {
-        put8(static_cast<T*>(p.C) + at, v, width);
+        rows(std::integral_constant<int, ACT_NONE>{});
+      }
+    } else {
+#pragma nounroll
+      for (int r = 0; r < AT; r += RPI) {
+        if (i + r >= p.I || width <= 0) continue;
+        float v[8];
+        take(v, r);
+        const int64_t at = int64_t(i + r) * p.J + j;
+        if (parts) put8(to_parts + at, v, width);
+        else if constexpr (OUT == OUT_LAYER) layer_out<T>(v, p, at, width);
+        else put8(static_cast<T*>(p.C) + at, v, width);
       }
     }
   }
