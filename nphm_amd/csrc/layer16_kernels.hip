@@ -333,7 +333,7 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   // fragments of A into its last 32 k: the last read of this step is then old enough not to be waited for, and behind it the first
   // fragments of the next step are read and the loads of the one after it start, each behind a product too (a wavefront issues in
   // order: a burst of either would leave the matrix pipe idle).
-  constexpr int NMUL = TM * TN, NREAD = TM + TN, LEAD = TM >= 8 ? 2 : 1, EARLY = NMUL + LEAD * TN, LATE = NMUL - LEAD * TN;
+  constexpr int NMUL = TM * TN, NREAD = TM + TN, LEAD = TM < 8 ? 1 : TA ? 2 : 4, EARLY = NMUL + LEAD * TN, LATE = NMUL - LEAD * TN;
   frag fa[TM], fb[2][TN];
   auto read_one = [&](int set, const char* at, const char* bt, int ks, int n) __attribute__((always_inline)) {
     if (n < TN) fb[set][n] = rb.template read<frag>(bt, n, ks);
