@@ -2,10 +2,10 @@
 //   z = x W^T + b,   y = a(z) + r            and its gradients   gz = g a'(z),  dx = gz W,  dW = gz^T x,  db = sum_m gz
 // All three products are C[i, j] = sum_k A(i, k) B(j, k) with either operand as it lies in memory, k beside k or row beside row (nothing is
 // transposed on the way).  Bound by the matrix cores: M = 8192, N = K = 4096 in bf16 take 190 us a product on random numbers, 1.45
-// PFLOP/s, with the matrix pipe busy in 71 to 74 % of the cycles (library: 175 us, 77 %); the same kernel on zeros runs a third faster: the
-// clock follows the power that the operands' bits take.  M = 16384, N = K = 1024 with Softplus: forward 44 us, dx 33, dW 39 and 5 to
-// join its halves, gz and db 23; one tile a CU, so that what a tile stores (67 MB, 13 us at the copy's rate) hides behind nothing.
-// Rows that do not start on 16 bytes are copied to such first (16384 x 515: 6 us).
+// PFLOP/s (library: 174 us); the matrix pipe is busy in 68 to 70 % of the cycles (78 %), the rest is the step's barrier and the loads in
+// front of it.  M = 16384, N = K = 1024 with Softplus: forward 41 us, dx 33, dW 43 and 5 to join its quarters, gz and db 23; one tile a
+// CU, so that what a tile stores (67 MB, 13 us at the copy's rate) hides behind nothing.  Rows that do not start on 16 bytes are copied to
+// such first (4095 x 515 and 1024 x 515: 7 us).
 // Roundings to 16 bits: the outputs, z as it is kept for the backward pass (a' moves by at most z 2^-9 a''(z), which is below the
 // rounding of the gradients themselves for every activation here), and gz before the two products that read it (the matrix
 // instructions take 16-bit operands).  Sums over k, over m and over splits are in fp32, in a fixed order.
@@ -290,9 +290,9 @@ __device__ __forceinline__ void layer_rows(float (&v)[U][8], const GemmArgs& p, 
 enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
 
 // One tile BM x BN of C[i, j] = sum_k A(i, k) B(j, k), by WM x WN wavefronts.  256 x 256 by eight: a wavefront's 128 x 64 is 128 accumulators a
-// lane, and its fragments take 6 LDS reads for 8 matrix instructions.  Four wavefronts of 128 x 128 read less, but
-// nothing stands in for one that waits (8192 x 4096 x 4096: 218 us, 206 with eight); slots of 32 k have a barrier twice as often.  Blocks that
-// stay and fetch the next tile's first steps while the last one's results leave: 209 us, for loads wait behind a wavefront's stores.
+// lane, and its fragments take 12 KiB of LDS reads for 32 k.  Tried with 32 x 32 x 16 instructions (8192 x 4096 x 4096: 206 us): four
+// wavefronts of 128 x 128 read less, but nothing stands in for one that waits (218); blocks that stay and fetch the next tile's first steps
+// while the last one's results leave (209: loads wait behind a wavefront's stores); slots of 32 k, a barrier twice as often, slower.
 template <class T, int BM, int BN, int WM, int WN, bool TA, bool TB, int OUT>
 __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   constexpr int WAVES = WM * WN, TM = BM / WM / 16, TN = BN / WN / 16;
@@ -332,7 +332,8 @@ __device__ __forceinline__ void gemm_tile(const GemmArgs& p, int block) {
   // in use, an A fragment's successor into its own registers as soon as its last product is issued.  The step's barrier stands LEAD
   // fragments of A into its last 32 k: the last read of this step is then old enough not to be waited for, and behind it the first
   // fragments of the next step are read and the loads of the one after it start, each behind a product too (a wavefront issues in
-  // order: a burst of either would leave the matrix pipe idle).
+  // order: a burst of either would leave the matrix pipe idle).  16384 x 16384 x 4096: 1609 us with LEAD 2, 1556 with 4; where A lies row beside
+  // row 2 is a little better.
   constexpr int NMUL = TM * TN, NREAD = TM + TN, LEAD = TM < 8 ? 1 : TA ? 2 : 4, EARLY = NMUL + LEAD * TN, LATE = NMUL - LEAD * TN;
   frag fa[TM], fb[2][TN];
   auto read_one = [&](int set, const char* at, const char* bt, int ks, int n) __attribute__((always_inline)) {
