@@ -573,9 +573,6 @@ __device__ __forceinline__ void join_splits(const GemmArgs& p, int block, int bl
   }
 }
 
-template <class T, int OUT>
-__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p) { join_splits<T, OUT>(p, blockIdx.x, gridDim.x); }
-
 // both products' partial products: blocks below `first` take p, the others q
 template <class T>
 __global__ __launch_bounds__(256) void join_pair_kernel(GemmArgs p, GemmArgs q, int first) {
@@ -682,6 +679,14 @@ template <class T>
 __global__ __launch_bounds__(256) void column_sums16_kernel(Columns c) {
   __shared__ float part[8][32];
   column_sums<T>(c, blockIdx.x, part);
+}
+
+// blocks below `own` join p, the others add up columns
+template <class T, int OUT>
+__global__ __launch_bounds__(256) void join_splits_kernel(GemmArgs p, int own, Columns c) {
+  __shared__ float part[8][32];
+  if (int(blockIdx.x) < own) join_splits<T, OUT>(p, blockIdx.x, own);
+  else column_sums<T>(c, blockIdx.x - own, part);
 }
 
 // dx, dW and the last sums of db side by side in one launch, where none of them fills the chip: blocks [0, bx) make dx in tiles of BX,
@@ -791,9 +796,15 @@ inline int64_t join_blocks(const GemmArgs& a) {
   return want < 8192 ? want : 8192;
 }
 
-// the product, with its k range in t.splits pieces where that is more than one: `a.parts` has room for parts_bytes
+inline unsigned column_blocks(const Columns& c) { return c.tiles ? unsigned(c.N + 31) / 32 : 0; }
+template <class T>
+inline void sum_columns(hipStream_t st, const Columns& c) {
+  if (c.tiles) hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(column_blocks(c)), dim3(256), 0, st, c);
+}
+
+// the product, with its k range in t.splits pieces where that is more than one: `a.parts` has room for parts_bytes; and db's last sums
 template <class T, bool TA, bool TB, int OUT>
-inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
+inline void gemm(hipStream_t st, GemmArgs a, Tiling t, const Columns& columns = {}) {
   split(a, t.splits);
   auto launch = [&](auto out) {
     constexpr int O = decltype(out)::value;
@@ -801,9 +812,13 @@ inline void gemm(hipStream_t st, GemmArgs a, Tiling t) {
     else if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, O>(st, a);
     else launch_gemm<T, 64, 2, 2, TA, TB, O>(st, a);
   };
-  if (a.splits == 1) return launch(std::integral_constant<int, OUT>{});
+  if (a.splits == 1) {
+    sum_columns<T>(st, columns);
+    return launch(std::integral_constant<int, OUT>{});
+  }
   launch(std::integral_constant<int, OUT_PARTS>{});
-  hipLaunchKernelGGL((join_splits_kernel<T, OUT>), dim3(unsigned(join_blocks(a))), dim3(256), 0, st, a);
+  const int own = int(join_blocks(a));
+  hipLaunchKernelGGL((join_splits_kernel<T, OUT>), dim3(own + column_blocks(columns)), dim3(256), 0, st, a, own, columns);
 }
 
 // dx, dW and db together (x, w: their own tilings of 64 or 128, rooms of their own for partial products)
@@ -811,7 +826,7 @@ template <class T, int BX, int BW>
 inline void launch_gradients(hipStream_t st, GemmArgs x, GemmArgs w, const Columns& c) {
   constexpr unsigned LDS = lds_of(BX > BW ? BX : BW);
   allow_lds<&gradients_kernel<T, BX, BW>>(LDS);
-  const int64_t bx = blocks_of(x, BX), bw = bx + blocks_of(w, BW), all = bw + (c.tiles ? (c.N + 31) / 32 : 0);
+  const int64_t bx = blocks_of(x, BX), bw = bx + blocks_of(w, BW), all = bw + column_blocks(c);
   hipLaunchKernelGGL((gradients_kernel<T, BX, BW>), dim3(unsigned(all)), dim3(256), LDS, st, x, w, c, int(bx), int(bw));
   const int64_t jx = x.splits > 1 ? join_blocks(x) : 0, jw = w.splits > 1 ? join_blocks(w) : 0;
   if (jx + jw == 0) return;
@@ -962,10 +977,9 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
         else if (plan.w_t.size == 128) launch_gradients<T, 64, 128>(st, ax, aw, columns);
         else launch_gradients<T, 64, 64>(st, ax, aw, columns);
       } else {
-        if (columns.tiles)
-          hipLaunchKernelGGL((column_sums16_kernel<T>), dim3(unsigned((N + 31) / 32)), dim3(256), 0, st, columns);
         if (dx) gemm<T, false, true, OUT_PLAIN>(st, ax, plan.x_t);
-        if (dweight) gemm<T, true, true, OUT_PLAIN>(st, aw, plan.w_t);
+        if (dweight) gemm<T, true, true, OUT_PLAIN>(st, aw, plan.w_t, columns);
+        else sum_columns<T>(st, columns);
       }
     }
   });

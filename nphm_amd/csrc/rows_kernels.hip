@@ -489,6 +489,7 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   flush(live == n && after == key);
 }
 
+// A block a chunk, most of which have nothing to join (eight chunks a block: 10.2 us for the 4 of 4097 indices, one run waits for another).
 constexpr int JOINERS = 8;             // wavefronts that join a run
 
 template <class T, bool MERGE>
