@@ -123,11 +123,10 @@ __device__ __forceinline__ void scale_chunk(const ClipTable& t, int i, uint32_t 
   const uint32_t n = t.elements[i], begin = (chunk - t.first_chunk[i]) * PER, end = min(n, begin + PER);
   const uint32_t full = begin + (end - begin) / V * V;
   for (uint32_t c = begin + threadIdx.x * V; c < full; c += 256 * V) {
-    const auto* from = reinterpret_cast<const typename Vec<T>::type*>(g + c);
-    typename Vec<T>::type v = STREAM ? __builtin_nontemporal_load(from) : *from;
+    typename Vec<T>::type v = load_vec<STREAM>(g + c);
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = T(float(v[k]) * f);
-    __builtin_nontemporal_store(v, reinterpret_cast<typename Vec<T>::type*>(o + c));
+    store_vec<true>(o + c, v);
   }
   if (full + threadIdx.x < end) o[full + threadIdx.x] = T(float(g[full + threadIdx.x]) * f);
 }
@@ -144,9 +143,8 @@ struct Factor {
   bool stream;
 };
 
-// What is scaled is not read again: above the last cache's 256 MiB its lines are not kept, to the good of what the norm has left there (290
+// What is scaled is not read again: where all do not fit into the last cache its lines are not kept, to the good of what the norm has left there (290
 // bf16 tensors, 606 MB: 361 us, 336 so; 8 MB: 12.4, 14.7 so).  What is written never is (378, 361 so).
-constexpr int64_t CACHED = int64_t(256) << 20;
 
 template <bool STREAM>
 __device__ __forceinline__ void scale_any(const ClipTable& t, int i, uint32_t c, float f) {

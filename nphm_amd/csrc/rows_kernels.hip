@@ -32,8 +32,11 @@ __device__ __forceinline__ int64_t load_index(const void* idx, int idx64, int64_
 }
 
 // A group of LPR lanes takes one row (LPR * 16 bytes of it at a time); a wavefront 64 / LPR rows, so that narrow rows fill it too.  Few rows
-// are cut along blockIdx.y.  Bound by memory: 16384 rows of 4096 bf16 out of 50000 take 54.6 us, 248 MB at 4.5 TB/s (a copy: 5.1).
-template <class T, int LPR>
+// are cut along blockIdx.y.  Bound by memory: 16384 rows of 4096 bf16 out of 50000 take 44.8 us, 248 MB at 5.5 TB/s (a copy: 5.1).  IN, from rows
+// and result together that fill the last cache: rows are not kept once read (54.6 us if they are; with a call behind it that reads the
+// result 81 and 86; 8192 rows, which fit: 24.6 and 21.5; 65536, some of them named twice: 201 and 177).  OUT, from a result that fills
+// it by itself: nor is that kept (65536 rows and a call that reads them: 345 us, 353 if it is).
+template <class T, int LPR, bool IN, bool OUT>
 __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs p) {
   constexpr int V = Vec<T>::N, ROWS = 256 / LPR;
   typedef typename Vec<T>::type vec;
@@ -47,10 +50,10 @@ __global__ __launch_bounds__(256) void lookup_kernel(LookupArgs p) {
   const int full = p.dim / V * V;
   for (int c = (blockIdx.y * LPR + sub) * V; c < full; c += gridDim.y * LPR * V) {
     vec v;
-    if (ok) v = *reinterpret_cast<const vec*>(src + c);
+    if (ok) v = load_vec<IN>(src + c);
 #pragma unroll
     for (int k = 0; k < V; ++k) v[k] = ok ? T(float(v[k]) * p.scale) : T(__builtin_nanf(""));
-    *reinterpret_cast<vec*>(dst + c) = v;
+    store_vec<OUT>(dst + c, v);
   }
   if (blockIdx.y == 0) {
     const int c = full + sub;                       // V - 1 elements at most, LPR >= 8 lanes
@@ -117,14 +120,14 @@ __device__ __forceinline__ void load_cols(float (&v)[Vec<T>::N], const T* row, i
     for (int k = 0; k < V; ++k) v[k] = c + k < dim ? float(row[c + k]) : 0.f;
   }
 }
-template <class T>
+template <class T, bool STREAM = false>
 __device__ __forceinline__ void store_cols(T* row, int c, int dim, const float (&v)[Vec<T>::N], float scale) {
   constexpr int V = Vec<T>::N;
   if (c + V <= dim) {
     typename Vec<T>::type x;
 #pragma unroll
     for (int k = 0; k < V; ++k) x[k] = T(v[k] * scale);
-    *reinterpret_cast<typename Vec<T>::type*>(row + c) = x;
+    store_vec<STREAM>(row + c, x);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k) if (c + k < dim) row[c + k] = T(v[k] * scale);
@@ -132,14 +135,12 @@ __device__ __forceinline__ void store_cols(T* row, int c, int dim, const float (
 }
 
 // `count` elements from `to` on become zeros, by `threads` threads of which this is number `t`: whole 16-byte places but for the ends
-template <class T>
+template <bool STREAM, class T>
 __device__ __forceinline__ void zero_run(T* to, int64_t count, int t, int threads) {
   constexpr int V = Vec<T>::N;
-  typedef unsigned u32x4 __attribute__((ext_vector_type(4)));
   const int head = int(min(count, int64_t((16 - (reinterpret_cast<uintptr_t>(to) & 15)) & 15) / int64_t(sizeof(T))));
   const int64_t whole = (count - head) / V;
-  u32x4* p = reinterpret_cast<u32x4*>(to + head);
-  for (int64_t i = t; i < whole; i += threads) p[i] = u32x4{};
+  for (int64_t i = t; i < whole; i += threads) store_vec<STREAM>(to + head + i * V, typename Vec<T>::type{});
   if (t < head) to[t] = T(0.f);
   const int64_t last = head + whole * V + t;
   if (last < count) to[last] = T(0.f);                               // (V - 1 elements at most on either end, at least 64 threads)
@@ -151,7 +152,7 @@ __device__ __forceinline__ void zero_run(T* to, int64_t count, int t, int thread
 // becomes the sum of its own, in the order of the indices.
 constexpr int FEW = 256, SPAN = 1024;
 
-template <class T>
+template <class T, bool OUT>
 __global__ __launch_bounds__(256) void grad_few_kernel(GradArgs p, int rows_each) {
   constexpr int V = Vec<T>::N;
   __shared__ uint64_t found[4], lead[4];
@@ -165,8 +166,8 @@ __global__ __launch_bounds__(256) void grad_few_kernel(GradArgs p, int rows_each
   const uint64_t hit = __ballot(in);
   if ((t & 63) == 0) found[t >> 6] = hit;
   T* out = static_cast<T*>(p.out);
-  if (c0 == 0 && c1 == p.dim) zero_run(out + v0 * p.dim, (v1 - v0) * p.dim, t, 256);
-  else zero_run(out + v0 * p.dim + c0, c1 - c0, t, 256);             // (one row)
+  if (c0 == 0 && c1 == p.dim) zero_run<OUT>(out + v0 * p.dim, (v1 - v0) * p.dim, t, 256);
+  else zero_run<OUT>(out + v0 * p.dim + c0, c1 - c0, t, 256);             // (one row)
   __syncthreads();
   if (!(found[0] | found[1] | found[2] | found[3])) return;
   bool leads = in;                                                   // the first index of its row
@@ -253,6 +254,7 @@ struct Zero {
   int64_t row;                         // units of one
 };
 constexpr int64_t ZERO_UNITS = 32768;                                // 64 KiB a block
+template <bool OUT>
 __device__ __forceinline__ bool cleared(const GradArgs& p, const Zero& z) {      // whether this was one of the blocks that clear
   if (int(blockIdx.x) < z.blocks) return false;
   if (z.mark) {
@@ -264,11 +266,11 @@ __device__ __forceinline__ bool cleared(const GradArgs& p, const Zero& z) {     
       open = m < 0 || m >= p.count || key_of(p, m) != v;
     }
     for (uint64_t rows = __ballot(open); rows; rows &= rows - 1)
-      zero_run(static_cast<bf16*>(z.out) + (v0 + __builtin_ctzll(rows)) * z.row, z.row, lane, 64);
+      zero_run<OUT>(static_cast<bf16*>(z.out) + (v0 + __builtin_ctzll(rows)) * z.row, z.row, lane, 64);
     return true;
   }
   const int64_t at = z.first + int64_t(blockIdx.x - z.blocks) * ZERO_UNITS;
-  zero_run(static_cast<bf16*>(z.out) + at, min(ZERO_UNITS, z.last - at), threadIdx.x, blockDim.x);
+  zero_run<OUT>(static_cast<bf16*>(z.out) + at, min(ZERO_UNITS, z.last - at), threadIdx.x, blockDim.x);
   return true;
 }
 
@@ -280,11 +282,12 @@ constexpr int MIDDLE = 8192, PLACED = 16, RANGE = 64;               // keys a bl
 
 __host__ __device__ inline int rank_room(int count) { return (count + 4 * RANGE - 1) / (4 * RANGE) * (4 * RANGE); }     // (whole reads a range)
 
+template <bool OUT>
 __global__ __launch_bounds__(PLACED * RANGE) void rank_kernel(GradArgs p, SortArgs s, Zero z) {
   extern __shared__ __attribute__((aligned(16))) int all[];
   __shared__ int part[RANGE][PLACED];
   typedef int i32x4 __attribute__((ext_vector_type(4)));
-  if (cleared(p, z)) return;
+  if (cleared<OUT>(p, z)) return;
   const int count = int(p.count), padded = rank_room(count), each = padded / RANGE;
 #pragma unroll 8
   for (int n = threadIdx.x; n < padded; n += PLACED * RANGE) all[n] = n < count ? key_of(p, n) : 0x7ffffffe;
@@ -323,10 +326,10 @@ __global__ __launch_bounds__(PLACED * RANGE) void rank_kernel(GradArgs p, SortAr
 // the indices.
 constexpr int MAX_DIGIT = 9;
 
-template <bool FIRST>
+template <bool FIRST, bool OUT>
 __global__ __launch_bounds__(1024) void radix_hist_kernel(GradArgs p, const int* __restrict__ keys, SortArgs s, int* mark, Zero z) {
   __shared__ int bins[1 << MAX_DIGIT];
-  if (cleared(p, z)) return;
+  if (cleared<OUT>(p, z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x;
   for (int d = t; d < digits; d += 1024) bins[d] = 0;
   __syncthreads();
@@ -343,11 +346,11 @@ __global__ __launch_bounds__(1024) void radix_hist_kernel(GradArgs p, const int*
 
 // Every block finds where its keys of each digit begin (the digits below it in all blocks, its own in the blocks before), then places its
 // keys in order, 1024 at a time: in a wavefront the lanes of one digit find each other by ballots, wavefront follows wavefront.
-template <bool FIRST>
+template <bool FIRST, bool OUT>
 __global__ __launch_bounds__(1024) void radix_place_kernel(GradArgs p, const int* __restrict__ keys, const int* __restrict__ perm, SortArgs s,
                                                            int* __restrict__ keys_out, int* __restrict__ perm_out, Zero z) {
   __shared__ int base[1 << MAX_DIGIT], scan[1 << MAX_DIGIT], seen[16][1 << MAX_DIGIT];
-  if (cleared(p, z)) return;
+  if (cleared<OUT>(p, z)) return;
   const int digits = 1 << s.bits, t = threadIdx.x, lane = t & 63, wave = t >> 6;
   {
     // 1024 / digits threads a digit, each over every so many blocks
@@ -416,8 +419,10 @@ __global__ __launch_bounds__(1024) void radix_place_kernel(GradArgs p, const int
 // A wavefront adds the rows of `chunk` consecutive places (64 vectors of columns): a run that lies inside goes out, one that the
 // chunk's borders cut goes to partial[2 chunk + (begun before ? 0 : 1)] in fp32; join adds those in order, from the chunk where the run
 // begins.  So a row that takes half of all indices costs no more than any other half.
-// Bound by memory: 32768 rows of 2048 bf16 for 50000, 51 us (134 MB read once, named rows written once); sorting takes 38 with the clearing
-// beside it and joining 8, most of it the way through six launches.
+// Bound by memory: 32768 rows of 2048 bf16 for 50000, 34 us (134 MB read once, named rows written once); sorting takes 36 with the clearing
+// beside it and joining 8, most of it the way through six launches.  IN, where gradient and result do not fit into the last cache: rows
+// are not kept once read (the whole: 96 us if they are, 83 so; 16384 rows of 1024, which fit: 44.3 and 46.6); OUT, nor is a result that does
+// not fit by itself (32768 rows of 2048 into 100000 and a norm over it: 217 us if it is, 192 so).
 struct SumArgs {
   const int *sorted, *perm;
   float* partial;
@@ -425,12 +430,12 @@ struct SumArgs {
   int64_t pitch;                       // floats a partial row
 };
 
-template <class T>
+template <class T, bool STREAM>
 __device__ __forceinline__ typename Vec<T>::type load_raw(const T* row, int c, int dim) {
   constexpr int V = Vec<T>::N;
   typename Vec<T>::type x;
   if (c + V <= dim) {
-    x = *reinterpret_cast<const typename Vec<T>::type*>(row + c);
+    x = load_vec<STREAM>(row + c);
   } else {
 #pragma unroll
     for (int k = 0; k < V; ++k) x[k] = c + k < dim ? row[c + k] : T(0.f);
@@ -438,7 +443,7 @@ __device__ __forceinline__ typename Vec<T>::type load_raw(const T* row, int c, i
   return x;
 }
 
-template <class T, bool MERGE>
+template <class T, bool MERGE, bool IN, bool OUT>
 __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   constexpr int V = Vec<T>::N, AHEAD = 8;                            // rows on their way
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -458,7 +463,7 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   bool begun = before == key;
   auto flush = [&](bool goes_on) __attribute__((always_inline)) {
     if (!begun && !goes_on) {
-      store_cols(out + int64_t(MERGE ? head : key) * p.dim, c, p.dim, acc, p.scale);
+      store_cols<T, OUT>(out + int64_t(MERGE ? head : key) * p.dim, c, p.dim, acc, p.scale);
     } else {
       float* to = s.partial + (2 * int64_t(chunk) + (begun ? 0 : 1)) * s.pitch + c;
       typedef float f32x4 __attribute__((ext_vector_type(4)));
@@ -469,7 +474,7 @@ __global__ __launch_bounds__(256) void sum_kernel(GradArgs p, SumArgs s) {
   typename Vec<T>::type x[AHEAD];
   for (int q = 0; q < live; q += AHEAD) {
 #pragma unroll
-    for (int a = 0; a < AHEAD; ++a) x[a] = load_raw(grad + int64_t(__builtin_amdgcn_readlane(rows, min(q + a, live - 1))) * p.ld, c, p.dim);
+    for (int a = 0; a < AHEAD; ++a) x[a] = load_raw<T, IN>(grad + int64_t(__builtin_amdgcn_readlane(rows, min(q + a, live - 1))) * p.ld, c, p.dim);
 #pragma unroll
     for (int a = 0; a < AHEAD; ++a) {
       if (q + a >= live) break;
@@ -574,7 +579,7 @@ inline GradPlan grad_plan(int64_t rows, int64_t dim, int64_t count, int element)
   return g;
 }
 
-template <class T, bool MERGE>
+template <class T, bool MERGE, bool OUT>
 inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char* ws) {
   const unsigned tiles = unsigned((a.dim + 64 * Vec<T>::N - 1) / (64 * Vec<T>::N));
   const int64_t out_rows = MERGE ? a.count : a.rows;
@@ -585,7 +590,7 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
       // up to 64 KiB of rows a block, as long as there are 1024 blocks
       const int span = SPAN * Vec<T>::N;
       const int64_t fit = a.dim <= span ? 65536 / (int64_t(a.dim) * int64_t(sizeof(T))) : 1, each = std::max<int64_t>(1, std::min(a.rows / 1024, fit));
-      hipLaunchKernelGGL((grad_few_kernel<T>), dim3(unsigned((a.rows + each - 1) / each), unsigned((a.dim + span - 1) / span)), dim3(256), 0, st, a,
+      hipLaunchKernelGGL((grad_few_kernel<T, OUT>), dim3(unsigned((a.rows + each - 1) / each), unsigned((a.dim + span - 1) / span)), dim3(256), 0, st, a,
                          int(each));
     }
     return;
@@ -618,7 +623,7 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   unsigned grid = 0;
   if (!g.passes) {
     const Zero z = zero(0, int((a.count + PLACED - 1) / PLACED), grid);
-    hipLaunchKernelGGL(rank_kernel, dim3(grid), dim3(PLACED * RANGE), unsigned(rank_room(int(a.count)) * 4), st, a, s, z);
+    hipLaunchKernelGGL((rank_kernel<OUT>), dim3(grid), dim3(PLACED * RANGE), unsigned(rank_room(int(a.count)) * 4), st, a, s, z);
   }
   const int *kin = nullptr, *pin = nullptr;
   for (int pass = 0; pass < g.passes; ++pass) {                      // indices -> other -> ... -> sorted, whatever the number of passes
@@ -626,11 +631,11 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
     int *kout = to_sorted ? s.sorted : s.sorted2, *pout = to_sorted ? s.perm : s.perm2;
     s.shift = pass * g.bits;
     Zero z = zero(2 * pass, g.blocks, grid);
-    if (pass == 0) hipLaunchKernelGGL((radix_hist_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
-    else hipLaunchKernelGGL((radix_hist_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
+    if (pass == 0) hipLaunchKernelGGL((radix_hist_kernel<true, OUT>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
+    else hipLaunchKernelGGL((radix_hist_kernel<false, OUT>), dim3(grid), dim3(1024), 0, st, a, kin, s, marks, z);
     z = zero(2 * pass + 1, g.blocks, grid);
-    if (pass == 0) hipLaunchKernelGGL((radix_place_kernel<true>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
-    else hipLaunchKernelGGL((radix_place_kernel<false>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
+    if (pass == 0) hipLaunchKernelGGL((radix_place_kernel<true, OUT>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
+    else hipLaunchKernelGGL((radix_place_kernel<false, OUT>), dim3(grid), dim3(1024), 0, st, a, kin, pin, s, kout, pout, z);
     kin = kout;
     pin = pout;
   }
@@ -642,7 +647,9 @@ inline void grad_run(hipStream_t st, const GradArgs& a, const GradPlan& g, char*
   u.chunks = g.chunks;
   u.tiles = g.tiles;
   u.pitch = int64_t(g.tiles) * 64 * Vec<T>::N;
-  hipLaunchKernelGGL((sum_kernel<T, MERGE>), dim3(unsigned((int64_t(g.chunks) * g.tiles + 3) / 4)), dim3(256), 0, st, a, u);
+  const dim3 wide(unsigned((int64_t(g.chunks) * g.tiles + 3) / 4));
+  if (OUT || (a.count + out_rows) * a.dim * int64_t(sizeof(T)) > CACHED) hipLaunchKernelGGL((sum_kernel<T, MERGE, true, OUT>), wide, dim3(256), 0, st, a, u);
+  else hipLaunchKernelGGL((sum_kernel<T, MERGE, false, OUT>), wide, dim3(256), 0, st, a, u);
   hipLaunchKernelGGL((join_kernel<T, MERGE>), dim3(unsigned(g.chunks), tiles), dim3(64 * JOINERS), 0, st, a, u);
 }
 
@@ -709,11 +716,18 @@ int nphm_rows_lookup(const void* table, int64_t rows, int64_t dim, int64_t ld, i
   if (int rc = check_table("nphm_rows_lookup", table, rows, dim, ld, dtype, idx, idx_bits, count)) return rc;
   if (count == 0) return 0;
   if (!out) return nphm_fail_msg("nphm_rows_lookup: null pointer");
-  LookupArgs a{table, idx, out, ld, count, rows, int(dim), idx_bits == 64, scale};
+  const int64_t bytes = count * dim * dtype_size(dtype);
+  const bool in = 2 * bytes >= CACHED && count <= rows, to = bytes >= CACHED;
+  const LookupArgs a{table, idx, out, ld, count, rows, int(dim), idx_bits == 64, scale};
   with_dtype(dtype, [&](auto t) {
     using T = decltype(t);
     for_rows(count, (dim + Vec<T>::N - 1) / Vec<T>::N, [&](auto lanes, dim3 grid) {
-      hipLaunchKernelGGL((lookup_kernel<T, decltype(lanes)::value>), grid, dim3(256), 0, static_cast<hipStream_t>(stream), a);
+      constexpr int L = decltype(lanes)::value;
+      hipStream_t st = static_cast<hipStream_t>(stream);
+      if (in && to) hipLaunchKernelGGL((lookup_kernel<T, L, true, true>), grid, dim3(256), 0, st, a);
+      else if (in) hipLaunchKernelGGL((lookup_kernel<T, L, true, false>), grid, dim3(256), 0, st, a);
+      else if (to) hipLaunchKernelGGL((lookup_kernel<T, L, false, true>), grid, dim3(256), 0, st, a);
+      else hipLaunchKernelGGL((lookup_kernel<T, L, false, false>), grid, dim3(256), 0, st, a);
     });
   });
   hipError_t e = hipGetLastError();
@@ -732,7 +746,10 @@ int nphm_rows_grad(const void* grad, int64_t count, int64_t dim, int64_t ld, int
   const GradPlan g = grad_plan(rows, dim, count, dtype_size(dtype));
   if (workspace_bytes < g.total || (g.total && !workspace)) return nphm_fail_msg("nphm_rows_grad: workspace too small");
   GradArgs a{grad, idx, out, ld, count, rows, int(dim), idx_bits == 64, padding, scale};
-  with_dtype(dtype, [&](auto t) { grad_run<decltype(t), false>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
+  with_dtype(dtype, [&](auto t) {
+    if (rows * dim * dtype_size(dtype) > CACHED) grad_run<decltype(t), false, true>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace));
+    else grad_run<decltype(t), false, false>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace));
+  });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_grad launch", e);
   return 0;
@@ -763,7 +780,7 @@ int nphm_rows_merge(const void* grad, int64_t count, int64_t dim, int dtype, con
   const GradPlan g = grad_plan(rows, dim, count, dtype_size(dtype));
   if (workspace_bytes < g.total || (g.total && !workspace)) return nphm_fail_msg("nphm_rows_merge: workspace too small");
   GradArgs a{grad, idx, out, dim, count, rows, int(dim), idx_bits == 64, -1, 1.f};
-  with_dtype(dtype, [&](auto t) { grad_run<decltype(t), true>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
+  with_dtype(dtype, [&](auto t) { grad_run<decltype(t), true, false>(static_cast<hipStream_t>(stream), a, g, static_cast<char*>(workspace)); });
   hipError_t e = hipGetLastError();
   if (e != hipSuccess) return nphm_fail("nphm_rows_merge launch", e);
   return 0;

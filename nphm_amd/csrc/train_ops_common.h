@@ -21,6 +21,23 @@ template <> struct Vec<float> { typedef f32x4_u type; static constexpr int N = 4
 template <> struct Vec<bf16> { typedef bf16x8_u type; static constexpr int N = 8; };
 template <> struct Vec<fp16> { typedef fp16x8_u type; static constexpr int N = 8; };
 
+// the last cache, bytes.  Work that does not fit into it says so: what it reads for the last time, or writes without a chance to be read from
+// there, is not kept
+constexpr int64_t CACHED = int64_t(256) << 20;
+// (the choice is made at compile time: of two accesses that differ in nothing else the compiler makes one, without the hint)
+template <bool STREAM, class T>
+__device__ __forceinline__ typename Vec<T>::type load_vec(const T* p) {
+  const auto* from = reinterpret_cast<const typename Vec<T>::type*>(p);
+  if constexpr (STREAM) return __builtin_nontemporal_load(from);
+  else return *from;
+}
+template <bool STREAM, class T>
+__device__ __forceinline__ void store_vec(T* p, const typename Vec<T>::type& v) {
+  auto* to = reinterpret_cast<typename Vec<T>::type*>(p);
+  if constexpr (STREAM) __builtin_nontemporal_store(v, to);
+  else *to = v;
+}
+
 enum { DT_F32 = 0, DT_BF16 = 1, DT_F16 = 2 };
 inline bool dtype_ok(int d) { return d >= DT_F32 && d <= DT_F16; }
 inline int dtype_size(int d) { return d == DT_F32 ? 4 : 2; }
