@@ -236,6 +236,24 @@ def test_long_rows_named_by_many_indices(dev, t, V, D, N):
 
 
 @gpu
+def test_rows_that_fill_the_last_cache(dev):
+    """the ways through memory that only large calls take (results above 256 MiB, odd rows), for every number of indices; whole numbers, so
+    that any order of sums is exact"""
+    V, D = 17000, 4099
+    gen = torch.Generator(device=dev).manual_seed(8)
+    table = torch.randint(-8, 9, (V, D), device=dev, generator=gen).float()
+    for N in (9000, V, V + 1):
+        idx = torch.randint(0, V, (N,), device=dev, generator=gen)
+        assert torch.equal(T.lookup_rows(table, idx), table.index_select(0, idx))
+    for N in (200, 4000, 9000):
+        idx = torch.randint(0, V, (N,), device=dev, generator=gen)
+        idx[N // 2:] %= 40
+        got = T.lookup_rows_grad(table[:N], idx, V)
+        assert torch.equal(got, torch.zeros(V, D, device=dev).index_add_(0, idx, table[:N]))
+        del got
+
+
+@gpu
 def test_row_gradients_do_not_overflow_in_sums(dev):
     """fp16 rows whose partial sums leave the type's range and come back"""
     g = torch.full((2000, 24), 60000.0, dtype=torch.float16, device=dev)
