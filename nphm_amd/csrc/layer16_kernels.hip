@@ -83,7 +83,14 @@ struct GemmArgs {
   void* z;                               // [I, J] or null: the value before the activation
   int act;
   float beta;
+  bool stream_z, stream_c;               // not kept in the caches
 };
+
+// z is read again in the backward pass, after all that follows in this one: from 32 MiB on it is not kept, and neither are it and g when they
+// are read for gz (six layers of 16384 x 1024 x 1024 with SiLU, forward and backward: 860 us if they are, 823 so; eight of 4096 x 512 x 512:
+// 242 and 250).  y is for the next layer: it is kept unless it fills the last cache by itself (16384 x 16384: 1644 us if it is, 1625
+// so; the six layers' forward pass 211 us, 215 if y never is).
+constexpr int64_t Z_KEPT = CACHED / 8;
 
 // z as it is kept: finite where z is (a' of an infinity is no number for some activations)
 template <class T>
@@ -201,11 +208,16 @@ struct Reader {
 
 // eight values beside each other, `width` of them there (more than eight: all); a row may start anywhere
 template <class T>
-__device__ __forceinline__ void put8(T* to, const float (&v)[8], int width) {
+__device__ __forceinline__ typename Vec<T>::type round8(const float (&v)[8]) {
   typename Vec<T>::type o;
 #pragma unroll
   for (int e = 0; e < 8; ++e) o[e] = T(v[e]);
-  if (width >= 8) { *reinterpret_cast<typename Vec<T>::type*>(to) = o; return; }
+  return o;
+}
+template <class T>
+__device__ __forceinline__ void put8(T* to, const float (&v)[8], int width) {
+  const typename Vec<T>::type o = round8<T>(v);
+  if (width >= 8) { store_vec<false>(to, o); return; }
 #pragma unroll
   for (int e = 0; e < 8; ++e) if (e < width) to[e] = o[e];
 }
@@ -256,19 +268,31 @@ __device__ __forceinline__ void layer_out(float (&v)[8], const GemmArgs& p, int6
   put8(static_cast<T*>(p.C) + at, v, width);
 }
 
-// the same for U rows `row` elements apart, all there: what is asked once for them stands between them, not in front of each
+// U rows `row` elements apart, all there.  (The empty asm keeps the compiler from making one store, without the hint, of the two.)
+template <class T, int U>
+__device__ __forceinline__ void put_rows(T* to, const typename Vec<T>::type (&o)[U], int64_t row, bool stream) {
+  if (stream) {
+    asm volatile("");
+#pragma unroll
+    for (int u = 0; u < U; ++u) store_vec<true>(to + u * row, o[u]);
+    asm volatile("");
+  } else {
+#pragma unroll
+    for (int u = 0; u < U; ++u) store_vec<false>(to + u * row, o[u]);
+  }
+}
+
+// the same for U rows: what is asked once for them stands between them, not in front of each
 template <class T, int ACT, int U>
 __device__ __forceinline__ void layer_rows(float (&v)[U][8], const GemmArgs& p, int64_t at, int64_t row) {
+  typename Vec<T>::type r[U];
   if (p.z) {
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      float k[8];
+    for (int u = 0; u < U; ++u)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) k[e] = float(keep<T>(v[u][e]));
-      put8(static_cast<T*>(p.z) + at + u * row, k, 8);
-    }
+      for (int e = 0; e < 8; ++e) r[u][e] = keep<T>(v[u][e]);
+    put_rows<T, U>(static_cast<T*>(p.z) + at, r, row, p.stream_z);
   }
-  typename Vec<T>::type r[U];
   if (p.residual) {
 #pragma unroll
     for (int u = 0; u < U; ++u) r[u] = *reinterpret_cast<const typename Vec<T>::type*>(static_cast<const T*>(p.residual) + at + u * row);
@@ -284,7 +308,8 @@ __device__ __forceinline__ void layer_rows(float (&v)[U][8], const GemmArgs& p, 
       for (int e = 0; e < 8; ++e) v[u][e] += float(r[u][e]);
   }
 #pragma unroll
-  for (int u = 0; u < U; ++u) put8(static_cast<T*>(p.C) + at + u * row, v[u], 8);
+  for (int u = 0; u < U; ++u) r[u] = round8<T>(v[u]);
+  put_rows<T, U>(static_cast<T*>(p.C) + at, r, row, p.stream_c);
 }
 
 enum { OUT_LAYER = 0, OUT_PLAIN = 1, OUT_PARTS = 2, OUT_EITHER = 3 };       // EITHER: PARTS where the k range is split, else PLAIN
@@ -591,7 +616,7 @@ struct Packs {
   int cols, ld;
 };
 
-template <class T, int LPR, int ROWS>
+template <class T, int LPR, int ROWS, bool STREAM>
 __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, float* sums, T* dbias, int M, int N, int ld, int act, float beta,
                                                  int tiles, unsigned own, Packs packs) {
   constexpr int SIDE = 256 / LPR;
@@ -609,11 +634,11 @@ __global__ __launch_bounds__(256) void gz_kernel(const T* g, const T* z, T* gz, 
       const int64_t at = int64_t(m) * N + c;
       float v[8] = {}, zz[8] = {};
       if (c + 8 <= N) {
-        const vec x = *reinterpret_cast<const vec*>(g + at);
+        const vec x = load_vec<STREAM>(g + at);
 #pragma unroll
         for (int e = 0; e < 8; ++e) v[e] = float(x[e]);
         if (z) {
-          const vec y = *reinterpret_cast<const vec*>(z + at);
+          const vec y = load_vec<STREAM>(z + at);
 #pragma unroll
           for (int e = 0; e < 8; ++e) zz[e] = float(y[e]);
         }
@@ -719,8 +744,10 @@ inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sum
   const bool many = gz_rows(M, ld) == 16;
   auto go = [&](auto lanes_c) {
     constexpr int L = decltype(lanes_c)::value;
-    if (many) hipLaunchKernelGGL((gz_kernel<T, L, 16>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
-    else hipLaunchKernelGGL((gz_kernel<T, L, 4>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
+    if (many && gz && int64_t(M) * N * 2 >= Z_KEPT)
+      hipLaunchKernelGGL((gz_kernel<T, L, 16, true>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
+    else if (many) hipLaunchKernelGGL((gz_kernel<T, L, 16, false>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
+    else hipLaunchKernelGGL((gz_kernel<T, L, 4, false>), dim3(grid), dim3(256), 0, st, g, z, gz, s, dbias, M, N, ld, act, beta, tiles, own, packs);
   };
   if (lanes == 8) go(std::integral_constant<int, 8>{});
   else if (lanes == 16) go(std::integral_constant<int, 16>{});
@@ -729,7 +756,7 @@ inline Columns make_gz(hipStream_t st, const T* g, const T* z, T* gz, float* sum
   return Columns{sums, dbias, dbias && tiles > 1 ? tiles : 0, N};
 }
 
-inline int64_t round8(int64_t v) { return (v + 7) / 8 * 8; }
+inline int64_t whole8(int64_t v) { return (v + 7) / 8 * 8; }
 
 struct Tiling { int size, splits; };               // size: 256, 128 or 64
 // Among the tiles that fill the 256 CUs the size whose fullest CU is done first: a tile takes its steps of 64 k, times what an element of it
@@ -839,7 +866,7 @@ inline void pack(hipStream_t st, const Packs& k) {
   const unsigned blocks = k.blocks + pack_blocks(k.q);
   if (blocks) hipLaunchKernelGGL((pack_kernel<T>), dim3(blocks), dim3(256), 0, st, k.p, k.q, k.blocks, k.cols, k.ld);
 }
-inline Packs packs_of(const Pack& p, const Pack& q, int64_t cols) { return Packs{p, q, pack_blocks(p), int(cols), int(round8(cols))}; }
+inline Packs packs_of(const Pack& p, const Pack& q, int64_t cols) { return Packs{p, q, pack_blocks(p), int(cols), int(whole8(cols))}; }
 
 inline bool aligned(const void* p, unsigned to) { return (reinterpret_cast<uintptr_t>(p) & (to - 1)) == 0; }
 
@@ -865,8 +892,8 @@ inline Forward forward_plan(const void* x, const void* weight, int64_t M, int64_
   Forward p;
   p.t = tiling(M, N, K);
   p.x = 0;
-  p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
-  p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
+  p.weight = p.x + (packed(x, K) ? up(size_t(M) * whole8(K) * 2) : 0);
+  p.parts = p.weight + (packed(weight, K) ? up(size_t(N) * whole8(K) * 2) : 0);
   p.total = p.parts + parts_bytes(p.t, M, N);
   return p;
 }
@@ -882,10 +909,10 @@ inline Backward backward_plan(const void* g, const void* x, const void* weight, 
   p.w_t = tiling(N, K, M);
   p.same = act == ACT_NONE && !packed(g, N);
   p.gz = 0;
-  p.sums = p.gz + (p.same ? 0 : up(size_t(M) * round8(N) * 2));
-  p.x = p.sums + up(size_t(gz_tiles(M, round8(N))) * N * 4);
-  p.weight = p.x + (packed(x, K) ? up(size_t(M) * round8(K) * 2) : 0);
-  p.parts_x = p.weight + (packed(weight, K) ? up(size_t(N) * round8(K) * 2) : 0);
+  p.sums = p.gz + (p.same ? 0 : up(size_t(M) * whole8(N) * 2));
+  p.x = p.sums + up(size_t(gz_tiles(M, whole8(N))) * N * 4);
+  p.weight = p.x + (packed(x, K) ? up(size_t(M) * whole8(K) * 2) : 0);
+  p.parts_x = p.weight + (packed(weight, K) ? up(size_t(N) * whole8(K) * 2) : 0);
   p.parts_w = p.parts_x + parts_bytes(p.x_t, M, K);
   p.total = p.parts_w + parts_bytes(p.w_t, N, K);
   return p;
@@ -918,10 +945,12 @@ int nphm_layer16_forward(const void* x, const void* weight, const void* bias, co
       a.B = weight; a.ldb = K;
       const bool px = packed(x, K), pw = packed(weight, K);
       pack<T>(st, packs_of(Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K));
-      if (px) { a.A = ws + plan.x; a.lda = round8(K); }
-      if (pw) { a.B = ws + plan.weight; a.ldb = round8(K); }
+      if (px) { a.A = ws + plan.x; a.lda = whole8(K); }
+      if (pw) { a.B = ws + plan.weight; a.ldb = whole8(K); }
       a.I = int(M); a.J = int(N); a.K = int(K);
       a.C = y; a.bias = bias; a.residual = residual; a.z = z; a.act = act; a.beta = beta;
+      a.stream_z = M * N * 2 >= Z_KEPT;
+      a.stream_c = M * N * 2 >= CACHED;
       a.parts = reinterpret_cast<float*>(ws + plan.parts);
       gemm<T, false, false, OUT_LAYER>(st, a, plan.t);
     }
@@ -946,7 +975,7 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
   with_dtype(dtype, [&](auto t) {
     typedef decltype(t) T;
     if constexpr (sizeof(T) == 2) {
-      const int64_t ldn = round8(N), ldk = round8(K);
+      const int64_t ldn = whole8(N), ldk = whole8(K);
       T* gz = plan.same ? const_cast<T*>(static_cast<const T*>(g)) : reinterpret_cast<T*>(ws + plan.gz);
       const bool px = dweight && packed(x, K), pw = dx && packed(weight, K);
       const Packs packs = packs_of(Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
