@@ -608,7 +608,7 @@ __global__ __launch_bounds__(256) void join_pair_kernel(GemmArgs p, GemmArgs q, 
 
 // gz = g a'(z) (rows `ld` elements apart, zeros behind them) and the column sums of every tile of rows of it (before it is rounded).  A
 // thread takes eight columns of ROWS rows; LPR threads a row, 256 / LPR rows side by side.  Bound by memory: 16384 x 1024 with Softplus,
-// 101 MB in 18 us (5.5 TB/s, some of it still in the last cache).
+// 101 MB in 18 to 23 us (4.4 TB/s and more, as much as is still in the last cache).
 // The blocks behind its own pack the operands of the products that follow (a launch less: 4095 x 515 -> 1024, 4 us).
 struct Packs {
   Pack p, q;
