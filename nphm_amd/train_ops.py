@@ -99,7 +99,7 @@ class LatentCodes(nn.Embedding):
 # ---- dense layer in 16 bits --------------------------------------------------------------------------------------------------
 
 def linear_act(x, weight, bias=None, activation="none", beta=1.0, residual=None):
-    """activation(x weight^T + bias) + residual in one launch: x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16 (fp32
+    """activation(x weight^T + bias) + residual, all of it behind the product in the same pass: x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16 (fp32
     layers run on the decoders' own dense tier); products accumulate in fp32.  activation: "none", "relu", "silu", "gelu"
     (erf), "softplus" (with `beta`, as nn.Softplus).  Differentiable once w.r.t. the four tensors: the value before the activation is
     kept in 16 bits for it.  No broadcasting: residual has the result's shape."""
@@ -157,8 +157,8 @@ def _merge_rows_(g):
 @torch.no_grad()
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (training.py:128-131) with one norm over dense and row-sparse gradients: clips the ``.grad`` of `parameters`
-    (a tensor or an iterable) in place and returns the norm before it (0-dim fp32).  Sparse gradients have one sparse dimension;
-    entries that name the same row count as their sum.  ``error_if_nonfinite`` waits for the device and raises before
+    (a tensor or an iterable, none of them twice) in place and returns the norm before it (0-dim fp32).  Sparse gradients have one sparse
+    dimension; entries that name the same row count as their sum.  ``error_if_nonfinite`` waits for the device and raises before
     anything is scaled."""
     what = "clip_grad_norm_"
     kind, limit = _kind(what, norm_type), _limit(what, max_norm)
