@@ -99,10 +99,10 @@ class LatentCodes(nn.Embedding):
 # ---- dense layer in 16 bits --------------------------------------------------------------------------------------------------
 
 def linear_act(x, weight, bias=None, activation="none", beta=1.0, residual=None):
-    """activation(x weight^T + bias) + residual, all of it behind the product in the same pass: x [..., K], weight [N, K], bias [N], residual [..., N], all bf16 or all fp16 (fp32
-    layers run on the decoders' own dense tier); products accumulate in fp32.  activation: "none", "relu", "silu", "gelu"
-    (erf), "softplus" (with `beta`, as nn.Softplus).  Differentiable once w.r.t. the four tensors: the value before the activation is
-    kept in 16 bits for it.  No broadcasting: residual has the result's shape."""
+    """activation(x weight^T + bias) + residual, all of it behind the product in the same pass: x [..., K], weight [N, K], bias [N],
+    residual [..., N], all bf16 or all fp16 (fp32 layers run on the decoders' own dense tier); products accumulate in fp32.
+    activation: "none", "relu", "silu", "gelu" (erf), "softplus" (with `beta`, as nn.Softplus).  Differentiable once w.r.t. the four
+    tensors: the value before the activation is kept in 16 bits for it.  No broadcasting: residual has the result's shape."""
     act = _ACTIVATIONS.get("none" if activation is None else activation)
     if act is None:
         raise ValueError(f"linear_act: activation is one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
