@@ -56,8 +56,9 @@ _ops = _Ops()
 def lookup_rows(table, idx, scale=1.0, padding_idx=None, sparse=False):
     """scale * table[idx] for a table [V, D] (fp32, bf16 or fp16) and int32 / int64 indices of any shape: [*idx.shape, D] in the table's type,
     the product in fp32.  Differentiable (once) w.r.t. the table: a dense gradient (``lookup_rows_grad``) or, with ``sparse``, a
-    sparse one with an entry for every index.  Row `padding_idx` is read like any other and gets no gradient.  An index outside
-    the table gives a row of NaN and adds nothing to the gradient (nothing on the host looks at the indices)."""
+    sparse one with an entry for every index (``LatentCodes`` and ``clip_grad_norm_`` coalesce it where torch's optimisers cannot).  Row
+    `padding_idx` is read like any other and gets no gradient.  An index outside the table gives a row of NaN and adds nothing to the
+    gradient (nothing on the host looks at the indices)."""
     return _ops.lookup_rows(table, idx, scale, padding_idx, sparse)
 
 
@@ -75,10 +76,38 @@ def renorm_rows_(table, idx, max_norm):
     return table
 
 
+# torch.sparse's coalesce, which torch.optim.SparseAdam calls, leaves the columns of wide rows as the memory was (PyTorch 2.10 on ROCm: of D
+# columns the first 256 + 4 (ceil(D / 256) - 1) are written, found with rows of 64 to 2048).  It leaves a coalesced gradient alone.
+_COALESCED_BY_TORCH = 256
+
+
+def _needs_fold(g):
+    """whether torch would coalesce the row gradient `g` on the device and lose columns"""
+    v = g._values()
+    return (v.is_cuda and v.dtype in _CODES and g.sparse_dim() == 1 and not g.is_coalesced() and v.shape[0] > 0
+            and v[0].numel() > _COALESCED_BY_TORCH and not torch.cuda.is_current_stream_capturing())
+
+
+@torch.no_grad()
+def _folded(g):
+    """The row gradient `g` coalesced: every row once, in ascending order, the sums in fp32 in the order of the entries (waits for the device)."""
+    v = g._values()
+    rows, place = torch.unique(g._indices()[0], return_inverse=True)
+    sums = lookup_rows_grad(v.reshape(v.shape[0], -1), place, rows.numel()).view(rows.numel(), *v.shape[1:])
+    return torch.sparse_coo_tensor(rows[None], sums, g.shape, is_coalesced=True, check_invariants=False)
+
+
+def _fold_grad(p):
+    if p.grad is not None and p.grad.is_sparse and _needs_fold(p.grad):
+        p.grad = _folded(p.grad)
+
+
 class LatentCodes(nn.Embedding):
     """The table of latent codes of the trainers (nn.Embedding(n, lat_dim, max_norm=1.0, sparse=True), training.py:36-40) on
     ``lookup_rows`` / ``renorm_rows_``; parameters, initialisation and state_dict are nn.Embedding's.  ``scale`` multiplies the looked-up
-    rows.  ``backend = "composite"`` computes the same with torch's embedding (CPU tensors need it, as in the decoders)."""
+    rows.  With ``sparse``, codes of more than 256 entries get their ``weight.grad`` coalesced when a backward pass has left it (which waits for
+    the device; not while a graph is captured): torch.optim.SparseAdam takes it as it is, where torch would lose columns of it.
+    ``backend = "composite"`` computes the same with torch's embedding (CPU tensors need it, as in the decoders)."""
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, scale=1.0, sparse=False, device=None, dtype=None):
         super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, max_norm=max_norm, sparse=sparse, device=device, dtype=dtype)
@@ -88,6 +117,11 @@ class LatentCodes(nn.Embedding):
         self.backend = "hip"            # "hip" | "composite"
 
     def forward(self, idx):
+        w = self.weight
+        if self.sparse and w.is_cuda and w.is_leaf and w.requires_grad and w.shape[1] > _COALESCED_BY_TORCH:
+            # (looked for in every call: a copied or unpickled module's weight has no hooks)
+            if _fold_grad not in (w._post_accumulate_grad_hooks or {}).values():
+                w.register_post_accumulate_grad_hook(_fold_grad)
         if self.backend == "composite":
             rows = super().forward(idx)
             return rows if self.scale == 1.0 else rows * self.scale
@@ -158,8 +192,9 @@ def _merge_rows_(g):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (training.py:128-131) with one norm over dense and row-sparse gradients: clips the ``.grad`` of `parameters`
     (a tensor or an iterable, none of them twice) in place and returns the norm before it (0-dim fp32).  Sparse gradients have one sparse
-    dimension; entries that name the same row count as their sum.  ``error_if_nonfinite`` waits for the device and raises before
-    anything is scaled."""
+    dimension; entries that name the same row count as their sum.  One that is not coalesced and has rows of more than 256 entries is
+    replaced by its coalesced form (as ``LatentCodes`` does; waits for the device, not while a graph is captured).
+    ``error_if_nonfinite`` waits for the device and raises before anything is scaled."""
     what = "clip_grad_norm_"
     kind, limit = _kind(what, norm_type), _limit(what, max_norm)
     if isinstance(parameters, torch.Tensor):
@@ -175,7 +210,10 @@ def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=Fals
             v = g._values()
             if not (v.is_cuda and v.dtype in _CODES):
                 raise TypeError(f"{what}: sparse fp32, bf16 or fp16 gradients on a ROCm device")
-            if not g.is_coalesced():
+            if _needs_fold(g):
+                p.grad = _folded(g)
+                v = p.grad._values()
+            elif not g.is_coalesced():
                 _merge_rows_(g)
             g = v
         grads.append(g)

@@ -802,6 +802,134 @@ def test_duplicates_of_a_sparse_gradient_are_folded(dev, N, rows, D):
     assert not got[rest].any()
 
 
+def dirty_memory(dev):
+    """small blocks that are handed out again hold NaN: what a later call leaves unwritten shows"""
+    held = [torch.full((n * 1344,), math.nan, device=dev) for n in (1, 2, 3, 4, 6, 8, 12, 24) for _ in range(4)]
+    torch.cuda.synchronize()
+    del held
+
+
+def sparse_adam_bound(steps, lr, w):
+    """A step of Adam adds lr sqrt(1 - b2^t) / (1 - b1^t) m / (sqrt(v) + eps) to an entry: 0.316 lr m / sqrt(v) at most, the factor's largest
+    value that of t = 1.  m comes from eight fp32 roundings of magnitudes up to the largest gradient's, sqrt(v) is at least 0.0316 of that
+    (its last one's share), so the two sides are 2 x 8 x 2^-24 x 0.316 / 0.0316 lr apart, and a rounding of the sum."""
+    return steps * (160 * lr * F32 + float(w.abs().max()) * F32)
+
+
+@gpu
+@pytest.mark.parametrize("D", [200, 256, 257, 300, 513, 1344, 2048])
+@pytest.mark.parametrize("way", ["plain", "clipped", "twice", "summed", "embedding", "copied"])
+def test_row_gradients_step_sparse_adam(dev, way, D):
+    """three steps of the trainer's optimiser on codes of this width, against the same optimiser on the host, which is handed the gradient in its
+    dense form: no column is lost, whether the gradient is one call's, clipped, of two calls, summed over two backward passes, or torch's"""
+    import copy
+    gen = torch.Generator().manual_seed(D)
+    start = torch.randn(9, D, generator=gen) * 0.01
+    codes = (torch.nn.Embedding(9, D, sparse=True) if way == "embedding" else T.LatentCodes(9, D, sparse=True)).to(dev)
+    with torch.no_grad():
+        codes.weight.copy_(start)
+    if way == "copied":
+        codes = copy.deepcopy(codes)
+    host = torch.nn.Parameter(start.clone())
+    ours, ref = torch.optim.SparseAdam([codes.weight], lr=1e-3), torch.optim.SparseAdam([host], lr=1e-3)
+    for k, idx in enumerate(([3, 1, 3, 0], [5, 0, 5], [1, 3, 8, 7, 3])):
+        idx = torch.tensor(idx)
+        go = torch.randn(len(idx), D, generator=gen)
+        mags = torch.zeros(9, D).index_add_(0, idx, go.abs())
+        want = torch.zeros(9, D, dtype=torch.float64).index_add_(0, idx, go.double())
+        dirty_memory(dev)
+        codes.weight.grad = None
+        if way == "twice":
+            ((codes(idx.to(dev)) * go.to(dev)).sum() * 0.25 + (codes(idx.to(dev)) * go.to(dev)).sum() * 0.75).backward()
+        elif way == "summed":
+            for f in (0.25, 0.75):
+                ((codes(idx.to(dev)) * go.to(dev)).sum() * f).backward()
+        else:
+            (codes(idx.to(dev)) * go.to(dev)).sum().backward()
+        if way in ("clipped", "embedding"):
+            norm = float(T.clip_grad_norm_(codes.parameters(), 0.5))
+            assert abs(norm - float(want.norm())) <= 16 * F32 * float(mags.double().norm())
+            want, mags = want * (0.5 / (norm + 1e-6)), mags * (0.5 / (norm + 1e-6))
+        g = codes.weight.grad
+        assert g.is_sparse and (D <= 256 or g.is_coalesced())
+        dense = g.to_dense().cpu()
+        within(dense, want, mags.double() * 24 * F32 + 1e-30)            # (two products, four sums and the factor's six roundings, each on either way)
+        rows = torch.unique(idx)
+        host.grad = torch.sparse_coo_tensor(rows[None], dense[rows], (9, D))
+        dirty_memory(dev)
+        ours.step()
+        ref.step()
+        assert float((codes.weight.detach().cpu() - host.detach()).abs().max()) <= sparse_adam_bound(k + 1, 1e-3, start), k
+
+
+@gpu
+@pytest.mark.parametrize("t", FLOATS)
+def test_a_folded_row_gradient_holds_every_row_once(dev, t):
+    gen = torch.Generator(device=dev).manual_seed(2)
+    for V, shape, N in ((1, (300,), 5), (70, (257,), 1), (70, (3, 200), 900), (50000, (300,), 9001)):
+        idx = (torch.rand(N, device=dev, generator=gen) ** 2 * V).long().clamp_(0, V - 1)
+        values = torch.randn(N, *shape, device=dev, generator=gen).to(t)
+        g = torch.sparse_coo_tensor(idx[None], values, (V, *shape), is_coalesced=False)
+        assert T._needs_fold(g)
+        f = T._folded(g)
+        assert f.is_coalesced() and f.dtype == t and f.shape == g.shape and not T._needs_fold(f)
+        rows = torch.unique(idx.cpu())
+        assert torch.equal(f._indices()[0].cpu(), rows)
+        want = torch.zeros(V, *shape, dtype=torch.float64, device=dev).index_put_((idx,), values.double(), accumulate=True)[rows.to(dev)]
+        mag = torch.zeros(V, *shape, dtype=torch.float64, device=dev).index_put_((idx,), values.double().abs(), accumulate=True)[rows.to(dev)]
+        within(f._values(), want, want.abs() * half_step(t) * (1 + half_step(t)) + mag * N * F32 + tiny(t))
+    assert not T._needs_fold(torch.sparse_coo_tensor(idx[None], values[:, :256], (V, 256)))      # torch takes these itself
+
+
+@gpu
+def test_every_stage_of_the_training_script_stays_finite(dev):
+    """the trainer's step; after each stage the code table, its gradient and the optimiser's state hold finite numbers, and what a stage does not
+    write keeps its bits"""
+    from nphm_amd.loss_functions import compute_loss, weighted_total
+    decoder = U.build_identity(device=dev).train()
+    gen = torch.Generator().manual_seed(13)
+    B = 4
+    pts = lambda n: (torch.rand(B, n, 3, generator=gen) - 0.5) * 0.5  # noqa: E731
+    nrm = lambda n: torch.nn.functional.normalize(torch.randn(B, n, 3, generator=gen), dim=-1)  # noqa: E731
+    batch = {"points_face": pts(60), "normals_face": nrm(60), "points_non_face": pts(9), "normals_non_face": nrm(9), "sup_grad_far": nrm(11) * 0.4,
+             "sup_grad_near": pts(33), "gt_anchors": torch.from_numpy(U.anchors_mean()).float().reshape(1, 39, 3).repeat(B, 1, 1),
+             "idx": torch.tensor([[3], [1], [3], [0]]), "path": ["x"] * B}
+    lambdas = {"surf_sdf": 2.0, "normals": 0.3, "space_sdf": 0.01, "grad": 0.1, "lat_reg": 0.005, "anchors": 7.5, "symm_dist": 0.005, "middle_dist": 0.001}
+    codes = T.LatentCodes(6, decoder.lat_dim, max_norm=1.0, sparse=True, device=dev)
+    with torch.no_grad():
+        codes.weight.copy_(torch.randn(6, decoder.lat_dim, generator=gen) * 0.1)
+    optims = torch.optim.AdamW(decoder.parameters(), lr=1e-4), torch.optim.SparseAdam(codes.parameters(), lr=1e-3)
+    idle = codes.weight.detach()[[2, 4, 5]].clone()
+
+    def finite(stage, *tensors):
+        for t in tensors:
+            assert bool(torch.isfinite(t).all()), (stage, (~torch.isfinite(t)).nonzero()[:4].tolist())
+
+    for k in range(3):
+        dirty_memory(dev)
+        for o in optims:
+            o.zero_grad()
+        loss = weighted_total(compute_loss(dict(batch), decoder, codes, dev), lambdas)
+        finite("forward", loss.detach(), codes.weight.detach())
+        dirty_memory(dev)
+        loss.backward()
+        finite("backward", codes.weight.grad._values(), *[p.grad for p in decoder.parameters() if p.grad is not None])
+        norms = T.clip_grad_norm_(decoder.parameters(), 0.1), T.clip_grad_norm_(codes.parameters(), 0.1)
+        grad = codes.weight.grad
+        finite("clips", *norms, grad._values(), *[p.grad for p in decoder.parameters() if p.grad is not None])
+        assert grad._indices()[0].tolist() == [0, 1, 3]
+        table, values = codes.weight.detach().clone(), grad._values().clone()
+        dirty_memory(dev)
+        optims[0].step()
+        assert torch.equal(codes.weight, table) and torch.equal(grad._values(), values)
+        optims[1].step()
+        state = optims[1].state[codes.weight]
+        finite("optimisers", codes.weight.detach(), state["exp_avg"], state["exp_avg_sq"])
+        assert float((codes.weight.detach() - table).abs().max()) <= 3.2e-3           # (Adam's largest step: lr (1 - b1) / sqrt(1 - b2))
+        assert torch.equal(codes.weight.detach()[[2, 4, 5]], idle)
+        assert not bool(state["exp_avg"][[2, 4, 5]].any()) and not bool(state["exp_avg_sq"][[2, 4, 5]].any())
+
+
 # ---- all of them -----------------------------------------------------------------------------------------------------------------
 
 def step(dev, codes, layers, idx, pts, target):
