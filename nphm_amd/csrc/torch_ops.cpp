@@ -129,8 +129,12 @@ Tensor rows_grad(const Tensor& grad, const Tensor& idx, int64_t rows, double sca
   return out;
 }
 
+// what the gradient of a lookup is: dense; an entry for every index, which is row 0 and zeros where it must not count; the same with
+// padding left on its own row (a module's: an optimiser that steps every row it finds named then moves no row by it)
+enum { GRAD_DENSE = 0, GRAD_ENTRIES = 1, GRAD_ENTRIES_PADDED = 2 };
+
 struct LookupNode : torch::autograd::Function<LookupNode> {
-  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& idx, double scale, int64_t padding, bool sparse) {
+  static Tensor forward(AutogradContext* ctx, const Tensor& table, const Tensor& idx, double scale, int64_t padding, int64_t sparse) {
     ctx->save_for_backward({idx});
     ctx->saved_data["meta"] = std::vector<int64_t>{table.size(0), padding, sparse};
     ctx->saved_data["scale"] = scale;
@@ -142,7 +146,7 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
     const int64_t rows = meta[0], padding = meta[1];
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor out;
-    if (!meta[2]) {
+    if (meta[2] == GRAD_DENSE) {
       out = rows_grad(g, idx, rows, scale, padding < 0 ? std::nullopt : std::optional<int64_t>(padding));
     } else {
       // an entry an index, as nn.Embedding(sparse=True) leaves it; an entry that must not count names a row that exists and adds zeros
@@ -155,13 +159,14 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
       Tensor index = at::empty({1, count}, i.options().dtype(at::kLong)), values = at::empty({count, D}, g.options());
       check(lib.rows_entries(const_of(g2), count, D, ld, code_of(g.scalar_type()), const_of(i), bits_of(i), rows, padding, float(scale),
                              static_cast<int64_t*>(at_of(index)), at_of(values), stream_of(g)), "nphm_rows_entries");
+      if (meta[2] == GRAD_ENTRIES_PADDED && padding >= 0) index.view({count}).masked_fill_(i.view({count}).eq(padding), padding);
       out = at::_sparse_coo_tensor_unsafe(index, values, {rows, D}, values.options().layout(at::kSparse));
     }
     return once({out, Tensor(), Tensor(), Tensor(), Tensor()}, "lookup_rows");
   }
 };
 
-Tensor lookup_rows(const Tensor& table, const Tensor& idx, double scale, std::optional<int64_t> padding_idx, bool sparse) {
+Tensor lookup_rows(const Tensor& table, const Tensor& idx, double scale, std::optional<int64_t> padding_idx, int64_t sparse) {
   const char* what = "lookup_rows";
   check_rows(what, table, idx, scale);
   check_table(what, table);
@@ -386,7 +391,7 @@ extern "C" __attribute__((visibility("default"))) PyObject* nphm_torch_clip(PyOb
 }
 
 TORCH_LIBRARY(nphm_amd, m) {
-  m.def("lookup_rows(Tensor table, Tensor idx, float scale, int? padding_idx, bool sparse) -> Tensor", &lookup_rows);
+  m.def("lookup_rows(Tensor table, Tensor idx, float scale, int? padding_idx, int sparse) -> Tensor", &lookup_rows);
   m.def("lookup_rows_grad(Tensor grad, Tensor idx, int num_rows, float scale, int? padding_idx) -> Tensor", &rows_grad);
   m.def("renorm_rows_(Tensor(a!) table, Tensor idx, float max_norm) -> ()", &renorm_rows);
   m.def("linear_act(Tensor x, Tensor weight, Tensor? bias, Tensor? residual, int act, float beta) -> Tensor", &linear_act);

@@ -59,7 +59,7 @@ def lookup_rows(table, idx, scale=1.0, padding_idx=None, sparse=False):
     sparse one with an entry for every index (``LatentCodes`` and ``clip_grad_norm_`` coalesce it where torch's optimisers cannot).  Row
     `padding_idx` is read like any other and gets no gradient.  An index outside the table gives a row of NaN and adds nothing to the
     gradient (nothing on the host looks at the indices)."""
-    return _ops.lookup_rows(table, idx, scale, padding_idx, sparse)
+    return _ops.lookup_rows(table, idx, scale, padding_idx, 1 if sparse else 0)
 
 
 def lookup_rows_grad(grad, idx, num_rows, scale=1.0, padding_idx=None):
@@ -106,7 +106,8 @@ class LatentCodes(nn.Embedding):
     """The table of latent codes of the trainers (nn.Embedding(n, lat_dim, max_norm=1.0, sparse=True), training.py:36-40) on
     ``lookup_rows`` / ``renorm_rows_``; parameters, initialisation and state_dict are nn.Embedding's.  ``scale`` multiplies the looked-up
     rows.  With ``sparse``, codes of more than 256 entries get their ``weight.grad`` coalesced when a backward pass has left it (which waits for
-    the device; not while a graph is captured): torch.optim.SparseAdam takes it as it is, where torch would lose columns of it.
+    the device; not while a graph is captured): torch.optim.SparseAdam takes it as it is, where torch would lose columns of it.  Padding in
+    a batch is an entry of zeros for its own row there: no optimiser moves a row by it.
     ``backend = "composite"`` computes the same with torch's embedding (CPU tensors need it, as in the decoders)."""
 
     def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, scale=1.0, sparse=False, device=None, dtype=None):
@@ -127,7 +128,7 @@ class LatentCodes(nn.Embedding):
             return rows if self.scale == 1.0 else rows * self.scale
         if self.max_norm is not None:
             renorm_rows_(self.weight, idx, self.max_norm)
-        return lookup_rows(self.weight, idx, self.scale, self.padding_idx, self.sparse)
+        return _ops.lookup_rows(w, idx, self.scale, self.padding_idx, 2 if self.sparse else 0)         # (2: padding stays on its own row)
 
 
 # ---- dense layer in 16 bits --------------------------------------------------------------------------------------------------

@@ -863,6 +863,29 @@ def test_row_gradients_step_sparse_adam(dev, way, D):
 
 
 @gpu
+@pytest.mark.parametrize("D", [40, 300])
+@pytest.mark.parametrize("kind", [torch.int64, torch.int32])
+def test_padding_in_a_batch_moves_no_row_of_a_sparse_table(dev, D, kind):
+    """row 0 has momentum from the first step; the batches behind it name padding and other rows, or padding alone: it keeps its bits, and so
+    does the padding row"""
+    codes = T.LatentCodes(6, D, padding_idx=-2, sparse=True, device=dev)
+    assert codes.padding_idx == 4
+    optim = torch.optim.SparseAdam(codes.parameters(), lr=1e-2)
+    kept = None
+    for idx in ([0, 4, 1, 0], [4, 2, 4], [4, 4], [4], [5, 4]):
+        optim.zero_grad()
+        before = codes.weight.detach().clone()
+        codes(torch.tensor(idx, device=dev, dtype=kind)).square().sum().add(codes.weight[0, 0].detach()).backward()
+        optim.step()
+        named = sorted(set(idx) - {4})
+        moved = [v for v in range(6) if not torch.equal(codes.weight[v], before[v])]
+        if kept is None:
+            kept = codes.weight[0].detach().clone()
+        assert torch.equal(codes.weight[0], kept) and set(moved) <= set(named), (idx, moved)
+        assert bool(torch.isfinite(codes.weight).all())
+
+
+@gpu
 @pytest.mark.parametrize("t", FLOATS)
 def test_a_folded_row_gradient_holds_every_row_once(dev, t):
     gen = torch.Generator(device=dev).manual_seed(2)
