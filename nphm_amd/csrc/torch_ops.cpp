@@ -55,6 +55,10 @@ void on_gpu(const char* what, const Tensor& t) {
   TORCH_CHECK_TYPE(t.is_cuda(), what, ": a tensor on a ROCm device (these operators have no CPU form)");
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
+// Forward-mode derivatives: none is computed, and none may be lost without a word.
+void no_tangent(const char* what, const Tensor& t) {
+  TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, ": no forward-mode derivative (torch.autograd.forward_ad)");
+}
 // (address 0 and no tensor where nothing is needed)
 Tensor workspace(size_t bytes, const Tensor& like) { return bytes ? at::empty({int64_t(bytes)}, like.options().dtype(at::kByte)) : Tensor(); }
 void* at_of(const Tensor& t) { return t.defined() ? t.mutable_data_ptr() : nullptr; }
@@ -76,6 +80,7 @@ variable_list once(variable_list grads, const char* what) {
 void check_rows(const char* what, const Tensor& rows, const Tensor& idx, double scale) {
   bound();
   on_gpu(what, rows);
+  no_tangent(what, rows);
   TORCH_CHECK_TYPE(code_of(rows.scalar_type()) >= 0, what, ": rows of fp32, bf16 or fp16, not ", rows.scalar_type());
   TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, what, ": idx is an int32 or int64 tensor");
   TORCH_CHECK_VALUE(idx.device() == rows.device(), what, ": idx is on ", idx.device(), ", the rows on ", rows.device());
@@ -146,6 +151,7 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
     const int64_t rows = meta[0], padding = meta[1];
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor out;
+    no_tangent("lookup_rows", g);
     if (meta[2] == GRAD_DENSE) {
       out = rows_grad(g, idx, rows, scale, padding < 0 ? std::nullopt : std::optional<int64_t>(padding));
     } else {
@@ -229,6 +235,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
     const int64_t meta = ctx->saved_data["meta"].toInt(), act = meta >> 4, asked = meta & 15;
     const double beta = ctx->saved_data["beta"].toDouble();
     variable_list out(7);                                            // (one for each argument of forward)
+    no_tangent("linear_act", g);
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(x.device());
@@ -262,6 +269,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
   const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
   on_gpu(what, x);
   on_gpu(what, weight);
+  no_tangent(what, x);
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what, ": bf16 or fp16 tensors, not ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.numel() > 0, what, ": x ", x.sizes(),
                     " does not fit weight ", weight.sizes());
@@ -274,6 +282,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
   int bit = 2;
   for (const Tensor* t : {&weight, &bias, &residual}) {
     if (t->defined()) {
+      no_tangent(what, *t);
       TORCH_CHECK_TYPE(t->scalar_type() == x.scalar_type() && t->device() == x.device(), what, ": all tensors on one device, of one type");
       if (t->requires_grad()) asked |= bit;
     }
@@ -324,6 +333,8 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
     const Tensor *g = grads[i], *o = writes ? out[i] : g;
     TORCH_CHECK_VALUE(in_place || (o->numel() == g->numel() && o->scalar_type() == g->scalar_type() && o->device() == device && o->layout() == at::kStrided),
                       what, ": out has a tensor of the size, type and device of each gradient");
+    no_tangent(what.c_str(), *g);
+    no_tangent(what.c_str(), *o);
     counts[i] = g->numel();
     codes[i] = code_of(g->scalar_type());
     // any order of dimensions will do, if it is the same on both sides and leaves no gap

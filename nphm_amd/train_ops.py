@@ -11,7 +11,7 @@ clip_grad_norm_ between ``compute_loss`` and the optimisers, src/NPHM/models/tra
 Every function runs on libnphm_amd.so (csrc/rows_kernels.hip, clip_kernels.hip, layer16_kernels.hip; csrc/torch_ops.cpp checks its
 arguments, allocates and holds its autograd node), on the current stream of its tensors' device.  It raises ``ValueError`` /
 ``TypeError`` for what it does not take and ``NphmAmdError`` if the library is missing or a call fails; there is no PyTorch fallback,
-CPU tensors are refused.  Results are the same bits from run to run.  All of it can be captured into a graph, except where a
+CPU tensors are refused, and so are forward-mode (dual) tensors, with ``NotImplementedError``.  Results are the same bits from run to run.  All of it can be captured into a graph, except where a
 line says that it waits for the device.  (A backward pass is captured on leaves of which no graph of eager calls is alive: autograd would
 make the capturing stream wait for work outside the capture.)"""
 from __future__ import annotations

@@ -802,6 +802,31 @@ def test_duplicates_of_a_sparse_gradient_are_folded(dev, N, rows, D):
     assert not got[rest].any()
 
 
+@gpu
+@pytest.mark.parametrize("asks", [False, True])
+def test_forward_mode_inputs_are_refused(dev, asks):
+    """a dual tensor would come out without its tangent; whether it requires a gradient or not, in every place that takes one"""
+    import torch.autograd.forward_ad as fwAD
+    idx = torch.tensor([1, 0], device=dev)
+    plain = lambda *s, t=torch.bfloat16: torch.randn(*s, device=dev).to(t)  # noqa: E731
+    with fwAD.dual_level():
+        dual = lambda *s, t=torch.bfloat16: fwAD.make_dual(plain(*s, t=t).requires_grad_(asks), plain(*s, t=t))  # noqa: E731
+        table, x, w, b, r = dual(4, 8, t=torch.float32), dual(3, 8), dual(5, 8), dual(5), dual(3, 5)
+        for call in (lambda: T.lookup_rows(table, idx), lambda: T.lookup_rows(table, idx, sparse=True), lambda: T.lookup_rows_grad(table[:2], idx, 4),
+                     lambda: T.renorm_rows_(table, idx, 1e-3), lambda: T.linear_act(x, plain(5, 8)), lambda: T.linear_act(plain(3, 8), w, activation="relu"),
+                     lambda: T.linear_act(plain(3, 8), plain(5, 8), b), lambda: T.linear_act(plain(3, 8), plain(5, 8), residual=r),
+                     lambda: T.grad_norm([plain(3), w]), lambda: T.clip_grads([w], 1.0, out=[plain(5, 8)]), lambda: T.clip_grads([plain(5, 8)], 1.0, out=[w])):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                call()
+        with torch.no_grad(), pytest.raises(NotImplementedError, match="forward-mode"):
+            T.linear_act(x, plain(5, 8))
+        leaf, codes = plain(5, 8).requires_grad_(), plain(4, 8).requires_grad_()
+        for y, p in ((T.linear_act(plain(3, 8), leaf), leaf), (T.lookup_rows(codes, idx), codes), (T.lookup_rows(codes, idx, sparse=True), codes)):
+            with pytest.raises(NotImplementedError, match="forward-mode"):
+                torch.autograd.grad(y, p, fwAD.make_dual(plain(*y.shape), plain(*y.shape)))
+    T.lookup_rows(plain(4, 8), idx)
+
+
 def dirty_memory(dev):
     """small blocks that are handed out again hold NaN: what a later call leaves unwritten shows"""
     held = [torch.full((n * 1344,), math.nan, device=dev) for n in (1, 2, 3, 4, 6, 8, 12, 24) for _ in range(4)]
