@@ -307,6 +307,22 @@ std::vector<const Tensor*> tensors_of(const std::string& what, PyObject* list) {
   return all;
 }
 
+// whether two elements of a tensor lie in one place, or cannot be told apart simply: sorted by stride, each dimension has to step over
+// all that the ones below it reach (views of a dense tensor do; expanded and unfolded ones do not)
+bool meets_itself(const Tensor& t) {
+  if (t.is_contiguous() || t.numel() < 2) return false;
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  for (int64_t d = 0; d < t.dim(); ++d)
+    if (t.size(d) > 1) dims.emplace_back(t.stride(d), t.size(d));
+  std::sort(dims.begin(), dims.end());
+  int64_t reach = 0;
+  for (const auto& [stride, size] : dims) {
+    if (stride <= reach) return true;
+    reach += stride * (size - 1);
+  }
+  return false;
+}
+
 // -> norm; `out` None: the norm alone, the list itself: in place.  out[i] may be grads[i].
 Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, int kind, double limit) {
   bound();
@@ -343,6 +359,7 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
       held.push_back(g->contiguous());
       from[i] = held.back().const_data_ptr();
       if (!writes) continue;
+      TORCH_CHECK(!meets_itself(*o), "nphm: ", what, ": a tensor to be written has several elements in one place");
       back.emplace_back(*o, at::empty_like(held.back()));
       to[i] = back.back().second.mutable_data_ptr();
       continue;

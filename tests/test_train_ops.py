@@ -731,6 +731,27 @@ def test_clip_refuses_a_tensor_named_twice(dev):
 
 
 @gpu
+def test_clip_refuses_what_meets_itself_before_it_writes(dev):
+    """expanded or unfolded tensors to be written: refused, with the tensors in front of them as they were; read they count as what they hold"""
+    base = torch.randn(6, 8, device=dev)
+    for shared in (base[:1].expand(4, 8), base[:, :1].expand(6, 5), base.view(-1).unfold(0, 8, 3), base.view(-1).as_strided((3, 4), (2, 3))):
+        other, kept = torch.ones(50, device=dev), base.clone()
+        with pytest.raises(NphmAmdError, match="in one place"):
+            T.clip_grads([other, shared], 0.1)
+        with pytest.raises(NphmAmdError, match="in one place"):
+            T.clip_grads([other, torch.ones(shared.shape, device=dev)], 0.1, out=[other, shared])
+        assert torch.equal(base, kept) and torch.equal(other, torch.ones(50, device=dev))
+        out = torch.zeros(shared.shape, device=dev)
+        norm, _ = T.clip_grads([shared], 0.1, out=[out])
+        want = shared.double() * min(1.0, 0.1 / (float(shared.double().norm()) + 1e-6))
+        within(out, want, clip_bound(want, torch.float32))
+    for fine in (base.t(), base[::2, 1::3], base[:, 2:3], base.view(2, 3, 8)[:, 1].t()):
+        want = fine.double() * min(1.0, 0.1 / (float(fine.double().norm()) + 1e-6))
+        T.clip_grads([fine], 0.1)
+        within(fine, want, clip_bound(want, torch.float32))
+
+
+@gpu
 def test_norm_of_huge_and_tiny_gradients(dev):
     """squares of these leave fp32 on both sides; the norm does not"""
     for v in (1e30, 1e-30):
