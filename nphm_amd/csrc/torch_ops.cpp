@@ -323,6 +323,61 @@ bool meets_itself(const Tensor& t) {
   return false;
 }
 
+// the bytes of a tensor: from its first on, dimensions of more than one place as (stride, places), a single byte the smallest
+struct Places {
+  uintptr_t first, end;
+  std::vector<std::pair<int64_t, int64_t>> dims;
+  explicit Places(const Tensor& t) : first(reinterpret_cast<uintptr_t>(t.const_data_ptr())) {
+    const int64_t e = int64_t(t.element_size());
+    int64_t reach = e - 1;
+    if (t.is_non_overlapping_and_dense()) {                          // (whatever the order of its dimensions)
+      reach = t.numel() * e - 1;
+      dims.emplace_back(1, t.numel() * e);
+    } else {
+      dims.emplace_back(1, e);
+      for (int64_t d = 0; d < t.dim(); ++d)
+        if (t.size(d) > 1 && t.stride(d)) dims.emplace_back(t.stride(d) * e, t.size(d)), reach += t.stride(d) * e * (t.size(d) - 1);
+    }
+    end = t.numel() ? first + uintptr_t(reach) + 1 : first;
+  }
+  bool apart(const Places& o) const { return first == end || o.first == o.end || end <= o.first || o.end <= first; }
+};
+
+// Whether two tensors share a byte: a.first + sum x_i s_i = b.first + sum y_j t_j, 0 <= x_i, y_j < their places.  Dimensions of one stride
+// are one unknown with a range; from the largest stride down, only values from which the smaller ones reach the rest are tried
+// (one or two each for views of one buffer).  Strides that have nothing to do with each other could take long: they count as
+// meeting after 100 000 tries.
+bool share(const Places& a, const Places& b) {
+  if (a.apart(b)) return false;
+  struct Term { int64_t stride, lo, hi; };
+  std::vector<Term> terms;
+  auto add = [&](int64_t stride, int64_t lo, int64_t hi) {
+    for (Term& t : terms)
+      if (t.stride == stride) { t.lo += lo; t.hi += hi; return; }
+    terms.push_back({stride, lo, hi});
+  };
+  for (const auto& [stride, places] : a.dims) add(stride, 0, places - 1);
+  for (const auto& [stride, places] : b.dims) add(stride, 1 - places, 0);
+  std::sort(terms.begin(), terms.end(), [](const Term& x, const Term& y) { return x.stride > y.stride; });
+  std::vector<int64_t> low(terms.size() + 1), high(terms.size() + 1);          // what the terms from i on reach
+  for (size_t i = terms.size(); i-- > 0;) {
+    low[i] = low[i + 1] + terms[i].lo * terms[i].stride;
+    high[i] = high[i + 1] + terms[i].hi * terms[i].stride;
+  }
+  int tries = 100000;
+  auto down = [](int64_t v, int64_t s) { return v >= 0 ? v / s : -((-v + s - 1) / s); };
+  auto reaches = [&](auto&& self, size_t i, int64_t rest) -> bool {
+    if (rest < low[i] || rest > high[i]) return false;
+    if (i == terms.size() || --tries < 0) return true;
+    const Term& t = terms[i];
+    const int64_t from = std::max(t.lo, -down(high[i + 1] - rest, t.stride)), to = std::min(t.hi, down(rest - low[i + 1], t.stride));
+    for (int64_t x = from; x <= to; ++x)
+      if (self(self, i + 1, rest - x * t.stride)) return true;
+    return false;
+  };
+  return reaches(reaches, 0, int64_t(b.first) - int64_t(a.first));
+}
+
 // -> norm; `out` None: the norm alone, the list itself: in place.  out[i] may be grads[i].
 Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, int kind, double limit) {
   bound();
@@ -345,6 +400,7 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
   std::vector<int> codes(n);
   std::vector<Tensor> held;                                          // copies that the launches read or write
   std::vector<std::pair<Tensor, Tensor>> back;
+  std::vector<size_t> copied;
   for (size_t i = 0; i < n; ++i) {
     const Tensor *g = grads[i], *o = writes ? out[i] : g;
     TORCH_CHECK_VALUE(in_place || (o->numel() == g->numel() && o->scalar_type() == g->scalar_type() && o->device() == device && o->layout() == at::kStrided),
@@ -357,6 +413,7 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
     if (!(g->is_contiguous() && (in_place || o->is_contiguous()))
         && !(g->is_non_overlapping_and_dense() && g->sizes() == o->sizes() && g->strides() == o->strides())) {
       held.push_back(g->contiguous());
+      copied.push_back(i);
       from[i] = held.back().const_data_ptr();
       if (!writes) continue;
       TORCH_CHECK(!meets_itself(*o), "nphm: ", what, ": a tensor to be written has several elements in one place");
@@ -367,11 +424,18 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
     from[i] = g->const_data_ptr();
     if (writes) to[i] = o->mutable_data_ptr();
   }
-  if (back.size() > 1) {                                             // (the others' memory is compared behind the C entry)
-    std::vector<const void*> starts;
-    for (const auto& pair : back) starts.push_back(pair.first.const_data_ptr());
-    std::sort(starts.begin(), starts.end());
-    TORCH_CHECK(std::adjacent_find(starts.begin(), starts.end()) == starts.end(), "nphm: ", what, ": two of the tensors share memory");
+  // tensors of which the launches see copies, or whose results come from a copy, against all others; those whose own memory is handed to the C
+  // entry are compared with each other behind it
+  if (!held.empty() && writes) {
+    std::vector<Places> read, wrote;
+    for (size_t i = 0; i < n; ++i) {
+      read.emplace_back(*grads[i]);
+      wrote.emplace_back(*out[i]);
+    }
+    for (const size_t i : copied)
+      for (size_t k = 0; k < n; ++k)
+        TORCH_CHECK(k == i || !(share(wrote[i], wrote[k]) || (!in_place && (share(wrote[i], read[k]) || share(read[i], wrote[k])))), "nphm: ", what,
+                    ": two of the tensors share memory");
   }
   const size_t need = lib.clip_ws(counts.data(), int(n));
   const Tensor ws = workspace(need, *grads[0]), norm = at::empty({}, grads[0]->options().dtype(at::kFloat).requires_grad(false));

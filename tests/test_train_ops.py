@@ -752,6 +752,38 @@ def test_clip_refuses_what_meets_itself_before_it_writes(dev):
 
 
 @gpu
+def test_clip_refuses_views_with_gaps_that_share_memory(dev):
+    """whatever their starts and orders, beside dense tensors and each other, in place and as results; interleaved views share nothing"""
+    buf, kept = torch.randn(24, 40, device=dev), None
+    spare = lambda like: torch.zeros(like.shape, device=dev)  # noqa: E731
+    pairs = [(buf, buf[:, ::2]), (buf[:, ::2], buf), (buf[:, ::2], buf[:, 2::2]), (buf[:, 1::2], buf[:, ::3]), (buf[::2], buf[:, 5:9]), (buf.t()[3:], buf[5, 7:8]),
+             (buf[1:, :-1], buf.view(-1)[900:]), (buf.view(-1)[7:-1:9], buf[20:])]
+    for a, b in pairs:
+        kept = buf.clone()
+        for grads, out in (([a, b], [a, b]), ([spare(a), spare(b)], [a, b]), ([a, spare(b)], [spare(a), b]), ([spare(a), b], [a, spare(b)]),
+                           ([spare(buf), a, b], [spare(buf), a, b])):
+            with pytest.raises(NphmAmdError, match="share memory"):
+                T.clip_grads(grads, 1e-3, out=out)
+        with pytest.raises(NphmAmdError, match="share memory"):
+            T.clip_grads([a, b], 1e-3)
+        assert torch.equal(buf, kept)
+        assert abs(float(T.grad_norm([a, b])) - math.hypot(float(a.double().norm()), float(b.double().norm()))) <= 4 * F32 * 2 * float(buf.norm())
+    for views in ([buf[:, ::2], buf[:, 1::2]], [buf[:, :15], buf[:, 15:]], [buf[::3, ::2], buf[1::3], buf[2::3, 3:], buf[::3, 1::2]], [buf.t()[:7], buf.t()[7:].t()]):
+        kept, before = buf.clone(), [v.double() for v in views]
+        total = math.sqrt(sum(float(v.square().sum()) for v in before))
+        norm, out = T.clip_grads(views, 0.5 * total)
+        assert abs(float(norm) - total) <= 4 * F32 * total
+        for v, w in zip(out, before):
+            want = w * (0.5 * total / (total + 1e-6))
+            within(v, want, clip_bound(want, torch.float32))
+        buf.copy_(kept)
+    # the two halves of one buffer
+    square = torch.randn(16, 16, device=dev)
+    T.clip_grads([square[:, :8]], 1e9, out=[square[:, 8:]])
+    assert torch.equal(square[:, 8:], square[:, :8])
+
+
+@gpu
 def test_norm_of_huge_and_tiny_gradients(dev):
     """squares of these leave fp32 on both sides; the norm does not"""
     for v in (1e30, 1e-30):
