@@ -689,7 +689,8 @@ int nphm_clip_grads(const void* const* in, void* const* out, const int64_t* coun
 /*   nphm_layer16_forward : z = x W^T + bias, y = a(z) + residual; x [M, K], weight [N, K], y / z / residual [M, N], bias [N], all
  *     contiguous bf16 or fp16; bias, residual, z (kept for the backward pass) may be NULL.  act: 0 none, 1 ReLU, 2 SiLU, 3 GELU
  *     (erf), 4 Softplus(beta).  M up to 2^22, N and K up to 2^20.
- *   nphm_layer16_backward : gz = g a'(z); dx = gz W, dweight = gz^T x, dbias = column sums of gz (each may be NULL).
+ *   nphm_layer16_backward : gz = g a'(z); dx = gz W, dweight = gz^T x, dbias = column sums of gz (each may be NULL; weight without dx and x
+ *     without dweight may be, too: the workspace is then smaller).
  *     Workspaces: nphm_layer16_*_workspace_bytes of the same operands (0: none is needed, NULL will do), 256-byte aligned. */
 size_t nphm_layer16_forward_workspace_bytes(const void* x, const void* weight, int64_t M, int64_t N, int64_t K);
 int nphm_layer16_forward(const void* x, const void* weight, const void* bias, const void* residual, void* y, void* z, int64_t M, int64_t N,

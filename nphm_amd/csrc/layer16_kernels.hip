@@ -909,12 +909,12 @@ inline Backward backward_plan(const void* g, const void* x, const void* weight, 
   p.w_t = tiling(N, K, M);
   p.same = act == ACT_NONE && !packed(g, N);
   p.gz = 0;
-  p.sums = p.gz + (p.same ? 0 : up(size_t(M) * whole8(N) * 2));
+  p.sums = p.gz + (p.same || !(x || weight) ? 0 : up(size_t(M) * whole8(N) * 2));      // (db alone: nobody reads gz)
   p.x = p.sums + up(size_t(gz_tiles(M, whole8(N))) * N * 4);
-  p.weight = p.x + (packed(x, K) ? up(size_t(M) * whole8(K) * 2) : 0);
-  p.parts_x = p.weight + (packed(weight, K) ? up(size_t(N) * whole8(K) * 2) : 0);
-  p.parts_w = p.parts_x + parts_bytes(p.x_t, M, K);
-  p.total = p.parts_w + parts_bytes(p.w_t, N, K);
+  p.weight = p.x + (x && packed(x, K) ? up(size_t(M) * whole8(K) * 2) : 0);
+  p.parts_x = p.weight + (weight && packed(weight, K) ? up(size_t(N) * whole8(K) * 2) : 0);
+  p.parts_w = p.parts_x + (weight ? parts_bytes(p.x_t, M, K) : 0);
+  p.total = p.parts_w + (x ? parts_bytes(p.w_t, N, K) : 0);
   return p;
 }
 
@@ -981,7 +981,7 @@ int nphm_layer16_backward(const void* g, const void* x, const void* weight, cons
       const Packs packs = packs_of(Pack{x, ws + plan.x, px ? M : 0}, Pack{weight, ws + plan.weight, pw ? N : 0}, K);
       Columns columns{};
       if (!plan.same || dbias)
-        columns = make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same ? nullptr : gz,
+        columns = make_gz<T>(st, static_cast<const T*>(g), act == ACT_NONE ? nullptr : static_cast<const T*>(z), plan.same || !(dx || dweight) ? nullptr : gz,
                              reinterpret_cast<float*>(ws + plan.sums), static_cast<T*>(dbias), int(M), int(N), int(ldn), act, beta, packs);
       else
         pack<T>(st, packs);

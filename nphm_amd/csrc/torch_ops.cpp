@@ -220,38 +220,45 @@ std::tuple<Tensor, Tensor> layer_forward(const Tensor& x, const Tensor& weight, 
 }
 
 struct LayerNode : torch::autograd::Function<LayerNode> {
-  // the inputs that ask for a gradient: one bit each (x, weight, bias, residual)
+  // asked: the inputs that ask for a gradient, one bit each (x, weight, bias, residual).  x is kept for weight's gradient, weight for x's, z for
+  // the first three.
   static Tensor forward(AutogradContext* ctx, const Tensor& x, const Tensor& weight, const std::optional<Tensor>& bias,
                         const std::optional<Tensor>& residual, int64_t act, double beta, int64_t asked) {
-    auto [y, z] = layer_forward(x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), act, beta, true);
-    ctx->save_for_backward({x, weight, z});
-    ctx->saved_data["meta"] = act << 4 | asked;
+    auto [y, z] = layer_forward(x, weight, bias.value_or(Tensor()), residual.value_or(Tensor()), act, beta, (asked & 7) != 0);
+    ctx->save_for_backward({asked & 2 ? x : Tensor(), asked & 1 ? weight : Tensor(), z});
+    const int64_t there = 3 | (bias && bias->defined() ? 4 : 0) | (residual && residual->defined() ? 8 : 0);
+    ctx->saved_data["meta"] = std::vector<int64_t>{act, asked, there, weight.size(0), weight.size(1)};
+    ctx->saved_data["sizes"] = x.sizes().vec();
     ctx->saved_data["beta"] = beta;
     return y;
   }
   static variable_list backward(AutogradContext* ctx, variable_list grads) {
     const auto saved = ctx->get_saved_variables();
     const Tensor &x = saved[0], &weight = saved[1], &z = saved[2], &g = grads[0];
-    const int64_t meta = ctx->saved_data["meta"].toInt(), act = meta >> 4, asked = meta & 15;
+    const auto meta = ctx->saved_data["meta"].toIntVector(), sizes = ctx->saved_data["sizes"].toIntVector();
+    const int64_t act = meta[0], N = meta[3], K = meta[4];
     const double beta = ctx->saved_data["beta"].toDouble();
+    // of those that asked, the ones that this pass is for (an edge for every tensor there is)
+    int64_t asked = 0;
+    for (int64_t bit = 1, edge = 0; bit <= 8; bit *= 2)
+      if (meta[2] & bit) asked |= ctx->needs_input_grad(size_t(edge++)) ? meta[1] & bit : 0;
     variable_list out(7);                                            // (one for each argument of forward)
     no_tangent("linear_act", g);
     {
       const at::NoGradGuard no_grad;
-      const c10::DeviceGuard guard(x.device());
-      const Tensor w = weight.contiguous();
-      const int64_t N = w.size(0), K = w.size(1), M = x.numel() / K;
-      auto made = [&](int64_t bit, at::IntArrayRef sizes) {
+      const c10::DeviceGuard guard(g.device());
+      const int64_t M = g.numel() / N;
+      auto made = [&](int64_t bit, at::IntArrayRef shape) {
         if (!(asked & bit)) return Tensor();
-        return M ? at::empty(sizes, x.options()) : at::zeros(sizes, x.options());
+        return M ? at::empty(shape, g.options()) : at::zeros(shape, g.options());
       };
-      const Tensor dx = made(1, x.sizes()), dw = made(2, {N, K}), db = made(4, {N});
+      const Tensor dx = made(1, sizes), dw = made(2, {N, K}), db = made(4, {N});
       if (M && (asked & 7)) {
-        const Tensor g2 = rows_of(g), x2 = rows_of(x);
+        const Tensor g2 = rows_of(g), x2 = asked & 2 ? rows_of(x) : Tensor(), w = asked & 1 ? weight.contiguous() : Tensor();
         const size_t need = lib.backward_ws(const_of(g2), const_of(x2), const_of(w), M, N, K, int(act));
-        const Tensor ws = workspace(need, x);
-        check(lib.backward(const_of(g2), const_of(x2), const_of(w), const_of(z), at_of(dx), at_of(dw), at_of(db), M, N, K, code_of(x.scalar_type()),
-                           int(act), float(beta), at_of(ws), need, stream_of(x)), "nphm_layer16_backward");
+        const Tensor ws = workspace(need, g);
+        check(lib.backward(const_of(g2), const_of(x2), const_of(w), const_of(z), at_of(dx), at_of(dw), at_of(db), M, N, K, code_of(g.scalar_type()),
+                           int(act), float(beta), at_of(ws), need, stream_of(g)), "nphm_layer16_backward");
       }
       out[0] = dx;
       out[1] = dw;

@@ -631,6 +631,79 @@ def test_decoder_trains_with_16_bit_hidden_layers(dev, t):
         net.evaluate_train_hip(xyz, lat)
 
 
+def test_backward_workspace_is_for_the_operands_handed_over():
+    """no x: no gradient of the weight, no weight: none of x - and no room for what they would need (host arithmetic, no GPU)"""
+    from nphm_amd import _lib
+    lib = _lib.load()
+    for M, N, K in ((4095, 1024, 515), (128, 128, 100000), (1, 4096, 4096), (100000, 128, 128), (3, 7, 5)):
+        for act in (0, 4):
+            full, x, w, none = [lib.nphm_layer16_backward_workspace_bytes(4096, *p, M, N, K, act) for p in ((4096, 4096), (4096, None), (None, 4096), (None, None))]
+            assert none <= min(x, w) and max(x, w) <= full
+            assert none < full or (N % 8 == 0 and K % 8 == 0 and act == 0 and full == x == w)      # (nothing but db's partial sums)
+
+
+@gpu
+@pytest.mark.parametrize("t", HALVES)
+@pytest.mark.parametrize("M,N,K", [(37, 64, 48), (130, 33, 21), (4095, 96, 515), (300, 512, 2000), (0, 8, 8)])
+@pytest.mark.parametrize("act", ["none", "silu"])
+def test_only_the_gradients_that_are_asked_for(dev, t, M, N, K, act):
+    """every choice of inputs that require one, and of those one pass asks for: the same bits as all of them together"""
+    x, w, b, r, g = layer_inputs(dev, t, M, N, K, True, True)
+    names = ("x", "weight", "bias", "residual")
+    leaves = [v.clone().requires_grad_() for v in (x, w, b, r)]
+    full = dict(zip(names, torch.autograd.grad(T.linear_act(*leaves[:3], act, residual=leaves[3]), leaves, g)))
+    for need in range(1, 16):
+        own = [v.clone().requires_grad_(bool(need >> i & 1)) for i, v in enumerate((x, w, b, r))]
+        for ask in range(1, 16):
+            if ask & ~need:
+                continue
+            picked = [i for i in range(4) if ask >> i & 1]
+            got = torch.autograd.grad(T.linear_act(*own[:3], act, residual=own[3]), [own[i] for i in picked], g)
+            for i, v in zip(picked, got):
+                assert torch.equal(v, full[names[i]]), (need, ask, names[i])
+    # no bias, no residual: the places of the others stay theirs
+    two = [x.clone().requires_grad_(), r.clone().requires_grad_()]
+    got = torch.autograd.grad(T.linear_act(two[0], w, None, act, residual=two[1]), two[1], g)
+    assert torch.equal(got[0], g)
+    got = torch.autograd.grad(T.linear_act(two[0], w, None, act, residual=two[1]), two[0], g)
+    assert got[0].shape == x.shape
+
+
+@gpu
+def test_a_layer_keeps_what_its_gradients_read(dev):
+    """a frozen weight's layer does not keep x (nor mind that it changes), frozen inputs' not the weight, the residual alone keeps nothing"""
+    M, N, K = 1024, 512, 2048
+    x, w, b, r, g = layer_inputs(dev, torch.bfloat16, M, N, K, True, True)
+    leaf = x.clone().requires_grad_()
+    want, = torch.autograd.grad(T.linear_act(leaf, w, b, "silu"), leaf, g)
+    moving = leaf * 1
+    y = T.linear_act(moving, w, b, "silu")
+    moving.detach().zero_()                                          # (no gradient of the weight: x is not read again)
+    got, = torch.autograd.grad(y, moving, g)
+    assert torch.equal(got, want)
+    weight = w.clone().requires_grad_()
+    moving = weight * 1
+    y = T.linear_act(x, moving, b, "silu")
+    want, = torch.autograd.grad(T.linear_act(x, weight, b, "silu"), weight, g)
+    moving.detach().zero_()
+    got, = torch.autograd.grad(y, moving, g)
+    assert torch.equal(got, want)
+    residual = r.clone().requires_grad_()
+    del y
+    before = torch.cuda.memory_allocated()
+    y = T.linear_act(x, w, b, "silu", residual=residual)
+    assert torch.cuda.memory_allocated() - before == y.numel() * 2   # the result alone, no z beside it
+    del y
+    bias, free = b.clone().requires_grad_(), x.clone()
+    before = torch.cuda.memory_allocated()
+    y = T.linear_act(free, w, bias, "silu")
+    del free
+    assert torch.cuda.memory_allocated() - before == (2 * M * N - M * K) * 2         # y and z, and x has gone
+    got, = torch.autograd.grad(y, bias, g)
+    every = [v.clone().requires_grad_() for v in (x, w, b)]
+    assert torch.equal(got, torch.autograd.grad(T.linear_act(*every, "silu"), every, g)[2])
+
+
 # ---- gradient norm and clipping ---------------------------------------------------------------------------------------------------
 
 def clip_bound(want, t):
