@@ -7,6 +7,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
+from importlib.metadata import version
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -20,11 +21,17 @@ TRAIN_FLAGS = ["-fhonor-nans", "-Xclang", "-target-feature", "-Xclang", "-packed
 TRAIN_PARTS = [(src, TRAIN_FLAGS, os.path.splitext(src)[0]) for src in ("layer16_kernels.hip", "rows_kernels.hip", "clip_kernels.hip")]
 OUT = os.path.join(HERE, "libnphm_amd.so")
 TORCH_OUT = os.path.join(HERE, "libnphm_torch.so")       # the training operators' side towards PyTorch (host code only)
+STAMP = os.path.join(HERE, "libnphm.stamp")              # what both were made with; it travels with them
 OBJ_CACHE = os.path.join(HERE, "..", ".build_cache")      # objects by content hash (git- and gpurun-ignored)
 
 
+def _made_with() -> str:
+    """what the built libraries depend on beside their sources: flags, and the PyTorch whose headers and C++ interface libnphm_torch.so was made for"""
+    return hashlib.sha256(repr((FLAGS, EVAL_PARTS, TRAIN_PARTS, SOURCES, version("torch"))).encode()).hexdigest()
+
+
 def _stale() -> bool:
-    if not os.path.exists(OUT) or not os.path.exists(TORCH_OUT):
+    if not os.path.exists(OUT) or not os.path.exists(TORCH_OUT) or not os.path.exists(STAMP) or open(STAMP).read() != _made_with():
         return True
     t = min(os.path.getmtime(OUT), os.path.getmtime(TORCH_OUT))
     deps = [os.path.join(CSRC, f) for f in os.listdir(CSRC)] + [os.path.join(HERE, "..", "include", "nphm_amd.h")]
@@ -72,7 +79,6 @@ def build(force: bool = False, verbose: bool = False) -> str:
         if proc.wait() != 0:
             raise subprocess.CalledProcessError(proc.returncode, cmd)
         os.replace(tmp, obj)
-    _build_torch(force, verbose)
     out_tmp = f"{OUT}.{os.getpid()}.tmp"
     link = [hipcc, "--offload-arch=gfx950", "-shared", "-fPIC", "-pthread"] + objs + ["-o", out_tmp]
     if verbose:
@@ -85,6 +91,10 @@ def build(force: bool = False, verbose: bool = False) -> str:
     for f in os.listdir(OBJ_CACHE):
         if f.endswith(".o") and f not in keep and f.rsplit("-", 1)[0] in stems:
             os.remove(os.path.join(OBJ_CACHE, f))
+    _build_torch(force, verbose)                            # (last: the C library does not need PyTorch or a host compiler)
+    with open(f"{STAMP}.{os.getpid()}.tmp", "w") as f:
+        f.write(_made_with())
+    os.replace(f"{STAMP}.{os.getpid()}.tmp", STAMP)
     return OUT
 
 

@@ -110,6 +110,50 @@ def test_c_entries_refuse_before_any_launch():
     assert clip([big], [big], [1], [7]) != 0 and b"dtype" in lib.nphm_last_error()
 
 
+def test_build_notices_another_pytorch_and_makes_the_c_library_first(tmp_path, monkeypatch):
+    """with compilers that only write their output's name down: nothing of the tree is touched"""
+    import subprocess
+    from nphm_amd import build as B
+    for name, path in (("OUT", "a.so"), ("TORCH_OUT", "b.so"), ("STAMP", "s.stamp"), ("OBJ_CACHE", "cache")):
+        monkeypatch.setattr(B, name, str(tmp_path / path))
+    made, broken = [], []
+
+    def run(cmd, **kw):
+        if "-o" in cmd:
+            if broken and broken[0] in cmd[cmd.index("-o") + 1]:
+                raise subprocess.CalledProcessError(1, cmd)
+            made.append(cmd[cmd.index("-o") + 1])
+            open(made[-1], "w").close()
+        return subprocess.CompletedProcess(cmd, 0, b"", b"")
+
+    class Popen:
+        def __init__(self, cmd, **kw):
+            run(cmd)
+
+        def wait(self):
+            return 0
+
+    monkeypatch.setattr(B.subprocess, "run", run)
+    monkeypatch.setattr(B.subprocess, "Popen", Popen)
+    broken.append("torch_ops")
+    assert B._stale()
+    with pytest.raises(subprocess.CalledProcessError):
+        B.build()
+    assert (tmp_path / "a.so").exists() and not (tmp_path / "b.so").exists() and B._stale()
+    broken.clear()
+    B.build()
+    assert (tmp_path / "b.so").exists() and not B._stale()
+    made.clear()
+    B.build()
+    assert not made
+    monkeypatch.setattr(B, "version", lambda name: "0.0")            # another PyTorch: its side is made again, with time stamps as they were
+    assert B._stale()
+    B.build()
+    assert any("b.so" in m for m in made) and not B._stale()
+    monkeypatch.setattr(B, "FLAGS", B.FLAGS + ["-g"])
+    assert B._stale()
+
+
 # ---- rows of a table ------------------------------------------------------------------------------------------------------------
 
 @pytest.fixture(scope="module")
