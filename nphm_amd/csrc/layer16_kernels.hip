@@ -835,8 +835,9 @@ inline void gemm(hipStream_t st, GemmArgs a, Tiling t, const Columns& columns = 
   split(a, t.splits);
   auto launch = [&](auto out) {
     constexpr int O = decltype(out)::value;
-    if (t.size == 256) launch_gemm<T, 256, 2, 4, TA, TB, O>(st, a);
-    else if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, O>(st, a);
+    if constexpr (O != OUT_PARTS)                                    // (tiling() cuts k ranges for tiles of 128 and 64 alone)
+      if (t.size == 256) return launch_gemm<T, 256, 2, 4, TA, TB, O>(st, a);
+    if (t.size == 128) launch_gemm<T, 128, 2, 2, TA, TB, O>(st, a);
     else launch_gemm<T, 64, 2, 2, TA, TB, O>(st, a);
   };
   if (a.splits == 1) {
