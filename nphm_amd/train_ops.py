@@ -108,10 +108,13 @@ class LatentCodes(nn.Embedding):
     rows.  With ``sparse``, codes of more than 256 entries get their ``weight.grad`` coalesced when a backward pass has left it (which waits for
     the device; not while a graph is captured): torch.optim.SparseAdam takes it as it is, where torch would lose columns of it.  Padding in
     a batch is an entry of zeros for its own row there: no optimiser moves a row by it.
-    ``backend = "composite"`` computes the same with torch's embedding (CPU tensors need it, as in the decoders)."""
+    ``backend = "composite"`` computes the same with torch's embedding (CPU tensors need it, as in the decoders, and so do ``norm_type`` other than
+    2 and ``scale_grad_by_freq``)."""
 
-    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, scale=1.0, sparse=False, device=None, dtype=None):
-        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, max_norm=max_norm, sparse=sparse, device=device, dtype=dtype)
+    def __init__(self, num_embeddings, embedding_dim, padding_idx=None, max_norm=None, scale=1.0, sparse=False, device=None, dtype=None,
+                 norm_type=2.0, scale_grad_by_freq=False, _weight=None, _freeze=False):
+        super().__init__(num_embeddings, embedding_dim, padding_idx=padding_idx, max_norm=max_norm, norm_type=norm_type,
+                         scale_grad_by_freq=scale_grad_by_freq, sparse=sparse, _weight=_weight, _freeze=_freeze, device=device, dtype=dtype)
         if not math.isfinite(scale):
             raise ValueError(f"LatentCodes: scale {scale}")
         self.scale = float(scale)
@@ -126,6 +129,8 @@ class LatentCodes(nn.Embedding):
         if self.backend == "composite":
             rows = super().forward(idx)
             return rows if self.scale == 1.0 else rows * self.scale
+        if self.scale_grad_by_freq or (self.max_norm is not None and self.norm_type != 2):
+            raise ValueError("LatentCodes: scale_grad_by_freq and other norms than the 2-norm need backend = \"composite\"")
         if self.max_norm is not None:
             renorm_rows_(self.weight, idx, self.max_norm)
         return _ops.lookup_rows(w, idx, self.scale, self.padding_idx, 2 if self.sparse else 0)         # (2: padding stays on its own row)

@@ -63,6 +63,31 @@ def test_module_on_cpu_needs_the_composite_backend():
     other.load_state_dict(codes.state_dict())
 
 
+def test_module_takes_what_an_embedding_takes():
+    """from_pretrained and its arguments; what the kernels do not compute is refused, not left out"""
+    rows = torch.randn(6, 5)
+    codes = T.LatentCodes.from_pretrained(rows, freeze=False, padding_idx=-1, max_norm=0.5, norm_type=1.0, scale_grad_by_freq=True)
+    assert isinstance(codes, T.LatentCodes) and codes.weight.requires_grad and codes.padding_idx == 5 and codes.scale == 1.0 and codes.weight.data_ptr() == rows.data_ptr()
+    idx = torch.tensor([1, 5, 1, 2])
+    with pytest.raises(ValueError, match="composite"):
+        codes(idx)
+    codes.backend = "composite"
+    twin = torch.nn.Embedding.from_pretrained(rows.clone(), freeze=False, padding_idx=-1, max_norm=0.5, norm_type=1.0, scale_grad_by_freq=True)
+    a, b = codes(idx), twin(idx)
+    a.sum().backward()
+    b.sum().backward()
+    assert torch.equal(a, b) and torch.equal(codes.weight.grad, twin.weight.grad)
+    frozen = T.LatentCodes.from_pretrained(rows)
+    assert not frozen.weight.requires_grad and frozen.max_norm is None
+    for codes in (T.LatentCodes(4, 3, scale_grad_by_freq=True), T.LatentCodes(4, 3, max_norm=1.0, norm_type=math.inf)):
+        with pytest.raises(ValueError, match="composite"):
+            codes(idx[:1])
+    with pytest.raises(TypeError):                                  # the norm of rows that are not bounded matters to nobody: on to the device's check
+        T.LatentCodes(4, 3, norm_type=1.0)(idx[:1])
+    with pytest.raises(AssertionError):
+        T.LatentCodes.from_pretrained(rows[0])
+
+
 def test_bad_arguments_are_refused():
     for kind in (1.0, 3.0, 0.0):
         with pytest.raises(ValueError):
@@ -1078,6 +1103,24 @@ def test_padding_in_a_batch_moves_no_row_of_a_sparse_table(dev, D, kind):
             kept = codes.weight[0].detach().clone()
         assert torch.equal(codes.weight[0], kept) and set(moved) <= set(named), (idx, moved)
         assert bool(torch.isfinite(codes.weight).all())
+
+
+@gpu
+@pytest.mark.parametrize("sparse", [False, True])
+def test_pretrained_codes_look_up_and_learn(dev, sparse):
+    rows = torch.randn(7, 300, device=dev)
+    idx = torch.tensor([[2, 2], [6, 0]], device=dev)
+    codes, ref = T.LatentCodes.from_pretrained(rows.clone(), freeze=False, sparse=sparse), torch.nn.Embedding.from_pretrained(rows.clone(), freeze=False)
+    go = torch.randn(2, 2, 300, device=dev)
+    a, b = codes(idx), ref(idx)
+    assert torch.equal(a, b)
+    a.backward(go)
+    b.backward(go)
+    assert codes.weight.grad.is_sparse == sparse
+    got = codes.weight.grad.to_dense() if sparse else codes.weight.grad
+    mags = torch.zeros_like(got).index_add_(0, idx.view(-1), go.view(-1, 300).abs()).double()
+    within(got, ref.weight.grad.double(), 4 * F32 * mags)
+    assert not T.LatentCodes.from_pretrained(rows)(idx).requires_grad
 
 
 @gpu
