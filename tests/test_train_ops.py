@@ -700,6 +700,41 @@ def test_decoder_trains_with_16_bit_hidden_layers(dev, t):
         net.evaluate_train_hip(xyz, lat)
 
 
+@gpu
+@pytest.mark.parametrize("t", ["bf16", "fp16"])
+@pytest.mark.parametrize("rows", [600, 20000])
+def test_small_gradients_come_through_16_bit_layers(dev, t, rows):
+    """a loss of 2^-k times the size (a mean over points, a small weight) gives 2^-k times the gradients.  At their own size fp16 would hold the
+    smaller ones as zero.  Both passes round to 16 bits alike but for entries near fp16's smallest, off by half of 2^-24 where the
+    largest is 2^10 over the number of rows: a rounding of the gradient's 2-norm covers them, a few bits lost do not pass."""
+    torch.manual_seed(0)
+    net = DeepSDF(lat_dim=32, hidden_dim=128, nlayers=6, beta=100, out_dim=1).to(dev).train()
+    net.train_precision = t
+    xyz = torch.randn(1, rows, 3, device=dev) * 0.3
+    lat = (torch.randn(1, 1, 32, device=dev) * 0.1).requires_grad_()
+    go = torch.randn(1, rows, 1, device=dev)
+    leaves = [lat, *net.parameters()]
+    want = torch.autograd.grad(net.evaluate_train_hip(xyz, lat), leaves, go)
+    assert all(bool(torch.isfinite(g).all()) and float(g.abs().max()) > 0 for g in want)
+    for k in (12, 24, 60):
+        got = torch.autograd.grad(net.evaluate_train_hip(xyz, lat), leaves, go * 2.0 ** -k)
+        for a, b in zip(got, want):
+            assert float((a.double() * 2.0 ** k - b.double()).norm()) <= half_step(torch.float16) * float(b.double().norm()), k
+    zero = torch.autograd.grad(net.evaluate_train_hip(xyz, lat), leaves, go * 0)
+    assert not any(bool(g.any()) for g in zero)
+    net.lin1.weight.requires_grad_(False)                            # frozen parameters: none for them, the same for the others
+    net.lin4.bias.requires_grad_(False)
+    some = [p for p in leaves if p.requires_grad]
+    got = torch.autograd.grad(net.evaluate_train_hip(xyz, lat), some, go)
+    assert all(torch.equal(a, b) for a, b in zip(got, [g for g, p in zip(want, leaves) if p.requires_grad]))
+    for p in net.parameters():
+        p.requires_grad_(False)
+    assert torch.equal(torch.autograd.grad(net.evaluate_train_hip(xyz, lat), lat, go)[0], want[0])
+    net.requires_grad_(True)
+    go[0, 5] = math.inf                                              # shows, and is not scaled away
+    assert not all(bool(torch.isfinite(g).all()) for g in torch.autograd.grad(net.evaluate_train_hip(xyz, lat), leaves, go * 2.0 ** -24))
+
+
 def test_backward_workspace_is_for_the_operands_handed_over():
     """no x: no gradient of the weight, no weight: none of x - and no room for what they would need (host arithmetic, no GPU)"""
     from nphm_amd import _lib
