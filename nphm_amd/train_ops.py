@@ -65,7 +65,7 @@ def lookup_rows(table, idx, scale=1.0, padding_idx=None, sparse=False):
 def lookup_rows_grad(grad, idx, num_rows, scale=1.0, padding_idx=None):
     """Gradient of ``lookup_rows`` w.r.t. its table of `num_rows` rows: [num_rows, D] of grad's type, ``scale`` times the sum of the rows
     of `grad` [*idx.shape, D] that name a row; zeros in rows that none names and in row `padding_idx`.  Sums are in fp32, in the
-    order of the indices.  For programs that keep their own backward pass; autograd calls it by itself."""
+    order of the indices.  For programs that keep their own backward pass; autograd calls it by itself.  The result is part of no graph."""
     return _ops.lookup_rows_grad(grad, idx, num_rows, scale, padding_idx)
 
 
@@ -141,8 +141,11 @@ class LatentCodes(nn.Embedding):
 def linear_act(x, weight, bias=None, activation="none", beta=1.0, residual=None):
     """activation(x weight^T + bias) + residual, all of it behind the product in the same pass: x [..., K], weight [N, K], bias [N],
     residual [..., N], all bf16 or all fp16 (fp32 layers run on the decoders' own dense tier); products accumulate in fp32.
-    activation: "none", "relu", "silu", "gelu" (erf), "softplus" (with `beta`, as nn.Softplus).  Differentiable once w.r.t. the four
-    tensors: the value before the activation is kept in 16 bits for it.  No broadcasting: residual has the result's shape."""
+    activation: "none", "relu", "silu", "gelu" (erf), "softplus" (with `beta`, as nn.Softplus).  No broadcasting: residual has the result's
+    shape.  Up to 2^22 rows, N and K up to 2^20.  Differentiable once w.r.t. the four tensors.  Its gradients pass two roundings to the type
+    beside those of its results: the value z before the activation is kept in 16 bits, which moves the slope a'(z) by up to a third of half
+    a step (of 1, not of a'), and the gradient w.r.t. z is rounded before the two products that read it.  In fp16 the loss is scaled by
+    the program, as for any fp16 layer."""
     act = _ACTIVATIONS.get("none" if activation is None else activation)
     if act is None:
         raise ValueError(f"linear_act: activation is one of {', '.join(_ACTIVATIONS)}, not {activation!r}")
@@ -167,7 +170,7 @@ def _limit(what, max_norm):
 
 def grad_norm(grads, norm_type=2.0):
     """The 2-norm (squares added in fp64) or, with norm_type = inf, the largest magnitude over all tensors of `grads` (dense; fp32, bf16,
-    fp16, mixed): a 0-dim fp32 tensor on their device."""
+    fp16, mixed): a 0-dim fp32 tensor on their device, part of no graph."""
     kind = _kind("grad_norm", norm_type)
     grads = list(grads)
     return _ops.clip(grads, None, kind, 0.0, b"grad_norm") if grads else torch.zeros(())
@@ -177,7 +180,8 @@ def clip_grads(grads, max_norm, norm_type=2.0, out=None):
     """Scales the dense tensors of `grads` by min(1, max_norm / (norm + 1e-6)), in place, or into the tensors `out` (of the same sizes and types,
     in row-major order: pieces of a flat buffer will do).  A tensor that shares memory with another of the call, or is named twice, is
     refused.  -> (norm, the scaled tensors).  As torch's clip: a norm that is no number makes every result NaN, an infinite one makes the
-    finite entries 0."""
+    finite entries 0.  Norm and results are part of no graph.  Views with gaps go through a copy; strides so odd that it cannot be told in
+    100 000 steps whether two views meet count as meeting."""
     what = "clip_grads"
     kind, limit = _kind(what, norm_type), _limit(what, max_norm)
     grads = list(grads)
@@ -198,7 +202,7 @@ def _merge_rows_(g):
 def clip_grad_norm_(parameters, max_norm, norm_type=2.0, error_if_nonfinite=False):
     """torch.nn.utils.clip_grad_norm_ (training.py:128-131) with one norm over dense and row-sparse gradients: clips the ``.grad`` of `parameters`
     (a tensor or an iterable, none of them twice) in place and returns the norm before it (0-dim fp32).  Sparse gradients have one sparse
-    dimension; entries that name the same row count as their sum.  One that is not coalesced and has rows of more than 256 entries is
+    dimension; entries that name the same row count as their sum, in the gradient's type (as it stays in the gradient).  One that is not coalesced and has rows of more than 256 entries is
     replaced by its coalesced form (as ``LatentCodes`` does; waits for the device, not while a graph is captured).
     ``error_if_nonfinite`` waits for the device and raises before anything is scaled."""
     what = "clip_grad_norm_"
