@@ -10,6 +10,7 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/forward_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
@@ -17,6 +18,7 @@
 #include <algorithm>
 #include <cmath>
 #include <cstring>
+#include <initializer_list>
 #include <optional>
 #include <string>
 #include <tuple>
@@ -55,9 +57,15 @@ void on_gpu(const char* what, const Tensor& t) {
   TORCH_CHECK_TYPE(t.is_cuda(), what, ": a tensor on a ROCm device (these operators have no CPU form)");
 }
 void* stream_of(const Tensor& t) { return c10::hip::getCurrentHIPStream(t.get_device()).stream(); }
-// Forward-mode derivatives: none is computed, and none may be lost without a word.
+// Forward-mode derivatives: none is computed, and none may be lost without a word.  (A tensor is asked only inside a level, where alone it
+// can have a tangent: 500 gradients and their outputs took 15 us to ask.)
+bool in_forward_mode() { return torch::autograd::ForwardADLevel::try_get_by_idx(0) != nullptr; }
 void no_tangent(const char* what, const Tensor& t) {
   TORCH_CHECK_NOT_IMPLEMENTED(!t.defined() || !t._fw_grad(/*level=*/0).defined(), what, ": no forward-mode derivative (torch.autograd.forward_ad)");
+}
+void no_tangent(const char* what, std::initializer_list<const Tensor*> all) {
+  if (in_forward_mode())
+    for (const Tensor* t : all) no_tangent(what, *t);
 }
 // (address 0 and no tensor where nothing is needed)
 Tensor workspace(size_t bytes, const Tensor& like) { return bytes ? at::empty({int64_t(bytes)}, like.options().dtype(at::kByte)) : Tensor(); }
@@ -80,7 +88,7 @@ variable_list once(variable_list grads, const char* what) {
 void check_rows(const char* what, const Tensor& rows, const Tensor& idx, double scale) {
   bound();
   on_gpu(what, rows);
-  no_tangent(what, rows);
+  no_tangent(what, {&rows});
   TORCH_CHECK_TYPE(code_of(rows.scalar_type()) >= 0, what, ": rows of fp32, bf16 or fp16, not ", rows.scalar_type());
   TORCH_CHECK_TYPE(idx.scalar_type() == at::kLong || idx.scalar_type() == at::kInt, what, ": idx is an int32 or int64 tensor");
   TORCH_CHECK_VALUE(idx.device() == rows.device(), what, ": idx is on ", idx.device(), ", the rows on ", rows.device());
@@ -151,7 +159,7 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
     const int64_t rows = meta[0], padding = meta[1];
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor out;
-    no_tangent("lookup_rows", g);
+    no_tangent("lookup_rows", {&g});
     if (meta[2] == GRAD_DENSE) {
       out = rows_grad(g, idx, rows, scale, padding < 0 ? std::nullopt : std::optional<int64_t>(padding));
     } else {
@@ -243,7 +251,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
     for (int64_t bit = 1, edge = 0; bit <= 8; bit *= 2)
       if (meta[2] & bit) asked |= ctx->needs_input_grad(size_t(edge++)) ? meta[1] & bit : 0;
     variable_list out(7);                                            // (one for each argument of forward)
-    no_tangent("linear_act", g);
+    no_tangent("linear_act", {&g});
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(g.device());
@@ -276,7 +284,7 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
   const Tensor bias = bias_.value_or(Tensor()), residual = residual_.value_or(Tensor());
   on_gpu(what, x);
   on_gpu(what, weight);
-  no_tangent(what, x);
+  no_tangent(what, {&x, &weight, &bias, &residual});
   TORCH_CHECK_TYPE(x.scalar_type() == at::kBFloat16 || x.scalar_type() == at::kHalf, what, ": bf16 or fp16 tensors, not ", x.scalar_type());
   TORCH_CHECK_VALUE(x.dim() >= 1 && weight.dim() == 2 && x.size(-1) == weight.size(1) && weight.numel() > 0, what, ": x ", x.sizes(),
                     " does not fit weight ", weight.sizes());
@@ -289,7 +297,6 @@ Tensor linear_act(const Tensor& x, const Tensor& weight, const std::optional<Ten
   int bit = 2;
   for (const Tensor* t : {&weight, &bias, &residual}) {
     if (t->defined()) {
-      no_tangent(what, *t);
       TORCH_CHECK_TYPE(t->scalar_type() == x.scalar_type() && t->device() == x.device(), what, ": all tensors on one device, of one type");
       if (t->requires_grad()) asked |= bit;
     }
@@ -391,7 +398,7 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
   const std::vector<const Tensor*> grads = tensors_of(what, grad_list),
                                    out = out_list == Py_None ? std::vector<const Tensor*>{} : out_list == grad_list ? grads : tensors_of(what, out_list);
   const size_t n = grads.size();
-  const bool writes = !out.empty(), in_place = out_list == grad_list;
+  const bool writes = !out.empty(), in_place = out_list == grad_list, forward_mode = in_forward_mode();
   TORCH_CHECK_VALUE(n && (!writes || out.size() == n), what, ": ", n, " gradients, ", out.size(), " tensors in out");
   const at::NoGradGuard no_grad;
   const at::Device device = grads[0]->device();
@@ -412,8 +419,10 @@ Tensor clip(const std::string& what, PyObject* grad_list, PyObject* out_list, in
     const Tensor *g = grads[i], *o = writes ? out[i] : g;
     TORCH_CHECK_VALUE(in_place || (o->numel() == g->numel() && o->scalar_type() == g->scalar_type() && o->device() == device && o->layout() == at::kStrided),
                       what, ": out has a tensor of the size, type and device of each gradient");
-    no_tangent(what.c_str(), *g);
-    no_tangent(what.c_str(), *o);
+    if (forward_mode) {
+      no_tangent(what.c_str(), *g);
+      no_tangent(what.c_str(), *o);
+    }
     counts[i] = g->numel();
     codes[i] = code_of(g->scalar_type());
     // any order of dimensions will do, if it is the same on both sides and leaves no gap
