@@ -7,10 +7,12 @@
 
 #include <ATen/ATen.h>
 #include <c10/core/DeviceGuard.h>
+#include <c10/hip/HIPGraphsC10Utils.h>
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/forward_grad.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/library.h>
@@ -81,6 +83,20 @@ variable_list once(variable_list grads, const char* what) {
     if (g.defined()) g = g.detach().set_requires_grad(true);
   auto node = std::make_shared<torch::autograd::DelayedError>(std::string(what) + ": its gradients are not differentiable", int64_t(grads.size()));
   return (*node)(std::move(grads));
+}
+
+// A captured backward pass whose gradients go to a leaf of which a graph of eager calls is alive: autograd adds them on the stream of those calls,
+// and the default stream cannot be made to wait for a capture (the process may end by it).  Refused while nothing has happened yet.
+void check_leaves(const char* what) {
+  if (c10::hip::currentStreamCaptureStatusMayInitCtx() == c10::hip::CaptureStatus::None) return;
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  for (const auto& edge : node->next_edges()) {
+    if (!dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get())) continue;
+    const auto stream = edge.function->stream();
+    TORCH_CHECK(!stream || stream->id() != 0, "nphm: ", what, ": a backward pass is captured for a tensor of which a graph of eager calls is alive "
+                "(drop its outputs first, or capture on tensors of the graph's own)");
+  }
 }
 
 // ---- rows of a table -----------------------------------------------------------------------------------------------------------
@@ -160,6 +176,7 @@ struct LookupNode : torch::autograd::Function<LookupNode> {
     const double scale = ctx->saved_data["scale"].toDouble();
     Tensor out;
     no_tangent("lookup_rows", {&g});
+    check_leaves("lookup_rows");
     if (meta[2] == GRAD_DENSE) {
       out = rows_grad(g, idx, rows, scale, padding < 0 ? std::nullopt : std::optional<int64_t>(padding));
     } else {
@@ -252,6 +269,7 @@ struct LayerNode : torch::autograd::Function<LayerNode> {
       if (meta[2] & bit) asked |= ctx->needs_input_grad(size_t(edge++)) ? meta[1] & bit : 0;
     variable_list out(7);                                            // (one for each argument of forward)
     no_tangent("linear_act", {&g});
+    check_leaves("linear_act");
     {
       const at::NoGradGuard no_grad;
       const c10::DeviceGuard guard(g.device());

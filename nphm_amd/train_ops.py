@@ -13,7 +13,7 @@ arguments, allocates and holds its autograd node), on the current stream of its 
 ``TypeError`` for what it does not take and ``NphmAmdError`` if the library is missing or a call fails; there is no PyTorch fallback,
 CPU tensors are refused, and so are forward-mode (dual) tensors, with ``NotImplementedError``.  Results are the same bits from run to run.  All of it can be captured into a graph, except where a
 line says that it waits for the device.  (A backward pass is captured on leaves of which no graph of eager calls is alive: autograd would
-make the capturing stream wait for work outside the capture.)"""
+make the default stream wait for the capture, which it cannot.  Where the operators' own gradients would go to such a leaf they raise.)"""
 from __future__ import annotations
 
 import math

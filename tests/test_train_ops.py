@@ -1351,6 +1351,40 @@ def test_a_captured_step_replays_as_the_eager_one(dev):
 
 
 @gpu
+@pytest.mark.parametrize("op", ["layer", "lookup", "sparse lookup"])
+def test_a_captured_pass_into_an_eager_graphs_leaf_is_refused(dev, op):
+    """raised before autograd would add the gradient on the default stream; once the eager graph is gone the same capture goes through"""
+    idx, g = torch.tensor([1, 0, 1], device=dev), torch.randn(3, 8, device=dev)
+    leaf = (torch.randn(8, 8, device=dev).bfloat16() if op == "layer" else torch.randn(4, 8, device=dev)).requires_grad_()
+    x = torch.randn(3, 8, device=dev).bfloat16()
+    call = {"layer": lambda: T.linear_act(x, leaf, activation="silu"), "lookup": lambda: T.lookup_rows(leaf, idx),
+            "sparse lookup": lambda: T.lookup_rows(leaf, idx, sparse=True)}[op]
+    g = g.to(leaf.dtype)
+    alive = call()
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        with pytest.raises(NphmAmdError, match="eager calls"):
+            try:
+                call().backward(g)
+            except RuntimeError as e:                                # (autograd raises it: known by its text)
+                raise NphmAmdError(str(e)) from None
+    assert leaf.grad is None
+    alive.backward(g)
+    want = leaf.grad.to_dense() if leaf.grad.is_sparse else leaf.grad
+    leaf.grad = None
+    del alive
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        call().backward(g)
+    for _ in range(3):
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(leaf.grad.to_dense() if leaf.grad.is_sparse else leaf.grad, want)
+        leaf.grad._values().zero_() if leaf.grad.is_sparse else leaf.grad.zero_()        # (written again by the next replay)
+
+
+@gpu
 def test_operators_run_on_the_current_stream(dev):
     """work queued behind a long product on another stream: the operators wait for it there, and two streams at once do not meet"""
     x, w, b, r, g = layer_inputs(dev, torch.bfloat16, 256, 256, 256, True, True)
