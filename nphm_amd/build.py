@@ -7,7 +7,7 @@ import os
 import shutil
 import subprocess
 import sysconfig
-from importlib.metadata import version
+from importlib.metadata import PackageNotFoundError, version
 
 HERE = os.path.dirname(os.path.abspath(__file__))
 CSRC = os.path.join(HERE, "csrc")
@@ -27,7 +27,11 @@ OBJ_CACHE = os.path.join(HERE, "..", ".build_cache")      # objects by content h
 
 def _made_with() -> str:
     """what the built libraries depend on beside their sources: flags, and the PyTorch whose headers and C++ interface libnphm_torch.so was made for"""
-    return hashlib.sha256(repr((FLAGS, EVAL_PARTS, TRAIN_PARTS, SOURCES, version("torch"))).encode()).hexdigest()
+    try:
+        torch = version("torch")
+    except PackageNotFoundError:                            # (none, or one without package data: _build_torch says so where it matters)
+        torch = None
+    return hashlib.sha256(repr((FLAGS, EVAL_PARTS, TRAIN_PARTS, SOURCES, torch)).encode()).hexdigest()
 
 
 def _stale() -> bool:

@@ -178,6 +178,13 @@ def test_build_notices_another_pytorch_and_makes_the_c_library_first(tmp_path, m
     monkeypatch.setattr(B, "FLAGS", B.FLAGS + ["-g"])
     assert B._stale()
 
+    def unknown(name):
+        raise B.PackageNotFoundError(name)
+
+    monkeypatch.setattr(B, "version", unknown)
+    B.build()                                                        # a PyTorch without package data is no reason to fail
+    assert not B._stale()
+
 
 # ---- rows of a table ------------------------------------------------------------------------------------------------------------
 
