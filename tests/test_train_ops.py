@@ -1392,6 +1392,51 @@ def test_a_captured_pass_into_an_eager_graphs_leaf_is_refused(dev, op):
 
 
 @gpu
+def test_a_captured_step_of_a_wide_sparse_table(dev):
+    """inside a graph the gradient keeps an entry for every index (nothing can wait there), its duplicates folded by the clip: the same gradient as
+    the eager step's coalesced one, which the clip outside makes of it"""
+    gen = torch.Generator(device=dev).manual_seed(5)
+    start = torch.randn(12, 300, device=dev, generator=gen) * 0.1
+    own, eager = [T.LatentCodes(12, 300, max_norm=1.0, sparse=True, device=dev) for _ in range(2)]
+    idx, go = torch.tensor([3, 1, 3, 0, 3], device=dev), torch.randn(5, 300, device=dev, generator=gen)
+    s_idx, s_go = idx.clone(), go.clone()
+
+    def run(codes, i, g):
+        codes.weight.grad = None
+        codes(i).backward(g)
+        return T.clip_grad_norm_(codes.parameters(), 0.7)
+
+    for codes in (own, eager):
+        with torch.no_grad():
+            codes.weight.copy_(start)
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(own, s_idx, s_go)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        norm = run(own, s_idx, s_go)
+    captured = own.weight.grad
+    for k in range(4):
+        s_idx.copy_((idx + k) % 12)
+        s_go.copy_(go * (1 + k))
+        graph.replay()
+        torch.cuda.synchronize()
+        want = run(eager, s_idx.clone(), s_go.clone())
+        torch.cuda.synchronize()
+        mag = torch.zeros(12, 300, dtype=torch.float64, device=dev).index_add_(0, s_idx, s_go.abs().double()) * (0.7 / float(want))
+        assert abs(float(norm) - float(want)) <= 8 * F32 * float(want)
+        assert eager.weight.grad.is_coalesced() and not captured.is_coalesced() and captured._nnz() == 5
+        within(captured.to_dense(), eager.weight.grad.to_dense().double(), mag * 16 * F32 + 1e-30)
+        assert torch.equal(own.weight, eager.weight)
+    before = captured.to_dense()
+    own.weight.grad = captured
+    T.clip_grad_norm_(own.parameters(), 1e9)
+    assert own.weight.grad.is_coalesced() and float((own.weight.grad.to_dense() - before).abs().max()) <= 2 * F32 * float(before.abs().max())
+
+
+@gpu
 def test_operators_run_on_the_current_stream(dev):
     """work queued behind a long product on another stream: the operators wait for it there, and two streams at once do not meet"""
     x, w, b, r, g = layer_inputs(dev, torch.bfloat16, 256, 256, 256, True, True)
